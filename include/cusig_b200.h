@@ -255,6 +255,62 @@ int sigb200_sig_backprop_noalloc_d(const double* path, double* out, const double
                                    int synchronize);
 uint64_t sigb200_noalloc_scratch_bytes(void);
 
+/* --- sequence operators ---------------------------------------------------------------
+ * Element types: 0 float32, 1 float64, 2 bfloat16, 3 float16.  "State" arrays (initial, state,
+ * checkpoints, state_derivs, dinitial) are float64 for float64 inputs, else float32, and contiguous.
+ * Strides are in elements; channels are adjacent.  Device pointers run on the device that owns them, on
+ * `stream` (a cudaStream_t passed as void*), and return before completion unless synchronize != 0; host
+ * pointers are staged (contiguous arrays only) and return when the result is there.  None of these
+ * have a counterpart in the reference. */
+
+/* Gated linear recurrence along the rows of x (batch, length, dimension):
+ *   h_t = a_t h_{t-1} + b_t,   b_t = complement ? (1 - a_t) x_t : x_t,   h_{-1} = initial (or 0),
+ * with a_t = gate, exp(gate) or 1 / (1 + exp(-gate)) for gate_form 0, 1, 2.  `gates` divides dimension;
+ * gate (batch, length, gates) then serves dimension / gates neighbouring channels each.  gate_type is
+ * `type`, or 0 for 16-bit types.  Written: out (batch, length, dimension), contiguous; state (batch,
+ * dimension), the last h, optional; checkpoints (batch, ceil(length / 64), dimension), the states that
+ * enter rows 0, 64, .., optional, for the backward pass.
+ * sequences > 0: packed sequences, batch 1; sequence i holds rows offsets[i] to offsets[i + 1] - 1
+ * (sequences + 1 non-decreasing values within 0 .. length; int64 with wide_offsets, else int32), initial
+ * and state are (sequences, dimension); rows of no sequence come out as 0.  Offsets in device
+ * memory are not validated: wrong ones give wrong numbers, never an access out of bounds. */
+int sigb200_linear_recurrence(int type, int gate_type, const void* x, const void* gate, const void* initial,
+                              const void* offsets, void* out, void* state, void* checkpoints, uint64_t batch_size,
+                              uint64_t length, uint64_t dimension, uint64_t gates, uint64_t sequences,
+                              uint64_t x_batch_stride, uint64_t x_row_stride, uint64_t gate_batch_stride,
+                              uint64_t gate_row_stride, int gate_form, bool complement, bool wide_offsets,
+                              void* stream, int synchronize);
+
+/* Backward of the recurrence: from the derivatives of out (derivs, like x) and of state (state_derivs,
+ * optional) to dx (like out), dgate (batch, length, gates) and dinitial (optional).  checkpoints: those of
+ * the forward pass of the same inputs, or NULL (they are then recomputed by a pass over x and gate). */
+int sigb200_linear_recurrence_backprop(int type, int gate_type, const void* derivs, const void* x, const void* gate,
+                                       const void* initial, const void* offsets, const void* state_derivs,
+                                       const void* checkpoints, void* dx, void* dgate, void* dinitial,
+                                       uint64_t batch_size, uint64_t length, uint64_t dimension, uint64_t gates,
+                                       uint64_t sequences, uint64_t derivs_batch_stride, uint64_t derivs_row_stride,
+                                       uint64_t x_batch_stride, uint64_t x_row_stride, uint64_t gate_batch_stride,
+                                       uint64_t gate_row_stride, int gate_form, bool complement, bool wide_offsets,
+                                       void* stream, int synchronize);
+
+/* One row for each of batch_size states: state (batch_size, dimension) becomes a state + b, out its
+ * value in the type of x. */
+int sigb200_linear_recurrence_step(int type, int gate_type, const void* x, const void* gate, void* state, void* out,
+                                   uint64_t batch_size, uint64_t dimension, uint64_t gates, uint64_t x_stride,
+                                   uint64_t gate_stride, int gate_form, bool complement, void* stream, int synchronize);
+
+/* Rotary positions on x (outer, inner, length, dimension): the pair i < rotary_dimension / 2 of a row,
+ * channels (i, i + rotary_dimension / 2) or, interleaved, (2i, 2i + 1), is turned by position *
+ * frequencies[i] (radians) and multiplied by scale; the channels from rotary_dimension on are copied.
+ * inverse turns the other way, which is the adjoint.  position_type: 0 the row index (positions is
+ * ignored), 1 int32, 2 int64, 3 float32, 4 float64; position strides may be 0.  out must not overlap x. */
+int sigb200_rotary(int type, int position_type, const void* x, const double* frequencies, const void* positions,
+                   void* out, uint64_t outer, uint64_t inner, uint64_t length, uint64_t dimension,
+                   uint64_t rotary_dimension, uint64_t x_outer_stride, uint64_t x_inner_stride, uint64_t x_row_stride,
+                   uint64_t out_outer_stride, uint64_t out_inner_stride, uint64_t out_row_stride,
+                   uint64_t position_outer_stride, uint64_t position_inner_stride, uint64_t position_row_stride,
+                   bool interleaved, bool inverse, double scale, void* stream, int synchronize);
+
 /* Number of coefficients of a signature, scalar term included; 0 on overflow.
  * Same contract as the CPU library's sig_length (siglib/cpsig/cp_utils.cpp:91-105). */
 uint64_t sigb200_sig_length(uint64_t dimension, uint64_t degree);

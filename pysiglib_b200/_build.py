@@ -38,9 +38,11 @@ def _tile_parts():
 
 def _units():
     """(object name, source, extra flags) for every translation unit."""
-    units = [(n + ".o", n + ".cu", []) for n in ("abi", "dispatch", "runtime", "sig_generic", "sig_tile_dispatch", "sig_algebra", "sig_log", "sig_coef", "sig_chen", "sig_log_stream", "noalloc")]
+    units = [(n + ".o", n + ".cu", []) for n in ("abi", "dispatch", "runtime", "sig_generic", "sig_tile_dispatch", "sig_algebra", "sig_log", "sig_coef", "sig_chen", "sig_log_stream", "noalloc", "recurrence", "rotary")]
     for k in range(_tile_parts()):
         units.append(("sig_tile_inst_%d.o" % k, "sig_tile_inst.cu", ["-DSIG_TILE_PART=%d" % k]))
+    for k in range(6):  # pairs of element types of the recurrence kernels
+        units.append(("recurrence_inst_%d.o" % k, "recurrence_inst.cu", ["-DSIG_RECURRENCE_PART=%d" % k]))
     return units
 
 

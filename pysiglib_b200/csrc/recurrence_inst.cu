@@ -1,0 +1,133 @@
+// Launchers of the recurrence kernels for one pair of element types (SIG_RECURRENCE_PART picks it; one
+// object each, so that the pairs compile side by side).
+#include <algorithm>
+
+#include "recurrence.h"
+#include "recurrence_kernels.cuh"
+
+namespace sigb200 {
+namespace {
+
+// Channels a thread holds: 16 bytes of float32 or float64, 8 of the 16-bit types (whose gates and states
+// widen to the same registers).
+template <typename X> constexpr int kWide = sizeof(X) == 8 ? 2 : 4;
+// Rows a thread holds: 8 forward; 4 backward where V > 1, as the five arrays of S * V values stay in registers.
+template <int V> constexpr int kBackwardRows = V == 1 ? 8 : 4;
+constexpr int kForwardRows = 8;
+
+int log2_ceil(uint64_t n) {
+    int k = 0;
+    while ((1ull << k) < n) ++k;
+    return k;
+}
+
+// 256 threads: as many side by side as make 128 bytes of a row (full lines, and the narrowest strips,
+// hence the most CTAs), the others behind one another in the rows.  Short inputs trade parts for lanes.
+template <typename X>
+RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
+    const int columns = log2_ceil((p.dim + V - 1) / V), needed = log2_ceil((p.rows + S - 1) / S);
+    RecurrencePlan plan{};
+    plan.log_lanes = std::min({columns, log2_ceil(128 / (V * sizeof(X))), 5});
+    plan.log_parts = std::min({8 - plan.log_lanes, needed, 6});
+    plan.log_lanes = std::min(columns, 8 - plan.log_parts);
+    plan.log_parts = std::max(plan.log_parts, 5 - plan.log_lanes);  // at least a warp
+    const uint64_t lanes = 1ull << plan.log_lanes;
+    const uint64_t strips = ((p.dim + V - 1) / V + lanes - 1) / lanes;
+    if (strips > 0x7fffffffull / p.batch) throw std::invalid_argument("linear_recurrence: problem too large for one kernel launch");
+    plan.strips = static_cast<unsigned>(strips);
+    return plan;
+}
+
+void check(const char* what) {
+    count_launch();
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) throw CudaFailure(err, std::string(what) + ": " + cudaGetErrorString(err));
+}
+
+template <typename X, typename G, int V, bool SHARED>
+void forward(const RecurrenceArgs& p, cudaStream_t stream) {
+    const RecurrencePlan plan = make_plan<X>(p, V, kForwardRows);
+    const int lanes = 1 << plan.log_lanes, parts = 1 << plan.log_parts;
+    recurrence_forward_kernel<X, G, V, kForwardRows, SHARED>
+        <<<static_cast<unsigned>(p.batch * plan.strips), lanes * parts, recurrence_smem<Acc<X>, V>(2, lanes, parts), stream>>>(p, plan);
+    check("linear recurrence kernel");
+}
+
+template <typename X, typename G, int V, bool SHARED>
+void backward(const RecurrenceArgs& p, cudaStream_t stream) {
+    RecurrencePlan plan = make_plan<X>(p, V, kBackwardRows<V>);
+    const int lanes = 1 << plan.log_lanes, parts = 1 << plan.log_parts;
+    Acc<X>* partial = nullptr;
+    uint64_t per_gate = 0;
+    if (SHARED) {  // lanes whose channels share a gate, as far as a power of two goes
+        per_gate = p.dim / p.gate_dim / V;
+        while (plan.fold_log < std::min(plan.log_lanes, 5) && per_gate % 2 == 0) { per_gate /= 2; ++plan.fold_log; }
+    }
+    const uint64_t n = p.batch * p.rows * p.gate_dim;
+    Scratch scratch(per_gate > 1 ? checked_mul(n, per_gate * sizeof(Acc<X>), "linear_recurrence_backprop") : 0, stream);
+    if (per_gate > 1) partial = scratch.as<Acc<X>>();
+    recurrence_backward_kernel<X, G, V, kBackwardRows<V>, SHARED>
+        <<<static_cast<unsigned>(p.batch * plan.strips), lanes * parts, recurrence_smem<Acc<X>, V>(3, lanes, parts), stream>>>(p, plan, partial);
+    check("linear recurrence backward kernel");
+    if (partial) {
+        if (n / 256 >= 0x7fffffffull) throw std::invalid_argument("linear_recurrence_backprop: problem too large for one kernel launch");
+        fold_partials_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(partial, static_cast<G*>(p.dgate), n, per_gate);
+        check("linear recurrence gate gradient kernel");
+    }
+}
+
+template <typename X, typename G, int V, bool SHARED>
+void step(const RecurrenceArgs& p, cudaStream_t stream) {
+    const uint64_t n = p.rows * (p.dim / V);
+    if (n / 256 >= 0x7fffffffull) throw std::invalid_argument("linear_recurrence_step: problem too large for one kernel launch");
+    recurrence_step_kernel<X, G, V, SHARED><<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(p);
+    check("linear recurrence step kernel");
+}
+
+// Whether every access of a thread's V channels is one aligned load or store.
+template <typename X, typename G, int V>
+bool aligned(const RecurrenceArgs& p, bool shared) {
+    const auto fits = [](const void* ptr, size_t bytes) { return reinterpret_cast<uintptr_t>(ptr) % bytes == 0; };
+    const uint64_t group = p.dim / p.gate_dim;
+    if (p.dim % V || p.x_batch % V || p.x_row % V || p.d_batch % V || p.d_row % V) return false;
+    for (const void* ptr : {p.x, p.derivs, static_cast<const void*>(p.out), static_cast<const void*>(p.dx)})
+        if (!fits(ptr, V * sizeof(X))) return false;
+    if (!fits(p.state, V * sizeof(Acc<X>))) return false;
+    if (shared) return group % V == 0;
+    return p.gate_batch % V == 0 && p.gate_row % V == 0 && fits(p.gate, V * sizeof(G)) && fits(p.dgate, V * sizeof(G));
+}
+
+}  // namespace
+
+template <typename X, typename G>
+void launch_recurrence(RecurrencePass pass, const RecurrenceArgs& p, cudaStream_t stream) {
+    constexpr int W = kWide<X>;
+    const bool shared = p.gate_dim != p.dim;
+    const bool wide = aligned<X, G, W>(p, shared);
+#define SIG_RECURRENCE(fn)                                                                   \
+    wide ? (shared ? fn<X, G, W, true>(p, stream) : fn<X, G, W, false>(p, stream))           \
+         : (shared ? fn<X, G, 1, true>(p, stream) : fn<X, G, 1, false>(p, stream))
+    switch (pass) {
+        case RecurrencePass::forward: SIG_RECURRENCE(forward); break;
+        case RecurrencePass::backward: SIG_RECURRENCE(backward); break;
+        case RecurrencePass::step: SIG_RECURRENCE(step); break;
+    }
+#undef SIG_RECURRENCE
+}
+
+#define SIG_INSTANTIATE(X, G) template void launch_recurrence<X, G>(RecurrencePass, const RecurrenceArgs&, cudaStream_t);
+#if SIG_RECURRENCE_PART == 0
+SIG_INSTANTIATE(float, float)
+#elif SIG_RECURRENCE_PART == 1
+SIG_INSTANTIATE(double, double)
+#elif SIG_RECURRENCE_PART == 2
+SIG_INSTANTIATE(__nv_bfloat16, __nv_bfloat16)
+#elif SIG_RECURRENCE_PART == 3
+SIG_INSTANTIATE(__nv_bfloat16, float)
+#elif SIG_RECURRENCE_PART == 4
+SIG_INSTANTIATE(__half, __half)
+#else
+SIG_INSTANTIATE(__half, float)
+#endif
+
+}  // namespace sigb200

@@ -1,0 +1,245 @@
+"""Gated linear recurrences along paths: ``linear_recurrence``, its backward pass and its single-row step.
+
+``h_t = a_t h_{t-1} + b_t`` for every channel: a learned memory of a sequence, computed by a parallel scan.
+No counterpart in the reference; the conventions (paths ``(..., length, dimension)``, ``*_backprop``, NumPy
+or torch) are those of the signature operators."""
+from math import prod
+from typing import Union
+
+import numpy as np
+import torch
+
+from .param_checks import check_type
+from .sequence_inputs import (batched_rows, call, check_like, check_state, contiguous, element_type, empty, on_device, pointer,
+                              state_dtype, stream_of, zeros)
+
+GATE_FORMS = {"value": 0, "log": 1, "logit": 2}
+CHECKPOINT_ROWS = 64  # rows between two of the states kept for the backward pass
+
+
+class _Recurrence:
+    """Checked and flattened arguments of one call."""
+
+    def __init__(self, x, gate, initial, gate_form, complement, offsets):
+        self.type = element_type(x, "x")
+        self.gate_type = element_type(gate, "gate")
+        check_like(gate, "gate", x, "x")
+        if self.gate_type != self.type and not (self.gate_type == 0 and self.type >= 2):
+            raise TypeError("gate.dtype must be that of x, or float32 for 16-bit x; got %s for %s" % (gate.dtype, x.dtype))
+        check_type(gate_form, "gate_form", str)
+        if gate_form not in GATE_FORMS:
+            raise ValueError("gate_form must be one of 'value', 'log' or 'logit', got %r" % gate_form)
+        check_type(complement, "complement", bool)
+        self.form, self.complement = GATE_FORMS[gate_form], complement
+        shape = tuple(x.shape)
+        if len(shape) < 2:
+            raise ValueError("x must have at least rank 2, got rank %d." % len(shape))
+        self.rows, self.dim = shape[-2:]
+        self.gates = gate.shape[-1] if len(gate.shape) else 0
+        if self.dim == 0:
+            raise ValueError("x has 0 channels (dimension). Its dimension must be at least 1.")
+        if tuple(gate.shape[:-1]) != shape[:-1] or self.gates == 0 or self.dim % self.gates:
+            raise ValueError("gate must have shape %s + (G,) with G dividing %d, got %s"
+                             % (shape[:-1], self.dim, tuple(gate.shape)))
+        self.shape, self.gate_shape = shape, tuple(gate.shape)
+        self.batch = prod(shape[:-2])
+        self.offsets, self.wide, self.sequences = None, False, 0
+        self.state_shape = (*shape[:-2], self.dim)
+        if offsets is not None:
+            self._set_offsets(offsets, x)
+        self.initial = check_state(initial, "initial", self.state_shape, x)
+        self.x, self.x_batch, self.x_row = batched_rows(x)
+        self.gate, self.gate_batch, self.gate_row = batched_rows(gate)
+        self.marks_shape = (*shape[:-2], -(-self.rows // CHECKPOINT_ROWS), self.dim)
+        self.empty = self.batch == 0 or self.rows == 0
+
+    def _set_offsets(self, offsets, x):
+        check_type(offsets, "offsets", (np.ndarray, torch.Tensor))
+        if len(self.shape) != 2:
+            raise ValueError("packed sequences (offsets) need x of shape (rows, dimension), got %s" % (self.shape,))
+        if len(offsets.shape) != 1 or offsets.shape[0] < 2:
+            raise ValueError("offsets must be one row of at least 2 values, got shape %s" % (tuple(offsets.shape),))
+        if str(offsets.dtype).replace("torch.", "") not in ("int32", "int64"):
+            raise TypeError("offsets.dtype must be int32 or int64, got %s instead" % offsets.dtype)
+        if not on_device(offsets):
+            values = np.asarray(offsets).astype(np.int64)
+            if values[0] < 0 or values[-1] > self.rows or (np.diff(values) < 0).any():
+                raise ValueError("offsets must not decrease and must lie between 0 and %d" % self.rows)
+        if isinstance(x, torch.Tensor):
+            if on_device(offsets):
+                check_like(offsets, "offsets", x, "x")
+            else:
+                offsets = torch.as_tensor(offsets).to(x.device)
+        elif not isinstance(offsets, np.ndarray):
+            check_like(offsets, "offsets", x, "x")
+        self.offsets = contiguous(offsets)
+        self.wide = str(offsets.dtype).endswith("int64")
+        self.sequences = offsets.shape[0] - 1
+        self.state_shape = (self.sequences, self.dim)
+
+    def tail(self, x):
+        return self.form, self.complement, self.wide, stream_of(x), 0
+
+
+def linear_recurrence(
+        x: Union[np.ndarray, torch.Tensor],
+        gate: Union[np.ndarray, torch.Tensor],
+        initial: Union[np.ndarray, torch.Tensor, None] = None,
+        *,
+        gate_form: str = "value",
+        complement: bool = False,
+        offsets: Union[np.ndarray, torch.Tensor, None] = None,
+        return_state: bool = False,
+        return_checkpoints: bool = False
+):
+    """Gated linear recurrence ``h_t = a_t h_{t-1} + b_t`` along axis -2, channel by channel.
+
+    :param x: inputs ``(..., length, dimension)`` of type float32, float64, float16 or bfloat16.  CUDA
+        tensors are processed on their device and on its current stream, without waiting for the
+        result; views with adjacent channels are read in place.  NumPy arrays and CPU tensors go
+        through the current CUDA device.
+    :param gate: ``(..., length, G)`` with ``G`` dividing ``dimension``: gate ``g`` serves the channels
+        ``g * dimension / G`` up to the next gate's.  Its type is that of ``x``, or float32 for 16-bit ``x``.
+    :param initial: state before the first row, ``(..., dimension)``, float64 for float64 ``x``, else
+        float32; 0 if absent.
+    :param gate_form: how ``a`` comes from ``gate``: ``"value"`` a = gate, ``"log"`` a = exp(gate),
+        ``"logit"`` a = 1 / (1 + exp(-gate)).
+    :param complement: ``b_t = (1 - a_t) x_t`` instead of ``b_t = x_t``.
+    :param offsets: packed sequences: ``x`` is ``(rows, dimension)`` and sequence ``i`` holds the rows
+        ``offsets[i]`` to ``offsets[i + 1] - 1`` (int32 or int64, ``n + 1`` values that do not decrease).
+        Sequences may be empty; rows of no sequence come out as 0.  ``initial`` and the state are
+        ``(n, dimension)``.  Values on the host are checked, those on the device are trusted: wrong ones
+        give wrong numbers.
+    :param return_state: also return the state after the last row (``initial`` for an empty sequence),
+        ready for ``linear_recurrence_step``.
+    :param return_checkpoints: also return the states before rows 0, 64, 128, .., which
+        ``linear_recurrence_backprop`` would otherwise compute again.
+    :return: ``h`` like ``x`` (contiguous), or a tuple ``(h, state, checkpoints)`` without the parts not
+        asked for.
+
+    States and sums are held in float32 (float64 for float64 ``x``); ``h`` is rounded once, on its way out.
+    The scan multiplies the gates of neighbouring rows: where such a product leaves the range of the
+    state's type (gates well above 1 over many rows) the result is not finite.
+
+    Example::
+
+        import torch, pysiglib_b200 as psl
+        x, g = torch.randn(8, 1000, 64, device="cuda"), torch.randn(8, 1000, 64, device="cuda")
+        h, state = psl.linear_recurrence(x, g, gate_form="logit", complement=True, return_state=True)
+        y = psl.linear_recurrence_step(x[:, 0], g[:, 0], state, gate_form="logit", complement=True)
+    """
+    check_type(return_state, "return_state", bool)
+    check_type(return_checkpoints, "return_checkpoints", bool)
+    r = _Recurrence(x, gate, initial, gate_form, complement, offsets)
+    h = empty(x, r.shape, x.dtype)
+    wide = state_dtype(x)
+    state = empty(x, r.state_shape, wide) if return_state else None
+    marks = empty(x, r.marks_shape, wide) if return_checkpoints else None
+    if r.empty:
+        if return_state:
+            state[...] = 0 if r.initial is None else r.initial
+    else:
+        call("linear_recurrence", r.type, r.gate_type, pointer(r.x), pointer(r.gate), pointer(r.initial),
+             pointer(r.offsets), pointer(h), pointer(state), pointer(marks), r.batch, r.rows, r.dim, r.gates,
+             r.sequences, r.x_batch, r.x_row, r.gate_batch, r.gate_row, *r.tail(x))
+    if return_state:
+        return (h, state, marks) if return_checkpoints else (h, state)
+    return (h, marks) if return_checkpoints else h
+
+
+def linear_recurrence_backprop(
+        derivs: Union[np.ndarray, torch.Tensor],
+        x: Union[np.ndarray, torch.Tensor],
+        gate: Union[np.ndarray, torch.Tensor],
+        initial: Union[np.ndarray, torch.Tensor, None] = None,
+        *,
+        gate_form: str = "value",
+        complement: bool = False,
+        offsets: Union[np.ndarray, torch.Tensor, None] = None,
+        state_derivs: Union[np.ndarray, torch.Tensor, None] = None,
+        checkpoints: Union[np.ndarray, torch.Tensor, None] = None
+):
+    """Backward pass of ``linear_recurrence``: from ``dF/dh`` to ``(dF/dx, dF/dgate, dF/dinitial)``.
+
+    :param derivs: derivatives with respect to ``h``, of the shape and type of ``x``.
+    :param state_derivs: derivatives with respect to the final state, of its shape and type.
+    :param checkpoints: those that ``linear_recurrence`` returned for the same inputs; without them a pass
+        over ``x`` and ``gate`` computes them again.
+    :return: gradients in the shapes and types of ``x``, ``gate`` and ``initial`` (``None`` without an
+        ``initial``); rows of no sequence get 0.
+
+    The other parameters are those of ``linear_recurrence``.  Results do not depend on the order in
+    which threads finish: the same call gives the same bits.
+    """
+    r = _Recurrence(x, gate, initial, gate_form, complement, offsets)
+    check_like(derivs, "derivs", x, "x")
+    if derivs.dtype != x.dtype:
+        raise TypeError("derivs.dtype must be that of x, got %s for %s" % (derivs.dtype, x.dtype))
+    if tuple(derivs.shape) != r.shape:
+        raise ValueError("derivs must have the shape of x, %s, got %s" % (r.shape, tuple(derivs.shape)))
+    state_derivs = check_state(state_derivs, "state_derivs", r.state_shape, x)
+    checkpoints = check_state(checkpoints, "checkpoints", r.marks_shape, x)
+    d, d_batch, d_row = batched_rows(derivs)
+    dx, dgate = empty(x, r.shape, x.dtype), empty(x, r.gate_shape, gate.dtype)
+    dinitial = None if initial is None else empty(x, r.state_shape, state_dtype(x))
+    if r.empty:
+        if dinitial is not None:
+            dinitial[...] = 0 if state_derivs is None else state_derivs
+        return dx, dgate, dinitial
+    call("linear_recurrence_backprop", r.type, r.gate_type, pointer(d), pointer(r.x), pointer(r.gate),
+         pointer(r.initial), pointer(r.offsets), pointer(state_derivs), pointer(checkpoints), pointer(dx),
+         pointer(dgate), pointer(dinitial), r.batch, r.rows, r.dim, r.gates, r.sequences, d_batch, d_row, r.x_batch,
+         r.x_row, r.gate_batch, r.gate_row, *r.tail(x))
+    return dx, dgate, dinitial
+
+
+def linear_recurrence_step(
+        x: Union[np.ndarray, torch.Tensor],
+        gate: Union[np.ndarray, torch.Tensor],
+        state: Union[np.ndarray, torch.Tensor],
+        *,
+        gate_form: str = "value",
+        complement: bool = False
+) -> Union[np.ndarray, torch.Tensor]:
+    """One more row for each of a batch of recurrences: ``state`` becomes ``a state + b``.
+
+    :param x: the new rows, ``(..., dimension)``.
+    :param gate: their gates, ``(..., G)`` as in ``linear_recurrence``.
+    :param state: ``(..., dimension)``, contiguous, float64 for float64 ``x``, else float32.  Overwritten.
+    :return: the new state in the type of ``x``.
+
+    Stepping through a sequence gives what ``linear_recurrence`` gives for it, up to rounding.
+    """
+    shape = tuple(getattr(x, "shape", ()))
+    code = element_type(x, "x")
+    gate_code = element_type(gate, "gate")
+    check_like(gate, "gate", x, "x")
+    check_like(state, "state", x, "x")
+    if gate_code != code and not (gate_code == 0 and code >= 2):
+        raise TypeError("gate.dtype must be that of x, or float32 for 16-bit x; got %s for %s" % (gate.dtype, x.dtype))
+    check_type(gate_form, "gate_form", str)
+    if gate_form not in GATE_FORMS:
+        raise ValueError("gate_form must be one of 'value', 'log' or 'logit', got %r" % gate_form)
+    check_type(complement, "complement", bool)
+    if len(shape) < 1:
+        raise ValueError("x must have at least rank 1, got rank 0.")
+    dim, gates = shape[-1], gate.shape[-1] if len(gate.shape) else 0
+    if dim == 0:
+        raise ValueError("x has 0 channels (dimension). Its dimension must be at least 1.")
+    if tuple(gate.shape[:-1]) != shape[:-1] or gates == 0 or dim % gates:
+        raise ValueError("gate must have shape %s + (G,) with G dividing %d, got %s" % (shape[:-1], dim, tuple(gate.shape)))
+    if state.dtype != state_dtype(x):
+        raise TypeError("state.dtype must be %s for x of type %s, got %s instead" % (state_dtype(x), x.dtype, state.dtype))
+    if tuple(state.shape) != shape:
+        raise ValueError("state must have the shape of x, %s, got %s" % (shape, tuple(state.shape)))
+    if not (state.is_contiguous() if isinstance(state, torch.Tensor) else state.flags["C_CONTIGUOUS"] and state.flags["WRITEABLE"]):
+        raise ValueError("state is overwritten: it must be contiguous and writeable")
+    if isinstance(state, torch.Tensor) and state.requires_grad:
+        raise ValueError("state is overwritten: it cannot require a gradient (use linear_recurrence to differentiate)")
+    x, gate = contiguous(x), contiguous(gate)
+    out = empty(x, shape, x.dtype)
+    batch = prod(shape[:-1])
+    if batch:
+        call("linear_recurrence_step", code, gate_code, pointer(x), pointer(gate), pointer(state), pointer(out), batch,
+             dim, gates, dim, gates, GATE_FORMS[gate_form], complement, stream_of(x), 0)
+    return out

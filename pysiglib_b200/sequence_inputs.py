@@ -1,0 +1,112 @@
+"""Arrays of the sequence operators (``linear_recurrence``, ``rotary``): element types, strides, outputs.
+
+Besides float32 and float64 these take float16 and (torch) bfloat16.  Torch views whose channels are
+adjacent are read in place, whatever their batch and row strides (an expanded axis included); others are
+copied once.  NumPy in gives NumPy out, torch in torch out on the same device."""
+import numpy as np
+import torch
+
+from . import load_cusig
+from .error_codes import err_msg
+from .param_checks import check_type
+
+TORCH_TYPES = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.float16: 3}
+NUMPY_TYPES = {np.dtype(np.float32): 0, np.dtype(np.float64): 1, np.dtype(np.float16): 3}
+
+
+def element_type(array, name):
+    """Number of the element type in the C ABI."""
+    if isinstance(array, torch.Tensor):
+        code = TORCH_TYPES.get(array.dtype)
+    else:
+        check_type(array, name, (np.ndarray, torch.Tensor))
+        code = NUMPY_TYPES.get(array.dtype)
+    if code is None:
+        raise TypeError("%s.dtype must be float32, float64, float16 or bfloat16, got %s instead" % (name, array.dtype))
+    return code
+
+
+def state_dtype(array):
+    """Type of states: float64 for float64 inputs, else float32."""
+    if isinstance(array, torch.Tensor):
+        return torch.float64 if array.dtype is torch.float64 else torch.float32
+    return np.dtype(np.float64 if array.dtype == np.float64 else np.float32)
+
+
+def check_like(array, name, like, like_name):
+    """Same kind and device as ``like``."""
+    check_type(array, name, (np.ndarray, torch.Tensor))
+    if isinstance(array, torch.Tensor) != isinstance(like, torch.Tensor):
+        raise ValueError("%s and %s must both be numpy arrays or both torch tensors" % (name, like_name))
+    if isinstance(array, torch.Tensor) and array.device != like.device:
+        raise ValueError("%s and %s must be on the same device" % (name, like_name))
+
+
+def check_state(array, name, shape, x):
+    """A contiguous state-shaped input, or None."""
+    if array is None:
+        return None
+    check_like(array, name, x, "x")
+    if array.dtype != state_dtype(x):
+        raise TypeError("%s.dtype must be %s for x of type %s, got %s instead" % (name, state_dtype(x), x.dtype, array.dtype))
+    if tuple(array.shape) != tuple(shape):
+        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(array.shape)))
+    return contiguous(array)
+
+
+def contiguous(array):
+    return array.contiguous() if isinstance(array, torch.Tensor) else np.ascontiguousarray(array)
+
+
+def on_device(array):
+    return isinstance(array, torch.Tensor) and array.is_cuda
+
+
+def pointer(array):
+    if array is None:
+        return None
+    return array.data_ptr() if isinstance(array, torch.Tensor) else array.ctypes.data
+
+
+def empty(like, shape, dtype):
+    if isinstance(like, torch.Tensor):
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    return np.empty(shape, dtype=dtype)
+
+
+def zeros(like, shape, dtype):
+    if isinstance(like, torch.Tensor):
+        return torch.zeros(shape, dtype=dtype, device=like.device)
+    return np.zeros(shape, dtype=dtype)
+
+
+def batched_rows(array):
+    """``(array, batch stride, row stride)`` of (..., L, C) with the batch axes read as one: in place where
+    the strides allow it, else a contiguous copy."""
+    shape = array.shape
+    width, rows = shape[-1], shape[-2]
+    if on_device(array):
+        strides = array.stride()
+        if strides[-1] == 1 or width == 1:
+            if array.dim() == 2:
+                return array, 0, strides[0]
+            if array.dim() == 3:
+                return array, strides[0], strides[1]
+            axis = array.dim() - 3
+            while axis > 0 and (shape[axis - 1] == 1 or strides[axis - 1] == strides[axis] * shape[axis]):
+                axis -= 1
+            if axis == 0:
+                return array, strides[-3], strides[-2]
+    array = contiguous(array)
+    return array, rows * width, width
+
+
+def stream_of(array):
+    return torch.cuda.current_stream(array.device).cuda_stream if on_device(array) else None
+
+
+def call(name, *args):
+    """One native call; raises what the package's other operators raise."""
+    code = getattr(load_cusig.library(), "sigb200_" + name)(*args)
+    if code:
+        raise Exception("Error in pysiglib.%s: %s" % (name, err_msg(code)))

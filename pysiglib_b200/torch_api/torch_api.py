@@ -8,6 +8,7 @@ from typing import Union
 import numpy as np
 import torch
 
+from ..param_checks import check_type
 from ..sig import sig as sig_forward
 from ..sig import sig_combine as sig_combine_forward
 from ..sig import sig_combine_backprop
@@ -19,6 +20,10 @@ from ..sig_coef import sig_coef as sig_coef_forward
 from ..sig_coef import sig_coef_backprop
 from ..sig_join import sig_join as sig_join_forward
 from ..sig_join import sig_join_backprop
+from ..linear_recurrence import linear_recurrence as linear_recurrence_forward
+from ..linear_recurrence import linear_recurrence_backprop
+from ..rotary import rotary as rotary_forward
+from ..rotary import rotary_backprop
 from ..transform_path import transform_path as transform_path_forward
 from ..transform_path import transform_path_backprop
 
@@ -224,3 +229,78 @@ def sig_coef(path, words, *, time_aug: bool = False, lead_lag: bool = False, end
 
 
 sig_coef.__doc__ = sig_coef_forward.__doc__
+
+
+class LinearRecurrence(torch.autograd.Function):
+    """Keeps x, the gates and one state of 64 for the backward pass, not h."""
+
+    @staticmethod
+    def forward(ctx, x, gate, initial, gate_form, complement, offsets):
+        h, state, marks = linear_recurrence_forward(x, gate, initial, gate_form=gate_form, complement=complement,
+                                                    offsets=offsets, return_state=True, return_checkpoints=True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, gate, initial, offsets, marks)
+        ctx.args = (gate_form, complement)
+        return h, state
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_h, grad_state):
+        x, gate, initial, offsets, marks = ctx.saved_tensors
+        gate_form, complement = ctx.args
+        if grad_h is None:
+            if grad_state is None:
+                return (None,) * 6
+            grad_h = torch.zeros_like(x)
+        dx, dgate, dinitial = linear_recurrence_backprop(grad_h, x, gate, initial, gate_form=gate_form,
+                                                         complement=complement, offsets=offsets,
+                                                         state_derivs=grad_state, checkpoints=marks)
+        return dx, dgate, dinitial, None, None, None
+
+
+def linear_recurrence(x, gate, initial=None, *, gate_form: str = "value", complement: bool = False, offsets=None,
+                      return_state: bool = False, return_checkpoints: bool = False):
+    if not isinstance(x, torch.Tensor) or return_checkpoints:
+        if isinstance(x, torch.Tensor) and torch.is_grad_enabled() and any(
+                isinstance(t, torch.Tensor) and t.requires_grad for t in (x, gate, initial)):
+            raise ValueError("checkpoints are kept by the autograd graph: return_checkpoints needs inputs without gradients")
+        return linear_recurrence_forward(x, gate, initial, gate_form=gate_form, complement=complement, offsets=offsets,
+                                         return_state=return_state, return_checkpoints=return_checkpoints)
+    check_type(return_state, "return_state", bool)
+    if isinstance(offsets, np.ndarray):
+        offsets = torch.from_numpy(offsets)
+    h, state = LinearRecurrence.apply(x, gate, initial, gate_form, complement, offsets)
+    return (h, state) if return_state else h
+
+
+linear_recurrence.__doc__ = linear_recurrence_forward.__doc__
+
+
+class Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, frequencies, positions, interleaved, scale, inverse):
+        out = rotary_forward(x, frequencies, positions, interleaved=interleaved, scale=scale, inverse=inverse)
+        ctx.save_for_backward(frequencies, positions)
+        ctx.args = (interleaved, scale, inverse)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output):
+        frequencies, positions = ctx.saved_tensors
+        interleaved, scale, inverse = ctx.args
+        grad = rotary_backprop(grad_output, frequencies, positions, interleaved=interleaved, scale=scale,
+                               inverse=inverse)
+        return grad, None, None, None, None, None
+
+
+def rotary(x, frequencies, positions=None, *, interleaved: bool = False, scale: float = 1., inverse: bool = False):
+    if not isinstance(x, torch.Tensor):
+        return rotary_forward(x, frequencies, positions, interleaved=interleaved, scale=scale, inverse=inverse)
+    for t, name in ((frequencies, "frequencies"), (positions, "positions")):
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            raise ValueError("rotary has no gradient with respect to %s: detach them" % name)
+    return Rotary.apply(x, frequencies, positions, interleaved, scale, inverse)
+
+
+rotary.__doc__ = rotary_forward.__doc__

@@ -1,0 +1,304 @@
+"""Gated linear recurrences on the GPU against the row-by-row float64 definition, within the bounds that the
+roundings of the arithmetic allow (sequence_oracle)."""
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+import pysiglib_b200 as psl
+import sequence_oracle as so
+from pysiglib_b200 import load_cusig, torch_api
+
+pytestmark = pytest.mark.gpu
+
+F32, F64, BF16, F16 = torch.float32, torch.float64, torch.bfloat16, torch.float16
+
+
+def make(seed, batch, rows, dim, gates, dtype, gate_dtype, form, initial, sequences=0, dense_offsets=True):
+    g = torch.Generator().manual_seed(seed)
+    lead = () if sequences else (batch,)
+    x = torch.randn(*lead, rows, dim, generator=g, dtype=F64).to(dtype)
+    logits = 2.0 + 1.5 * torch.randn(*lead, rows, gates, generator=g, dtype=F64)
+    gate = {"value": torch.sigmoid(logits) * torch.where(torch.rand(logits.shape, generator=g) < 0.1, -1.0, 1.0).double(),
+            "log": torch.nn.functional.logsigmoid(logits), "logit": logits}[form].to(gate_dtype)
+    derivs = torch.randn(*lead, rows, dim, generator=g, dtype=F64).to(dtype)
+    count = sequences or batch
+    wide = so.state_type(dtype)
+    start = torch.randn(count, dim, generator=g, dtype=F64).to(wide) if initial else None
+    tail = torch.randn(count, dim, generator=g, dtype=F64).to(wide)
+    offsets = None
+    if sequences:
+        lo, hi = (0, rows) if dense_offsets else (min(3, rows), max(min(3, rows), rows - 5))
+        cuts = torch.randint(lo, hi + 1, (sequences - 1,), generator=g).sort().values
+        offsets = torch.cat([torch.tensor([lo]), cuts, torch.tensor([hi])])
+    return x, gate, start, derivs, tail, offsets
+
+
+def cuda(t):
+    return None if t is None else t.cuda()
+
+
+def run_and_check(data, form, complement, checkpoints=True, tail=True, **kw):
+    x, gate, start, derivs, state_derivs, offsets = data
+    state_derivs = state_derivs if tail else None
+    expect = so.recurrence(x, gate, start, form, complement, offsets, derivs, state_derivs)
+    how = {"gate_form": form, "complement": complement, "offsets": cuda(offsets)}
+    X, G, S = cuda(x), cuda(gate), cuda(start)
+    before = load_cusig.launch_count()
+    h, state, marks = psl.linear_recurrence(X, G, S, return_state=True, return_checkpoints=True, **how)
+    dx, dgate, dinitial = psl.linear_recurrence_backprop(cuda(derivs), X, G, S, state_derivs=cuda(state_derivs),
+                                                         checkpoints=marks if checkpoints else None, **how)
+    assert load_cusig.launch_count() > before
+    assert h.dtype == x.dtype and dgate.dtype == gate.dtype and state.dtype == so.state_type(x.dtype)
+    for name, got in (("h", h), ("state", state), ("dx", dx), ("dgate", dgate)):
+        so.check(got, expect[name], name)
+    if start is None:
+        assert dinitial is None
+    else:
+        so.check(dinitial, expect["dinitial"], "dinitial")
+    return h
+
+
+TYPES = [(F32, F32), (F64, F64), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)]
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 7, 8, 9, 31, 33, 63, 64, 65, 127, 129, 200, 513, 1030])
+@pytest.mark.parametrize("dim", [1, 3, 4, 17, 32, 100])
+def test_sizes(rows, dim):
+    form = ("value", "log", "logit")[rows % 3]
+    run_and_check(make(rows * 7 + dim, 2, rows, dim, dim, F32, F32, form, rows % 2 == 0), form, rows % 4 > 1)
+
+
+@pytest.mark.parametrize("dtype,gate_dtype", TYPES)
+@pytest.mark.parametrize("form", ["value", "log", "logit"])
+@pytest.mark.parametrize("complement", [False, True])
+def test_types_and_forms(dtype, gate_dtype, form, complement):
+    for dim in (24, 21):
+        run_and_check(make(dim, 3, 150, dim, dim, dtype, gate_dtype, form, True), form, complement)
+
+
+@pytest.mark.parametrize("dim,gates", [(64, 1), (64, 2), (64, 16), (96, 2), (40, 8), (340, 85), (34, 17), (15, 3), (51, 3),
+                                       (384, 3), (1024, 4), (260, 1)])
+@pytest.mark.parametrize("dtype,gate_dtype", [(F32, F32), (F64, F64), (BF16, F32), (F16, F16)])
+def test_shared_gates(dim, gates, dtype, gate_dtype):
+    run_and_check(make(dim + gates, 2, 75, dim, gates, dtype, gate_dtype, "logit", True), "logit", gates % 2 == 0)
+
+
+@pytest.mark.parametrize("rows,sequences", [(1, 1), (1, 5), (6, 9), (40, 3), (64, 64), (150, 7), (300, 1), (515, 40), (1300, 300)])
+@pytest.mark.parametrize("dense", [True, False])
+@pytest.mark.parametrize("dtype,gate_dtype,dim", [(F32, F32, 36), (BF16, F32, 35), (F64, F64, 6)])
+def test_packed_sequences(rows, sequences, dense, dtype, gate_dtype, dim):
+    data = make(rows + sequences, 1, rows, dim, dim, dtype, gate_dtype, "log", rows % 2 == 0, sequences, dense)
+    h = run_and_check(data, "log", rows % 3 == 0)
+    offsets = data[-1]
+    outside = torch.ones(rows, dtype=torch.bool)
+    outside[int(offsets[0]):int(offsets[-1])] = False
+    assert (h.cpu()[outside] == 0).all()
+
+
+def test_packed_is_each_sequence_alone():
+    x, gate, start, derivs, tail, offsets = make(3, 1, 400, 20, 5, F32, F32, "logit", True, 11)
+    how = {"gate_form": "logit", "complement": True}
+    packed, state = psl.linear_recurrence(cuda(x), cuda(gate), cuda(start), offsets=offsets.to(torch.int32), return_state=True, **how)
+    expect = so.recurrence(x, gate, start, "logit", True, offsets)
+    for k, (lo, hi) in enumerate(so.spans_of(offsets, 400)):
+        h, s = psl.linear_recurrence(cuda(x)[lo:hi], cuda(gate)[lo:hi], cuda(start)[k], return_state=True, **how)
+        so.check(h, (packed[lo:hi].cpu().double(), 2 * expect["h"][1][lo:hi]), "h")
+        so.check(s, (state[k].cpu().double(), 2 * expect["state"][1][k]), "state")
+
+
+@pytest.mark.parametrize("checkpoints,tail,initial", list(itertools.product([True, False], repeat=3)))
+def test_backward_with_and_without_its_optional_parts(checkpoints, tail, initial):
+    run_and_check(make(5, 2, 333, 48, 48, BF16, F32, "log", initial), "log", False, checkpoints, tail)
+    run_and_check(make(6, 1, 333, 10, 5, F32, F32, "value", initial, 9, False), "value", True, checkpoints, tail)
+
+
+def test_many_channels_and_long_rows():
+    run_and_check(make(1, 3, 70, 1999, 1999, F32, F32, "logit", True), "logit", True)
+    run_and_check(make(2, 70, 20, 260, 260, BF16, BF16, "log", True), "log", False)
+    run_and_check(make(3, 1, 20000, 8, 8, F32, F32, "log", True), "log", True)
+    run_and_check(make(4, 1, 9000, 12, 3, BF16, F32, "logit", False, 13), "logit", False)
+    run_and_check(make(5, 2, 5000, 1, 1, F64, F64, "value", True), "value", False)
+
+
+def test_views_are_read_in_place():
+    g = torch.Generator().manual_seed(1)
+    wide = torch.randn(2, 3, 90, 4 * 24, generator=g)
+    x, gate, derivs = wide[..., :24], wide[..., 24:48], wide[..., 48:72]
+    expect = so.recurrence(x.reshape(6, 90, 24), gate.reshape(6, 90, 24), None, "logit", True, None, derivs.reshape(6, 90, 24))
+    W = wide.cuda()
+    X, G, D = W[..., :24], W[..., 24:48], W[..., 48:72]
+    h, marks = psl.linear_recurrence(X, G, gate_form="logit", complement=True, return_checkpoints=True)
+    dx, dgate, _ = psl.linear_recurrence_backprop(D, X, G, gate_form="logit", complement=True, checkpoints=marks)
+    for name, got in (("h", h), ("dx", dx), ("dgate", dgate)):
+        so.check(got.reshape(6, 90, 24), expect[name], name)
+    # rows and batch swapped, an odd start, channels apart, a gate for all rows and batch entries
+    for view in (lambda t: t.transpose(0, 1), lambda t: t[:, 1:, 3:20], lambda t: t[..., ::2], lambda t: t[:, ::3]):
+        base = torch.randn(40, 41, 24, generator=g)
+        v = view(base)
+        one = torch.randn(1, 1, v.shape[-1], generator=g).expand(*v.shape)
+        expect = so.recurrence(v.contiguous(), one.contiguous(), None, "logit", False, None, v.contiguous())
+        V, O = view(base.cuda()), one[:1, :1].contiguous().cuda().expand(*v.shape)
+        so.check(psl.linear_recurrence(V, O, gate_form="logit"), expect["h"], "h")
+        dx, dgate, _ = psl.linear_recurrence_backprop(V, V, O, gate_form="logit")
+        so.check(dx, expect["dx"], "dx")
+        so.check(dgate, expect["dgate"], "dgate")
+
+
+def test_a_sequence_keeps_its_nan_and_infinities_to_itself():
+    x, gate, start, derivs, tail, offsets = make(9, 1, 700, 33, 33, F32, F32, "log", True, 6)
+    offsets = torch.tensor([0, 5, 130, 131, 300, 600, 700])
+    expect = so.recurrence(x, gate, start, "log", False, offsets, derivs, tail)
+    bad = x.clone()
+    bad_gate = gate.clone()
+    bad[200], bad[400], bad_gate[130], derivs_bad = float("nan"), float("inf"), float("nan"), derivs.clone()
+    derivs_bad[200] = float("nan")
+    how = {"gate_form": "log", "offsets": cuda(offsets)}
+    h, state = psl.linear_recurrence(cuda(bad), cuda(bad_gate), cuda(start), return_state=True, **how)
+    dx, dgate, dinitial = psl.linear_recurrence_backprop(cuda(derivs_bad), cuda(bad), cuda(bad_gate), cuda(start), state_derivs=cuda(tail), **how)
+    clean = [0, 1, 5]
+    for k in clean:
+        lo, hi = int(offsets[k]), int(offsets[k + 1])
+        for name, got in (("h", h), ("dx", dx), ("dgate", dgate)):
+            so.check(got[lo:hi], (expect[name][0][lo:hi], expect[name][1][lo:hi]), "%s of %d" % (name, k))
+        so.check(state[k], (expect["state"][0][k], expect["state"][1][k]), "state")
+        so.check(dinitial[k], (expect["dinitial"][0][k], expect["dinitial"][1][k]), "dinitial")
+    assert torch.isnan(h[200:300]).all() and not torch.isfinite(h[400:600]).any() and torch.isnan(h[130]).all()
+
+
+@pytest.mark.parametrize("form,closed,open_", [("value", 0.0, 1.0), ("log", -float("inf"), 0.0), ("logit", -float("inf"), float("inf"))])
+def test_gates_that_are_closed_or_open(form, closed, open_):
+    x = torch.randn(2, 300, 20, generator=torch.Generator().manual_seed(2))
+    gate = torch.full((2, 300, 20), open_)
+    gate[:, ::50] = closed
+    so.check(psl.linear_recurrence(x.cuda(), gate.cuda(), gate_form=form), so.recurrence(x, gate, None, form, False)["h"], "h")
+    h = psl.linear_recurrence(x.cuda(), gate.cuda(), gate_form=form, complement=True)
+    so.check(h, so.recurrence(x, gate, None, form, True)["h"], "h")
+    lowest = torch.full((2, 300, 20), torch.finfo(F32).min if form != "value" else 0.0)
+    h = psl.linear_recurrence(x.cuda(), lowest.cuda(), gate_form=form, complement=True)
+    assert torch.equal(h.cpu(), x)
+
+
+@pytest.mark.parametrize("dtype,gate_dtype", TYPES)
+@pytest.mark.parametrize("dim,gates", [(32, 32), (32, 4), (7, 7), (9, 3)])
+def test_steps_continue_a_prompt(dtype, gate_dtype, dim, gates):
+    x, gate, start, *_ = make(11, 3, 40, dim, gates, dtype, gate_dtype, "logit", True)
+    for complement in (False, True):
+        expect = so.recurrence(x, gate, start, "logit", complement)
+        X, G = cuda(x), cuda(gate)
+        _, state = psl.linear_recurrence(X[:, :25], G[:, :25], cuda(start), gate_form="logit", complement=complement, return_state=True)
+        for t in range(25, 40):
+            out = psl.linear_recurrence_step(X[:, t], G[:, t], state, gate_form="logit", complement=complement)
+            so.check(out, (expect["h"][0][:, t], expect["h"][1][:, t]), "row %d" % t)
+        so.check(state, expect["state"], "state")
+
+
+def test_gradients_against_differences():
+    x, gate, start, derivs, tail, offsets = (t.cuda() if t is not None else None for t in make(21, 1, 12, 6, 2, F64, F64, "logit", True, 3))
+    for form, complement in itertools.product(("value", "log", "logit"), (False, True)):
+        leaves = [t.clone().requires_grad_() for t in (x, gate if form != "log" else -gate.abs(), start)]
+
+        def f(*args):
+            return torch_api.linear_recurrence(*args, gate_form=form, complement=complement, offsets=offsets, return_state=True)
+        assert torch.autograd.gradcheck(f, leaves, eps=1e-6, atol=1e-6, rtol=1e-5)
+
+
+def test_autograd_partial_gradients():
+    x, gate, start, derivs, tail, _ = make(22, 2, 70, 8, 8, F32, F32, "logit", True)
+    expect = so.recurrence(x, gate, start, "logit", False, None, torch.zeros_like(derivs), tail)
+    X, G, S = (t.cuda().requires_grad_() for t in (x, gate, start))
+    h, state = torch_api.linear_recurrence(X, G, S, gate_form="logit", return_state=True)
+    gx, gg, gs = torch.autograd.grad(state, (X, G, S), tail.cuda())
+    for name, got in (("dx", gx), ("dgate", gg), ("dinitial", gs)):
+        so.check(got, expect[name], name)
+    only = torch_api.linear_recurrence(X, G.detach(), gate_form="logit")
+    only.sum().backward()
+    expect = so.recurrence(x, gate, None, "logit", False, None, torch.ones_like(derivs))
+    so.check(X.grad, expect["dx"], "dx")
+    assert G.grad is None
+
+
+def test_same_bits_on_every_run():
+    x, gate, start, derivs, tail, offsets = (cuda(t) for t in make(23, 1, 3000, 192, 3, BF16, F32, "log", True, 17))
+    def once():
+        h, marks = psl.linear_recurrence(x, gate, start, gate_form="log", offsets=offsets, return_checkpoints=True)
+        return (h, *psl.linear_recurrence_backprop(derivs, x, gate, start, gate_form="log", offsets=offsets, checkpoints=marks))
+    first = once()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, once()))
+
+
+def test_side_streams_and_graphs():
+    sets = [make(30 + k, 2, 260, 96, 1, F32, F32, "logit", True) for k in range(2)]
+    expects = [so.recurrence(x, gate, start, "logit", True, None, derivs) for x, gate, start, derivs, *_ in sets]
+    static = [[cuda(t) for t in s[:4]] for s in sets]
+
+    def both(x, gate, start, derivs):
+        h, marks = psl.linear_recurrence(x, gate, start, gate_form="logit", complement=True, return_checkpoints=True)
+        return (h, *psl.linear_recurrence_backprop(derivs, x, gate, start, gate_form="logit", complement=True, checkpoints=marks))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    results = []
+    for k in range(2):
+        with torch.cuda.stream(streams[k]):
+            results.append(both(*static[k]))
+    torch.cuda.synchronize()
+    names = ("h", "dx", "dgate", "dinitial")
+    for k in range(2):
+        for name, got in zip(names, results[k]):
+            so.check(got, expects[k][name], name)
+    # two captured calls, replayed in turns and on other inputs
+    graphs, outs = [], []
+    for k in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(both(*static[k]))
+        graphs.append(graph)
+    for order in ((0, 1), (1, 0)):
+        for k in order:
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        for k in range(2):
+            for name, got in zip(names, outs[k]):
+                so.check(got, expects[k][name], name)
+    for a, b in zip(static[0], static[1]):
+        a.copy_(b)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    for name, got in zip(names, outs[0]):
+        so.check(got, expects[1][name], name)
+
+
+def test_more_than_32_bits_of_elements():
+    rows, dim = (1 << 31) // 1024 + 4096, 1024
+    x = torch.zeros(rows, dim, dtype=BF16, device="cuda")
+    gate = torch.full((1, 1), 0.5, dtype=BF16, device="cuda").expand(rows, 1)
+    x[rows - 3] = 1.0
+    h, state = psl.linear_recurrence(x, gate, return_state=True)
+    assert float(h[: rows - 3].abs().max()) == 0
+    assert h[rows - 3:, 7].tolist() == [1.0, 0.5, 0.25] and h[rows - 1].unique().numel() == 1
+    assert float(state.min()) == float(state.max()) == 0.25
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64, np.float16])
+def test_host_arrays(dtype):
+    t = {np.float32: F32, np.float64: F64, np.float16: F16}[dtype]
+    x, gate, start, derivs, tail, offsets = make(40, 1, 90, 12, 4, t, t, "logit", True, 5)
+    expect = so.recurrence(x, gate, start, "logit", True, offsets, derivs, tail)
+    to = lambda v: v.numpy()
+    how = {"gate_form": "logit", "complement": True, "offsets": to(offsets)}
+    h, state, marks = psl.linear_recurrence(to(x), to(gate), to(start), return_state=True, return_checkpoints=True, **how)
+    assert isinstance(h, np.ndarray) and h.dtype == dtype
+    for m in (marks, None):
+        dx, dgate, dinitial = psl.linear_recurrence_backprop(to(derivs), to(x), to(gate), to(start), state_derivs=to(tail), checkpoints=m, **how)
+        for name, got in (("h", h), ("state", state), ("dx", dx), ("dgate", dgate), ("dinitial", dinitial)):
+            so.check(torch.from_numpy(got), expect[name], name)
+    cpu = psl.linear_recurrence(x.to(t), gate, start, gate_form="logit", complement=True, offsets=offsets)
+    assert cpu.device.type == "cpu"
+    so.check(cpu, expect["h"], "h")
+    s = to(start).copy()
+    out = psl.linear_recurrence_step(to(x)[:5], to(gate)[:5], s, gate_form="logit", complement=True)
+    one = so.recurrence(x[:5, None], gate[:5, None], start, "logit", True)
+    so.check(torch.from_numpy(out), (one["h"][0][:, 0], one["h"][1][:, 0]), "step")
+    so.check(torch.from_numpy(s), one["state"], "state")
