@@ -21,19 +21,25 @@ int log2_ceil(uint64_t n) {
     return k;
 }
 
-// 256 threads: as many side by side as make 128 bytes of a row (full lines, and the narrowest strips,
-// hence the most CTAs), the others behind one another in the rows.  Short inputs trade parts for lanes.
+// Up to 8 warps whose lanes lie side by side in the channels as far as 128 bytes of a row go (full lines, and
+// the narrowest strips, hence the most CTAs) and behind one another in the rows beyond that.
 template <typename X>
 RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     const int columns = log2_ceil((p.dim + V - 1) / V), needed = log2_ceil((p.rows + S - 1) / S);
     RecurrencePlan plan{};
     plan.log_lanes = std::min({columns, log2_ceil(128 / (V * sizeof(X))), 5});
-    plan.log_parts = std::min({8 - plan.log_lanes, needed, 6});
-    plan.log_lanes = std::min(columns, 8 - plan.log_parts);
-    plan.log_parts = std::max(plan.log_parts, 5 - plan.log_lanes);  // at least a warp
+    // short inputs: no more parts than there are rows for, the lanes go to the channels instead
+    plan.log_lanes = std::max(plan.log_lanes, std::min(columns, 5 - std::min(needed, 5)));
+    plan.warps = 1 << std::min(3, std::max(0, needed - (5 - plan.log_lanes)));
     const uint64_t lanes = 1ull << plan.log_lanes;
     const uint64_t strips = ((p.dim + V - 1) / V + lanes - 1) / lanes;
-    if (strips > 0x7fffffffull / p.batch) throw std::invalid_argument("linear_recurrence: problem too large for one kernel launch");
+    const uint64_t span = uint64_t(plan.warps) * (32 >> plan.log_lanes) * S;
+    // two CTAs an SM at a time: share strips while that many are not there, as long as every CTA has rows
+    const uint64_t slots = 2 * uint64_t(device_context(current_device()).sm_count);
+    plan.cluster = 1;
+    while (plan.cluster < 8 && p.batch * strips * plan.cluster * 2 <= slots && span * plan.cluster < p.rows) plan.cluster *= 2;
+    if (strips * plan.cluster > 0x7fffffffull / p.batch)
+        throw std::invalid_argument("linear_recurrence: problem too large for one kernel launch");
     plan.strips = static_cast<unsigned>(strips);
     return plan;
 }
@@ -44,30 +50,52 @@ void check(const char* what) {
     if (err != cudaSuccess) throw CudaFailure(err, std::string(what) + ": " + cudaGetErrorString(err));
 }
 
+template <typename... Params, typename... Args>
+void launch(void (*kernel)(Params...), const RecurrenceArgs& p, const RecurrencePlan& plan, size_t smem, cudaStream_t stream, Args... args) {
+    if (smem > 48 * 1024) SIG_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(p.batch * plan.strips * plan.cluster));
+    config.blockDim = dim3(32 * plan.warps);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = plan.cluster;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = plan.cluster > 1 ? 1 : 0;
+    SIG_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, p, plan, args...));
+}
+
 template <typename X, typename G, int V, bool SHARED>
 void forward(const RecurrenceArgs& p, cudaStream_t stream) {
     const RecurrencePlan plan = make_plan<X>(p, V, kForwardRows);
-    const int lanes = 1 << plan.log_lanes, parts = 1 << plan.log_parts;
-    recurrence_forward_kernel<X, G, V, kForwardRows, SHARED>
-        <<<static_cast<unsigned>(p.batch * plan.strips), lanes * parts, recurrence_smem<Acc<X>, V>(2, lanes, parts), stream>>>(p, plan);
+    const int threads = 32 * plan.warps;
+    const size_t smem = Prefetch<X, V, kForwardRows>::smem(threads) + (Prefetch<G, SHARED ? 1 : V, kForwardRows>::smem(threads) + 15) / 16 * 16 +
+                        scan_bytes<Acc<X>, V>(1 << plan.log_lanes, plan.warps, plan.cluster, 1);
+    if (p.sequences) launch(recurrence_forward_kernel<X, G, V, kForwardRows, SHARED, true>, p, plan, smem, stream);
+    else launch(recurrence_forward_kernel<X, G, V, kForwardRows, SHARED, false>, p, plan, smem, stream);
     check("linear recurrence kernel");
 }
 
 template <typename X, typename G, int V, bool SHARED>
 void backward(const RecurrenceArgs& p, cudaStream_t stream) {
-    RecurrencePlan plan = make_plan<X>(p, V, kBackwardRows<V>);
-    const int lanes = 1 << plan.log_lanes, parts = 1 << plan.log_parts;
+    constexpr int S = kBackwardRows<V>;
+    RecurrencePlan plan = make_plan<X>(p, V, S);
     Acc<X>* partial = nullptr;
     uint64_t per_gate = 0;
     if (SHARED) {  // lanes whose channels share a gate, as far as a power of two goes
         per_gate = p.dim / p.gate_dim / V;
-        while (plan.fold_log < std::min(plan.log_lanes, 5) && per_gate % 2 == 0) { per_gate /= 2; ++plan.fold_log; }
+        while (plan.fold_log < plan.log_lanes && per_gate % 2 == 0) { per_gate /= 2; ++plan.fold_log; }
     }
     const uint64_t n = p.batch * p.rows * p.gate_dim;
     Scratch scratch(per_gate > 1 ? checked_mul(n, per_gate * sizeof(Acc<X>), "linear_recurrence_backprop") : 0, stream);
     if (per_gate > 1) partial = scratch.as<Acc<X>>();
-    recurrence_backward_kernel<X, G, V, kBackwardRows<V>, SHARED>
-        <<<static_cast<unsigned>(p.batch * plan.strips), lanes * parts, recurrence_smem<Acc<X>, V>(3, lanes, parts), stream>>>(p, plan, partial);
+    const int threads = 32 * plan.warps;
+    const size_t smem = 2 * Prefetch<X, V, S>::smem(threads) + (Prefetch<G, SHARED ? 1 : V, S>::smem(threads) + 15) / 16 * 16 +
+                        scan_bytes<Acc<X>, V>(1 << plan.log_lanes, plan.warps, plan.cluster, 2);
+    if (p.sequences) launch(recurrence_backward_kernel<X, G, V, S, SHARED, true>, p, plan, smem, stream, partial);
+    else launch(recurrence_backward_kernel<X, G, V, S, SHARED, false>, p, plan, smem, stream, partial);
     check("linear recurrence backward kernel");
     if (partial) {
         if (n / 256 >= 0x7fffffffull) throw std::invalid_argument("linear_recurrence_backprop: problem too large for one kernel launch");

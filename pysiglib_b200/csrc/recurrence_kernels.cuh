@@ -6,19 +6,24 @@
 // same recurrence from the other end in u_t = a_t g_t, the gradient handed to row t - 1: with d_t the
 // derivatives of h_t, g_t = d_t + u_{t+1}, dx_t = g_t (or (1 - a_t) g_t) and da_t = g_t (h_{t-1} - [x_t]).
 //
-// Split.  One element costs three to six values of traffic and a handful of operations, so everything
-// here is about keeping enough loads in flight.  A CTA owns a strip of CL * V neighbouring channels and
-// TP * S rows at a time: thread (tt, tc) holds S consecutive rows of V channels in registers, reduces them
-// to one (A, B), and reads the (A, B) of the threads before it from shared memory to get the state that
-// enters its rows; a second walk over its registers then gives the S states.  Every input is read once,
-// every output written once, and the state that crosses an iteration stays in registers, in 32 bits (64
-// for float64 inputs).  A run is folded into the state one S-row map at a time, so the products of gates
-// that are formed are S long (CTA-row long across a cluster) and no longer.
+// Split.  A value costs three to five values of traffic and a few dozen operations at most, so the loads have to
+// be in flight all the time.  A CTA owns a strip of CL * V neighbouring channels and walks down the rows, W warps
+// times 32 / CL parts times S rows at a time: each thread holds S consecutive rows of V channels in
+// registers and reduces them to one map.  The maps of a warp are composed by shuffles, those of the warps go
+// through shared memory, and a second walk over the registers gives the S states.  The next
+// iteration's inputs are copied into shared memory (asynchronously, into slots that only the thread itself reads)
+// while this one's are folded and stored.  Every input is read once, every output written once, and the
+// state that crosses an iteration stays in registers, in 32 bits (64 for float64 inputs).
+//
+// Where strips are too few to fill the GPU, a cluster of CTAs shares one: each takes a block of rows of every
+// iteration and writes its map into the shared memory of the others; the cluster's barrier is the only wait.
 //
 // Packed sequences are one scan over all rows in which the first row of a sequence drops what enters it:
 // the drop is a flag beside (A, B), not a gate of 0, so that a NaN or an infinity of one sequence
 // stays inside it.
 #pragma once
+
+#include <cooperative_groups.h>
 
 #include "sequence.h"
 #include "sequence_types.cuh"
@@ -26,8 +31,9 @@
 namespace sigb200 {
 
 struct RecurrencePlan {
-    int log_lanes;     // CL = 1 << log_lanes threads side by side in the channels
-    int log_parts;     // TP = 1 << log_parts threads behind each other in the rows
+    int log_lanes;     // CL = 1 << log_lanes threads side by side in the channels, 32 / CL parts in a warp
+    int warps;         // W
+    int cluster;       // CTAs that share a strip
     unsigned strips;   // strips of CL * V channels
     int fold_log;      // backward, shared gates: lanes folded into one partial sum, log2
 };
@@ -63,6 +69,9 @@ struct SequenceWalk {
     __device__ __forceinline__ void advance(int64_t row) {
         while (next <= row) { ++seq; settle(); }
     }
+    __device__ __forceinline__ void retreat(int64_t row) {
+        while (begin > row) { --seq; settle(); }
+    }
     __device__ __forceinline__ bool inside() const { return seq >= 0 && seq < count; }
     // no sequence starts or ends in [row, row + n), and all of those rows are in one
     __device__ __forceinline__ bool quiet(int64_t row, int n) const { return inside() && begin < row && next > row + n; }
@@ -94,19 +103,22 @@ __device__ __forceinline__ int64_t sequence_of(SequenceWalk walk, int64_t row) {
     return walk.seq;
 }
 
-// a and 1 - a, neither by cancellation: exp and expm1 for logarithms; for logits both come from e^-|v|.
-__device__ __forceinline__ void gate_factors(int form, float v, float& a, float& rest) {
-    if (form == kGateValue) { a = v; rest = 1.0f - v; }
-    else if (form == kGateLog) { a = expf(v); rest = -expm1f(v); }
+// a and 1 - a, neither by cancellation: exp and expm1 for logarithms; for logits both from e^-|v|, with the
+// hardware's reciprocal (within 2 ulp on [1, 2]) in place of a division.
+template <int FORM>
+__device__ __forceinline__ void gate_factors(float v, float& a, float& rest) {
+    if (FORM == kGateValue) { a = v; rest = 1.0f - v; }
+    else if (FORM == kGateLog) { a = expf(v); rest = -expm1f(v); }
     else {
-        const float e = expf(-fabsf(v)), r = 1.0f / (1.0f + e), s = e * r;
+        const float e = expf(-fabsf(v)), r = __fdividef(1.0f, 1.0f + e), s = e * r;
         a = v >= 0.0f ? r : s;
         rest = v >= 0.0f ? s : r;
     }
 }
-__device__ __forceinline__ void gate_factors(int form, double v, double& a, double& rest) {
-    if (form == kGateValue) { a = v; rest = 1.0 - v; }
-    else if (form == kGateLog) { a = exp(v); rest = -expm1(v); }
+template <int FORM>
+__device__ __forceinline__ void gate_factors(double v, double& a, double& rest) {
+    if (FORM == kGateValue) { a = v; rest = 1.0 - v; }
+    else if (FORM == kGateLog) { a = exp(v); rest = -expm1(v); }
     else {
         const double e = exp(-fabs(v)), r = 1.0 / (1.0 + e), s = e * r;
         a = v >= 0.0 ? r : s;
@@ -117,99 +129,289 @@ __device__ __forceinline__ void gate_factors(int form, double v, double& a, doub
 __device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_(double a, double b, double c) { return fma(a, b, c); }
 
-// S rows of V values each; rows at or beyond `rows` and channels beyond the last one read as zero.
+// The next iteration's S rows of V values of one array.  4 bytes and more go asynchronously to
+// slot [row][thread] of shared memory; single 16-bit values, which that copy does not know, to registers.
+// Rows before 0, at or beyond `rows`, and channels beyond the last one read as zero.
 template <typename T, int V, int S>
-__device__ __forceinline__ void load_rows(Pack<T, V> (&r)[S], const T* base, int64_t row0, int64_t rows, int64_t stride,
-                                          bool live) {
-#pragma unroll
-    for (int s = 0; s < S; ++s)
-        r[s] = live && row0 + s < rows ? load_pack<T, V>(base + (row0 + s) * stride) : Pack<T, V>{};
-}
+struct Prefetch {
+    static constexpr int kBytes = sizeof(T) * V;
+    static constexpr bool kShared = kBytes >= 4;
+    static constexpr size_t smem(int threads) { return kShared ? size_t(kBytes) * S * threads : 0; }
+    Pack<T, V> held[kShared ? 1 : S];
+    Pack<T, V>* slot;
 
-// Bytes of shared memory: `kinds` value arrays (A and the Bs) and the drop flags, of both buffers.
+    __device__ __forceinline__ void issue(const T* base, int64_t row0, int64_t rows, int64_t stride, bool live) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const bool on = live && row0 + s >= 0 && row0 + s < rows;
+            const T* from = base + (on ? (row0 + s) * stride : 0);
+            if constexpr (kShared) {
+                const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(slot + s * blockDim.x));
+                const int bytes = on ? kBytes : 0;
+                if constexpr (kBytes == 16)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+                else
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(kBytes), "r"(bytes) : "memory");
+            } else {
+                held[s] = on ? *reinterpret_cast<const Pack<T, V>*>(from) : Pack<T, V>{};
+            }
+        }
+    }
+    __device__ __forceinline__ Pack<T, V> take(int s) const {
+        if constexpr (kShared) return slot[s * blockDim.x];
+        else return held[s];
+    }
+};
+
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void await_copies() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// The affine map of a run of rows on V channels; `drop`: what enters the run does not leave it.
 template <typename A, int V>
-constexpr size_t recurrence_smem(int kinds, int lanes, int parts) {
-    return 2 * (sizeof(A) * size_t(kinds) * lanes * parts * V + size_t(parts));
-}
+struct Map {
+    A a[V], b[V];
+    bool drop;
 
-// Folds the maps of the parts, in the direction of the scan, into the
-// state that enters each: `run` goes from the state entering the CTA's rows to the one leaving them, `in`
-// is the state entering part tt.
-template <typename A, int V, bool REVERSE>
-__device__ __forceinline__ void fold_parts(const A* ma, const A* mb, const unsigned char* md, unsigned bit, int parts,
-                                           int lanes, int tt, int tc, A (&run)[V], A (&in)[V]) {
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int v = 0; v < V; ++v) in[v] = run[v];
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-        const int t = REVERSE ? parts - 1 - i : i;
-        const bool drop = md[t] & bit;
-        const Pack<A, V> fa = load_pack<A, V>(ma + (t * lanes + tc) * V), fb = load_pack<A, V>(mb + (t * lanes + tc) * V);
+        for (int v = 0; v < V; ++v) { a[v] = A(1); b[v] = A(0); }
+        drop = false;
+    }
+    // this map behind `earlier`
+    __device__ __forceinline__ void behind(const Map& earlier) {
+        if (drop) return;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            if (t == tt) in[v] = run[v];
-            run[v] = drop ? fb.v[v] : fma_(fa.v[v], run[v], fb.v[v]);
+            b[v] = fma_(a[v], earlier.b[v], b[v]);
+            a[v] *= earlier.a[v];
+        }
+        drop = earlier.drop;
+    }
+    __device__ __forceinline__ void apply(A (&h)[V]) const {
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = drop ? b[v] : fma_(a[v], h[v], b[v]);
+    }
+};
+
+// Maps in shared memory: [warp or CTA][A, B][lane of the strip], with a flag each.
+template <typename A, int V>
+struct MapStore {
+    Pack<A, V>* values;
+    unsigned char* drops;
+    int lanes;
+
+    __device__ __forceinline__ void put(int i, int tc, const Map<A, V>& m) const {
+        Pack<A, V> a, b;
+#pragma unroll
+        for (int v = 0; v < V; ++v) { a.v[v] = m.a[v]; b.v[v] = m.b[v]; }
+        values[(2 * i) * lanes + tc] = a;
+        values[(2 * i + 1) * lanes + tc] = b;
+        if (tc == 0) drops[i] = m.drop;
+    }
+    template <bool PACKED>
+    __device__ __forceinline__ Map<A, V> get(int i, int tc) const {
+        const Pack<A, V> a = values[(2 * i) * lanes + tc], b = values[(2 * i + 1) * lanes + tc];
+        Map<A, V> m;
+#pragma unroll
+        for (int v = 0; v < V; ++v) { m.a[v] = a.v[v]; m.b[v] = b.v[v]; }
+        m.drop = PACKED && drops[i];
+        return m;
+    }
+};
+
+// Bytes of shared memory behind the prefetch slots: both buffers of the warps' maps (`scans` of them) and of
+// the cluster's maps, flags included.
+template <typename A, int V>
+__host__ __device__ constexpr size_t map_bytes(int lanes, int count) { return 2 * sizeof(A) * V * size_t(lanes) * count + 16 * ((count + 15) / 16); }
+template <typename A, int V>
+__host__ __device__ constexpr size_t scan_bytes(int lanes, int warps, int cluster, int scans) {
+    return 2 * (scans * map_bytes<A, V>(lanes, warps) + (cluster > 1 ? map_bytes<A, V>(lanes, cluster) : 0));
+}
+
+template <typename A, int V>
+__device__ __forceinline__ MapStore<A, V> map_store(unsigned char* at, int lanes, int count) {
+    MapStore<A, V> m;
+    m.values = reinterpret_cast<Pack<A, V>*>(at);
+    m.drops = at + 2 * sizeof(A) * V * size_t(lanes) * count;
+    m.lanes = lanes;
+    return m;
+}
+
+// Scan of the threads' maps over the parts of a warp (REVERSE: from the last part to the first).  On return
+// `m` is the map of everything in the warp that comes before this part, and lanes of the last part in scan
+// order have put the whole warp's map into `store`.
+template <typename A, int V, bool REVERSE, bool PACKED>
+__device__ __forceinline__ void scan_warp(Map<A, V>& m, int log_lanes, const MapStore<A, V>& store) {
+    const int lane = threadIdx.x & 31, lanes = 1 << log_lanes, parts = 32 >> log_lanes;
+    const int part = REVERSE ? parts - 1 - (lane >> log_lanes) : lane >> log_lanes;
+    for (int k = 1; k < parts; k <<= 1) {
+        Map<A, V> e;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            e.a[v] = REVERSE ? __shfl_down_sync(0xffffffffu, m.a[v], k << log_lanes) : __shfl_up_sync(0xffffffffu, m.a[v], k << log_lanes);
+            e.b[v] = REVERSE ? __shfl_down_sync(0xffffffffu, m.b[v], k << log_lanes) : __shfl_up_sync(0xffffffffu, m.b[v], k << log_lanes);
+        }
+        e.drop = false;
+        if (PACKED) e.drop = REVERSE ? __shfl_down_sync(0xffffffffu, int(m.drop), k << log_lanes) : __shfl_up_sync(0xffffffffu, int(m.drop), k << log_lanes);
+        if (part >= k) m.behind(e);
+    }
+    if (part == parts - 1) store.put(threadIdx.x >> 5, lane & (lanes - 1), m);
+    if (parts > 1) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            m.a[v] = REVERSE ? __shfl_down_sync(0xffffffffu, m.a[v], lanes) : __shfl_up_sync(0xffffffffu, m.a[v], lanes);
+            m.b[v] = REVERSE ? __shfl_down_sync(0xffffffffu, m.b[v], lanes) : __shfl_up_sync(0xffffffffu, m.b[v], lanes);
+        }
+        if (PACKED) m.drop = REVERSE ? __shfl_down_sync(0xffffffffu, int(m.drop), lanes) : __shfl_up_sync(0xffffffffu, int(m.drop), lanes);
+    }
+    if (part == 0) m.clear();
+}
+
+// The state that enters this thread's rows, from `run`, the state that enters the iteration's first row (in
+// scan order), and `m`, the map of the parts before it in its warp; `run` moves on to the next iteration.
+// One CTA: the warps' maps are applied in their order.  A cluster: each CTA composes its own, hands the
+// composition to all and applies what lies before it.
+template <typename A, int V, bool REVERSE, bool PACKED>
+__device__ __forceinline__ void enter(A (&run)[V], A (&in)[V], const Map<A, V>& m, const MapStore<A, V>& store,
+                                      const MapStore<A, V>& shared, int warps, int cluster, int rank, int tc) {
+    const int warp = threadIdx.x >> 5;
+    if (cluster == 1) {
+#pragma unroll 4
+        for (int i = 0; i < warps; ++i) {
+            const int w = REVERSE ? warps - 1 - i : i;
+            if (w == warp) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) in[v] = run[v];
+            }
+            store.template get<PACKED>(w, tc).apply(run);
+        }
+    } else {
+        Map<A, V> all;
+        all.clear();
+        for (int i = 0; i < warps; ++i) {
+            Map<A, V> next = store.template get<PACKED>(REVERSE ? warps - 1 - i : i, tc);
+            next.behind(all);
+            all = next;
+        }
+        auto group = cooperative_groups::this_cluster();
+        // each warp serves some of the CTAs
+        if ((threadIdx.x & 31) < (1 << (31 - __clz(store.lanes))))
+            for (int r = warp; r < cluster; r += warps) {
+                MapStore<A, V> there = shared;
+                there.values = group.map_shared_rank(shared.values, r);
+                there.drops = group.map_shared_rank(shared.drops, r);
+                there.put(rank, tc, all);
+            }
+        group.sync();
+#pragma unroll
+        for (int v = 0; v < V; ++v) in[v] = run[v];
+        for (int i = 0; i < cluster; ++i) {
+            const int r = REVERSE ? cluster - 1 - i : i;
+            if (r == rank) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) in[v] = run[v];
+            }
+            shared.template get<PACKED>(r, tc).apply(run);
+        }
+        for (int i = 0; i < (REVERSE ? warps - 1 - warp : warp); ++i)
+            store.template get<PACKED>(REVERSE ? warps - 1 - i : i, tc).apply(in);
+    }
+    m.apply(in);
+}
+
+// a, x and, where REST, 1 - a of S rows from the prefetched inputs; without REST x is b already.
+template <int FORM, bool REST, typename X, typename G, int V, int GV, int S, typename A>
+__device__ __forceinline__ void factors(const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, bool complement,
+                                        A (&a)[S][V], A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const Pack<X, V> x = fx.take(s);
+        const Pack<G, GV> g = fg.take(s);
+        A ga[GV], gr[GV];
+#pragma unroll
+        for (int v = 0; v < GV; ++v) gate_factors<FORM>(A(widen(g.v[v])), ga[v], gr[v]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            a[s][v] = ga[v % GV];
+            u[s][v] = widen(x.v[v]);
+            if (REST) rest[s % (REST ? S : 1)][v] = gr[v % GV];
+            else if (complement) u[s][v] *= gr[v % GV];
         }
     }
 }
 
-template <typename X, typename G, int V, int S, bool SHARED>
-__global__ void __launch_bounds__(256) recurrence_forward_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
+template <bool REST, typename X, typename G, int V, int GV, int S, typename A>
+__device__ __forceinline__ void factors(int form, const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, bool complement,
+                                        A (&a)[S][V], A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
+    if (form == kGateValue) factors<kGateValue, REST>(fx, fg, complement, a, u, rest);
+    else if (form == kGateLog) factors<kGateLog, REST>(fx, fg, complement, a, u, rest);
+    else factors<kGateLogit, REST>(fx, fg, complement, a, u, rest);
+}
+
+template <typename X, typename G, int V, int S, bool SHARED, bool PACKED>
+__global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
     using A = Acc<X>;
     constexpr int GV = SHARED ? 1 : V;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int lanes = 1 << plan.log_lanes, parts = 1 << plan.log_parts, width = lanes * V;
-    const int tc = threadIdx.x & (lanes - 1), tt = threadIdx.x >> plan.log_lanes;
-    A* maps = reinterpret_cast<A*>(smem);  // [buffer][A, B][parts][width]
-    unsigned char* drops = smem + sizeof(A) * 4 * parts * width;  // [buffer][parts]
-
-    const uint64_t b = blockIdx.x / plan.strips;
-    const uint64_t c0 = (uint64_t(blockIdx.x % plan.strips) * lanes + tc) * V;
-    const bool live = c0 < p.dim, packed = p.sequences > 0;
+    const int lanes = 1 << plan.log_lanes, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tc = lane & (lanes - 1), parts = 32 >> plan.log_lanes;
+    const int cluster = plan.cluster, rank = cluster > 1 ? int(blockIdx.x % cluster) : 0;
+    const uint64_t strip = blockIdx.x / cluster, b = strip / plan.strips;
+    const uint64_t c0 = ((strip % plan.strips) * lanes + tc) * V;
+    const bool live = c0 < p.dim;
     const int64_t rows = int64_t(p.rows), dim = int64_t(p.dim);
-    const X* x = static_cast<const X*>(p.x) + b * p.x_batch + c0;
-    const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (SHARED ? c0 / (p.dim / p.gate_dim) : c0);
+    const X* x = static_cast<const X*>(p.x) + b * p.x_batch + (live ? c0 : 0);
+    const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
     const A* initial = p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr;
     X* out = p.out ? static_cast<X*>(p.out) + b * p.rows * p.dim + c0 : nullptr;
     A* state = p.state ? static_cast<A*>(p.state) + c0 : nullptr;
     A* marks = p.checkpoints
         ? static_cast<A*>(p.checkpoints) + b * ((p.rows + kCheckpointRows - 1) / kCheckpointRows) * p.dim + c0 : nullptr;
 
+    Prefetch<X, V, S> fx;
+    Prefetch<G, GV, S> fg;
+    fx.slot = reinterpret_cast<Pack<X, V>*>(smem) + threadIdx.x;
+    unsigned char* at = smem + fx.smem(blockDim.x);
+    fg.slot = reinterpret_cast<Pack<G, GV>*>(at) + threadIdx.x;
+    at += (fg.smem(blockDim.x) + 15) / 16 * 16;
+    MapStore<A, V> stores[2], shared[2];
+    for (int k = 0; k < 2; ++k, at += map_bytes<A, V>(lanes, plan.warps)) stores[k] = map_store<A, V>(at, lanes, plan.warps);
+    for (int k = 0; k < 2 && cluster > 1; ++k, at += map_bytes<A, V>(lanes, cluster)) shared[k] = map_store<A, V>(at, lanes, cluster);
+
     A run[V];  // the state that enters the iteration's first row
 #pragma unroll
-    for (int v = 0; v < V; ++v) run[v] = !packed && initial && live ? initial[b * p.dim + v] : A(0);
-    if (packed && state && live)  // sequences without rows hand their initial state on
-        for (int64_t j = tt; j < int64_t(p.sequences); j += parts)
+    for (int v = 0; v < V; ++v) run[v] = !PACKED && initial && live ? initial[b * p.dim + v] : A(0);
+    const int part = warp * parts + (lane >> plan.log_lanes);
+    if (PACKED && state && live && rank == 0)  // sequences without rows hand their initial state on
+        for (int64_t j = part; j < int64_t(p.sequences); j += plan.warps * parts)
             if (offset_at(p.offsets, p.wide_offsets, j + 1) <= offset_at(p.offsets, p.wide_offsets, j))
                 for (int v = 0; v < V; ++v) state[j * dim + v] = initial ? initial[j * dim + v] : A(0);
 
+    const int64_t span = int64_t(plan.warps) * parts * cluster * S;
+    int64_t row0 = (int64_t(rank) * plan.warps * parts + part) * S;
     SequenceWalk walk;
-    if (packed) walk.seek(p.offsets, p.wide_offsets, p.sequences, int64_t(tt) * S);
+    if (PACKED) walk.seek(p.offsets, p.wide_offsets, p.sequences, row0);
+    fx.issue(x, row0, rows, p.x_row, live);
+    fg.issue(gate, row0, rows, p.gate_row, live);
+    commit_copies();
     int buf = 0;
-    for (int64_t base = 0; base < rows; base += int64_t(parts) * S, buf ^= 1) {
-        const int64_t row0 = base + int64_t(tt) * S;
-        Pack<X, V> rx[S];
-        Pack<G, GV> rg[S];
-        load_rows<X, V, S>(rx, x, row0, rows, p.x_row, live);
-        load_rows<G, GV, S>(rg, gate, row0, rows, p.gate_row, live);
+    for (int64_t base = 0; base < rows; base += span, row0 += span, buf ^= 1) {
         RowEvents e;
-        if (packed) {
+        if (PACKED) {
             walk.advance(row0);
             e = row_events<S>(walk, row0, rows);
         }
-        A a[S][V], u[S][V];
+        A a[S][V], u[S][V], unused[1][V];
+        await_copies();
+        factors<false>(p.form, fx, fg, p.complement, a, u, unused);
+        if (row0 + S > rows || (PACKED && e.dead))
 #pragma unroll
-        for (int s = 0; s < S; ++s)
+            for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                A rest;
-                gate_factors(p.form, widen(rg[s].v[SHARED ? 0 : v]), a[s][v], rest);
-                u[s][v] = widen(rx[s].v[v]);
-                if (p.complement) u[s][v] *= rest;
-                if (row0 + s >= rows || (e.dead >> s & 1u)) { a[s][v] = A(1); u[s][v] = A(0); }
-            }
+                for (int v = 0; v < V; ++v)
+                    if (row0 + s >= rows || (e.dead >> s & 1u)) { a[s][v] = A(1); u[s][v] = A(0); }
         // the initial state of a sequence that starts here joins b: its first row is then b alone
-        if (e.starts && initial && live)
+        if (PACKED && e.starts && initial && live)
 #pragma unroll
             for (int s = 0; s < S; ++s)
                 if (e.starts >> s & 1u) {
@@ -217,25 +419,23 @@ __global__ void __launch_bounds__(256) recurrence_forward_kernel(const Recurrenc
 #pragma unroll
                     for (int v = 0; v < V; ++v) u[s][v] = fma_(a[s][v], in[v], u[s][v]);
                 }
-        Pack<A, V> fa, fb;
-#pragma unroll
-        for (int v = 0; v < V; ++v) { fa.v[v] = A(1); fb.v[v] = A(0); }
+        Map<A, V> m;
+        m.clear();
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                fb.v[v] = (e.starts >> s & 1u) ? u[s][v] : fma_(a[s][v], fb.v[v], u[s][v]);
-                fa.v[v] *= a[s][v];
+                m.b[v] = PACKED && (e.starts >> s & 1u) ? u[s][v] : fma_(a[s][v], m.b[v], u[s][v]);
+                m.a[v] *= a[s][v];
             }
-        A* ma = maps + buf * 2 * parts * width;
-        A* mb = ma + parts * width;
-        unsigned char* md = drops + buf * parts;
-        store_pack<A, V>(ma + threadIdx.x * V, fa);
-        store_pack<A, V>(mb + threadIdx.x * V, fb);
-        if (tc == 0) md[tt] = e.starts != 0;
+        m.drop = PACKED && e.starts;
+        scan_warp<A, V, false, PACKED>(m, plan.log_lanes, stores[buf]);
         __syncthreads();
+        fx.issue(x, row0 + span, rows, p.x_row, live);  // the slots were read before the barrier
+        fg.issue(gate, row0 + span, rows, p.gate_row, live);
+        commit_copies();
         A h[V];
-        fold_parts<A, V, false>(ma, mb, md, 1u, parts, lanes, tt, tc, run, h);
+        enter<A, V, false, PACKED>(run, h, m, stores[buf], shared[buf], plan.warps, cluster, rank, tc);
         if (!live || row0 >= rows) continue;
         if (marks && row0 % int64_t(kCheckpointRows) == 0)
 #pragma unroll
@@ -245,18 +445,18 @@ __global__ void __launch_bounds__(256) recurrence_forward_kernel(const Recurrenc
             Pack<X, V> y;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                h[v] = (e.starts >> s & 1u) ? u[s][v] : fma_(a[s][v], h[v], u[s][v]);
-                y.v[v] = narrow<X>((e.dead >> s & 1u) ? A(0) : h[v]);
+                h[v] = PACKED && (e.starts >> s & 1u) ? u[s][v] : fma_(a[s][v], h[v], u[s][v]);
+                y.v[v] = narrow<X>(PACKED && (e.dead >> s & 1u) ? A(0) : h[v]);
             }
             if (out && row0 + s < rows) store_pack<X, V>(out + (row0 + s) * dim, y);
-            if (state && (e.ends >> s & 1u)) {
+            if (PACKED && state && (e.ends >> s & 1u)) {
                 A* to = state + sequence_of(walk, row0 + s) * dim;
 #pragma unroll
                 for (int v = 0; v < V; ++v) to[v] = h[v];
             }
         }
     }
-    if (!packed && state && live && tt == 0)
+    if (!PACKED && state && live && part == 0 && rank == 0)
 #pragma unroll
         for (int v = 0; v < V; ++v) state[b * p.dim + v] = run[v];
 }
@@ -266,24 +466,22 @@ __global__ void __launch_bounds__(256) recurrence_forward_kernel(const Recurrenc
 // rounded or not, is not read at all.
 // Shared gates: each thread sums its V channels, 1 << fold_log neighbouring lanes are folded by shuffles,
 // and `partial` takes one value per row and fold (dgate itself where a fold is a whole gate).
-template <typename X, typename G, int V, int S, bool SHARED>
-__global__ void __launch_bounds__(256) recurrence_backward_kernel(const RecurrenceArgs p, const RecurrencePlan plan,
-                                                                  Acc<X>* partial) {
+template <typename X, typename G, int V, int S, bool SHARED, bool PACKED>
+__global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const RecurrenceArgs p, const RecurrencePlan plan,
+                                                                     Acc<X>* partial) {
     using A = Acc<X>;
     constexpr int GV = SHARED ? 1 : V;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int lanes = 1 << plan.log_lanes, parts = 1 << plan.log_parts, width = lanes * V;
-    const int tc = threadIdx.x & (lanes - 1), tt = threadIdx.x >> plan.log_lanes;
-    A* maps = reinterpret_cast<A*>(smem);  // [buffer][A, forward B, backward B][parts][width]
-    unsigned char* drops = smem + sizeof(A) * 6 * parts * width;  // [buffer][parts], bit 0 starts, bit 1 ends
-
-    const uint64_t b = blockIdx.x / plan.strips;
-    const uint64_t c0 = (uint64_t(blockIdx.x % plan.strips) * lanes + tc) * V;
-    const bool live = c0 < p.dim, packed = p.sequences > 0;
+    const int lanes = 1 << plan.log_lanes, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tc = lane & (lanes - 1), parts = 32 >> plan.log_lanes;
+    const int cluster = plan.cluster, rank = cluster > 1 ? int(blockIdx.x % cluster) : 0;
+    const uint64_t strip = blockIdx.x / cluster, b = strip / plan.strips;
+    const uint64_t c0 = ((strip % plan.strips) * lanes + tc) * V;
+    const bool live = c0 < p.dim;
     const int64_t rows = int64_t(p.rows), dim = int64_t(p.dim);
-    const X* x = static_cast<const X*>(p.x) + b * p.x_batch + c0;
-    const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (SHARED ? c0 / (p.dim / p.gate_dim) : c0);
-    const X* derivs = static_cast<const X*>(p.derivs) + b * p.d_batch + c0;
+    const X* x = static_cast<const X*>(p.x) + b * p.x_batch + (live ? c0 : 0);
+    const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
+    const X* derivs = static_cast<const X*>(p.derivs) + b * p.d_batch + (live ? c0 : 0);
     const A* initial = p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr;
     const A* state_derivs = p.state_derivs ? static_cast<const A*>(p.state_derivs) + c0 : nullptr;
     const A* marks = static_cast<const A*>(p.marks) + b * ((p.rows + kCheckpointRows - 1) / kCheckpointRows) * p.dim + c0;
@@ -292,45 +490,63 @@ __global__ void __launch_bounds__(256) recurrence_backward_kernel(const Recurren
     const int64_t folds = SHARED ? (dim / V) >> plan.fold_log : 0;
     G* dgate = static_cast<G*>(p.dgate) + b * p.rows * p.gate_dim + (SHARED ? 0 : c0);
 
+    Prefetch<X, V, S> fx, fd;
+    Prefetch<G, GV, S> fg;
+    fx.slot = reinterpret_cast<Pack<X, V>*>(smem) + threadIdx.x;
+    fd.slot = fx.slot + S * blockDim.x;
+    unsigned char* at = smem + 2 * fx.smem(blockDim.x);
+    fg.slot = reinterpret_cast<Pack<G, GV>*>(at) + threadIdx.x;
+    at += (fg.smem(blockDim.x) + 15) / 16 * 16;
+    MapStore<A, V> ahead[2], stores[2], shared[2];
+    for (int k = 0; k < 2; ++k, at += map_bytes<A, V>(lanes, plan.warps)) ahead[k] = map_store<A, V>(at, lanes, plan.warps);
+    for (int k = 0; k < 2; ++k, at += map_bytes<A, V>(lanes, plan.warps)) stores[k] = map_store<A, V>(at, lanes, plan.warps);
+    for (int k = 0; k < 2 && cluster > 1; ++k, at += map_bytes<A, V>(lanes, cluster)) shared[k] = map_store<A, V>(at, lanes, cluster);
+
     A run[V];  // the gradient that enters the iteration's last row from behind
 #pragma unroll
-    for (int v = 0; v < V; ++v) run[v] = !packed && state_derivs && live ? state_derivs[b * p.dim + v] : A(0);
-    if (packed && dinitial && live)
-        for (int64_t j = tt; j < int64_t(p.sequences); j += parts)
+    for (int v = 0; v < V; ++v) run[v] = !PACKED && state_derivs && live ? state_derivs[b * p.dim + v] : A(0);
+    const int part = warp * parts + (lane >> plan.log_lanes);
+    if (PACKED && dinitial && live && rank == 0)
+        for (int64_t j = part; j < int64_t(p.sequences); j += plan.warps * parts)
             if (offset_at(p.offsets, p.wide_offsets, j + 1) <= offset_at(p.offsets, p.wide_offsets, j))
                 for (int v = 0; v < V; ++v) dinitial[j * dim + v] = state_derivs ? state_derivs[j * dim + v] : A(0);
 
-    const int64_t span = int64_t(parts) * S;
+    const int64_t block = int64_t(plan.warps) * parts * S, span = block * cluster;
+    int64_t base = (rows - 1) / span * span, row0 = base + rank * block + int64_t(part) * S;
+    SequenceWalk walk;
+    if (PACKED) walk.seek(p.offsets, p.wide_offsets, p.sequences, row0);
+    fx.issue(x, row0, rows, p.x_row, live);
+    fg.issue(gate, row0, rows, p.gate_row, live);
+    fd.issue(derivs, row0, rows, p.d_row, live);
+    commit_copies();
     int buf = 0;
-    for (int64_t base = (rows - 1) / span * span; base >= 0; base -= span, buf ^= 1) {
-        const int64_t row0 = base + int64_t(tt) * S;
-        Pack<X, V> rx[S], rd[S];
-        Pack<G, GV> rg[S];
-        load_rows<X, V, S>(rx, x, row0, rows, p.x_row, live);
-        load_rows<G, GV, S>(rg, gate, row0, rows, p.gate_row, live);
-        load_rows<X, V, S>(rd, derivs, row0, rows, p.d_row, live);
+    for (; base >= 0; base -= span, row0 -= span, buf ^= 1) {
         A h[V];
+        const int64_t own = base + rank * block;  // the CTA's first row
 #pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = live ? marks[base / int64_t(kCheckpointRows) * dim + v] : A(0);
+        for (int v = 0; v < V; ++v) h[v] = live && own < rows ? marks[own / int64_t(kCheckpointRows) * dim + v] : A(0);
         RowEvents e;
-        SequenceWalk walk;
-        if (packed && row0 < rows) {
-            walk.seek(p.offsets, p.wide_offsets, p.sequences, row0);
+        if (PACKED) {
+            walk.retreat(row0);
             e = row_events<S>(walk, row0, rows);
         }
-        A a[S][V], rest[S][V], u[S][V], d[S][V];
+        A a[S][V], rest[S][V], x_[S][V], d[S][V];
+        await_copies();
+        factors<true>(p.form, fx, fg, p.complement, a, x_, rest);
 #pragma unroll
-        for (int s = 0; s < S; ++s)
+        for (int s = 0; s < S; ++s) {
+            const Pack<X, V> rd = fd.take(s);
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                gate_factors(p.form, widen(rg[s].v[SHARED ? 0 : v]), a[s][v], rest[s][v]);
-                u[s][v] = widen(rx[s].v[v]);
-                if (p.complement) u[s][v] *= rest[s][v];
-                d[s][v] = widen(rd[s].v[v]);
-                if (row0 + s >= rows || (e.dead >> s & 1u)) { a[s][v] = A(1); u[s][v] = d[s][v] = A(0); }
-            }
+            for (int v = 0; v < V; ++v) d[s][v] = widen(rd.v[v]);
+        }
+        if (row0 + S > rows || (PACKED && e.dead))
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int v = 0; v < V; ++v)
+                    if (row0 + s >= rows || (e.dead >> s & 1u)) { a[s][v] = A(1); rest[s][v] = x_[s][v] = d[s][v] = A(0); }
         // the gradient of a state joins the derivatives of the row that it was taken from
-        if (e.ends && state_derivs && live)
+        if (PACKED && e.ends && state_derivs && live)
 #pragma unroll
             for (int s = 0; s < S; ++s)
                 if (e.ends >> s & 1u) {
@@ -338,70 +554,78 @@ __global__ void __launch_bounds__(256) recurrence_backward_kernel(const Recurren
 #pragma unroll
                     for (int v = 0; v < V; ++v) d[s][v] += in[v];
                 }
-        Pack<A, V> fa, fb, gb;
-#pragma unroll
-        for (int v = 0; v < V; ++v) { fa.v[v] = A(1); fb.v[v] = gb.v[v] = A(0); }
+        Map<A, V> m, g;
+        m.clear();
+        g.clear();
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            if (e.starts >> s & 1u) {
+            if (PACKED && (e.starts >> s & 1u)) {
                 const A* in = initial && live ? initial + sequence_of(walk, row0 + s) * dim : nullptr;
 #pragma unroll
-                for (int v = 0; v < V; ++v) fb.v[v] = in ? in[v] : A(0);
+                for (int v = 0; v < V; ++v) m.b[v] = in ? in[v] : A(0);
             }
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                fb.v[v] = fma_(a[s][v], fb.v[v], u[s][v]);
-                fa.v[v] *= a[s][v];
+                m.b[v] = fma_(a[s][v], m.b[v], p.complement ? rest[s][v] * x_[s][v] : x_[s][v]);
+                m.a[v] *= a[s][v];
             }
         }
 #pragma unroll
         for (int s = S - 1; s >= 0; --s)
 #pragma unroll
             for (int v = 0; v < V; ++v)
-                gb.v[v] = a[s][v] * ((e.ends >> s & 1u) ? d[s][v] : d[s][v] + gb.v[v]);
-        A* ma = maps + buf * 3 * parts * width;
-        A* mf = ma + parts * width;
-        A* mg = mf + parts * width;
-        unsigned char* md = drops + buf * parts;
-        store_pack<A, V>(ma + threadIdx.x * V, fa);
-        store_pack<A, V>(mf + threadIdx.x * V, fb);
-        store_pack<A, V>(mg + threadIdx.x * V, gb);
-        if (tc == 0) md[tt] = (e.starts ? 1 : 0) | (e.ends ? 2 : 0);
+                g.b[v] = a[s][v] * (PACKED && (e.ends >> s & 1u) ? d[s][v] : d[s][v] + g.b[v]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) g.a[v] = m.a[v];
+        m.drop = PACKED && e.starts;
+        g.drop = PACKED && e.ends;
+        scan_warp<A, V, false, PACKED>(m, plan.log_lanes, ahead[buf]);
+        scan_warp<A, V, true, PACKED>(g, plan.log_lanes, stores[buf]);
         __syncthreads();
-        A w[V], in[V];
-        fold_parts<A, V, false>(ma, mf, md, 1u, parts, lanes, tt, tc, h, in);
-        fold_parts<A, V, true>(ma, mg, md, 2u, parts, lanes, tt, tc, run, w);
-        A before[S][V];
+        fx.issue(x, row0 - span, rows, p.x_row, live);  // the slots were read before the barrier
+        fg.issue(gate, row0 - span, rows, p.gate_row, live);
+        fd.issue(derivs, row0 - span, rows, p.d_row, live);
+        commit_copies();
+        A in[V], w[V];
+        enter<A, V, false, PACKED>(h, in, m, ahead[buf], ahead[buf], plan.warps, 1, 0, tc);
+        enter<A, V, true, PACKED>(run, w, g, stores[buf], shared[buf], plan.warps, cluster, rank, tc);
+        // backward through the rows: d becomes g
+#pragma unroll
+        for (int s = S - 1; s >= 0; --s) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (!(PACKED && (e.ends >> s & 1u))) d[s][v] += w[v];
+                w[v] = a[s][v] * d[s][v];
+            }
+            if (PACKED && dinitial && live && (e.starts >> s & 1u)) {
+                A* to = dinitial + sequence_of(walk, row0 + s) * dim;
+#pragma unroll
+                for (int v = 0; v < V; ++v) to[v] = w[v];
+            }
+        }
+        // forward through them with h_{t-1} in `in`
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            if (e.starts >> s & 1u) {
+            if (PACKED && (e.starts >> s & 1u)) {
                 const A* from = initial && live ? initial + sequence_of(walk, row0 + s) * dim : nullptr;
 #pragma unroll
                 for (int v = 0; v < V; ++v) in[v] = from ? from[v] : A(0);
             }
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                before[s][v] = in[v];
-                in[v] = fma_(a[s][v], in[v], u[s][v]);
-            }
-        }
-#pragma unroll
-        for (int s = S - 1; s >= 0; --s) {
-            const bool dead = e.dead >> s & 1u, stored = live && row0 + s < rows;
+            const bool dead = PACKED && (e.dead >> s & 1u), stored = live && row0 + s < rows;
             Pack<X, V> gx;
             Pack<G, V> gg;
             A sum = A(0);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const A g = (e.ends >> s & 1u) ? d[s][v] : d[s][v] + w[v];
-                gx.v[v] = narrow<X>(dead ? A(0) : p.complement ? rest[s][v] * g : g);
-                A da = g * (p.complement ? before[s][v] - widen(rx[s].v[v]) : before[s][v]);
+                const A g_ = d[s][v];
+                gx.v[v] = narrow<X>(dead ? A(0) : p.complement ? rest[s][v] * g_ : g_);
+                A da = g_ * (p.complement ? in[v] - x_[s][v] : in[v]);
                 if (p.form != kGateValue) da *= a[s][v];
                 if (p.form == kGateLogit) da *= rest[s][v];
                 if (dead) da = A(0);
                 gg.v[v] = narrow<G>(da);
                 sum += da;
-                w[v] = a[s][v] * g;
+                in[v] = fma_(a[s][v], in[v], p.complement ? rest[s][v] * x_[s][v] : x_[s][v]);
             }
             if (stored) store_pack<X, V>(dx + (row0 + s) * dim, gx);
             if (SHARED) {
@@ -415,14 +639,9 @@ __global__ void __launch_bounds__(256) recurrence_backward_kernel(const Recurren
             } else if (stored) {
                 store_pack<G, V>(dgate + (row0 + s) * dim, gg);
             }
-            if (dinitial && live && (e.starts >> s & 1u)) {
-                A* to = dinitial + sequence_of(walk, row0 + s) * dim;
-#pragma unroll
-                for (int v = 0; v < V; ++v) to[v] = w[v];
-            }
         }
     }
-    if (!packed && dinitial && live && tt == 0)
+    if (!PACKED && dinitial && live && part == 0 && rank == 0)
 #pragma unroll
         for (int v = 0; v < V; ++v) dinitial[b * p.dim + v] = run[v];
 }
@@ -455,7 +674,10 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(const RecurrenceAr
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         A a, rest, u = widen(x.v[v]);
-        gate_factors(p.form, widen(g.v[SHARED ? 0 : v]), a, rest);
+        const A t = widen(g.v[SHARED ? 0 : v]);
+        if (p.form == kGateValue) gate_factors<kGateValue>(t, a, rest);
+        else if (p.form == kGateLog) gate_factors<kGateLog>(t, a, rest);
+        else gate_factors<kGateLogit>(t, a, rest);
         if (p.complement) u *= rest;
         h.v[v] = fma_(a, h.v[v], u);
         y.v[v] = narrow<X>(h.v[v]);
