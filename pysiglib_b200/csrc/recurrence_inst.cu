@@ -72,7 +72,7 @@ void forward(const RecurrenceArgs& p, cudaStream_t stream) {
     const RecurrencePlan plan = make_plan<X>(p, V, kForwardRows);
     const int threads = 32 * plan.warps;
     const size_t smem = Prefetch<X, V, kForwardRows>::smem(threads) + (Prefetch<G, SHARED ? 1 : V, kForwardRows>::smem(threads) + 15) / 16 * 16 +
-                        scan_bytes<Acc<X>, V>(1 << plan.log_lanes, plan.warps, plan.cluster, 1);
+                        ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, plan.cluster);
     if (p.sequences) launch(recurrence_forward_kernel<X, G, V, kForwardRows, SHARED, true>, p, plan, smem, stream);
     else launch(recurrence_forward_kernel<X, G, V, kForwardRows, SHARED, false>, p, plan, smem, stream);
     check("linear recurrence kernel");
@@ -93,7 +93,7 @@ void backward(const RecurrenceArgs& p, cudaStream_t stream) {
     if (per_gate > 1) partial = scratch.as<Acc<X>>();
     const int threads = 32 * plan.warps;
     const size_t smem = 2 * Prefetch<X, V, S>::smem(threads) + (Prefetch<G, SHARED ? 1 : V, S>::smem(threads) + 15) / 16 * 16 +
-                        scan_bytes<Acc<X>, V>(1 << plan.log_lanes, plan.warps, plan.cluster, 2);
+                        ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, 1) + ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, plan.cluster);
     if (p.sequences) launch(recurrence_backward_kernel<X, G, V, S, SHARED, true>, p, plan, smem, stream, partial);
     else launch(recurrence_backward_kernel<X, G, V, S, SHARED, false>, p, plan, smem, stream, partial);
     check("linear recurrence backward kernel");

@@ -103,58 +103,67 @@ __device__ __forceinline__ int64_t sequence_of(SequenceWalk walk, int64_t row) {
     return walk.seq;
 }
 
-// a and 1 - a, neither by cancellation: exp and expm1 for logarithms; for logits both from e^-|v|, with the
-// hardware's reciprocal (within 2 ulp on [1, 2]) in place of a division.
-template <int FORM>
+// a and 1 - a, neither by cancellation: exp and expm1 for logarithms; for logits a = 1 / (1 + e^-v), and 1 - a
+// is e^-v a where v > 0.  The reciprocal is the hardware's (within 1 ulp; a = 0 for e^-v = inf).
+// FAST (gates of 16 bits): e^-v as 2^(-v log2 e) in single precision, off by up to 2 + 1.2 |v| ulp.  A gate of
+// 8 or 11 bits leaves e^-v uncertain by |v| 2^-9 or 2^-12 of itself, thousands of times more.
+__device__ __forceinline__ float reciprocal(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+template <int FORM, bool FAST>
 __device__ __forceinline__ void gate_factors(float v, float& a, float& rest) {
     if (FORM == kGateValue) { a = v; rest = 1.0f - v; }
-    else if (FORM == kGateLog) { a = expf(v); rest = -expm1f(v); }
+    else if (FORM == kGateLog) { a = FAST ? __expf(v) : expf(v); rest = -expm1f(v); }
     else {
-        const float e = expf(-fabsf(v)), r = __fdividef(1.0f, 1.0f + e), s = e * r;
-        a = v >= 0.0f ? r : s;
-        rest = v >= 0.0f ? s : r;
+        const float e = FAST ? __expf(-v) : expf(-v);
+        a = reciprocal(1.0f + e);
+        rest = v > 0.0f ? e * a : 1.0f - a;
     }
 }
-template <int FORM>
+template <int FORM, bool FAST>
 __device__ __forceinline__ void gate_factors(double v, double& a, double& rest) {
     if (FORM == kGateValue) { a = v; rest = 1.0 - v; }
     else if (FORM == kGateLog) { a = exp(v); rest = -expm1(v); }
     else {
-        const double e = exp(-fabs(v)), r = 1.0 / (1.0 + e), s = e * r;
-        a = v >= 0.0 ? r : s;
-        rest = v >= 0.0 ? s : r;
+        const double e = exp(-v);
+        a = 1.0 / (1.0 + e);
+        rest = v > 0.0 ? e * a : 1.0 - a;
     }
 }
 
 __device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_(double a, double b, double c) { return fma(a, b, c); }
 
+// One copy of B bytes (4, 8 or 16) to shared memory, asynchronous; `on` false writes zeros.
+template <int B>
+__device__ __forceinline__ void copy_async(void* to, const void* from, bool on) {
+    const unsigned at = static_cast<unsigned>(__cvta_generic_to_shared(to));
+    const int bytes = on ? B : 0;
+    if constexpr (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(at), "l"(from), "n"(B), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void await_copies() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
 // The next iteration's S rows of V values of one array.  4 bytes and more go asynchronously to
 // slot [row][thread] of shared memory; single 16-bit values, which that copy does not know, to registers.
-// Rows before 0, at or beyond `rows`, and channels beyond the last one read as zero.
+// Rows from `count` on read as zero.
 template <typename T, int V, int S>
 struct Prefetch {
     static constexpr int kBytes = sizeof(T) * V;
     static constexpr bool kShared = kBytes >= 4;
-    static constexpr size_t smem(int threads) { return kShared ? size_t(kBytes) * S * threads : 0; }
+    __host__ __device__ static constexpr size_t smem(int threads) { return kShared ? size_t(kBytes) * S * threads : 0; }
     Pack<T, V> held[kShared ? 1 : S];
     Pack<T, V>* slot;
 
-    __device__ __forceinline__ void issue(const T* base, int64_t row0, int64_t rows, int64_t stride, bool live) {
+    __device__ __forceinline__ void issue(const T* base, const T* from, int64_t stride, int count) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const bool on = live && row0 + s >= 0 && row0 + s < rows;
-            const T* from = base + (on ? (row0 + s) * stride : 0);
-            if constexpr (kShared) {
-                const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(slot + s * blockDim.x));
-                const int bytes = on ? kBytes : 0;
-                if constexpr (kBytes == 16)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-                else
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(kBytes), "r"(bytes) : "memory");
-            } else {
-                held[s] = on ? *reinterpret_cast<const Pack<T, V>*>(from) : Pack<T, V>{};
-            }
+        for (int s = 0; s < S; ++s, from += stride) {
+            const bool on = s < count;
+            if constexpr (kShared) copy_async<kBytes>(slot + s * blockDim.x, on ? from : base, on);
+            else held[s] = on ? *reinterpret_cast<const Pack<T, V>*>(from) : Pack<T, V>{};
         }
     }
     __device__ __forceinline__ Pack<T, V> take(int s) const {
@@ -162,9 +171,6 @@ struct Prefetch {
         else return held[s];
     }
 };
-
-__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void await_copies() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
 // The affine map of a run of rows on V channels; `drop`: what enters the run does not leave it.
 template <typename A, int V>
@@ -177,175 +183,181 @@ struct Map {
         for (int v = 0; v < V; ++v) { a[v] = A(1); b[v] = A(0); }
         drop = false;
     }
-    // this map behind `earlier`
-    __device__ __forceinline__ void behind(const Map& earlier) {
-        if (drop) return;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            b[v] = fma_(a[v], earlier.b[v], b[v]);
-            a[v] *= earlier.a[v];
-        }
-        drop = earlier.drop;
-    }
     __device__ __forceinline__ void apply(A (&h)[V]) const {
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = drop ? b[v] : fma_(a[v], h[v], b[v]);
     }
 };
 
-// Maps in shared memory: [warp or CTA][A, B][lane of the strip], with a flag each.
-template <typename A, int V>
-struct MapStore {
-    Pack<A, V>* values;
-    unsigned char* drops;
-    int lanes;
+// Shared memory of one scan: the maps of the warps, the state that enters each of them, the state that enters
+// the next iteration, and, twice by turns, the maps that the CTAs of a cluster hand to one another.
+template <typename A>
+struct ScanMemory {
+    A *maps, *carry, *run, *others;  // [warp][A, B][width], [warp][width], [width], [turn][CTA][A, B][width]
+    unsigned char *drops, *other_drops;  // [warp], [turn][CTA]
+    int width;
 
-    __device__ __forceinline__ void put(int i, int tc, const Map<A, V>& m) const {
-        Pack<A, V> a, b;
-#pragma unroll
-        for (int v = 0; v < V; ++v) { a.v[v] = m.a[v]; b.v[v] = m.b[v]; }
-        values[(2 * i) * lanes + tc] = a;
-        values[(2 * i + 1) * lanes + tc] = b;
-        if (tc == 0) drops[i] = m.drop;
+    __host__ __device__ static constexpr size_t bytes(int width, int warps, int cluster) {
+        return sizeof(A) * width * (3 * size_t(warps) + 1 + (cluster > 1 ? 4 * size_t(cluster) : 0)) + 16 * size_t(1 + (warps + 2 * cluster) / 16);
     }
-    template <bool PACKED>
-    __device__ __forceinline__ Map<A, V> get(int i, int tc) const {
-        const Pack<A, V> a = values[(2 * i) * lanes + tc], b = values[(2 * i + 1) * lanes + tc];
-        Map<A, V> m;
-#pragma unroll
-        for (int v = 0; v < V; ++v) { m.a[v] = a.v[v]; m.b[v] = b.v[v]; }
-        m.drop = PACKED && drops[i];
-        return m;
+    __device__ __forceinline__ void place(unsigned char* at, int w, int warps, int cluster) {
+        width = w;
+        maps = reinterpret_cast<A*>(at);
+        carry = maps + 2 * warps * width;
+        run = carry + warps * width;
+        others = run + width;
+        drops = reinterpret_cast<unsigned char*>(others + (cluster > 1 ? 4 * cluster * width : 0));
+        other_drops = drops + warps;
     }
 };
 
-// Bytes of shared memory behind the prefetch slots: both buffers of the warps' maps (`scans` of them) and of
-// the cluster's maps, flags included.
-template <typename A, int V>
-__host__ __device__ constexpr size_t map_bytes(int lanes, int count) { return 2 * sizeof(A) * V * size_t(lanes) * count + 16 * ((count + 15) / 16); }
-template <typename A, int V>
-__host__ __device__ constexpr size_t scan_bytes(int lanes, int warps, int cluster, int scans) {
-    return 2 * (scans * map_bytes<A, V>(lanes, warps) + (cluster > 1 ? map_bytes<A, V>(lanes, cluster) : 0));
-}
-
-template <typename A, int V>
-__device__ __forceinline__ MapStore<A, V> map_store(unsigned char* at, int lanes, int count) {
-    MapStore<A, V> m;
-    m.values = reinterpret_cast<Pack<A, V>*>(at);
-    m.drops = at + 2 * sizeof(A) * V * size_t(lanes) * count;
-    m.lanes = lanes;
-    return m;
-}
-
 // Scan of the threads' maps over the parts of a warp (REVERSE: from the last part to the first).  On return
-// `m` is the map of everything in the warp that comes before this part, and lanes of the last part in scan
-// order have put the whole warp's map into `store`.
+// `m` is the map of everything in the warp that comes before this part; the whole warp's is in `memory`.
 template <typename A, int V, bool REVERSE, bool PACKED>
-__device__ __forceinline__ void scan_warp(Map<A, V>& m, int log_lanes, const MapStore<A, V>& store) {
+__device__ __forceinline__ void scan_warp(Map<A, V>& m, int log_lanes, const ScanMemory<A>& memory) {
     const int lane = threadIdx.x & 31, lanes = 1 << log_lanes, parts = 32 >> log_lanes;
     const int part = REVERSE ? parts - 1 - (lane >> log_lanes) : lane >> log_lanes;
+    const auto from = [&](auto value, int by) {
+        return REVERSE ? __shfl_down_sync(0xffffffffu, value, by) : __shfl_up_sync(0xffffffffu, value, by);
+    };
     for (int k = 1; k < parts; k <<= 1) {
-        Map<A, V> e;
+        const bool earlier_drop = PACKED && from(int(m.drop), k << log_lanes);
+        const bool take = part >= k && !(PACKED && m.drop);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            e.a[v] = REVERSE ? __shfl_down_sync(0xffffffffu, m.a[v], k << log_lanes) : __shfl_up_sync(0xffffffffu, m.a[v], k << log_lanes);
-            e.b[v] = REVERSE ? __shfl_down_sync(0xffffffffu, m.b[v], k << log_lanes) : __shfl_up_sync(0xffffffffu, m.b[v], k << log_lanes);
+            const A ea = from(m.a[v], k << log_lanes), eb = from(m.b[v], k << log_lanes);
+            if (take) {
+                m.b[v] = fma_(m.a[v], eb, m.b[v]);
+                m.a[v] *= ea;
+            }
         }
-        e.drop = false;
-        if (PACKED) e.drop = REVERSE ? __shfl_down_sync(0xffffffffu, int(m.drop), k << log_lanes) : __shfl_up_sync(0xffffffffu, int(m.drop), k << log_lanes);
-        if (part >= k) m.behind(e);
+        if (take) m.drop = earlier_drop;
     }
-    if (part == parts - 1) store.put(threadIdx.x >> 5, lane & (lanes - 1), m);
+    if (part == parts - 1) {
+        Pack<A, V> a, b;
+#pragma unroll
+        for (int v = 0; v < V; ++v) { a.v[v] = m.a[v]; b.v[v] = m.b[v]; }
+        A* to = memory.maps + 2 * int(threadIdx.x >> 5) * memory.width + (lane & (lanes - 1)) * V;
+        store_pack<A, V>(to, a);
+        store_pack<A, V>(to + memory.width, b);
+        if (PACKED && (lane & (lanes - 1)) == 0) memory.drops[threadIdx.x >> 5] = m.drop;
+    }
     if (parts > 1) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            m.a[v] = REVERSE ? __shfl_down_sync(0xffffffffu, m.a[v], lanes) : __shfl_up_sync(0xffffffffu, m.a[v], lanes);
-            m.b[v] = REVERSE ? __shfl_down_sync(0xffffffffu, m.b[v], lanes) : __shfl_up_sync(0xffffffffu, m.b[v], lanes);
-        }
-        if (PACKED) m.drop = REVERSE ? __shfl_down_sync(0xffffffffu, int(m.drop), lanes) : __shfl_up_sync(0xffffffffu, int(m.drop), lanes);
+        for (int v = 0; v < V; ++v) { m.a[v] = from(m.a[v], lanes); m.b[v] = from(m.b[v], lanes); }
+        if (PACKED) m.drop = from(int(m.drop), lanes);
     }
     if (part == 0) m.clear();
 }
 
-// The state that enters this thread's rows, from `run`, the state that enters the iteration's first row (in
-// scan order), and `m`, the map of the parts before it in its warp; `run` moves on to the next iteration.
-// One CTA: the warps' maps are applied in their order.  A cluster: each CTA composes its own, hands the
-// composition to all and applies what lies before it.
-template <typename A, int V, bool REVERSE, bool PACKED>
-__device__ __forceinline__ void enter(A (&run)[V], A (&in)[V], const Map<A, V>& m, const MapStore<A, V>& store,
-                                      const MapStore<A, V>& shared, int warps, int cluster, int rank, int tc) {
-    const int warp = threadIdx.x >> 5;
-    if (cluster == 1) {
+// Column c of the strip, one thread each: the state `r` that enters the CTA's rows goes through the warps'
+// maps, and what enters each warp is left in `carry`.
+template <typename A, bool REVERSE, bool PACKED>
+__device__ __forceinline__ A carry_through(const ScanMemory<A>& m, int warps, int c, A r) {
 #pragma unroll 4
+    for (int i = 0; i < warps; ++i) {
+        const int w = REVERSE ? warps - 1 - i : i;
+        m.carry[w * m.width + c] = r;
+        const A b = m.maps[(2 * w + 1) * m.width + c];
+        r = PACKED && m.drops[w] ? b : fma_(m.maps[2 * w * m.width + c], r, b);
+    }
+    return r;
+}
+
+// The same across a cluster: each CTA composes its warps' maps and writes the composition into every CTA's
+// memory; behind the cluster's barrier each applies those before its own.  All threads call it.
+template <typename A, bool REVERSE, bool PACKED>
+__device__ __forceinline__ void carry_across(const ScanMemory<A>& m, int warps, int cluster, int rank, int turn) {
+    auto group = cooperative_groups::this_cluster();
+    A* others = m.others + turn * 2 * cluster * m.width;
+    unsigned char* drops = m.other_drops + turn * cluster;
+    for (int c = threadIdx.x; c < m.width; c += blockDim.x) {
+        A a = A(1), b = A(0);
+        bool drop = false;
         for (int i = 0; i < warps; ++i) {
             const int w = REVERSE ? warps - 1 - i : i;
-            if (w == warp) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) in[v] = run[v];
-            }
-            store.template get<PACKED>(w, tc).apply(run);
+            const A wa = m.maps[2 * w * m.width + c], wb = m.maps[(2 * w + 1) * m.width + c];
+            const bool wd = PACKED && m.drops[w];
+            b = wd ? wb : fma_(wa, b, wb);
+            a *= wa;
+            drop |= wd;
         }
-    } else {
-        Map<A, V> all;
-        all.clear();
-        for (int i = 0; i < warps; ++i) {
-            Map<A, V> next = store.template get<PACKED>(REVERSE ? warps - 1 - i : i, tc);
-            next.behind(all);
-            all = next;
+        for (int r = 0; r < cluster; ++r) {
+            A* there = group.map_shared_rank(others, r) + 2 * rank * m.width + c;
+            there[0] = a;
+            there[m.width] = b;
+            if (PACKED && c == 0) group.map_shared_rank(drops, r)[rank] = drop;
         }
-        auto group = cooperative_groups::this_cluster();
-        // each warp serves some of the CTAs
-        if ((threadIdx.x & 31) < (1 << (31 - __clz(store.lanes))))
-            for (int r = warp; r < cluster; r += warps) {
-                MapStore<A, V> there = shared;
-                there.values = group.map_shared_rank(shared.values, r);
-                there.drops = group.map_shared_rank(shared.drops, r);
-                there.put(rank, tc, all);
-            }
-        group.sync();
-#pragma unroll
-        for (int v = 0; v < V; ++v) in[v] = run[v];
-        for (int i = 0; i < cluster; ++i) {
-            const int r = REVERSE ? cluster - 1 - i : i;
-            if (r == rank) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) in[v] = run[v];
-            }
-            shared.template get<PACKED>(r, tc).apply(run);
-        }
-        for (int i = 0; i < (REVERSE ? warps - 1 - warp : warp); ++i)
-            store.template get<PACKED>(REVERSE ? warps - 1 - i : i, tc).apply(in);
     }
-    m.apply(in);
+    group.sync();
+    for (int c = threadIdx.x; c < m.width; c += blockDim.x) {
+        A r = m.run[c], mine = r;
+        for (int i = 0; i < cluster; ++i) {
+            const int k = REVERSE ? cluster - 1 - i : i;
+            if (k == rank) mine = r;
+            const A b = others[(2 * k + 1) * m.width + c];
+            r = PACKED && drops[k] ? b : fma_(others[2 * k * m.width + c], r, b);
+        }
+        m.run[c] = r;
+        carry_through<A, REVERSE, PACKED>(m, warps, c, mine);
+    }
 }
 
 // a, x and, where REST, 1 - a of S rows from the prefetched inputs; without REST x is b already.
-template <int FORM, bool REST, typename X, typename G, int V, int GV, int S, typename A>
-__device__ __forceinline__ void factors(const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, bool complement,
-                                        A (&a)[S][V], A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
+template <int FORM, bool REST, bool COMPLEMENT, typename X, typename G, int V, int GV, int S, typename A>
+__device__ __forceinline__ void factors(const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, A (&a)[S][V],
+                                        A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         const Pack<X, V> x = fx.take(s);
         const Pack<G, GV> g = fg.take(s);
         A ga[GV], gr[GV];
 #pragma unroll
-        for (int v = 0; v < GV; ++v) gate_factors<FORM>(A(widen(g.v[v])), ga[v], gr[v]);
+        for (int v = 0; v < GV; ++v) gate_factors<FORM, sizeof(G) == 2>(A(widen(g.v[v])), ga[v], gr[v]);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             a[s][v] = ga[v % GV];
             u[s][v] = widen(x.v[v]);
+            if (COMPLEMENT) u[s][v] *= gr[v % GV];
             if (REST) rest[s % (REST ? S : 1)][v] = gr[v % GV];
-            else if (complement) u[s][v] *= gr[v % GV];
         }
     }
 }
 
-template <bool REST, typename X, typename G, int V, int GV, int S, typename A>
-__device__ __forceinline__ void factors(int form, const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, bool complement,
-                                        A (&a)[S][V], A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
-    if (form == kGateValue) factors<kGateValue, REST>(fx, fg, complement, a, u, rest);
-    else if (form == kGateLog) factors<kGateLog, REST>(fx, fg, complement, a, u, rest);
-    else factors<kGateLogit, REST>(fx, fg, complement, a, u, rest);
+template <bool REST, bool COMPLEMENT, typename X, typename G, int V, int GV, int S, typename A>
+__device__ __forceinline__ void factors(int form, const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, A (&a)[S][V],
+                                        A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
+    if (form == kGateValue) factors<kGateValue, REST, COMPLEMENT>(fx, fg, a, u, rest);
+    else if (form == kGateLog) factors<kGateLog, REST, COMPLEMENT>(fx, fg, a, u, rest);
+    else factors<kGateLogit, REST, COMPLEMENT>(fx, fg, a, u, rest);
+}
+
+// Where a thread stands: its strip, channels and rows.
+struct Place {
+    int lanes, lane, warp, tc, parts, part, cluster, rank;
+    uint64_t batch, first, c0;  // batch entry, first channel of the strip and of the thread
+    bool live;
+
+    __device__ __forceinline__ Place(const RecurrencePlan& plan, uint64_t dim, int V) {
+        lanes = 1 << plan.log_lanes;
+        lane = threadIdx.x & 31;
+        warp = threadIdx.x >> 5;
+        tc = lane & (lanes - 1);
+        parts = 32 >> plan.log_lanes;
+        part = warp * parts + (lane >> plan.log_lanes);
+        cluster = plan.cluster;
+        rank = cluster > 1 ? int(blockIdx.x % cluster) : 0;
+        const uint64_t strip = cluster > 1 ? blockIdx.x / cluster : blockIdx.x;
+        batch = strip / plan.strips;
+        first = (strip % plan.strips) * lanes * V;
+        c0 = first + uint64_t(tc) * V;
+        live = c0 < dim;
+    }
+};
+
+__device__ __forceinline__ int rows_left(int64_t rows, int64_t row0, int most, bool live) {
+    const int64_t n = rows - row0;
+    return !live || row0 < 0 || n <= 0 ? 0 : n < most ? int(n) : most;
 }
 
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED>
@@ -353,49 +365,47 @@ __global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const Recurr
     using A = Acc<X>;
     constexpr int GV = SHARED ? 1 : V;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int lanes = 1 << plan.log_lanes, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int tc = lane & (lanes - 1), parts = 32 >> plan.log_lanes;
-    const int cluster = plan.cluster, rank = cluster > 1 ? int(blockIdx.x % cluster) : 0;
-    const uint64_t strip = blockIdx.x / cluster, b = strip / plan.strips;
-    const uint64_t c0 = ((strip % plan.strips) * lanes + tc) * V;
-    const bool live = c0 < p.dim;
+    const Place at(plan, p.dim, V);
+    const uint64_t b = at.batch, c0 = at.c0;
+    const bool live = at.live;
     const int64_t rows = int64_t(p.rows), dim = int64_t(p.dim);
-    const X* x = static_cast<const X*>(p.x) + b * p.x_batch + (live ? c0 : 0);
-    const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
     const A* initial = p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr;
-    X* out = p.out ? static_cast<X*>(p.out) + b * p.rows * p.dim + c0 : nullptr;
     A* state = p.state ? static_cast<A*>(p.state) + c0 : nullptr;
     A* marks = p.checkpoints
         ? static_cast<A*>(p.checkpoints) + b * ((p.rows + kCheckpointRows - 1) / kCheckpointRows) * p.dim + c0 : nullptr;
 
     Prefetch<X, V, S> fx;
     Prefetch<G, GV, S> fg;
-    fx.slot = reinterpret_cast<Pack<X, V>*>(smem) + threadIdx.x;
-    unsigned char* at = smem + fx.smem(blockDim.x);
-    fg.slot = reinterpret_cast<Pack<G, GV>*>(at) + threadIdx.x;
-    at += (fg.smem(blockDim.x) + 15) / 16 * 16;
-    MapStore<A, V> stores[2], shared[2];
-    for (int k = 0; k < 2; ++k, at += map_bytes<A, V>(lanes, plan.warps)) stores[k] = map_store<A, V>(at, lanes, plan.warps);
-    for (int k = 0; k < 2 && cluster > 1; ++k, at += map_bytes<A, V>(lanes, cluster)) shared[k] = map_store<A, V>(at, lanes, cluster);
-
-    A run[V];  // the state that enters the iteration's first row
-#pragma unroll
-    for (int v = 0; v < V; ++v) run[v] = !PACKED && initial && live ? initial[b * p.dim + v] : A(0);
-    const int part = warp * parts + (lane >> plan.log_lanes);
-    if (PACKED && state && live && rank == 0)  // sequences without rows hand their initial state on
-        for (int64_t j = part; j < int64_t(p.sequences); j += plan.warps * parts)
+    unsigned char* next = smem;
+    fx.slot = reinterpret_cast<Pack<X, V>*>(next) + threadIdx.x;
+    next += fx.smem(blockDim.x);
+    fg.slot = reinterpret_cast<Pack<G, GV>*>(next) + threadIdx.x;
+    next += (fg.smem(blockDim.x) + 15) / 16 * 16;
+    ScanMemory<A> memory;
+    memory.place(next, at.lanes * V, plan.warps, at.cluster);
+    for (int c = threadIdx.x; c < memory.width; c += blockDim.x)
+        memory.run[c] = !PACKED && p.initial && at.first + c < p.dim ? static_cast<const A*>(p.initial)[b * p.dim + at.first + c] : A(0);
+    if (PACKED && state && live && at.rank == 0)  // sequences without rows hand their initial state on
+        for (int64_t j = at.part; j < int64_t(p.sequences); j += plan.warps * at.parts)
             if (offset_at(p.offsets, p.wide_offsets, j + 1) <= offset_at(p.offsets, p.wide_offsets, j))
                 for (int v = 0; v < V; ++v) state[j * dim + v] = initial ? initial[j * dim + v] : A(0);
 
-    const int64_t span = int64_t(plan.warps) * parts * cluster * S;
-    int64_t row0 = (int64_t(rank) * plan.warps * parts + part) * S;
+    const int64_t span = int64_t(plan.warps) * at.parts * at.cluster * S;
+    int64_t row0 = (int64_t(at.rank) * plan.warps * at.parts + at.part) * S;
+    const X* x = static_cast<const X*>(p.x) + b * p.x_batch + (live ? c0 : 0);
+    const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
+    const int64_t x_row = int64_t(p.x_row), gate_row = int64_t(p.gate_row);
+    const X* px = x + row0 * x_row;
+    const G* pg = gate + row0 * gate_row;
+    X* out = p.out ? static_cast<X*>(p.out) + (b * p.rows + row0) * p.dim + c0 : nullptr;
+    int count = rows_left(rows, row0, S, live);
+    fx.issue(x, px, x_row, count);
+    fg.issue(gate, pg, gate_row, count);
+    commit_copies();
     SequenceWalk walk;
     if (PACKED) walk.seek(p.offsets, p.wide_offsets, p.sequences, row0);
-    fx.issue(x, row0, rows, p.x_row, live);
-    fg.issue(gate, row0, rows, p.gate_row, live);
-    commit_copies();
-    int buf = 0;
-    for (int64_t base = 0; base < rows; base += span, row0 += span, buf ^= 1) {
+    int turn = 0;
+    for (int64_t base = 0; base < rows; base += span, row0 += span, turn ^= 1) {
         RowEvents e;
         if (PACKED) {
             walk.advance(row0);
@@ -403,15 +413,19 @@ __global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const Recurr
         }
         A a[S][V], u[S][V], unused[1][V];
         await_copies();
-        factors<false>(p.form, fx, fg, p.complement, a, u, unused);
-        if (row0 + S > rows || (PACKED && e.dead))
+        if (p.complement) factors<false, true>(p.form, fx, fg, a, u, unused);
+        else factors<false, false>(p.form, fx, fg, a, u, unused);
+        if (count < S || (PACKED && e.dead)) {
 #pragma unroll
             for (int s = 0; s < S; ++s)
+                if (s >= count || (e.dead >> s & 1u)) {
 #pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (row0 + s >= rows || (e.dead >> s & 1u)) { a[s][v] = A(1); u[s][v] = A(0); }
+                    for (int v = 0; v < V; ++v) { a[s][v] = A(1); u[s][v] = A(0); }
+                }
+        }
+        const bool events = PACKED && e.starts | e.ends | e.dead;
         // the initial state of a sequence that starts here joins b: its first row is then b alone
-        if (PACKED && e.starts && initial && live)
+        if (events && e.starts && initial && live) {
 #pragma unroll
             for (int s = 0; s < S; ++s)
                 if (e.starts >> s & 1u) {
@@ -419,51 +433,89 @@ __global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const Recurr
 #pragma unroll
                     for (int v = 0; v < V; ++v) u[s][v] = fma_(a[s][v], in[v], u[s][v]);
                 }
+        }
         Map<A, V> m;
         m.clear();
+        if (!events) {
 #pragma unroll
-        for (int s = 0; s < S; ++s)
+            for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                m.b[v] = PACKED && (e.starts >> s & 1u) ? u[s][v] : fma_(a[s][v], m.b[v], u[s][v]);
-                m.a[v] *= a[s][v];
-            }
-        m.drop = PACKED && e.starts;
-        scan_warp<A, V, false, PACKED>(m, plan.log_lanes, stores[buf]);
+                for (int v = 0; v < V; ++v) {
+                    m.b[v] = s ? fma_(a[s][v], m.b[v], u[s][v]) : u[s][v];
+                    m.a[v] = s ? m.a[v] * a[s][v] : a[s][v];
+                }
+        } else {
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    m.b[v] = e.starts >> s & 1u ? u[s][v] : fma_(a[s][v], m.b[v], u[s][v]);
+                    m.a[v] *= a[s][v];
+                }
+            m.drop = e.starts;
+        }
+        __syncwarp();
+        scan_warp<A, V, false, PACKED>(m, plan.log_lanes, memory);
         __syncthreads();
-        fx.issue(x, row0 + span, rows, p.x_row, live);  // the slots were read before the barrier
-        fg.issue(gate, row0 + span, rows, p.gate_row, live);
+        // the slots were read before the barrier: the next rows may come
+        px += span * x_row;
+        pg += span * gate_row;
+        const int now = count;
+        count = rows_left(rows, row0 + span, S, live);
+        fx.issue(x, px, x_row, count);
+        fg.issue(gate, pg, gate_row, count);
         commit_copies();
-        A h[V];
-        enter<A, V, false, PACKED>(run, h, m, stores[buf], shared[buf], plan.warps, cluster, rank, tc);
-        if (!live || row0 >= rows) continue;
-        if (marks && row0 % int64_t(kCheckpointRows) == 0)
+        if (at.cluster == 1) {
+            for (int c = threadIdx.x; c < memory.width; c += blockDim.x)
+                memory.run[c] = carry_through<A, false, PACKED>(memory, plan.warps, c, memory.run[c]);
+        } else {
+            carry_across<A, false, PACKED>(memory, plan.warps, at.cluster, at.rank, turn);
+        }
+        __syncthreads();
+        if (now) {
+            const Pack<A, V> in = load_pack<A, V>(memory.carry + at.warp * memory.width + at.tc * V);
+            A h[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) marks[row0 / int64_t(kCheckpointRows) * dim + v] = h[v];
+            for (int v = 0; v < V; ++v) h[v] = in.v[v];
+            m.apply(h);
+            if (marks && row0 % int64_t(kCheckpointRows) == 0)
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            Pack<X, V> y;
+                for (int v = 0; v < V; ++v) marks[row0 / int64_t(kCheckpointRows) * dim + v] = h[v];
+            if (!events) {
+                X* to = out;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                h[v] = PACKED && (e.starts >> s & 1u) ? u[s][v] : fma_(a[s][v], h[v], u[s][v]);
-                y.v[v] = narrow<X>(PACKED && (e.dead >> s & 1u) ? A(0) : h[v]);
-            }
-            if (out && row0 + s < rows) store_pack<X, V>(out + (row0 + s) * dim, y);
-            if (PACKED && state && (e.ends >> s & 1u)) {
-                A* to = state + sequence_of(walk, row0 + s) * dim;
+                for (int s = 0; s < S; ++s, to += dim) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) to[v] = h[v];
+                    for (int v = 0; v < V; ++v) h[v] = fma_(a[s][v], h[v], u[s][v]);
+                    if (out && s < now) store_pack<X, V>(to, narrow_pack<X, V>(h));
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    A y[V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        h[v] = e.starts >> s & 1u ? u[s][v] : fma_(a[s][v], h[v], u[s][v]);
+                        y[v] = e.dead >> s & 1u ? A(0) : h[v];
+                    }
+                    if (out && s < now) store_pack<X, V>(out + s * dim, narrow_pack<X, V>(y));
+                    if (state && (e.ends >> s & 1u)) {
+                        A* to = state + sequence_of(walk, row0 + s) * dim;
+#pragma unroll
+                        for (int v = 0; v < V; ++v) to[v] = h[v];
+                    }
+                }
             }
         }
+        if (out) out += span * dim;
     }
-    if (!PACKED && state && live && part == 0 && rank == 0)
-#pragma unroll
-        for (int v = 0; v < V; ++v) state[b * p.dim + v] = run[v];
+    if (!PACKED && p.state && at.rank == 0)
+        for (int c = threadIdx.x; c < memory.width && at.first + c < p.dim; c += blockDim.x)
+            static_cast<A*>(p.state)[b * p.dim + at.first + c] = memory.run[c];
 }
 
-// One iteration goes forward through its rows from a checkpoint (for h_{t-1}, kept in registers) and
-// backward through the same registers, so that x, the gates and the derivatives are read once and h,
-// rounded or not, is not read at all.
+// One iteration takes its rows backward and then, from a checkpoint, forward again (for h_{t-1}), both in
+// registers, so that x, the gates and the derivatives are read once and h, rounded or not, is not read at all.
 // Shared gates: each thread sums its V channels, 1 << fold_log neighbouring lanes are folded by shuffles,
 // and `partial` takes one value per row and fold (dgate itself where a fold is a whole gate).
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED>
@@ -472,59 +524,61 @@ __global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const Recur
     using A = Acc<X>;
     constexpr int GV = SHARED ? 1 : V;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int lanes = 1 << plan.log_lanes, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int tc = lane & (lanes - 1), parts = 32 >> plan.log_lanes;
-    const int cluster = plan.cluster, rank = cluster > 1 ? int(blockIdx.x % cluster) : 0;
-    const uint64_t strip = blockIdx.x / cluster, b = strip / plan.strips;
-    const uint64_t c0 = ((strip % plan.strips) * lanes + tc) * V;
-    const bool live = c0 < p.dim;
+    const Place at(plan, p.dim, V);
+    const uint64_t b = at.batch, c0 = at.c0;
+    const bool live = at.live;
     const int64_t rows = int64_t(p.rows), dim = int64_t(p.dim);
-    const X* x = static_cast<const X*>(p.x) + b * p.x_batch + (live ? c0 : 0);
-    const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
-    const X* derivs = static_cast<const X*>(p.derivs) + b * p.d_batch + (live ? c0 : 0);
     const A* initial = p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr;
     const A* state_derivs = p.state_derivs ? static_cast<const A*>(p.state_derivs) + c0 : nullptr;
-    const A* marks = static_cast<const A*>(p.marks) + b * ((p.rows + kCheckpointRows - 1) / kCheckpointRows) * p.dim + c0;
-    X* dx = static_cast<X*>(p.dx) + b * p.rows * p.dim + c0;
     A* dinitial = p.dinitial ? static_cast<A*>(p.dinitial) + c0 : nullptr;
-    const int64_t folds = SHARED ? (dim / V) >> plan.fold_log : 0;
-    G* dgate = static_cast<G*>(p.dgate) + b * p.rows * p.gate_dim + (SHARED ? 0 : c0);
+    const A* marks = static_cast<const A*>(p.marks) + b * ((p.rows + kCheckpointRows - 1) / kCheckpointRows) * p.dim + at.first;
 
     Prefetch<X, V, S> fx, fd;
     Prefetch<G, GV, S> fg;
-    fx.slot = reinterpret_cast<Pack<X, V>*>(smem) + threadIdx.x;
+    unsigned char* next = smem;
+    fx.slot = reinterpret_cast<Pack<X, V>*>(next) + threadIdx.x;
     fd.slot = fx.slot + S * blockDim.x;
-    unsigned char* at = smem + 2 * fx.smem(blockDim.x);
-    fg.slot = reinterpret_cast<Pack<G, GV>*>(at) + threadIdx.x;
-    at += (fg.smem(blockDim.x) + 15) / 16 * 16;
-    MapStore<A, V> ahead[2], stores[2], shared[2];
-    for (int k = 0; k < 2; ++k, at += map_bytes<A, V>(lanes, plan.warps)) ahead[k] = map_store<A, V>(at, lanes, plan.warps);
-    for (int k = 0; k < 2; ++k, at += map_bytes<A, V>(lanes, plan.warps)) stores[k] = map_store<A, V>(at, lanes, plan.warps);
-    for (int k = 0; k < 2 && cluster > 1; ++k, at += map_bytes<A, V>(lanes, cluster)) shared[k] = map_store<A, V>(at, lanes, cluster);
-
-    A run[V];  // the gradient that enters the iteration's last row from behind
-#pragma unroll
-    for (int v = 0; v < V; ++v) run[v] = !PACKED && state_derivs && live ? state_derivs[b * p.dim + v] : A(0);
-    const int part = warp * parts + (lane >> plan.log_lanes);
-    if (PACKED && dinitial && live && rank == 0)
-        for (int64_t j = part; j < int64_t(p.sequences); j += plan.warps * parts)
+    next += 2 * fx.smem(blockDim.x);
+    fg.slot = reinterpret_cast<Pack<G, GV>*>(next) + threadIdx.x;
+    next += (fg.smem(blockDim.x) + 15) / 16 * 16;
+    ScanMemory<A> ahead, back;
+    ahead.place(next, at.lanes * V, plan.warps, 1);
+    next += ScanMemory<A>::bytes(ahead.width, plan.warps, 1);
+    back.place(next, ahead.width, plan.warps, at.cluster);
+    for (int c = threadIdx.x; c < back.width; c += blockDim.x)
+        back.run[c] = !PACKED && p.state_derivs && at.first + c < p.dim ? static_cast<const A*>(p.state_derivs)[b * p.dim + at.first + c] : A(0);
+    if (PACKED && dinitial && live && at.rank == 0)
+        for (int64_t j = at.part; j < int64_t(p.sequences); j += plan.warps * at.parts)
             if (offset_at(p.offsets, p.wide_offsets, j + 1) <= offset_at(p.offsets, p.wide_offsets, j))
                 for (int v = 0; v < V; ++v) dinitial[j * dim + v] = state_derivs ? state_derivs[j * dim + v] : A(0);
 
-    const int64_t block = int64_t(plan.warps) * parts * S, span = block * cluster;
-    int64_t base = (rows - 1) / span * span, row0 = base + rank * block + int64_t(part) * S;
+    const int64_t block = int64_t(plan.warps) * at.parts * S, span = block * at.cluster;
+    int64_t base = (rows - 1) / span * span, row0 = base + at.rank * block + int64_t(at.part) * S;
+    const X* x = static_cast<const X*>(p.x) + b * p.x_batch + (live ? c0 : 0);
+    const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
+    const X* derivs = static_cast<const X*>(p.derivs) + b * p.d_batch + (live ? c0 : 0);
+    const int64_t x_row = int64_t(p.x_row), gate_row = int64_t(p.gate_row), d_row = int64_t(p.d_row);
+    const X* px = x + row0 * x_row;
+    const G* pg = gate + row0 * gate_row;
+    const X* pd = derivs + row0 * d_row;
+    // the checkpoint that enters the CTA's rows: each column's thread copies its own
+    const auto fetch_marks = [&](int64_t own) {
+        for (int c = threadIdx.x; c < ahead.width; c += blockDim.x) {
+            const bool on = own >= 0 && own < rows && at.first + c < p.dim;
+            const A* from = static_cast<const A*>(p.marks);
+            copy_async<sizeof(A)>(ahead.run + c, on ? marks + own / int64_t(kCheckpointRows) * dim + c : from, on);
+        }
+    };
+    int count = rows_left(rows, row0, S, live);
+    fx.issue(x, px, x_row, count);
+    fg.issue(gate, pg, gate_row, count);
+    fd.issue(derivs, pd, d_row, count);
+    fetch_marks(base + at.rank * block);
+    commit_copies();
     SequenceWalk walk;
     if (PACKED) walk.seek(p.offsets, p.wide_offsets, p.sequences, row0);
-    fx.issue(x, row0, rows, p.x_row, live);
-    fg.issue(gate, row0, rows, p.gate_row, live);
-    fd.issue(derivs, row0, rows, p.d_row, live);
-    commit_copies();
-    int buf = 0;
-    for (; base >= 0; base -= span, row0 -= span, buf ^= 1) {
-        A h[V];
-        const int64_t own = base + rank * block;  // the CTA's first row
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = live && own < rows ? marks[own / int64_t(kCheckpointRows) * dim + v] : A(0);
+    int turn = 0;
+    for (; base >= 0; base -= span, row0 -= span, turn ^= 1) {
         RowEvents e;
         if (PACKED) {
             walk.retreat(row0);
@@ -532,21 +586,24 @@ __global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const Recur
         }
         A a[S][V], rest[S][V], x_[S][V], d[S][V];
         await_copies();
-        factors<true>(p.form, fx, fg, p.complement, a, x_, rest);
+        factors<true, false>(p.form, fx, fg, a, x_, rest);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             const Pack<X, V> rd = fd.take(s);
 #pragma unroll
             for (int v = 0; v < V; ++v) d[s][v] = widen(rd.v[v]);
         }
-        if (row0 + S > rows || (PACKED && e.dead))
+        if (count < S || (PACKED && e.dead)) {
 #pragma unroll
             for (int s = 0; s < S; ++s)
+                if (s >= count || (e.dead >> s & 1u)) {
 #pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (row0 + s >= rows || (e.dead >> s & 1u)) { a[s][v] = A(1); rest[s][v] = x_[s][v] = d[s][v] = A(0); }
+                    for (int v = 0; v < V; ++v) { a[s][v] = A(1); rest[s][v] = x_[s][v] = d[s][v] = A(0); }
+                }
+        }
+        const bool events = PACKED && e.starts | e.ends | e.dead;
         // the gradient of a state joins the derivatives of the row that it was taken from
-        if (PACKED && e.ends && state_derivs && live)
+        if (events && e.ends && state_derivs && live) {
 #pragma unroll
             for (int s = 0; s < S; ++s)
                 if (e.ends >> s & 1u) {
@@ -554,41 +611,74 @@ __global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const Recur
 #pragma unroll
                     for (int v = 0; v < V; ++v) d[s][v] += in[v];
                 }
+        }
         Map<A, V> m, g;
         m.clear();
         g.clear();
+        const auto input = [&](int s, int v) { return p.complement ? rest[s][v] * x_[s][v] : x_[s][v]; };
+        if (!events) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            if (PACKED && (e.starts >> s & 1u)) {
-                const A* in = initial && live ? initial + sequence_of(walk, row0 + s) * dim : nullptr;
+            for (int s = 0; s < S; ++s)
 #pragma unroll
-                for (int v = 0; v < V; ++v) m.b[v] = in ? in[v] : A(0);
+                for (int v = 0; v < V; ++v) {
+                    const int q = S - 1 - s;
+                    m.b[v] = s ? fma_(a[s][v], m.b[v], input(s, v)) : input(s, v);
+                    m.a[v] = s ? m.a[v] * a[s][v] : a[s][v];
+                    g.b[v] = a[q][v] * (s ? d[q][v] + g.b[v] : d[q][v]);
+                }
+        } else {
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                if (e.starts >> s & 1u) {
+                    const A* in = initial && live ? initial + sequence_of(walk, row0 + s) * dim : nullptr;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) m.b[v] = in ? in[v] : A(0);
+                }
+                const int q = S - 1 - s;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    m.b[v] = fma_(a[s][v], m.b[v], input(s, v));
+                    m.a[v] *= a[s][v];
+                    g.b[v] = a[q][v] * (e.ends >> q & 1u ? d[q][v] : d[q][v] + g.b[v]);
+                }
             }
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                m.b[v] = fma_(a[s][v], m.b[v], p.complement ? rest[s][v] * x_[s][v] : x_[s][v]);
-                m.a[v] *= a[s][v];
-            }
+            m.drop = e.starts;
+            g.drop = e.ends;
         }
 #pragma unroll
-        for (int s = S - 1; s >= 0; --s)
-#pragma unroll
-            for (int v = 0; v < V; ++v)
-                g.b[v] = a[s][v] * (PACKED && (e.ends >> s & 1u) ? d[s][v] : d[s][v] + g.b[v]);
-#pragma unroll
         for (int v = 0; v < V; ++v) g.a[v] = m.a[v];
-        m.drop = PACKED && e.starts;
-        g.drop = PACKED && e.ends;
-        scan_warp<A, V, false, PACKED>(m, plan.log_lanes, ahead[buf]);
-        scan_warp<A, V, true, PACKED>(g, plan.log_lanes, stores[buf]);
+        __syncwarp();
+        scan_warp<A, V, false, PACKED>(m, plan.log_lanes, ahead);
+        scan_warp<A, V, true, PACKED>(g, plan.log_lanes, back);
         __syncthreads();
-        fx.issue(x, row0 - span, rows, p.x_row, live);  // the slots were read before the barrier
-        fg.issue(gate, row0 - span, rows, p.gate_row, live);
-        fd.issue(derivs, row0 - span, rows, p.d_row, live);
+        for (int c = threadIdx.x; c < ahead.width; c += blockDim.x) carry_through<A, false, PACKED>(ahead, plan.warps, c, ahead.run[c]);
+        if (at.cluster == 1) {
+            for (int c = threadIdx.x; c < back.width; c += blockDim.x)
+                back.run[c] = carry_through<A, true, PACKED>(back, plan.warps, c, back.run[c]);
+        } else {
+            carry_across<A, true, PACKED>(back, plan.warps, at.cluster, at.rank, turn);
+        }
+        __syncthreads();
+        // the slots and the checkpoint were read before the barrier: the rows before these may come
+        px -= span * x_row;
+        pg -= span * gate_row;
+        pd -= span * d_row;
+        const int now = count;
+        count = rows_left(rows, row0 - span, S, live);
+        fx.issue(x, px, x_row, count);
+        fg.issue(gate, pg, gate_row, count);
+        fd.issue(derivs, pd, d_row, count);
+        fetch_marks(base - span + at.rank * block);
         commit_copies();
         A in[V], w[V];
-        enter<A, V, false, PACKED>(h, in, m, ahead[buf], ahead[buf], plan.warps, 1, 0, tc);
-        enter<A, V, true, PACKED>(run, w, g, stores[buf], shared[buf], plan.warps, cluster, rank, tc);
+        {
+            const Pack<A, V> first = load_pack<A, V>(ahead.carry + at.warp * ahead.width + at.tc * V);
+            const Pack<A, V> last = load_pack<A, V>(back.carry + at.warp * back.width + at.tc * V);
+#pragma unroll
+            for (int v = 0; v < V; ++v) { in[v] = first.v[v]; w[v] = last.v[v]; }
+        }
+        m.apply(in);
+        g.apply(w);
         // backward through the rows: d becomes g
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {
@@ -604,46 +694,43 @@ __global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const Recur
             }
         }
         // forward through them with h_{t-1} in `in`
+        X* dx = static_cast<X*>(p.dx) + (b * rows + row0) * dim + c0;
+        G* dgate = static_cast<G*>(p.dgate) + (SHARED ? 0 : (b * rows + row0) * dim + c0);
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
+        for (int s = 0; s < S; ++s, dx += dim, dgate += SHARED ? 0 : dim) {
             if (PACKED && (e.starts >> s & 1u)) {
                 const A* from = initial && live ? initial + sequence_of(walk, row0 + s) * dim : nullptr;
 #pragma unroll
                 for (int v = 0; v < V; ++v) in[v] = from ? from[v] : A(0);
             }
-            const bool dead = PACKED && (e.dead >> s & 1u), stored = live && row0 + s < rows;
-            Pack<X, V> gx;
-            Pack<G, V> gg;
-            A sum = A(0);
+            A gx[V], gg[V], sum = A(0);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const A g_ = d[s][v];
-                gx.v[v] = narrow<X>(dead ? A(0) : p.complement ? rest[s][v] * g_ : g_);
-                A da = g_ * (p.complement ? in[v] - x_[s][v] : in[v]);
-                if (p.form != kGateValue) da *= a[s][v];
-                if (p.form == kGateLogit) da *= rest[s][v];
-                if (dead) da = A(0);
-                gg.v[v] = narrow<G>(da);
-                sum += da;
-                in[v] = fma_(a[s][v], in[v], p.complement ? rest[s][v] * x_[s][v] : x_[s][v]);
+                gx[v] = p.complement ? rest[s][v] * d[s][v] : d[s][v];
+                gg[v] = d[s][v] * (p.complement ? in[v] - x_[s][v] : in[v]);
+                if (p.form != kGateValue) gg[v] *= a[s][v];
+                if (p.form == kGateLogit) gg[v] *= rest[s][v];
+                if (PACKED && (e.dead >> s & 1u)) gx[v] = gg[v] = A(0);
+                sum += gg[v];
+                in[v] = fma_(a[s][v], in[v], input(s, v));
             }
-            if (stored) store_pack<X, V>(dx + (row0 + s) * dim, gx);
+            if (s < now) store_pack<X, V>(dx, narrow_pack<X, V>(gx));
             if (SHARED) {
-                sum = stored ? sum : A(0);
+                sum = s < now ? sum : A(0);
                 for (int k = 1; k < 1 << plan.fold_log; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-                const int64_t fold = int64_t(c0 / V) >> plan.fold_log;
-                if (stored && (tc & ((1 << plan.fold_log) - 1)) == 0) {
-                    if (partial) partial[(b * rows + row0 + s) * folds + fold] = sum;
-                    else dgate[(row0 + s) * int64_t(p.gate_dim) + fold] = narrow<G>(sum);
+                if (s < now && (at.tc & ((1 << plan.fold_log) - 1)) == 0) {
+                    const int64_t fold = int64_t(c0 / V) >> plan.fold_log, row = b * rows + row0 + s;
+                    if (partial) partial[row * ((dim / V) >> plan.fold_log) + fold] = sum;
+                    else dgate[row * int64_t(p.gate_dim) + fold] = narrow<G>(sum);
                 }
-            } else if (stored) {
-                store_pack<G, V>(dgate + (row0 + s) * dim, gg);
+            } else if (s < now) {
+                if constexpr (std::is_same_v<Acc<G>, A>) store_pack<G, V>(dgate, narrow_pack<G, V>(gg));
             }
         }
     }
-    if (!PACKED && dinitial && live && part == 0 && rank == 0)
-#pragma unroll
-        for (int v = 0; v < V; ++v) dinitial[b * p.dim + v] = run[v];
+    if (!PACKED && p.dinitial && at.rank == 0)
+        for (int c = threadIdx.x; c < back.width && at.first + c < p.dim; c += blockDim.x)
+            static_cast<A*>(p.dinitial)[b * p.dim + at.first + c] = back.run[c];
 }
 
 // dgate[row, h] = sum of the `count` partial sums of gate h, in their order.
@@ -675,9 +762,9 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(const RecurrenceAr
     for (int v = 0; v < V; ++v) {
         A a, rest, u = widen(x.v[v]);
         const A t = widen(g.v[SHARED ? 0 : v]);
-        if (p.form == kGateValue) gate_factors<kGateValue>(t, a, rest);
-        else if (p.form == kGateLog) gate_factors<kGateLog>(t, a, rest);
-        else gate_factors<kGateLogit>(t, a, rest);
+        if (p.form == kGateValue) gate_factors<kGateValue, sizeof(G) == 2>(t, a, rest);
+        else if (p.form == kGateLog) gate_factors<kGateLog, sizeof(G) == 2>(t, a, rest);
+        else gate_factors<kGateLogit, sizeof(G) == 2>(t, a, rest);
         if (p.complement) u *= rest;
         h.v[v] = fma_(a, h.v[v], u);
         y.v[v] = narrow<X>(h.v[v]);

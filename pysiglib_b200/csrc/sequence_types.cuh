@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace sigb200 {
 
@@ -28,6 +29,30 @@ template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {
     T v[V];
 };
+
+// V results rounded to T; pairs of 16-bit values by one conversion.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> narrow_pack(const Acc<T> (&v)[V]) {
+    Pack<T, V> r;
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const __half2 two = __floats2half2_rn(v[i], v[i + 1]);
+                r.v[i] = __low2half(two);
+                r.v[i + 1] = __high2half(two);
+            } else {
+                const __nv_bfloat162 two = __floats2bfloat162_rn(v[i], v[i + 1]);
+                r.v[i] = __low2bfloat16(two);
+                r.v[i + 1] = __high2bfloat16(two);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[i] = narrow<T>(v[i]);
+    }
+    return r;
+}
 
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
