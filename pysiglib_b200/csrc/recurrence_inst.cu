@@ -13,12 +13,32 @@ namespace {
 template <typename X> constexpr int kWide = sizeof(X) == 8 ? 2 : 4;
 // Rows a thread holds: 8 forward; 4 backward where V > 1, as the five arrays of S * V values stay in registers.
 template <int V> constexpr int kBackwardRows = V == 1 ? 8 : 4;
-constexpr int kForwardRows = 8;
+#ifndef SIG_F32S
+#define SIG_F32S 4
+#endif
+template <typename X, int V> constexpr int kForwardRows = V > 1 && sizeof(X) > 2 ? SIG_F32S : 8;
+#ifndef SIG_SLOTS
+#define SIG_SLOTS 2
+#endif
+#ifndef SIG_LINE
+#define SIG_LINE 128
+#endif
 
 int log2_ceil(uint64_t n) {
     int k = 0;
     while ((1ull << k) < n) ++k;
     return k;
+}
+
+// Whether the inputs' rows and the cuts between groups of `bytes` of their channels are aligned to `bytes`
+// (a shared gate's are not cut).
+bool aligned_to(const RecurrenceArgs& p, size_t bytes) {
+    const auto fits = [&](const void* ptr, size_t size, uint64_t width, uint64_t batch, uint64_t row) {
+        return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && width * size % bytes == 0 && batch * size % bytes == 0 && row * size % bytes == 0;
+    };
+    const size_t e = element_size(p.type);
+    return fits(p.x, e, p.dim, p.x_batch, p.x_row) && fits(p.derivs, e, p.dim, p.d_batch, p.d_row) &&
+           (p.gate_dim != p.dim || fits(p.gate, element_size(p.gate_type), p.dim, p.gate_batch, p.gate_row));
 }
 
 // Up to 8 warps whose lanes lie side by side in the channels as far as 128 bytes of a row go (full lines, and
@@ -27,15 +47,16 @@ template <typename X>
 RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     const int columns = log2_ceil((p.dim + V - 1) / V), needed = log2_ceil((p.rows + S - 1) / S);
     RecurrencePlan plan{};
-    plan.log_lanes = std::min({columns, log2_ceil(128 / (V * sizeof(X))), 5});
+    plan.log_lanes = std::min({columns, log2_ceil(SIG_LINE / (V * sizeof(X))), 5});
     // short inputs: no more parts than there are rows for, the lanes go to the channels instead
     plan.log_lanes = std::max(plan.log_lanes, std::min(columns, 5 - std::min(needed, 5)));
     plan.warps = 1 << std::min(3, std::max(0, needed - (5 - plan.log_lanes)));
+    plan.pairs = plan.log_lanes > 0 && aligned_to(p, 16);
     const uint64_t lanes = 1ull << plan.log_lanes;
     const uint64_t strips = ((p.dim + V - 1) / V + lanes - 1) / lanes;
     const uint64_t span = uint64_t(plan.warps) * (32 >> plan.log_lanes) * S;
     // two CTAs an SM at a time: share strips while that many are not there, as long as every CTA has rows
-    const uint64_t slots = 2 * uint64_t(device_context(current_device()).sm_count);
+    const uint64_t slots = SIG_SLOTS * uint64_t(device_context(current_device()).sm_count);
     plan.cluster = 1;
     while (plan.cluster < 8 && p.batch * strips * plan.cluster * 2 <= slots && span * plan.cluster < p.rows) plan.cluster *= 2;
     if (strips * plan.cluster > 0x7fffffffull / p.batch)
@@ -69,12 +90,12 @@ void launch(void (*kernel)(Params...), const RecurrenceArgs& p, const Recurrence
 
 template <typename X, typename G, int V, bool SHARED>
 void forward(const RecurrenceArgs& p, cudaStream_t stream) {
-    const RecurrencePlan plan = make_plan<X>(p, V, kForwardRows);
-    const int threads = 32 * plan.warps;
-    const size_t smem = Prefetch<X, V, kForwardRows>::smem(threads) + (Prefetch<G, SHARED ? 1 : V, kForwardRows>::smem(threads) + 15) / 16 * 16 +
+    const RecurrencePlan plan = make_plan<X>(p, V, kForwardRows<X, V>);
+    using Ring = Stages<X, G, V, SHARED ? 1 : V, kForwardRows<X, V>, 1>;
+    const size_t smem = Ring::kCount * Ring::kBytes +
                         ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, plan.cluster);
-    if (p.sequences) launch(recurrence_forward_kernel<X, G, V, kForwardRows, SHARED, true>, p, plan, smem, stream);
-    else launch(recurrence_forward_kernel<X, G, V, kForwardRows, SHARED, false>, p, plan, smem, stream);
+    if (p.sequences) launch(recurrence_forward_kernel<X, G, V, kForwardRows<X, V>, SHARED, true>, p, plan, smem, stream);
+    else launch(recurrence_forward_kernel<X, G, V, kForwardRows<X, V>, SHARED, false>, p, plan, smem, stream);
     check("linear recurrence kernel");
 }
 
@@ -91,11 +112,16 @@ void backward(const RecurrenceArgs& p, cudaStream_t stream) {
     const uint64_t n = p.batch * p.rows * p.gate_dim;
     Scratch scratch(per_gate > 1 ? checked_mul(n, per_gate * sizeof(Acc<X>), "linear_recurrence_backprop") : 0, stream);
     if (per_gate > 1) partial = scratch.as<Acc<X>>();
-    const int threads = 32 * plan.warps;
-    const size_t smem = 2 * Prefetch<X, V, S>::smem(threads) + (Prefetch<G, SHARED ? 1 : V, S>::smem(threads) + 15) / 16 * 16 +
+    using Ring = Stages<X, G, V, SHARED ? 1 : V, S, 2>;
+    const size_t smem = Ring::kCount * (Ring::kBytes + sizeof(Acc<X>) * (V << plan.log_lanes)) +
                         ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, 1) + ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, plan.cluster);
-    if (p.sequences) launch(recurrence_backward_kernel<X, G, V, S, SHARED, true>, p, plan, smem, stream, partial);
-    else launch(recurrence_backward_kernel<X, G, V, S, SHARED, false>, p, plan, smem, stream, partial);
+    if (p.complement) {
+        if (p.sequences) launch(recurrence_backward_kernel<X, G, V, S, SHARED, true, true>, p, plan, smem, stream, partial);
+        else launch(recurrence_backward_kernel<X, G, V, S, SHARED, false, true>, p, plan, smem, stream, partial);
+    } else {
+        if (p.sequences) launch(recurrence_backward_kernel<X, G, V, S, SHARED, true, false>, p, plan, smem, stream, partial);
+        else launch(recurrence_backward_kernel<X, G, V, S, SHARED, false, false>, p, plan, smem, stream, partial);
+    }
     check("linear recurrence backward kernel");
     if (partial) {
         if (n / 256 >= 0x7fffffffull) throw std::invalid_argument("linear_recurrence_backprop: problem too large for one kernel launch");

@@ -35,6 +35,7 @@ struct RecurrencePlan {
     int warps;         // W
     int cluster;       // CTAs that share a strip
     unsigned strips;   // strips of CL * V channels
+    bool pairs;        // 8-byte neighbours are aligned to 16 bytes in every array
     int fold_log;      // backward, shared gates: lanes folded into one partial sum, log2
 };
 
@@ -103,38 +104,49 @@ __device__ __forceinline__ int64_t sequence_of(SequenceWalk walk, int64_t row) {
     return walk.seq;
 }
 
-// a and 1 - a, neither by cancellation: exp and expm1 for logarithms; for logits a = 1 / (1 + e^-v), and 1 - a
-// is e^-v a where v > 0.  The reciprocal is the hardware's (within 1 ulp; a = 0 for e^-v = inf).
-// FAST (gates of 16 bits): e^-v as 2^(-v log2 e) in single precision, off by up to 2 + 1.2 |v| ulp.  A gate of
-// 8 or 11 bits leaves e^-v uncertain by |v| 2^-9 or 2^-12 of itself, thousands of times more.
+// a and 1 - a, neither by cancellation: exp and expm1 for logarithms; for logits, with e = e^-v kept finite,
+// a = 1 / (1 + e) and 1 - a = e a.  The reciprocal is the hardware's (within 1 ulp).
+// FAST (gates of 16 bits): exponentials as 2^(v log2 e) in single precision, off by up to 2 + 1.2 |v| ulp.  A gate
+// of 8 or 11 bits leaves e^v uncertain by |v| 2^-9 or 2^-12 of itself, thousands of times more.
+__device__ __forceinline__ float exponential(float v, bool fast) {
+    if (!fast) return expf(v);
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.4426950408889634f));
+    return r;
+}
+__device__ __forceinline__ double exponential(double v, bool) { return exp(v); }
+__device__ __forceinline__ float minus_expm1(float v) { return -expm1f(v); }
+__device__ __forceinline__ double minus_expm1(double v) { return -expm1(v); }
+__device__ __forceinline__ float below(float v) {  // at most 2^100, NaN kept
+    float r;
+    asm("min.NaN.f32 %0, %1, 0f71800000;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ double below(double v) { return v > 0x1p1000 ? 0x1p1000 : v; }
 __device__ __forceinline__ float reciprocal(float v) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-template <int FORM, bool FAST>
-__device__ __forceinline__ void gate_factors(float v, float& a, float& rest) {
-    if (FORM == kGateValue) { a = v; rest = 1.0f - v; }
-    else if (FORM == kGateLog) { a = FAST ? __expf(v) : expf(v); rest = -expm1f(v); }
+__device__ __forceinline__ double reciprocal(double v) { return 1.0 / v; }
+template <int FORM, bool FAST, typename A>
+__device__ __forceinline__ void gate_factors(A v, A& a, A& rest) {
+    if (FORM == kGateValue) { a = v; rest = A(1) - v; }
+    else if (FORM == kGateLog) { a = exponential(v, FAST); rest = minus_expm1(v); }
     else {
-        const float e = FAST ? __expf(-v) : expf(-v);
-        a = reciprocal(1.0f + e);
-        rest = v > 0.0f ? e * a : 1.0f - a;
-    }
-}
-template <int FORM, bool FAST>
-__device__ __forceinline__ void gate_factors(double v, double& a, double& rest) {
-    if (FORM == kGateValue) { a = v; rest = 1.0 - v; }
-    else if (FORM == kGateLog) { a = exp(v); rest = -expm1(v); }
-    else {
-        const double e = exp(-v);
-        a = 1.0 / (1.0 + e);
-        rest = v > 0.0 ? e * a : 1.0 - a;
+        const A e = below(exponential(-v, FAST));
+        a = reciprocal(A(1) + e);
+        rest = e * a;
     }
 }
 
 __device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_(double a, double b, double c) { return fma(a, b, c); }
+
+#ifndef SIG_ROOM
+#define SIG_ROOM 100
+#endif
+constexpr int kCtaThreads = 256;  // at most; also the stride of the prefetch slots
 
 // One copy of B bytes (4, 8 or 16) to shared memory, asynchronous; `on` false writes zeros.
 template <int B>
@@ -144,32 +156,84 @@ __device__ __forceinline__ void copy_async(void* to, const void* from, bool on) 
     if constexpr (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(bytes) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(at), "l"(from), "n"(B), "r"(bytes) : "memory");
 }
+template <int B>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+    const unsigned at = static_cast<unsigned>(__cvta_generic_to_shared(to));
+    if constexpr (B == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(B) : "memory");
+}
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void await_copies() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+// until all groups of the warp but the last N are there
+template <int N>
+__device__ __forceinline__ void await_copies() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    __syncwarp();
+}
 
-// The next iteration's S rows of V values of one array.  4 bytes and more go asynchronously to
-// slot [row][thread] of shared memory; single 16-bit values, which that copy does not know, to registers.
-// Rows from `count` on read as zero.
+// The coming iterations' S rows of V values of one array.  4 bytes and more go asynchronously to
+// slot [stage][row][thread] of shared memory; single 16-bit values, which that copy does not know, to
+// registers, one iteration ahead.  Rows from `count` on read as zero (as anything, where there are none).
+// Copies of less than 16 bytes pass through L1, whose free part bounds how many are in flight.  Where 8-byte
+// neighbours are aligned as a pair, the even thread therefore copies both of an even row and the odd thread
+// both of an odd row; a warp reads only what its own threads copied.
 template <typename T, int V, int S>
 struct Prefetch {
     static constexpr int kBytes = sizeof(T) * V;
-    static constexpr bool kShared = kBytes >= 4;
-    __host__ __device__ static constexpr size_t smem(int threads) { return kShared ? size_t(kBytes) * S * threads : 0; }
+    static constexpr bool kShared = kBytes >= 4, kPairs = V > 1 && kBytes == 8;
+    static constexpr size_t kStage = kShared ? size_t(kBytes) * S * kCtaThreads : 0;
     Pack<T, V> held[kShared ? 1 : S];
     Pack<T, V>* slot;
+    int odd;     // pairs: 1 for the thread that copies the odd rows
+    bool pairs;
 
-    __device__ __forceinline__ void issue(const T* base, const T* from, int64_t stride, int count) {
+    __device__ __forceinline__ void place(unsigned char* at, int tc, bool in_pairs) {
+        slot = reinterpret_cast<Pack<T, V>*>(at) + threadIdx.x;
+        pairs = kPairs && in_pairs;
+        odd = pairs ? tc & 1 : 0;
+    }
+    // where this thread's copies of the rows from `first` on start
+    __device__ __forceinline__ const T* start(const T* first, int64_t stride) const { return odd ? first + stride - V : first; }
+
+    __device__ __forceinline__ void issue(int stage, const T* base, const T* from, int64_t stride, int count) {
+        if constexpr (kShared) {
+            Pack<T, V>* to = slot + stage * S * kCtaThreads;
+            if (kPairs && pairs) {
+                to += odd * (kCtaThreads - 1);
+                const int left = count - odd;
+                stride *= 2;
+                if (count == S) {
 #pragma unroll
-        for (int s = 0; s < S; ++s, from += stride) {
-            const bool on = s < count;
-            if constexpr (kShared) copy_async<kBytes>(slot + s * blockDim.x, on ? from : base, on);
-            else held[s] = on ? *reinterpret_cast<const Pack<T, V>*>(from) : Pack<T, V>{};
+                    for (int s = 0; s < S; s += 2, from += stride) copy_async<16>(to + s * kCtaThreads, from);
+                } else if (count > 0) {
+#pragma unroll
+                    for (int s = 0; s < S; s += 2, from += stride) copy_async<16>(to + s * kCtaThreads, s < left ? from : base, s < left);
+                }
+            } else if (count == S) {
+#pragma unroll
+                for (int s = 0; s < S; ++s, from += stride) copy_async<kBytes>(to + s * kCtaThreads, from);
+            } else if (count > 0) {
+#pragma unroll
+                for (int s = 0; s < S; ++s, from += stride) copy_async<kBytes>(to + s * kCtaThreads, s < count ? from : base, s < count);
+            }
         }
     }
-    __device__ __forceinline__ Pack<T, V> take(int s) const {
-        if constexpr (kShared) return slot[s * blockDim.x];
+    __device__ __forceinline__ void hold(const T* from, int64_t stride, int count) {
+        if constexpr (!kShared) {
+#pragma unroll
+            for (int s = 0; s < S; ++s, from += stride) held[s] = s < count ? *reinterpret_cast<const Pack<T, V>*>(from) : Pack<T, V>{};
+        }
+    }
+    __device__ __forceinline__ Pack<T, V> take(int stage, int s) const {
+        if constexpr (kShared) return slot[(stage * S + s) * kCtaThreads];
         else return held[s];
     }
+};
+
+// Iterations whose inputs are in shared memory or on their way: as many as two CTAs an SM have room for.
+template <typename X, typename G, int V, int GV, int S, int ARRAYS>
+struct Stages {
+    static constexpr size_t kBytes = ARRAYS * Prefetch<X, V, S>::kStage + Prefetch<G, GV, S>::kStage;
+    static constexpr int kCount = kBytes * 4 <= SIG_ROOM * 1024 ? 4 : kBytes * 3 <= SIG_ROOM * 1024 ? 3 : 2;
 };
 
 // The affine map of a run of rows on V channels; `drop`: what enters the run does not leave it.
@@ -305,12 +369,12 @@ __device__ __forceinline__ void carry_across(const ScanMemory<A>& m, int warps, 
 
 // a, x and, where REST, 1 - a of S rows from the prefetched inputs; without REST x is b already.
 template <int FORM, bool REST, bool COMPLEMENT, typename X, typename G, int V, int GV, int S, typename A>
-__device__ __forceinline__ void factors(const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, A (&a)[S][V],
+__device__ __forceinline__ void factors(const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, int stage, A (&a)[S][V],
                                         A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        const Pack<X, V> x = fx.take(s);
-        const Pack<G, GV> g = fg.take(s);
+        const Pack<X, V> x = fx.take(stage, s);
+        const Pack<G, GV> g = fg.take(stage, s);
         A ga[GV], gr[GV];
 #pragma unroll
         for (int v = 0; v < GV; ++v) gate_factors<FORM, sizeof(G) == 2>(A(widen(g.v[v])), ga[v], gr[v]);
@@ -325,11 +389,11 @@ __device__ __forceinline__ void factors(const Prefetch<X, V, S>& fx, const Prefe
 }
 
 template <bool REST, bool COMPLEMENT, typename X, typename G, int V, int GV, int S, typename A>
-__device__ __forceinline__ void factors(int form, const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, A (&a)[S][V],
+__device__ __forceinline__ void factors(int form, const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, int stage, A (&a)[S][V],
                                         A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
-    if (form == kGateValue) factors<kGateValue, REST, COMPLEMENT>(fx, fg, a, u, rest);
-    else if (form == kGateLog) factors<kGateLog, REST, COMPLEMENT>(fx, fg, a, u, rest);
-    else factors<kGateLogit, REST, COMPLEMENT>(fx, fg, a, u, rest);
+    if (form == kGateValue) factors<kGateValue, REST, COMPLEMENT>(fx, fg, stage, a, u, rest);
+    else if (form == kGateLog) factors<kGateLog, REST, COMPLEMENT>(fx, fg, stage, a, u, rest);
+    else factors<kGateLogit, REST, COMPLEMENT>(fx, fg, stage, a, u, rest);
 }
 
 // Where a thread stands: its strip, channels and rows.
@@ -361,9 +425,9 @@ __device__ __forceinline__ int rows_left(int64_t rows, int64_t row0, int most, b
 }
 
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED>
-__global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
+__global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
     using A = Acc<X>;
-    constexpr int GV = SHARED ? 1 : V;
+    constexpr int GV = SHARED ? 1 : V, kStages = Stages<X, G, V, GV, S, 1>::kCount;
     extern __shared__ __align__(16) unsigned char smem[];
     const Place at(plan, p.dim, V);
     const uint64_t b = at.batch, c0 = at.c0;
@@ -377,10 +441,10 @@ __global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const Recurr
     Prefetch<X, V, S> fx;
     Prefetch<G, GV, S> fg;
     unsigned char* next = smem;
-    fx.slot = reinterpret_cast<Pack<X, V>*>(next) + threadIdx.x;
-    next += fx.smem(blockDim.x);
-    fg.slot = reinterpret_cast<Pack<G, GV>*>(next) + threadIdx.x;
-    next += (fg.smem(blockDim.x) + 15) / 16 * 16;
+    fx.place(next, at.tc, plan.pairs);
+    next += kStages * fx.kStage;
+    fg.place(next, at.tc, plan.pairs);
+    next += kStages * fg.kStage;
     ScanMemory<A> memory;
     memory.place(next, at.lanes * V, plan.warps, at.cluster);
     for (int c = threadIdx.x; c < memory.width; c += blockDim.x)
@@ -395,26 +459,43 @@ __global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const Recurr
     const X* x = static_cast<const X*>(p.x) + b * p.x_batch + (live ? c0 : 0);
     const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
     const int64_t x_row = int64_t(p.x_row), gate_row = int64_t(p.gate_row);
-    const X* px = x + row0 * x_row;
-    const G* pg = gate + row0 * gate_row;
+    const int64_t x_span = span * x_row, gate_span = span * gate_row;
+    const X* px = fx.start(x + row0 * x_row, x_row);
+    const G* pg = fg.start(gate + row0 * gate_row, gate_row);
     X* out = p.out ? static_cast<X*>(p.out) + (b * p.rows + row0) * p.dim + c0 : nullptr;
-    int count = rows_left(rows, row0, S, live);
-    fx.issue(x, px, x_row, count);
-    fg.issue(gate, pg, gate_row, count);
-    commit_copies();
+    int64_t coming = row0;  // the row that the next copies are for
+    const auto fetch = [&](int stage) {
+        const int n = rows_left(rows, coming, S, live);
+        fx.issue(stage, x, px, x_row, n);
+        fg.issue(stage, gate, pg, gate_row, n);
+        commit_copies();
+        px += x_span;
+        pg += gate_span;
+        coming += span;
+    };
+    const auto hold = [&](int64_t row) {
+        const int n = rows_left(rows, row, S, live);
+        fx.hold(x + row * x_row, x_row, n);
+        fg.hold(gate + row * gate_row, gate_row, n);
+    };
+    for (int k = 0; k < kStages - 1; ++k) fetch(k);
+    hold(row0);
     SequenceWalk walk;
     if (PACKED) walk.seek(p.offsets, p.wide_offsets, p.sequences, row0);
-    int turn = 0;
-    for (int64_t base = 0; base < rows; base += span, row0 += span, turn ^= 1) {
+    int turn = 0, stage = 0;
+    for (int64_t base = 0; base < rows; base += span, row0 += span, turn ^= 1, stage = stage + 1 == kStages ? 0 : stage + 1) {
+        const int count = rows_left(rows, row0, S, live);
+        fetch(stage == 0 ? kStages - 1 : stage - 1);  // its slots were read in the last iteration, before a barrier
         RowEvents e;
         if (PACKED) {
             walk.advance(row0);
             e = row_events<S>(walk, row0, rows);
         }
         A a[S][V], u[S][V], unused[1][V];
-        await_copies();
-        if (p.complement) factors<false, true>(p.form, fx, fg, a, u, unused);
-        else factors<false, false>(p.form, fx, fg, a, u, unused);
+        await_copies<kStages - 1>();
+        if (p.complement) factors<false, true>(p.form, fx, fg, stage, a, u, unused);
+        else factors<false, false>(p.form, fx, fg, stage, a, u, unused);
+        hold(row0 + span);
         if (count < S || (PACKED && e.dead)) {
 #pragma unroll
             for (int s = 0; s < S; ++s)
@@ -457,14 +538,6 @@ __global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const Recurr
         __syncwarp();
         scan_warp<A, V, false, PACKED>(m, plan.log_lanes, memory);
         __syncthreads();
-        // the slots were read before the barrier: the next rows may come
-        px += span * x_row;
-        pg += span * gate_row;
-        const int now = count;
-        count = rows_left(rows, row0 + span, S, live);
-        fx.issue(x, px, x_row, count);
-        fg.issue(gate, pg, gate_row, count);
-        commit_copies();
         if (at.cluster == 1) {
             for (int c = threadIdx.x; c < memory.width; c += blockDim.x)
                 memory.run[c] = carry_through<A, false, PACKED>(memory, plan.warps, c, memory.run[c]);
@@ -472,7 +545,7 @@ __global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const Recurr
             carry_across<A, false, PACKED>(memory, plan.warps, at.cluster, at.rank, turn);
         }
         __syncthreads();
-        if (now) {
+        if (count) {
             const Pack<A, V> in = load_pack<A, V>(memory.carry + at.warp * memory.width + at.tc * V);
             A h[V];
 #pragma unroll
@@ -483,11 +556,21 @@ __global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const Recurr
                 for (int v = 0; v < V; ++v) marks[row0 / int64_t(kCheckpointRows) * dim + v] = h[v];
             if (!events) {
                 X* to = out;
+                const int stored = out ? count : 0;
+                if (stored == S) {
 #pragma unroll
-                for (int s = 0; s < S; ++s, to += dim) {
+                    for (int s = 0; s < S; ++s, to += dim) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) h[v] = fma_(a[s][v], h[v], u[s][v]);
-                    if (out && s < now) store_pack<X, V>(to, narrow_pack<X, V>(h));
+                        for (int v = 0; v < V; ++v) h[v] = fma_(a[s][v], h[v], u[s][v]);
+                        store_pack<X, V>(to, narrow_pack<X, V>(h));
+                    }
+                } else {
+#pragma unroll
+                    for (int s = 0; s < S; ++s, to += dim) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) h[v] = fma_(a[s][v], h[v], u[s][v]);
+                        if (s < stored) store_pack<X, V>(to, narrow_pack<X, V>(h));
+                    }
                 }
             } else {
 #pragma unroll
@@ -498,7 +581,7 @@ __global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const Recurr
                         h[v] = e.starts >> s & 1u ? u[s][v] : fma_(a[s][v], h[v], u[s][v]);
                         y[v] = e.dead >> s & 1u ? A(0) : h[v];
                     }
-                    if (out && s < now) store_pack<X, V>(out + s * dim, narrow_pack<X, V>(y));
+                    if (out && s < count) store_pack<X, V>(out + s * dim, narrow_pack<X, V>(y));
                     if (state && (e.ends >> s & 1u)) {
                         A* to = state + sequence_of(walk, row0 + s) * dim;
 #pragma unroll
@@ -518,11 +601,11 @@ __global__ void __launch_bounds__(256, 2) recurrence_forward_kernel(const Recurr
 // registers, so that x, the gates and the derivatives are read once and h, rounded or not, is not read at all.
 // Shared gates: each thread sums its V channels, 1 << fold_log neighbouring lanes are folded by shuffles,
 // and `partial` takes one value per row and fold (dgate itself where a fold is a whole gate).
-template <typename X, typename G, int V, int S, bool SHARED, bool PACKED>
-__global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const RecurrenceArgs p, const RecurrencePlan plan,
+template <typename X, typename G, int V, int S, bool SHARED, bool PACKED, bool COMPLEMENT>
+__global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(const RecurrenceArgs p, const RecurrencePlan plan,
                                                                      Acc<X>* partial) {
     using A = Acc<X>;
-    constexpr int GV = SHARED ? 1 : V;
+    constexpr int GV = SHARED ? 1 : V, kStages = Stages<X, G, V, GV, S, 2>::kCount;
     extern __shared__ __align__(16) unsigned char smem[];
     const Place at(plan, p.dim, V);
     const uint64_t b = at.batch, c0 = at.c0;
@@ -536,15 +619,17 @@ __global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const Recur
     Prefetch<X, V, S> fx, fd;
     Prefetch<G, GV, S> fg;
     unsigned char* next = smem;
-    fx.slot = reinterpret_cast<Pack<X, V>*>(next) + threadIdx.x;
-    fd.slot = fx.slot + S * blockDim.x;
-    next += 2 * fx.smem(blockDim.x);
-    fg.slot = reinterpret_cast<Pack<G, GV>*>(next) + threadIdx.x;
-    next += (fg.smem(blockDim.x) + 15) / 16 * 16;
+    fx.place(next, at.tc, plan.pairs);
+    next += kStages * fx.kStage;
+    fd.place(next, at.tc, plan.pairs);
+    next += kStages * fd.kStage;
+    fg.place(next, at.tc, plan.pairs);
+    next += kStages * fg.kStage;
     ScanMemory<A> ahead, back;
     ahead.place(next, at.lanes * V, plan.warps, 1);
     next += ScanMemory<A>::bytes(ahead.width, plan.warps, 1);
     back.place(next, ahead.width, plan.warps, at.cluster);
+    A* entering = reinterpret_cast<A*>(next + ScanMemory<A>::bytes(ahead.width, plan.warps, at.cluster));  // [stage][width]
     for (int c = threadIdx.x; c < back.width; c += blockDim.x)
         back.run[c] = !PACKED && p.state_derivs && at.first + c < p.dim ? static_cast<const A*>(p.state_derivs)[b * p.dim + at.first + c] : A(0);
     if (PACKED && dinitial && live && at.rank == 0)
@@ -558,41 +643,58 @@ __global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const Recur
     const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
     const X* derivs = static_cast<const X*>(p.derivs) + b * p.d_batch + (live ? c0 : 0);
     const int64_t x_row = int64_t(p.x_row), gate_row = int64_t(p.gate_row), d_row = int64_t(p.d_row);
-    const X* px = x + row0 * x_row;
-    const G* pg = gate + row0 * gate_row;
-    const X* pd = derivs + row0 * d_row;
-    // the checkpoint that enters the CTA's rows: each column's thread copies its own
-    const auto fetch_marks = [&](int64_t own) {
+    const int64_t x_span = span * x_row, gate_span = span * gate_row, d_span = span * d_row;
+    const X* px = fx.start(x + row0 * x_row, x_row);
+    const G* pg = fg.start(gate + row0 * gate_row, gate_row);
+    const X* pd = fd.start(derivs + row0 * d_row, d_row);
+    int64_t coming = row0, coming_base = base;
+    const auto fetch = [&](int stage) {
+        const int n = rows_left(rows, coming, S, live);
+        fx.issue(stage, x, px, x_row, n);
+        fg.issue(stage, gate, pg, gate_row, n);
+        fd.issue(stage, derivs, pd, d_row, n);
+        // the checkpoint that enters the CTA's rows: each column's thread copies its own
+        const int64_t own = coming_base + at.rank * block;
         for (int c = threadIdx.x; c < ahead.width; c += blockDim.x) {
             const bool on = own >= 0 && own < rows && at.first + c < p.dim;
-            const A* from = static_cast<const A*>(p.marks);
-            copy_async<sizeof(A)>(ahead.run + c, on ? marks + own / int64_t(kCheckpointRows) * dim + c : from, on);
+            copy_async<sizeof(A)>(entering + stage * ahead.width + c, on ? marks + own / int64_t(kCheckpointRows) * dim + c : static_cast<const A*>(p.marks), on);
         }
+        commit_copies();
+        px -= x_span;
+        pg -= gate_span;
+        pd -= d_span;
+        coming -= span;
+        coming_base -= span;
     };
-    int count = rows_left(rows, row0, S, live);
-    fx.issue(x, px, x_row, count);
-    fg.issue(gate, pg, gate_row, count);
-    fd.issue(derivs, pd, d_row, count);
-    fetch_marks(base + at.rank * block);
-    commit_copies();
+    const auto hold = [&](int64_t row) {
+        const int n = rows_left(rows, row, S, live);
+        fx.hold(x + row * x_row, x_row, n);
+        fg.hold(gate + row * gate_row, gate_row, n);
+        fd.hold(derivs + row * d_row, d_row, n);
+    };
+    for (int k = 0; k < kStages - 1; ++k) fetch(k);
+    hold(row0);
     SequenceWalk walk;
     if (PACKED) walk.seek(p.offsets, p.wide_offsets, p.sequences, row0);
-    int turn = 0;
-    for (; base >= 0; base -= span, row0 -= span, turn ^= 1) {
+    int turn = 0, stage = 0;
+    for (; base >= 0; base -= span, row0 -= span, turn ^= 1, stage = stage + 1 == kStages ? 0 : stage + 1) {
+        const int count = rows_left(rows, row0, S, live);
+        fetch(stage == 0 ? kStages - 1 : stage - 1);  // its slots were read in the last iteration, before a barrier
         RowEvents e;
         if (PACKED) {
             walk.retreat(row0);
             e = row_events<S>(walk, row0, rows);
         }
         A a[S][V], rest[S][V], x_[S][V], d[S][V];
-        await_copies();
-        factors<true, false>(p.form, fx, fg, a, x_, rest);
+        await_copies<kStages - 1>();
+        factors<true, false>(p.form, fx, fg, stage, a, x_, rest);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const Pack<X, V> rd = fd.take(s);
+            const Pack<X, V> rd = fd.take(stage, s);
 #pragma unroll
             for (int v = 0; v < V; ++v) d[s][v] = widen(rd.v[v]);
         }
+        hold(row0 - span);
         if (count < S || (PACKED && e.dead)) {
 #pragma unroll
             for (int s = 0; s < S; ++s)
@@ -615,7 +717,7 @@ __global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const Recur
         Map<A, V> m, g;
         m.clear();
         g.clear();
-        const auto input = [&](int s, int v) { return p.complement ? rest[s][v] * x_[s][v] : x_[s][v]; };
+        const auto input = [&](int s, int v) { return COMPLEMENT ? rest[s][v] * x_[s][v] : x_[s][v]; };
         if (!events) {
 #pragma unroll
             for (int s = 0; s < S; ++s)
@@ -651,7 +753,7 @@ __global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const Recur
         scan_warp<A, V, false, PACKED>(m, plan.log_lanes, ahead);
         scan_warp<A, V, true, PACKED>(g, plan.log_lanes, back);
         __syncthreads();
-        for (int c = threadIdx.x; c < ahead.width; c += blockDim.x) carry_through<A, false, PACKED>(ahead, plan.warps, c, ahead.run[c]);
+        for (int c = threadIdx.x; c < ahead.width; c += blockDim.x) carry_through<A, false, PACKED>(ahead, plan.warps, c, entering[stage * ahead.width + c]);
         if (at.cluster == 1) {
             for (int c = threadIdx.x; c < back.width; c += blockDim.x)
                 back.run[c] = carry_through<A, true, PACKED>(back, plan.warps, c, back.run[c]);
@@ -659,17 +761,6 @@ __global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const Recur
             carry_across<A, true, PACKED>(back, plan.warps, at.cluster, at.rank, turn);
         }
         __syncthreads();
-        // the slots and the checkpoint were read before the barrier: the rows before these may come
-        px -= span * x_row;
-        pg -= span * gate_row;
-        pd -= span * d_row;
-        const int now = count;
-        count = rows_left(rows, row0 - span, S, live);
-        fx.issue(x, px, x_row, count);
-        fg.issue(gate, pg, gate_row, count);
-        fd.issue(derivs, pd, d_row, count);
-        fetch_marks(base - span + at.rank * block);
-        commit_copies();
         A in[V], w[V];
         {
             const Pack<A, V> first = load_pack<A, V>(ahead.carry + at.warp * ahead.width + at.tc * V);
@@ -706,24 +797,24 @@ __global__ void __launch_bounds__(256, 2) recurrence_backward_kernel(const Recur
             A gx[V], gg[V], sum = A(0);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                gx[v] = p.complement ? rest[s][v] * d[s][v] : d[s][v];
-                gg[v] = d[s][v] * (p.complement ? in[v] - x_[s][v] : in[v]);
+                gx[v] = COMPLEMENT ? rest[s][v] * d[s][v] : d[s][v];
+                gg[v] = d[s][v] * (COMPLEMENT ? in[v] - x_[s][v] : in[v]);
                 if (p.form != kGateValue) gg[v] *= a[s][v];
                 if (p.form == kGateLogit) gg[v] *= rest[s][v];
                 if (PACKED && (e.dead >> s & 1u)) gx[v] = gg[v] = A(0);
                 sum += gg[v];
                 in[v] = fma_(a[s][v], in[v], input(s, v));
             }
-            if (s < now) store_pack<X, V>(dx, narrow_pack<X, V>(gx));
+            if (s < count) store_pack<X, V>(dx, narrow_pack<X, V>(gx));
             if (SHARED) {
-                sum = s < now ? sum : A(0);
+                sum = s < count ? sum : A(0);
                 for (int k = 1; k < 1 << plan.fold_log; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-                if (s < now && (at.tc & ((1 << plan.fold_log) - 1)) == 0) {
+                if (s < count && (at.tc & ((1 << plan.fold_log) - 1)) == 0) {
                     const int64_t fold = int64_t(c0 / V) >> plan.fold_log, row = b * rows + row0 + s;
                     if (partial) partial[row * ((dim / V) >> plan.fold_log) + fold] = sum;
                     else dgate[row * int64_t(p.gate_dim) + fold] = narrow<G>(sum);
                 }
-            } else if (s < now) {
+            } else if (s < count) {
                 if constexpr (std::is_same_v<Acc<G>, A>) store_pack<G, V>(dgate, narrow_pack<G, V>(gg));
             }
         }
