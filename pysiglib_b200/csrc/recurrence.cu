@@ -30,10 +30,11 @@ Sizes checked(const RecurrenceArgs& p, const char* who) {
     if (!p.x || !p.gate) throw std::invalid_argument(name + " received a null pointer");
     if (p.sequences && (p.batch != 1 || !p.offsets))
         throw std::invalid_argument(name + ": packed sequences need offsets and a batch of 1");
+    if (p.rows >= kMaxRows || p.sequences >= kMaxRows) throw std::out_of_range(name + ": 2^30 rows or sequences and more are not supported");
     const uint64_t rows = checked_mul(p.batch, p.rows, who);
     Sizes s{};
     s.values = checked_mul(rows, p.dim, who);
-    if (s.values >= 1ull << 59 || p.sequences >= 1ull << 59) throw std::out_of_range(name + ": size overflow");
+    if (s.values >= 1ull << 59) throw std::out_of_range(name + ": size overflow");
     s.gates = rows * p.gate_dim;
     s.states = checked_mul(p.sequences ? p.sequences : p.batch, p.dim, who);
     s.marks = p.batch * ((p.rows + kCheckpointRows - 1) / kCheckpointRows) * p.dim;

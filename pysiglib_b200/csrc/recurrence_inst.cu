@@ -48,6 +48,11 @@ RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     const int columns = log2_ceil((p.dim + V - 1) / V), needed = log2_ceil((p.rows + S - 1) / S);
     RecurrencePlan plan{};
     plan.log_lanes = std::min({columns, log2_ceil(SIG_LINE / (V * sizeof(X))), 5});
+    // few strips: half and quarter lines, for as many CTAs as there are SMs and more
+    const uint64_t sms = device_context(current_device()).sm_count;
+    while ((V * sizeof(X)) << plan.log_lanes > 32 && plan.log_lanes > 0 &&
+           p.batch * (((p.dim + V - 1) / V + (1ull << plan.log_lanes) - 1) >> plan.log_lanes) * 8 < sms)
+        --plan.log_lanes;
     // short inputs: no more parts than there are rows for, the lanes go to the channels instead
     plan.log_lanes = std::max(plan.log_lanes, std::min(columns, 5 - std::min(needed, 5)));
     plan.warps = 1 << std::min(3, std::max(0, needed - (5 - plan.log_lanes)));
@@ -56,7 +61,7 @@ RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     const uint64_t strips = ((p.dim + V - 1) / V + lanes - 1) / lanes;
     const uint64_t span = uint64_t(plan.warps) * (32 >> plan.log_lanes) * S;
     // two CTAs an SM at a time: share strips while that many are not there, as long as every CTA has rows
-    const uint64_t slots = SIG_SLOTS * uint64_t(device_context(current_device()).sm_count);
+    const uint64_t slots = SIG_SLOTS * sms;
     plan.cluster = 1;
     while (plan.cluster < 8 && p.batch * strips * plan.cluster * 2 <= slots && span * plan.cluster < p.rows) plan.cluster *= 2;
     if (strips * plan.cluster > 0x7fffffffull / p.batch)
@@ -69,6 +74,10 @@ void check(const char* what) {
     count_launch();
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) throw CudaFailure(err, std::string(what) + ": " + cudaGetErrorString(err));
+}
+
+size_t offset_bytes(const RecurrenceArgs& p) {
+    return p.sequences && p.sequences < uint64_t(kLocalOffsets) ? (p.sequences + 1) * sizeof(int) : 0;
 }
 
 template <typename... Params, typename... Args>
@@ -93,7 +102,7 @@ void forward(const RecurrenceArgs& p, cudaStream_t stream) {
     const RecurrencePlan plan = make_plan<X>(p, V, kForwardRows<X, V>);
     using Ring = Stages<X, G, V, SHARED ? 1 : V, kForwardRows<X, V>, 1>;
     const size_t smem = Ring::kCount * Ring::kBytes +
-                        ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, plan.cluster);
+                        ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, plan.cluster) + offset_bytes(p);
     if (p.sequences) launch(recurrence_forward_kernel<X, G, V, kForwardRows<X, V>, SHARED, true>, p, plan, smem, stream);
     else launch(recurrence_forward_kernel<X, G, V, kForwardRows<X, V>, SHARED, false>, p, plan, smem, stream);
     check("linear recurrence kernel");
@@ -114,7 +123,8 @@ void backward(const RecurrenceArgs& p, cudaStream_t stream) {
     if (per_gate > 1) partial = scratch.as<Acc<X>>();
     using Ring = Stages<X, G, V, SHARED ? 1 : V, S, 2>;
     const size_t smem = Ring::kCount * (Ring::kBytes + sizeof(Acc<X>) * (V << plan.log_lanes)) +
-                        ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, 1) + ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, plan.cluster);
+                        ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, 1) +
+                        ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, plan.cluster) + offset_bytes(p);
     if (p.complement) {
         if (p.sequences) launch(recurrence_backward_kernel<X, G, V, S, SHARED, true, true>, p, plan, smem, stream, partial);
         else launch(recurrence_backward_kernel<X, G, V, S, SHARED, false, true>, p, plan, smem, stream, partial);

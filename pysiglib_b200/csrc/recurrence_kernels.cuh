@@ -25,6 +25,8 @@
 
 #include <cooperative_groups.h>
 
+#include <climits>
+
 #include "sequence.h"
 #include "sequence_types.cuh"
 
@@ -41,41 +43,56 @@ struct RecurrencePlan {
 
 namespace {
 
-__device__ __forceinline__ int64_t offset_at(const void* offsets, bool wide, int64_t i) {
-    return wide ? static_cast<const long long*>(offsets)[i] : static_cast<const int*>(offsets)[i];
+__device__ __forceinline__ int saturated(long long v) {
+    return v < INT_MIN ? INT_MIN : v > INT_MAX ? INT_MAX : int(v);
+}
+__device__ __forceinline__ int offset_at(const void* offsets, bool wide, int i) {
+    return wide ? saturated(static_cast<const long long*>(offsets)[i]) : static_cast<const int*>(offsets)[i];
 }
 
-// Walks the packed sequences along increasing rows.  `seq` is the last sequence whose offset is at or before
-// the row (-1 before the first, `count` behind the last); it spans rows [begin, next).  Offsets are only
-// compared with rows, so values that are out of order or out of range take no access out of bounds.
+// Offsets of packed sequences that a CTA keeps in shared memory, where there are no more of them.
+constexpr int kLocalOffsets = 512;
+
+// Walks the packed sequences along the rows.  `seq` is the last sequence whose offset is at or before the row
+// (-1 before the first, `count` behind the last); it spans rows [begin, next).  Offsets are only compared
+// with rows, so values that are out of order or out of range take no access out of bounds.
 struct SequenceWalk {
     const void* offsets;
-    int64_t count, seq, begin, next;
+    int count, seq, begin, next;
     bool wide;
 
     __device__ __forceinline__ void settle() {
-        begin = seq >= 0 ? offset_at(offsets, wide, seq) : INT64_MIN;
-        next = seq < count ? offset_at(offsets, wide, seq + 1) : INT64_MAX;
+        begin = seq >= 0 ? offset_at(offsets, wide, seq) : INT_MIN;
+        next = seq < count ? offset_at(offsets, wide, seq + 1) : INT_MAX;
     }
-    __device__ void seek(const void* o, bool w, int64_t n, int64_t row) {
-        offsets = o; wide = w; count = n;
-        int64_t lo = 0, hi = n + 1;  // first of the n + 1 offsets that is > row
+    __device__ void seek(int row) {
+        int lo = 0, hi = count + 1;  // first of the count + 1 offsets that is > row
         while (lo < hi) {
-            const int64_t mid = (lo + hi) >> 1;
-            if (offset_at(o, w, mid) <= row) lo = mid + 1; else hi = mid;
+            const int mid = (lo + hi) >> 1;
+            if (offset_at(offsets, wide, mid) <= row) lo = mid + 1; else hi = mid;
         }
         seq = lo - 1;
         settle();
     }
-    __device__ __forceinline__ void advance(int64_t row) {
-        while (next <= row) { ++seq; settle(); }
+    // all threads: copies the offsets to `local` where they fit (behind a barrier)
+    __device__ __forceinline__ void open(const RecurrenceArgs& p, int* local) {
+        offsets = p.offsets; wide = p.wide_offsets; count = int(p.sequences);
+        if (count + 1 <= kLocalOffsets) {
+            for (int i = threadIdx.x; i <= count; i += blockDim.x) local[i] = offset_at(p.offsets, p.wide_offsets, i);
+            __syncthreads();
+            offsets = local;
+            wide = false;
+        }
     }
-    __device__ __forceinline__ void retreat(int64_t row) {
-        while (begin > row) { --seq; settle(); }
+    __device__ __forceinline__ void advance(int row) {
+        while (next <= row && seq < count) { ++seq; settle(); }
+    }
+    __device__ __forceinline__ void retreat(int row) {
+        while (begin > row && seq >= 0) { --seq; settle(); }
     }
     __device__ __forceinline__ bool inside() const { return seq >= 0 && seq < count; }
     // no sequence starts or ends in [row, row + n), and all of those rows are in one
-    __device__ __forceinline__ bool quiet(int64_t row, int n) const { return inside() && begin < row && next > row + n; }
+    __device__ __forceinline__ bool quiet(int row, int n) const { return inside() && begin < row && next > row + n; }
 };
 
 // What happens in a thread's S rows, one bit a row: a sequence starts, a sequence ends, the row is in none.
@@ -84,7 +101,7 @@ struct RowEvents {
 };
 
 template <int S>
-__device__ __forceinline__ RowEvents row_events(SequenceWalk walk, int64_t row0, int64_t rows) {
+__device__ __forceinline__ RowEvents row_events(SequenceWalk walk, int row0, int rows) {
     RowEvents e;
     if (walk.quiet(row0, S)) return e;
     for (int s = 0; s < S && row0 + s < rows; ++s) {
@@ -99,7 +116,7 @@ __device__ __forceinline__ RowEvents row_events(SequenceWalk walk, int64_t row0,
 }
 
 // Sequence that row `row` belongs to, walking from a thread's first row.
-__device__ __forceinline__ int64_t sequence_of(SequenceWalk walk, int64_t row) {
+__device__ __forceinline__ int64_t sequence_of(SequenceWalk walk, int row) {
     walk.advance(row);
     return walk.seq;
 }
@@ -276,7 +293,7 @@ struct ScanMemory {
 };
 
 // Scan of the threads' maps over the parts of a warp (REVERSE: from the last part to the first).  On return
-// `m` is the map of everything in the warp that comes before this part; the whole warp's is in `memory`.
+// `m` is the map of this part and everything in the warp before it; the whole warp's is in `memory`.
 template <typename A, int V, bool REVERSE, bool PACKED>
 __device__ __forceinline__ void scan_warp(Map<A, V>& m, int log_lanes, const ScanMemory<A>& memory) {
     const int lane = threadIdx.x & 31, lanes = 1 << log_lanes, parts = 32 >> log_lanes;
@@ -306,12 +323,23 @@ __device__ __forceinline__ void scan_warp(Map<A, V>& m, int log_lanes, const Sca
         store_pack<A, V>(to + memory.width, b);
         if (PACKED && (lane & (lanes - 1)) == 0) memory.drops[threadIdx.x >> 5] = m.drop;
     }
-    if (parts > 1) {
+}
+
+// The state that enters this thread's rows, from the one that enters its warp's and the inclusive maps.
+template <typename A, int V, bool REVERSE>
+__device__ __forceinline__ void enter_rows(const Map<A, V>& m, int log_lanes, const A* carry, A (&h)[V]) {
+    const int lane = threadIdx.x & 31, lanes = 1 << log_lanes;
+    const Pack<A, V> in = load_pack<A, V>(carry);
+    A behind[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) { m.a[v] = from(m.a[v], lanes); m.b[v] = from(m.b[v], lanes); }
-        if (PACKED) m.drop = from(int(m.drop), lanes);
+    for (int v = 0; v < V; ++v) behind[v] = in.v[v];
+    m.apply(behind);
+    const bool first = REVERSE ? lane >= 32 - lanes : lane < lanes;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const A e = REVERSE ? __shfl_down_sync(0xffffffffu, behind[v], lanes) : __shfl_up_sync(0xffffffffu, behind[v], lanes);
+        h[v] = first ? in.v[v] : e;
     }
-    if (part == 0) m.clear();
 }
 
 // Column c of the strip, one thread each: the state `r` that enters the CTA's rows goes through the warps'
@@ -353,7 +381,12 @@ __device__ __forceinline__ void carry_across(const ScanMemory<A>& m, int warps, 
             if (PACKED && c == 0) group.map_shared_rank(drops, r)[rank] = drop;
         }
     }
-    group.sync();
+    // only the threads that wrote order their writes before the barrier: a release by all would wait for every
+    // thread's stores of outputs as well
+    if (threadIdx.x < m.width) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     for (int c = threadIdx.x; c < m.width; c += blockDim.x) {
         A r = m.run[c], mine = r;
         for (int i = 0; i < cluster; ++i) {
@@ -419,9 +452,10 @@ struct Place {
     }
 };
 
-__device__ __forceinline__ int rows_left(int64_t rows, int64_t row0, int most, bool live) {
-    const int64_t n = rows - row0;
-    return !live || row0 < 0 || n <= 0 ? 0 : n < most ? int(n) : most;
+// How many of the S rows from row0 on there are (row0 may lie before 0 as a whole).
+template <int S>
+__device__ __forceinline__ int rows_left(int rows, int row0, bool live) {
+    return live && row0 >= 0 ? max(0, min(S, rows - row0)) : 0;
 }
 
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED>
@@ -432,7 +466,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
     const Place at(plan, p.dim, V);
     const uint64_t b = at.batch, c0 = at.c0;
     const bool live = at.live;
-    const int64_t rows = int64_t(p.rows), dim = int64_t(p.dim);
+    const int rows = int(p.rows);
+    const int64_t dim = int64_t(p.dim);
     const A* initial = p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr;
     A* state = p.state ? static_cast<A*>(p.state) + c0 : nullptr;
     A* marks = p.checkpoints
@@ -449,23 +484,18 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
     memory.place(next, at.lanes * V, plan.warps, at.cluster);
     for (int c = threadIdx.x; c < memory.width; c += blockDim.x)
         memory.run[c] = !PACKED && p.initial && at.first + c < p.dim ? static_cast<const A*>(p.initial)[b * p.dim + at.first + c] : A(0);
-    if (PACKED && state && live && at.rank == 0)  // sequences without rows hand their initial state on
-        for (int64_t j = at.part; j < int64_t(p.sequences); j += plan.warps * at.parts)
-            if (offset_at(p.offsets, p.wide_offsets, j + 1) <= offset_at(p.offsets, p.wide_offsets, j))
-                for (int v = 0; v < V; ++v) state[j * dim + v] = initial ? initial[j * dim + v] : A(0);
-
-    const int64_t span = int64_t(plan.warps) * at.parts * at.cluster * S;
-    int64_t row0 = (int64_t(at.rank) * plan.warps * at.parts + at.part) * S;
+    const int span = plan.warps * at.parts * at.cluster * S;
+    int row0 = (at.rank * plan.warps * at.parts + at.part) * S;
     const X* x = static_cast<const X*>(p.x) + b * p.x_batch + (live ? c0 : 0);
     const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
     const int64_t x_row = int64_t(p.x_row), gate_row = int64_t(p.gate_row);
-    const int64_t x_span = span * x_row, gate_span = span * gate_row;
-    const X* px = fx.start(x + row0 * x_row, x_row);
-    const G* pg = fg.start(gate + row0 * gate_row, gate_row);
-    X* out = p.out ? static_cast<X*>(p.out) + (b * p.rows + row0) * p.dim + c0 : nullptr;
-    int64_t coming = row0;  // the row that the next copies are for
+    const int64_t x_span = span * x_row, gate_span = span * gate_row, out_span = span * dim;
+    const X* px = fx.start(x + int64_t(row0) * x_row, x_row);
+    const G* pg = fg.start(gate + int64_t(row0) * gate_row, gate_row);
+    X* out = p.out ? static_cast<X*>(p.out) + (int64_t(b * p.rows) + row0) * dim + c0 : nullptr;
+    int coming = row0;  // the row that the next copies are for
     const auto fetch = [&](int stage) {
-        const int n = rows_left(rows, coming, S, live);
+        const int n = rows_left<S>(rows, coming, live);
         fx.issue(stage, x, px, x_row, n);
         fg.issue(stage, gate, pg, gate_row, n);
         commit_copies();
@@ -473,18 +503,26 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
         pg += gate_span;
         coming += span;
     };
-    const auto hold = [&](int64_t row) {
-        const int n = rows_left(rows, row, S, live);
-        fx.hold(x + row * x_row, x_row, n);
-        fg.hold(gate + row * gate_row, gate_row, n);
+    const auto hold = [&](int row) {
+        const int n = rows_left<S>(rows, row, live);
+        fx.hold(x + int64_t(row) * x_row, x_row, n);
+        fg.hold(gate + int64_t(row) * gate_row, gate_row, n);
     };
     for (int k = 0; k < kStages - 1; ++k) fetch(k);
     hold(row0);
+    if (at.cluster > 1) cooperative_groups::this_cluster().sync();  // all of it runs before any writes to another
     SequenceWalk walk;
-    if (PACKED) walk.seek(p.offsets, p.wide_offsets, p.sequences, row0);
+    if (PACKED) {
+        walk.open(p, reinterpret_cast<int*>(next + ScanMemory<A>::bytes(memory.width, plan.warps, at.cluster)));
+        walk.seek(row0);
+        if (state && live && at.rank == 0)  // sequences without rows hand their initial state on
+            for (int j = at.part; j < walk.count; j += plan.warps * at.parts)
+                if (offset_at(walk.offsets, walk.wide, j + 1) <= offset_at(walk.offsets, walk.wide, j))
+                    for (int v = 0; v < V; ++v) state[j * dim + v] = initial ? initial[j * dim + v] : A(0);
+    }
     int turn = 0, stage = 0;
-    for (int64_t base = 0; base < rows; base += span, row0 += span, turn ^= 1, stage = stage + 1 == kStages ? 0 : stage + 1) {
-        const int count = rows_left(rows, row0, S, live);
+    for (int base = 0; base < rows; base += span, row0 += span, turn ^= 1, stage = stage + 1 == kStages ? 0 : stage + 1) {
+        const int count = rows_left<S>(rows, row0, live);
         fetch(stage == 0 ? kStages - 1 : stage - 1);  // its slots were read in the last iteration, before a barrier
         RowEvents e;
         if (PACKED) {
@@ -545,15 +583,12 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
             carry_across<A, false, PACKED>(memory, plan.warps, at.cluster, at.rank, turn);
         }
         __syncthreads();
+        A h[V];
+        enter_rows<A, V, false>(m, plan.log_lanes, memory.carry + at.warp * memory.width + at.tc * V, h);
         if (count) {
-            const Pack<A, V> in = load_pack<A, V>(memory.carry + at.warp * memory.width + at.tc * V);
-            A h[V];
+            if (marks && row0 % int(kCheckpointRows) == 0)
 #pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = in.v[v];
-            m.apply(h);
-            if (marks && row0 % int64_t(kCheckpointRows) == 0)
-#pragma unroll
-                for (int v = 0; v < V; ++v) marks[row0 / int64_t(kCheckpointRows) * dim + v] = h[v];
+                for (int v = 0; v < V; ++v) marks[int64_t(row0 / int(kCheckpointRows)) * dim + v] = h[v];
             if (!events) {
                 X* to = out;
                 const int stored = out ? count : 0;
@@ -590,7 +625,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
                 }
             }
         }
-        if (out) out += span * dim;
+        if (out) out += out_span;
     }
     if (!PACKED && p.state && at.rank == 0)
         for (int c = threadIdx.x; c < memory.width && at.first + c < p.dim; c += blockDim.x)
@@ -610,7 +645,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
     const Place at(plan, p.dim, V);
     const uint64_t b = at.batch, c0 = at.c0;
     const bool live = at.live;
-    const int64_t rows = int64_t(p.rows), dim = int64_t(p.dim);
+    const int rows = int(p.rows);
+    const int64_t dim = int64_t(p.dim);
     const A* initial = p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr;
     const A* state_derivs = p.state_derivs ? static_cast<const A*>(p.state_derivs) + c0 : nullptr;
     A* dinitial = p.dinitial ? static_cast<A*>(p.dinitial) + c0 : nullptr;
@@ -632,32 +668,31 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
     A* entering = reinterpret_cast<A*>(next + ScanMemory<A>::bytes(ahead.width, plan.warps, at.cluster));  // [stage][width]
     for (int c = threadIdx.x; c < back.width; c += blockDim.x)
         back.run[c] = !PACKED && p.state_derivs && at.first + c < p.dim ? static_cast<const A*>(p.state_derivs)[b * p.dim + at.first + c] : A(0);
-    if (PACKED && dinitial && live && at.rank == 0)
-        for (int64_t j = at.part; j < int64_t(p.sequences); j += plan.warps * at.parts)
-            if (offset_at(p.offsets, p.wide_offsets, j + 1) <= offset_at(p.offsets, p.wide_offsets, j))
-                for (int v = 0; v < V; ++v) dinitial[j * dim + v] = state_derivs ? state_derivs[j * dim + v] : A(0);
-
-    const int64_t block = int64_t(plan.warps) * at.parts * S, span = block * at.cluster;
-    int64_t base = (rows - 1) / span * span, row0 = base + at.rank * block + int64_t(at.part) * S;
+    const int block = plan.warps * at.parts * S, span = block * at.cluster;
+    int base = (rows - 1) / span * span, row0 = base + at.rank * block + at.part * S;
     const X* x = static_cast<const X*>(p.x) + b * p.x_batch + (live ? c0 : 0);
     const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
     const X* derivs = static_cast<const X*>(p.derivs) + b * p.d_batch + (live ? c0 : 0);
     const int64_t x_row = int64_t(p.x_row), gate_row = int64_t(p.gate_row), d_row = int64_t(p.d_row);
     const int64_t x_span = span * x_row, gate_span = span * gate_row, d_span = span * d_row;
-    const X* px = fx.start(x + row0 * x_row, x_row);
-    const G* pg = fg.start(gate + row0 * gate_row, gate_row);
-    const X* pd = fd.start(derivs + row0 * d_row, d_row);
-    int64_t coming = row0, coming_base = base;
+    const X* px = fx.start(x + int64_t(row0) * x_row, x_row);
+    const G* pg = fg.start(gate + int64_t(row0) * gate_row, gate_row);
+    const X* pd = fd.start(derivs + int64_t(row0) * d_row, d_row);
+    const int64_t out_span = span * dim;
+    X* dx = static_cast<X*>(p.dx) + (int64_t(b) * rows + row0) * dim + c0;
+    G* dgate = static_cast<G*>(p.dgate) + (SHARED ? 0 : (int64_t(b) * rows + row0) * dim + c0);
+    int coming = row0, coming_base = base;
     const auto fetch = [&](int stage) {
-        const int n = rows_left(rows, coming, S, live);
+        const int n = rows_left<S>(rows, coming, live);
         fx.issue(stage, x, px, x_row, n);
         fg.issue(stage, gate, pg, gate_row, n);
         fd.issue(stage, derivs, pd, d_row, n);
         // the checkpoint that enters the CTA's rows: each column's thread copies its own
-        const int64_t own = coming_base + at.rank * block;
+        const int own = coming_base + at.rank * block;
+        const A* mark = marks + int64_t(own / int(kCheckpointRows)) * dim;
         for (int c = threadIdx.x; c < ahead.width; c += blockDim.x) {
             const bool on = own >= 0 && own < rows && at.first + c < p.dim;
-            copy_async<sizeof(A)>(entering + stage * ahead.width + c, on ? marks + own / int64_t(kCheckpointRows) * dim + c : static_cast<const A*>(p.marks), on);
+            copy_async<sizeof(A)>(entering + stage * ahead.width + c, on ? mark + c : static_cast<const A*>(p.marks), on);
         }
         commit_copies();
         px -= x_span;
@@ -666,19 +701,27 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
         coming -= span;
         coming_base -= span;
     };
-    const auto hold = [&](int64_t row) {
-        const int n = rows_left(rows, row, S, live);
-        fx.hold(x + row * x_row, x_row, n);
-        fg.hold(gate + row * gate_row, gate_row, n);
-        fd.hold(derivs + row * d_row, d_row, n);
+    const auto hold = [&](int row) {
+        const int n = rows_left<S>(rows, row, live);
+        fx.hold(x + int64_t(row) * x_row, x_row, n);
+        fg.hold(gate + int64_t(row) * gate_row, gate_row, n);
+        fd.hold(derivs + int64_t(row) * d_row, d_row, n);
     };
     for (int k = 0; k < kStages - 1; ++k) fetch(k);
     hold(row0);
+    if (at.cluster > 1) cooperative_groups::this_cluster().sync();  // all of it runs before any writes to another
     SequenceWalk walk;
-    if (PACKED) walk.seek(p.offsets, p.wide_offsets, p.sequences, row0);
+    if (PACKED) {
+        walk.open(p, reinterpret_cast<int*>(entering + kStages * ahead.width));
+        walk.seek(row0);
+        if (dinitial && live && at.rank == 0)
+            for (int j = at.part; j < walk.count; j += plan.warps * at.parts)
+                if (offset_at(walk.offsets, walk.wide, j + 1) <= offset_at(walk.offsets, walk.wide, j))
+                    for (int v = 0; v < V; ++v) dinitial[j * dim + v] = state_derivs ? state_derivs[j * dim + v] : A(0);
+    }
     int turn = 0, stage = 0;
     for (; base >= 0; base -= span, row0 -= span, turn ^= 1, stage = stage + 1 == kStages ? 0 : stage + 1) {
-        const int count = rows_left(rows, row0, S, live);
+        const int count = rows_left<S>(rows, row0, live);
         fetch(stage == 0 ? kStages - 1 : stage - 1);  // its slots were read in the last iteration, before a barrier
         RowEvents e;
         if (PACKED) {
@@ -762,14 +805,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
         }
         __syncthreads();
         A in[V], w[V];
-        {
-            const Pack<A, V> first = load_pack<A, V>(ahead.carry + at.warp * ahead.width + at.tc * V);
-            const Pack<A, V> last = load_pack<A, V>(back.carry + at.warp * back.width + at.tc * V);
-#pragma unroll
-            for (int v = 0; v < V; ++v) { in[v] = first.v[v]; w[v] = last.v[v]; }
-        }
-        m.apply(in);
-        g.apply(w);
+        enter_rows<A, V, false>(m, plan.log_lanes, ahead.carry + at.warp * ahead.width + at.tc * V, in);
+        enter_rows<A, V, true>(g, plan.log_lanes, back.carry + at.warp * back.width + at.tc * V, w);
         // backward through the rows: d becomes g
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {
@@ -785,10 +822,12 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
             }
         }
         // forward through them with h_{t-1} in `in`
-        X* dx = static_cast<X*>(p.dx) + (b * rows + row0) * dim + c0;
-        G* dgate = static_cast<G*>(p.dgate) + (SHARED ? 0 : (b * rows + row0) * dim + c0);
+        X* to_x = dx;
+        G* to_gate = dgate;
+        dx -= out_span;
+        dgate -= SHARED ? 0 : out_span;
 #pragma unroll
-        for (int s = 0; s < S; ++s, dx += dim, dgate += SHARED ? 0 : dim) {
+        for (int s = 0; s < S; ++s, to_x += dim, to_gate += SHARED ? 0 : dim) {
             if (PACKED && (e.starts >> s & 1u)) {
                 const A* from = initial && live ? initial + sequence_of(walk, row0 + s) * dim : nullptr;
 #pragma unroll
@@ -805,17 +844,17 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
                 sum += gg[v];
                 in[v] = fma_(a[s][v], in[v], input(s, v));
             }
-            if (s < count) store_pack<X, V>(dx, narrow_pack<X, V>(gx));
+            if (s < count) store_pack<X, V>(to_x, narrow_pack<X, V>(gx));
             if (SHARED) {
                 sum = s < count ? sum : A(0);
                 for (int k = 1; k < 1 << plan.fold_log; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
                 if (s < count && (at.tc & ((1 << plan.fold_log) - 1)) == 0) {
-                    const int64_t fold = int64_t(c0 / V) >> plan.fold_log, row = b * rows + row0 + s;
+                    const int64_t fold = int64_t(c0 / V) >> plan.fold_log, row = int64_t(b) * rows + row0 + s;
                     if (partial) partial[row * ((dim / V) >> plan.fold_log) + fold] = sum;
-                    else dgate[row * int64_t(p.gate_dim) + fold] = narrow<G>(sum);
+                    else to_gate[row * int64_t(p.gate_dim) + fold] = narrow<G>(sum);
                 }
             } else if (s < count) {
-                if constexpr (std::is_same_v<Acc<G>, A>) store_pack<G, V>(dgate, narrow_pack<G, V>(gg));
+                if constexpr (std::is_same_v<Acc<G>, A>) store_pack<G, V>(to_gate, narrow_pack<G, V>(gg));
             }
         }
     }

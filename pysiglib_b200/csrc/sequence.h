@@ -24,6 +24,9 @@ inline size_t state_size(int type) { return type == kFloat64 ? 8 : 4; }
 // Rows between two checkpoints of a recurrence (the state entering rows 0, 64, 128, ..).
 constexpr uint64_t kCheckpointRows = 64;
 
+// Rows are counted in 32 bits, with room for the blocks that an iteration looks ahead.
+constexpr uint64_t kMaxRows = 1ull << 30;
+
 struct RecurrenceArgs {
     int type, gate_type;
     uint64_t batch, rows, dim, gate_dim, sequences;  // sequences > 0: packed, batch == 1

@@ -94,7 +94,8 @@ def linear_recurrence(
 ):
     """Gated linear recurrence ``h_t = a_t h_{t-1} + b_t`` along axis -2, channel by channel.
 
-    :param x: inputs ``(..., length, dimension)`` of type float32, float64, float16 or bfloat16.  CUDA
+    :param x: inputs ``(..., length, dimension)`` of type float32, float64, float16 or bfloat16, fewer than
+        2^30 rows long.  CUDA
         tensors are processed on their device and on its current stream, without waiting for the
         result; views with adjacent channels are read in place.  NumPy arrays and CPU tensors go
         through the current CUDA device.

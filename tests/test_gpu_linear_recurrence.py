@@ -85,7 +85,7 @@ def test_shared_gates(dim, gates, dtype, gate_dtype):
     run_and_check(make(dim + gates, 2, 75, dim, gates, dtype, gate_dtype, "logit", True), "logit", gates % 2 == 0)
 
 
-@pytest.mark.parametrize("rows,sequences", [(1, 1), (1, 5), (6, 9), (40, 3), (64, 64), (150, 7), (300, 1), (515, 40), (1300, 300)])
+@pytest.mark.parametrize("rows,sequences", [(1, 1), (1, 5), (6, 9), (40, 3), (64, 64), (150, 7), (300, 1), (515, 40), (1300, 300), (900, 700)])
 @pytest.mark.parametrize("dense", [True, False])
 @pytest.mark.parametrize("dtype,gate_dtype,dim", [(F32, F32, 36), (BF16, F32, 35), (F64, F64, 6)])
 def test_packed_sequences(rows, sequences, dense, dtype, gate_dtype, dim):

@@ -164,7 +164,7 @@ def test_native_entry_points_refuse_without_a_gpu():
                {"form": 3}, {"x": None}, {"gate": None}, {"out": None}, {"sequences": 1}, {"sequences": 1, "offsets": p}):
         assert recurrence(**kw) == 2, (kw, load_cusig.last_error_message())
         assert "linear_recurrence" in load_cusig.last_error_message()
-    assert recurrence(batch=1 << 40, rows=1 << 40) == 3
+    assert recurrence(batch=1 << 40, rows=1 << 20) == 3 and recurrence(rows=1 << 30) == 3
     assert recurrence(batch=0) == 0 and recurrence(rows=0) == 0
 
     def rotary(type=0, kind=0, x=p, f=p, positions=None, out=p, rows=4, dim=4, part=4):
