@@ -59,7 +59,7 @@ template <typename T> T staged(T host, void* device) { return host ? static_cast
 
 void backward_on_device(RecurrenceArgs p, const Sizes& s, cudaStream_t stream) {
     Scratch marks(p.marks ? 0 : s.marks * state_size(p.type), stream);
-    if (!p.marks) {  // the states entering every 64th row, by a forward pass that stores nothing else
+    if (!p.marks) {  // the states entering every 16th row, by a forward pass that stores nothing else
         RecurrenceArgs f = p;
         f.out = f.state = nullptr;
         f.derivs = nullptr;

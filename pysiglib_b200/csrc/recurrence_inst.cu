@@ -11,18 +11,9 @@ namespace {
 // Channels a thread holds: 16 bytes of float32 or float64, 8 of the 16-bit types (whose gates and states
 // widen to the same registers).
 template <typename X> constexpr int kWide = sizeof(X) == 8 ? 2 : 4;
-// Rows a thread holds: 8 forward; 4 backward where V > 1, as the five arrays of S * V values stay in registers.
+// Rows a thread holds: as many as leave the arrays of S * V values in registers and two CTAs an SM their stages.
 template <int V> constexpr int kBackwardRows = V == 1 ? 8 : 4;
-#ifndef SIG_F32S
-#define SIG_F32S 4
-#endif
-template <typename X, int V> constexpr int kForwardRows = V > 1 && sizeof(X) > 2 ? SIG_F32S : 8;
-#ifndef SIG_SLOTS
-#define SIG_SLOTS 2
-#endif
-#ifndef SIG_LINE
-#define SIG_LINE 128
-#endif
+template <typename X, int V> constexpr int kForwardRows = V > 1 && sizeof(X) > 2 ? 4 : 8;
 
 int log2_ceil(uint64_t n) {
     int k = 0;
@@ -41,32 +32,30 @@ bool aligned_to(const RecurrenceArgs& p, size_t bytes) {
            (p.gate_dim != p.dim || fits(p.gate, element_size(p.gate_type), p.dim, p.gate_batch, p.gate_row));
 }
 
-// Up to 8 warps whose lanes lie side by side in the channels as far as 128 bytes of a row go (full lines, and
-// the narrowest strips, hence the most CTAs) and behind one another in the rows beyond that.
+// Up to 8 warps whose lanes lie side by side in the channels as far as 128 bytes of a row go (full lines), and
+// behind one another in the rows beyond that.  Two CTAs an SM are there at a time.  Where full lines make fewer
+// strips than there are SMs, half lines do if that is enough; else the rows are cut into segments.
 template <typename X>
 RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
-    const int columns = log2_ceil((p.dim + V - 1) / V), needed = log2_ceil((p.rows + S - 1) / S);
+    const uint64_t per_row = (p.dim + V - 1) / V, sms = device_context(current_device()).sm_count;
+    const int columns = log2_ceil(per_row), needed = log2_ceil((p.rows + S - 1) / S);
     RecurrencePlan plan{};
-    plan.log_lanes = std::min({columns, log2_ceil(SIG_LINE / (V * sizeof(X))), 5});
-    // few strips: half and quarter lines, for as many CTAs as there are SMs and more
-    const uint64_t sms = device_context(current_device()).sm_count;
-    while ((V * sizeof(X)) << plan.log_lanes > 32 && plan.log_lanes > 0 &&
-           p.batch * (((p.dim + V - 1) / V + (1ull << plan.log_lanes) - 1) >> plan.log_lanes) * 8 < sms)
-        --plan.log_lanes;
+    plan.log_lanes = std::min({columns, log2_ceil(128 / (V * sizeof(X))), 5});
+    const auto ctas = [&](int log_lanes) { return p.batch * (((per_row - 1) >> log_lanes) + 1); };
+    if (plan.log_lanes > 0 && ctas(plan.log_lanes) < sms && ctas(plan.log_lanes - 1) >= sms) --plan.log_lanes;
     // short inputs: no more parts than there are rows for, the lanes go to the channels instead
     plan.log_lanes = std::max(plan.log_lanes, std::min(columns, 5 - std::min(needed, 5)));
     plan.warps = 1 << std::min(3, std::max(0, needed - (5 - plan.log_lanes)));
     plan.pairs = plan.log_lanes > 0 && aligned_to(p, 16);
-    const uint64_t lanes = 1ull << plan.log_lanes;
-    const uint64_t strips = ((p.dim + V - 1) / V + lanes - 1) / lanes;
-    const uint64_t span = uint64_t(plan.warps) * (32 >> plan.log_lanes) * S;
-    // two CTAs an SM at a time: share strips while that many are not there, as long as every CTA has rows
-    const uint64_t slots = SIG_SLOTS * sms;
-    plan.cluster = 1;
-    while (plan.cluster < 8 && p.batch * strips * plan.cluster * 2 <= slots && span * plan.cluster < p.rows) plan.cluster *= 2;
-    if (strips * plan.cluster > 0x7fffffffull / p.batch)
+    if (ctas(plan.log_lanes) > 0x7fffffffull)
         throw std::invalid_argument("linear_recurrence: problem too large for one kernel launch");
-    plan.strips = static_cast<unsigned>(strips);
+    plan.strips = static_cast<unsigned>(((per_row - 1) >> plan.log_lanes) + 1);
+    const uint64_t span = uint64_t(plan.warps) * (32 >> plan.log_lanes) * S, blocks = (p.rows + span - 1) / span;
+    uint64_t segments = 1;
+    if (ctas(plan.log_lanes) < sms) segments = std::min(blocks, 2 * sms / ctas(plan.log_lanes));
+    const uint64_t length = (blocks + segments - 1) / segments;
+    plan.segments = static_cast<int>((blocks + length - 1) / length);
+    plan.segment_rows = static_cast<int>(length * span);
     return plan;
 }
 
@@ -80,38 +69,67 @@ size_t offset_bytes(const RecurrenceArgs& p) {
     return p.sequences && p.sequences < uint64_t(kLocalOffsets) ? (p.sequences + 1) * sizeof(int) : 0;
 }
 
+// As many stages as two CTAs an SM have room for; returns the bytes of shared memory of a CTA.
+size_t shared_memory(RecurrencePlan& plan, size_t stage, size_t fixed) {
+    constexpr size_t kRoom = (228 * 1024 / 2) - 1024;
+    plan.stages = 4;
+    while (plan.stages > 2 && fixed + plan.stages * stage > kRoom) --plan.stages;
+    return fixed + plan.stages * stage;
+}
+
 template <typename... Params, typename... Args>
 void launch(void (*kernel)(Params...), const RecurrenceArgs& p, const RecurrencePlan& plan, size_t smem, cudaStream_t stream, Args... args) {
     if (smem > 48 * 1024) SIG_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(static_cast<unsigned>(p.batch * plan.strips * plan.cluster));
-    config.blockDim = dim3(32 * plan.warps);
-    config.dynamicSmemBytes = smem;
-    config.stream = stream;
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = plan.cluster;
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    config.attrs = &attribute;
-    config.numAttrs = plan.cluster > 1 ? 1 : 0;
-    SIG_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, p, plan, args...));
+    const unsigned grid = static_cast<unsigned>(p.batch) * plan.strips * unsigned(plan.segments);
+    kernel<<<grid, 32 * plan.warps, smem, stream>>>(p, plan, args...);
+    check("linear recurrence kernel");
+}
+
+// Scratch for the segments' maps and, behind them, their drops.
+template <typename A>
+size_t maps_bytes(const RecurrenceArgs& p, const RecurrencePlan& plan) {
+    return plan.segments > 1 ? p.batch * plan.segments * (2 * p.dim * sizeof(A) + sizeof(int)) : 0;
+}
+
+template <typename X, typename G, int V, bool SHARED, bool REVERSE>
+void reduce_segments(const RecurrenceArgs& p, RecurrencePlan plan, cudaStream_t stream) {
+    constexpr int S = V == 1 ? 8 : 4;  // divides the rows of a thread: a block's are a multiple of it
+    const size_t smem = shared_memory(plan, Prefetch<X, V, S>::kStage + Prefetch<G, SHARED ? 1 : V, S>::kStage,
+                                      plan.warps * (2 * sizeof(Acc<X>) * (V << plan.log_lanes) + sizeof(int)) + offset_bytes(p));
+    if (p.sequences) launch(recurrence_maps_kernel<X, G, V, S, SHARED, true, REVERSE>, p, plan, smem, stream);
+    else launch(recurrence_maps_kernel<X, G, V, S, SHARED, false, REVERSE>, p, plan, smem, stream);
+}
+
+template <typename A>
+void place_maps(const RecurrenceArgs& p, RecurrencePlan& plan, void* memory) {
+    plan.maps = memory;
+    plan.drops = reinterpret_cast<int*>(static_cast<A*>(memory) + p.batch * plan.segments * 2 * p.dim);
 }
 
 template <typename X, typename G, int V, bool SHARED>
 void forward(const RecurrenceArgs& p, cudaStream_t stream) {
-    const RecurrencePlan plan = make_plan<X>(p, V, kForwardRows<X, V>);
-    using Ring = Stages<X, G, V, SHARED ? 1 : V, kForwardRows<X, V>, 1>;
-    const size_t smem = Ring::kCount * Ring::kBytes +
-                        ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, plan.cluster) + offset_bytes(p);
-    if (p.sequences) launch(recurrence_forward_kernel<X, G, V, kForwardRows<X, V>, SHARED, true>, p, plan, smem, stream);
-    else launch(recurrence_forward_kernel<X, G, V, kForwardRows<X, V>, SHARED, false>, p, plan, smem, stream);
-    check("linear recurrence kernel");
+    constexpr int S = kForwardRows<X, V>;
+    RecurrencePlan plan = make_plan<X>(p, V, S);
+    Scratch maps(maps_bytes<Acc<X>>(p, plan), stream);
+    if (plan.segments > 1) {
+        place_maps<Acc<X>>(p, plan, maps.get());
+        reduce_segments<X, G, V, SHARED, false>(p, plan, stream);
+    }
+    const size_t smem = shared_memory(plan, Prefetch<X, V, S>::kStage + Prefetch<G, SHARED ? 1 : V, S>::kStage,
+                                      sizeof(Acc<X>) * (V << plan.log_lanes) * plan.warps + offset_bytes(p));
+    if (p.sequences) launch(recurrence_forward_kernel<X, G, V, S, SHARED, true>, p, plan, smem, stream);
+    else launch(recurrence_forward_kernel<X, G, V, S, SHARED, false>, p, plan, smem, stream);
 }
 
 template <typename X, typename G, int V, bool SHARED>
 void backward(const RecurrenceArgs& p, cudaStream_t stream) {
     constexpr int S = kBackwardRows<V>;
     RecurrencePlan plan = make_plan<X>(p, V, S);
+    Scratch maps(maps_bytes<Acc<X>>(p, plan), stream);
+    if (plan.segments > 1) {
+        place_maps<Acc<X>>(p, plan, maps.get());
+        reduce_segments<X, G, V, SHARED, true>(p, plan, stream);
+    }
     Acc<X>* partial = nullptr;
     uint64_t per_gate = 0;
     if (SHARED) {  // lanes whose channels share a gate, as far as a power of two goes
@@ -121,10 +139,9 @@ void backward(const RecurrenceArgs& p, cudaStream_t stream) {
     const uint64_t n = p.batch * p.rows * p.gate_dim;
     Scratch scratch(per_gate > 1 ? checked_mul(n, per_gate * sizeof(Acc<X>), "linear_recurrence_backprop") : 0, stream);
     if (per_gate > 1) partial = scratch.as<Acc<X>>();
-    using Ring = Stages<X, G, V, SHARED ? 1 : V, S, 2>;
-    const size_t smem = Ring::kCount * (Ring::kBytes + sizeof(Acc<X>) * (V << plan.log_lanes)) +
-                        ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, 1) +
-                        ScanMemory<Acc<X>>::bytes(V << plan.log_lanes, plan.warps, plan.cluster) + offset_bytes(p);
+    const size_t column = (V << plan.log_lanes) * sizeof(Acc<X>);
+    const size_t smem = shared_memory(plan, 2 * Prefetch<X, V, S>::kStage + Prefetch<G, SHARED ? 1 : V, S>::kStage + plan.warps * column,
+                                      2 * plan.warps * column + offset_bytes(p));
     if (p.complement) {
         if (p.sequences) launch(recurrence_backward_kernel<X, G, V, S, SHARED, true, true>, p, plan, smem, stream, partial);
         else launch(recurrence_backward_kernel<X, G, V, S, SHARED, false, true>, p, plan, smem, stream, partial);
@@ -132,7 +149,6 @@ void backward(const RecurrenceArgs& p, cudaStream_t stream) {
         if (p.sequences) launch(recurrence_backward_kernel<X, G, V, S, SHARED, true, false>, p, plan, smem, stream, partial);
         else launch(recurrence_backward_kernel<X, G, V, S, SHARED, false, false>, p, plan, smem, stream, partial);
     }
-    check("linear recurrence backward kernel");
     if (partial) {
         if (n / 256 >= 0x7fffffffull) throw std::invalid_argument("linear_recurrence_backprop: problem too large for one kernel launch");
         fold_partials_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(partial, static_cast<G*>(p.dgate), n, per_gate);
@@ -156,7 +172,8 @@ bool aligned(const RecurrenceArgs& p, bool shared) {
     if (p.dim % V || p.x_batch % V || p.x_row % V || p.d_batch % V || p.d_row % V) return false;
     for (const void* ptr : {p.x, p.derivs, static_cast<const void*>(p.out), static_cast<const void*>(p.dx)})
         if (!fits(ptr, V * sizeof(X))) return false;
-    if (!fits(p.state, V * sizeof(Acc<X>))) return false;
+    for (const void* ptr : {static_cast<const void*>(p.state), static_cast<const void*>(p.checkpoints), p.marks})
+        if (!fits(ptr, V * sizeof(Acc<X>))) return false;
     if (shared) return group % V == 0;
     return p.gate_batch % V == 0 && p.gate_row % V == 0 && fits(p.gate, V * sizeof(G)) && fits(p.dgate, V * sizeof(G));
 }

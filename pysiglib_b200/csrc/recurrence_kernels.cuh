@@ -7,23 +7,24 @@
 // derivatives of h_t, g_t = d_t + u_{t+1}, dx_t = g_t (or (1 - a_t) g_t) and da_t = g_t (h_{t-1} - [x_t]).
 //
 // Split.  A value costs three to five values of traffic and a few dozen operations at most, so the loads have to
-// be in flight all the time.  A CTA owns a strip of CL * V neighbouring channels and walks down the rows, W warps
-// times 32 / CL parts times S rows at a time: each thread holds S consecutive rows of V channels in
-// registers and reduces them to one map.  The maps of a warp are composed by shuffles, those of the warps go
-// through shared memory, and a second walk over the registers gives the S states.  The next
-// iteration's inputs are copied into shared memory (asynchronously, into slots that only the thread itself reads)
-// while this one's are folded and stored.  Every input is read once, every output written once, and the
-// state that crosses an iteration stays in registers, in 32 bits (64 for float64 inputs).
+// be in flight all the time and nothing may stand still.  A CTA owns a strip of CL * V neighbouring channels and
+// walks down the rows, W warps times 32 / CL parts times S rows at a time: each thread holds S consecutive
+// rows of V channels in registers and reduces them to one map, the maps of a warp are composed by shuffles, the
+// state goes round the ring of warps, each handing it to the next as soon as its map has been applied,
+// and a second walk over the registers gives the S states.  No barrier holds all warps: while some wait
+// for the state the others load and reduce.  The coming iterations' inputs are copied into shared memory
+// asynchronously, into slots that only the warp itself reads.  Every input is read once, every output
+// written once, and the state is held in 32 bits (64 for float64 inputs).
 //
-// Where strips are too few to fill the GPU, a cluster of CTAs shares one: each takes a block of rows of every
-// iteration and writes its map into the shared memory of the others; the cluster's barrier is the only wait.
+// Where the strips are too few to fill the GPU, the rows are cut into segments as well.  A first kernel reduces
+// every segment to its map, each thread a contiguous run of rows and without any exchange on the way; the
+// main kernel starts each segment from the maps before it.  That reads the inputs twice, the second
+// time from L2 where they fit.
 //
 // Packed sequences are one scan over all rows in which the first row of a sequence drops what enters it:
 // the drop is a flag beside (A, B), not a gate of 0, so that a NaN or an infinity of one sequence
 // stays inside it.
 #pragma once
-
-#include <cooperative_groups.h>
 
 #include <climits>
 
@@ -35,10 +36,14 @@ namespace sigb200 {
 struct RecurrencePlan {
     int log_lanes;     // CL = 1 << log_lanes threads side by side in the channels, 32 / CL parts in a warp
     int warps;         // W
-    int cluster;       // CTAs that share a strip
+    int stages;        // iterations whose inputs are in shared memory or on their way, 2 to 4
     unsigned strips;   // strips of CL * V channels
+    int segments;      // of the rows
+    int segment_rows;  // a multiple of the rows of an iteration and, where there are several, of a checkpoint's
     bool pairs;        // 8-byte neighbours are aligned to 16 bytes in every array
     int fold_log;      // backward, shared gates: lanes folded into one partial sum, log2
+    void* maps;        // [batch][segment][A, B][dim] of the segments, and
+    int* drops;        // [batch][segment]
 };
 
 namespace {
@@ -160,9 +165,6 @@ __device__ __forceinline__ void gate_factors(A v, A& a, A& rest) {
 __device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_(double a, double b, double c) { return fma(a, b, c); }
 
-#ifndef SIG_ROOM
-#define SIG_ROOM 100
-#endif
 constexpr int kCtaThreads = 256;  // at most; also the stride of the prefetch slots
 
 // One copy of B bytes (4, 8 or 16) to shared memory, asynchronous; `on` false writes zeros.
@@ -180,10 +182,12 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(B) : "memory");
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// until all groups of the warp but the last N are there
-template <int N>
-__device__ __forceinline__ void await_copies() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// until all groups of the warp but the last `stages - 1` are there
+__device__ __forceinline__ void await_copies(int stages) {
+    if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (stages == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
 }
 
@@ -246,13 +250,6 @@ struct Prefetch {
     }
 };
 
-// Iterations whose inputs are in shared memory or on their way: as many as two CTAs an SM have room for.
-template <typename X, typename G, int V, int GV, int S, int ARRAYS>
-struct Stages {
-    static constexpr size_t kBytes = ARRAYS * Prefetch<X, V, S>::kStage + Prefetch<G, GV, S>::kStage;
-    static constexpr int kCount = kBytes * 4 <= SIG_ROOM * 1024 ? 4 : kBytes * 3 <= SIG_ROOM * 1024 ? 3 : 2;
-};
-
 // The affine map of a run of rows on V channels; `drop`: what enters the run does not leave it.
 template <typename A, int V>
 struct Map {
@@ -270,33 +267,11 @@ struct Map {
     }
 };
 
-// Shared memory of one scan: the maps of the warps, the state that enters each of them, the state that enters
-// the next iteration, and, twice by turns, the maps that the CTAs of a cluster hand to one another.
-template <typename A>
-struct ScanMemory {
-    A *maps, *carry, *run, *others;  // [warp][A, B][width], [warp][width], [width], [turn][CTA][A, B][width]
-    unsigned char *drops, *other_drops;  // [warp], [turn][CTA]
-    int width;
-
-    __host__ __device__ static constexpr size_t bytes(int width, int warps, int cluster) {
-        return sizeof(A) * width * (3 * size_t(warps) + 1 + (cluster > 1 ? 4 * size_t(cluster) : 0)) + 16 * size_t(1 + (warps + 2 * cluster) / 16);
-    }
-    __device__ __forceinline__ void place(unsigned char* at, int w, int warps, int cluster) {
-        width = w;
-        maps = reinterpret_cast<A*>(at);
-        carry = maps + 2 * warps * width;
-        run = carry + warps * width;
-        others = run + width;
-        drops = reinterpret_cast<unsigned char*>(others + (cluster > 1 ? 4 * cluster * width : 0));
-        other_drops = drops + warps;
-    }
-};
-
-// Scan of the threads' maps over the parts of a warp (REVERSE: from the last part to the first).  On return
-// `m` is the map of this part and everything in the warp before it; the whole warp's is in `memory`.
+// Scan of the threads' maps over the parts of a warp (REVERSE: from the last part to the first): `m` becomes the map of
+// this part and everything in the warp before it.
 template <typename A, int V, bool REVERSE, bool PACKED>
-__device__ __forceinline__ void scan_warp(Map<A, V>& m, int log_lanes, const ScanMemory<A>& memory) {
-    const int lane = threadIdx.x & 31, lanes = 1 << log_lanes, parts = 32 >> log_lanes;
+__device__ __forceinline__ void scan_warp(Map<A, V>& m, int log_lanes) {
+    const int lane = threadIdx.x & 31, parts = 32 >> log_lanes;
     const int part = REVERSE ? parts - 1 - (lane >> log_lanes) : lane >> log_lanes;
     const auto from = [&](auto value, int by) {
         return REVERSE ? __shfl_down_sync(0xffffffffu, value, by) : __shfl_up_sync(0xffffffffu, value, by);
@@ -314,90 +289,49 @@ __device__ __forceinline__ void scan_warp(Map<A, V>& m, int log_lanes, const Sca
         }
         if (take) m.drop = earlier_drop;
     }
-    if (part == parts - 1) {
-        Pack<A, V> a, b;
-#pragma unroll
-        for (int v = 0; v < V; ++v) { a.v[v] = m.a[v]; b.v[v] = m.b[v]; }
-        A* to = memory.maps + 2 * int(threadIdx.x >> 5) * memory.width + (lane & (lanes - 1)) * V;
-        store_pack<A, V>(to, a);
-        store_pack<A, V>(to + memory.width, b);
-        if (PACKED && (lane & (lanes - 1)) == 0) memory.drops[threadIdx.x >> 5] = m.drop;
-    }
 }
 
-// The state that enters this thread's rows, from the one that enters its warp's and the inclusive maps.
+// The state that enters this thread's rows, from `in`, which enters its warp's, and the maps of scan_warp; lanes of the
+// part that comes last leave what leaves the warp at `leaving`.
 template <typename A, int V, bool REVERSE>
-__device__ __forceinline__ void enter_rows(const Map<A, V>& m, int log_lanes, const A* carry, A (&h)[V]) {
+__device__ __forceinline__ void enter_rows(const Map<A, V>& m, int log_lanes, const A (&in)[V], A (&h)[V], A* leaving) {
     const int lane = threadIdx.x & 31, lanes = 1 << log_lanes;
-    const Pack<A, V> in = load_pack<A, V>(carry);
-    A behind[V];
+    Pack<A, V> behind;
 #pragma unroll
-    for (int v = 0; v < V; ++v) behind[v] = in.v[v];
-    m.apply(behind);
+    for (int v = 0; v < V; ++v) behind.v[v] = m.drop ? m.b[v] : fma_(m.a[v], in[v], m.b[v]);
+    if (REVERSE ? lane < lanes : lane >= 32 - lanes) store_pack<A, V>(leaving, behind);
     const bool first = REVERSE ? lane >= 32 - lanes : lane < lanes;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const A e = REVERSE ? __shfl_down_sync(0xffffffffu, behind[v], lanes) : __shfl_up_sync(0xffffffffu, behind[v], lanes);
-        h[v] = first ? in.v[v] : e;
+        const A e = REVERSE ? __shfl_down_sync(0xffffffffu, behind.v[v], lanes) : __shfl_up_sync(0xffffffffu, behind.v[v], lanes);
+        h[v] = first ? in[v] : e;
     }
 }
 
-// Column c of the strip, one thread each: the state `r` that enters the CTA's rows goes through the warps'
-// maps, and what enters each warp is left in `carry`.
+// Hand-over between two warps of a CTA: the one that gives arrives, the one that takes waits for it.
+// Both in whole warps.
+__device__ __forceinline__ void give(int link) {
+    __syncwarp();
+    asm volatile("bar.arrive %0, 64;" ::"r"(link) : "memory");
+}
+__device__ __forceinline__ void take_over(int link) {
+    __syncwarp();
+    asm volatile("bar.sync %0, 64;" ::"r"(link) : "memory");
+}
+
+// The state that enters a segment: `r`, which enters the first one in scan order, through the maps of those before
+// it.  A state of 0 meets no factor, so that a product of large gates that overflowed does no harm to it.
 template <typename A, bool REVERSE, bool PACKED>
-__device__ __forceinline__ A carry_through(const ScanMemory<A>& m, int warps, int c, A r) {
+__device__ __forceinline__ A through_segments(const RecurrencePlan& plan, uint64_t batch, int segment, uint64_t dim, uint64_t c, A r) {
+    const int n = REVERSE ? plan.segments - 1 - segment : segment;
 #pragma unroll 4
-    for (int i = 0; i < warps; ++i) {
-        const int w = REVERSE ? warps - 1 - i : i;
-        m.carry[w * m.width + c] = r;
-        const A b = m.maps[(2 * w + 1) * m.width + c];
-        r = PACKED && m.drops[w] ? b : fma_(m.maps[2 * w * m.width + c], r, b);
+    for (int i = 0; i < n; ++i) {
+        const uint64_t k = batch * plan.segments + (REVERSE ? plan.segments - 1 - i : i);
+        const A* map = static_cast<const A*>(plan.maps) + 2 * k * dim + c;
+        const A b = map[dim];
+        r = (PACKED && plan.drops[k]) || r == A(0) ? b : fma_(map[0], r, b);
     }
     return r;
-}
-
-// The same across a cluster: each CTA composes its warps' maps and writes the composition into every CTA's
-// memory; behind the cluster's barrier each applies those before its own.  All threads call it.
-template <typename A, bool REVERSE, bool PACKED>
-__device__ __forceinline__ void carry_across(const ScanMemory<A>& m, int warps, int cluster, int rank, int turn) {
-    auto group = cooperative_groups::this_cluster();
-    A* others = m.others + turn * 2 * cluster * m.width;
-    unsigned char* drops = m.other_drops + turn * cluster;
-    for (int c = threadIdx.x; c < m.width; c += blockDim.x) {
-        A a = A(1), b = A(0);
-        bool drop = false;
-        for (int i = 0; i < warps; ++i) {
-            const int w = REVERSE ? warps - 1 - i : i;
-            const A wa = m.maps[2 * w * m.width + c], wb = m.maps[(2 * w + 1) * m.width + c];
-            const bool wd = PACKED && m.drops[w];
-            b = wd ? wb : fma_(wa, b, wb);
-            a *= wa;
-            drop |= wd;
-        }
-        for (int r = 0; r < cluster; ++r) {
-            A* there = group.map_shared_rank(others, r) + 2 * rank * m.width + c;
-            there[0] = a;
-            there[m.width] = b;
-            if (PACKED && c == 0) group.map_shared_rank(drops, r)[rank] = drop;
-        }
-    }
-    // only the threads that wrote order their writes before the barrier: a release by all would wait for every
-    // thread's stores of outputs as well
-    if (threadIdx.x < m.width) asm volatile("fence.acq_rel.cluster;" ::: "memory");
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    for (int c = threadIdx.x; c < m.width; c += blockDim.x) {
-        A r = m.run[c], mine = r;
-        for (int i = 0; i < cluster; ++i) {
-            const int k = REVERSE ? cluster - 1 - i : i;
-            if (k == rank) mine = r;
-            const A b = others[(2 * k + 1) * m.width + c];
-            r = PACKED && drops[k] ? b : fma_(others[2 * k * m.width + c], r, b);
-        }
-        m.run[c] = r;
-        carry_through<A, REVERSE, PACKED>(m, warps, c, mine);
-    }
 }
 
 // a, x and, where REST, 1 - a of S rows from the prefetched inputs; without REST x is b already.
@@ -429,10 +363,10 @@ __device__ __forceinline__ void factors(int form, const Prefetch<X, V, S>& fx, c
     else factors<kGateLogit, REST, COMPLEMENT>(fx, fg, stage, a, u, rest);
 }
 
-// Where a thread stands: its strip, channels and rows.
+// Where a thread stands: its strip, channels and segment of the rows.
 struct Place {
-    int lanes, lane, warp, tc, parts, part, cluster, rank;
-    uint64_t batch, first, c0;  // batch entry, first channel of the strip and of the thread
+    int lanes, lane, warp, tc, parts, part, segment;
+    uint64_t batch, c0;  // batch entry, the thread's first channel
     bool live;
 
     __device__ __forceinline__ Place(const RecurrencePlan& plan, uint64_t dim, int V) {
@@ -442,12 +376,12 @@ struct Place {
         tc = lane & (lanes - 1);
         parts = 32 >> plan.log_lanes;
         part = warp * parts + (lane >> plan.log_lanes);
-        cluster = plan.cluster;
-        rank = cluster > 1 ? int(blockIdx.x % cluster) : 0;
-        const uint64_t strip = cluster > 1 ? blockIdx.x / cluster : blockIdx.x;
-        batch = strip / plan.strips;
-        first = (strip % plan.strips) * lanes * V;
-        c0 = first + uint64_t(tc) * V;
+        unsigned block = blockIdx.x;
+        const unsigned strip = block % plan.strips;
+        block /= plan.strips;
+        segment = int(block % unsigned(plan.segments));
+        batch = block / unsigned(plan.segments);
+        c0 = (uint64_t(strip) * lanes + tc) * V;
         live = c0 < dim;
     }
 };
@@ -458,16 +392,81 @@ __device__ __forceinline__ int rows_left(int rows, int row0, bool live) {
     return live && row0 >= 0 ? max(0, min(S, rows - row0)) : 0;
 }
 
+// Rows of a thread with what a packed sequence does in them.
+template <typename A, int V, int S>
+struct Rows {
+    A a[S][V], u[S][V];  // u: b in the forward direction, d in the backward one
+    RowEvents e;
+    int count;
+};
+
+// Rows that are not there, or in no sequence, become the identity; the initial state of a sequence that starts here
+// joins b, and its first row is then b alone (in the backward direction: the gradient of a state joins
+// the derivatives of the row it was taken from).
+template <bool REVERSE, typename A, int V, int S>
+__device__ __forceinline__ void settle_rows(Rows<A, V, S>& r, const SequenceWalk& walk, int row0, const A* joins, int64_t dim, bool live) {
+    if (r.count < S || r.e.dead) {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if (s >= r.count || (r.e.dead >> s & 1u)) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) { r.a[s][v] = A(1); r.u[s][v] = A(0); }
+            }
+    }
+    const unsigned at = REVERSE ? r.e.ends : r.e.starts;
+    if (at && joins && live) {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if (at >> s & 1u) {
+                const A* in = joins + sequence_of(walk, row0 + s) * dim;
+#pragma unroll
+                for (int v = 0; v < V; ++v) r.u[s][v] = REVERSE ? r.u[s][v] + in[v] : fma_(r.a[s][v], in[v], r.u[s][v]);
+            }
+    }
+}
+
+// Appends the rows to a map, in scan order.
+template <bool REVERSE, bool PACKED, typename A, int V, int S>
+__device__ __forceinline__ void append_rows(Map<A, V>& m, const Rows<A, V, S>& r) {
+    const unsigned drops = REVERSE ? r.e.ends : r.e.starts;
+    if (PACKED && drops) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int s = REVERSE ? S - 1 - i : i;
+            const bool drop = drops >> s & 1u;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (REVERSE) m.b[v] = r.a[s][v] * (drop ? r.u[s][v] : r.u[s][v] + m.b[v]);
+                else m.b[v] = drop ? r.u[s][v] : fma_(r.a[s][v], m.b[v], r.u[s][v]);
+                m.a[v] *= r.a[s][v];
+            }
+        }
+        m.drop = true;
+    } else {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int s = REVERSE ? S - 1 - i : i;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (REVERSE) m.b[v] = r.a[s][v] * (r.u[s][v] + m.b[v]);
+                else m.b[v] = fma_(r.a[s][v], m.b[v], r.u[s][v]);
+                m.a[v] *= r.a[s][v];
+            }
+        }
+    }
+}
+
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED>
 __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
     using A = Acc<X>;
-    constexpr int GV = SHARED ? 1 : V, kStages = Stages<X, G, V, GV, S, 1>::kCount;
+    constexpr int GV = SHARED ? 1 : V;
     extern __shared__ __align__(16) unsigned char smem[];
     const Place at(plan, p.dim, V);
     const uint64_t b = at.batch, c0 = at.c0;
     const bool live = at.live;
-    const int rows = int(p.rows);
+    const int stages = plan.stages, warps = plan.warps;
     const int64_t dim = int64_t(p.dim);
+    const int first = at.segment * plan.segment_rows, rows = min(int(p.rows), first + plan.segment_rows);
     const A* initial = p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr;
     A* state = p.state ? static_cast<A*>(p.state) + c0 : nullptr;
     A* marks = p.checkpoints
@@ -477,15 +476,15 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
     Prefetch<G, GV, S> fg;
     unsigned char* next = smem;
     fx.place(next, at.tc, plan.pairs);
-    next += kStages * fx.kStage;
+    next += stages * fx.kStage;
     fg.place(next, at.tc, plan.pairs);
-    next += kStages * fg.kStage;
-    ScanMemory<A> memory;
-    memory.place(next, at.lanes * V, plan.warps, at.cluster);
-    for (int c = threadIdx.x; c < memory.width; c += blockDim.x)
-        memory.run[c] = !PACKED && p.initial && at.first + c < p.dim ? static_cast<const A*>(p.initial)[b * p.dim + at.first + c] : A(0);
-    const int span = plan.warps * at.parts * at.cluster * S;
-    int row0 = (at.rank * plan.warps * at.parts + at.part) * S;
+    next += stages * fg.kStage;
+    const int width = at.lanes * V;
+    A* carry = reinterpret_cast<A*>(next) + at.tc * V;  // [warp][width]: the state on its way into each warp
+    next += sizeof(A) * width * warps;
+
+    const int span = warps * at.parts * S;
+    int row0 = first + at.part * S;
     const X* x = static_cast<const X*>(p.x) + b * p.x_batch + (live ? c0 : 0);
     const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
     const int64_t x_row = int64_t(p.x_row), gate_row = int64_t(p.gate_row);
@@ -508,168 +507,147 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
         fx.hold(x + int64_t(row) * x_row, x_row, n);
         fg.hold(gate + int64_t(row) * gate_row, gate_row, n);
     };
-    for (int k = 0; k < kStages - 1; ++k) fetch(k);
+    for (int k = 0; k < stages - 1; ++k) fetch(k);
     hold(row0);
-    if (at.cluster > 1) cooperative_groups::this_cluster().sync();  // all of it runs before any writes to another
+    A in[V];  // the state that enters the warp's rows
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        in[v] = !PACKED && initial && live ? initial[b * p.dim + v] : A(0);
+        if (at.warp == 0 && live) in[v] = through_segments<A, false, PACKED>(plan, b, at.segment, p.dim, c0 + v, in[v]);
+    }
     SequenceWalk walk;
     if (PACKED) {
-        walk.open(p, reinterpret_cast<int*>(next + ScanMemory<A>::bytes(memory.width, plan.warps, at.cluster)));
+        walk.open(p, reinterpret_cast<int*>(next));
         walk.seek(row0);
-        if (state && live && at.rank == 0)  // sequences without rows hand their initial state on
-            for (int j = at.part; j < walk.count; j += plan.warps * at.parts)
+        if (state && live && at.segment == 0)  // sequences without rows hand their initial state on
+            for (int j = at.part; j < walk.count; j += warps * at.parts)
                 if (offset_at(walk.offsets, walk.wide, j + 1) <= offset_at(walk.offsets, walk.wide, j))
                     for (int v = 0; v < V; ++v) state[j * dim + v] = initial ? initial[j * dim + v] : A(0);
     }
-    int turn = 0, stage = 0;
-    for (int base = 0; base < rows; base += span, row0 += span, turn ^= 1, stage = stage + 1 == kStages ? 0 : stage + 1) {
-        const int count = rows_left<S>(rows, row0, live);
-        fetch(stage == 0 ? kStages - 1 : stage - 1);  // its slots were read in the last iteration, before a barrier
-        RowEvents e;
+    const int link = 1 + at.warp, link_before = at.warp ? at.warp : warps;
+    A* leaving = carry + (at.warp + 1 == warps ? 0 : at.warp + 1) * width;
+    int stage = 0;
+    for (int base = first; base < rows; base += span, row0 += span, stage = stage + 1 == stages ? 0 : stage + 1) {
+        __syncwarp();
+        fetch(stage == 0 ? stages - 1 : stage - 1);  // its slots were read in the last iteration
+        Rows<A, V, S> r;
+        r.count = rows_left<S>(rows, row0, live);
         if (PACKED) {
             walk.advance(row0);
-            e = row_events<S>(walk, row0, rows);
+            r.e = row_events<S>(walk, row0, rows);
         }
-        A a[S][V], u[S][V], unused[1][V];
-        await_copies<kStages - 1>();
-        if (p.complement) factors<false, true>(p.form, fx, fg, stage, a, u, unused);
-        else factors<false, false>(p.form, fx, fg, stage, a, u, unused);
+        A unused[1][V];
+        await_copies(stages);
+        if (p.complement) factors<false, true>(p.form, fx, fg, stage, r.a, r.u, unused);
+        else factors<false, false>(p.form, fx, fg, stage, r.a, r.u, unused);
         hold(row0 + span);
-        if (count < S || (PACKED && e.dead)) {
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-                if (s >= count || (e.dead >> s & 1u)) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) { a[s][v] = A(1); u[s][v] = A(0); }
-                }
-        }
-        const bool events = PACKED && e.starts | e.ends | e.dead;
-        // the initial state of a sequence that starts here joins b: its first row is then b alone
-        if (events && e.starts && initial && live) {
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-                if (e.starts >> s & 1u) {
-                    const A* in = initial + sequence_of(walk, row0 + s) * dim;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) u[s][v] = fma_(a[s][v], in[v], u[s][v]);
-                }
-        }
+        settle_rows<false>(r, walk, row0, initial, dim, live);
         Map<A, V> m;
         m.clear();
-        if (!events) {
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    m.b[v] = s ? fma_(a[s][v], m.b[v], u[s][v]) : u[s][v];
-                    m.a[v] = s ? m.a[v] * a[s][v] : a[s][v];
-                }
-        } else {
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    m.b[v] = e.starts >> s & 1u ? u[s][v] : fma_(a[s][v], m.b[v], u[s][v]);
-                    m.a[v] *= a[s][v];
-                }
-            m.drop = e.starts;
-        }
+        append_rows<false, PACKED>(m, r);
         __syncwarp();
-        scan_warp<A, V, false, PACKED>(m, plan.log_lanes, memory);
-        __syncthreads();
-        if (at.cluster == 1) {
-            for (int c = threadIdx.x; c < memory.width; c += blockDim.x)
-                memory.run[c] = carry_through<A, false, PACKED>(memory, plan.warps, c, memory.run[c]);
-        } else {
-            carry_across<A, false, PACKED>(memory, plan.warps, at.cluster, at.rank, turn);
-        }
-        __syncthreads();
-        A h[V];
-        enter_rows<A, V, false>(m, plan.log_lanes, memory.carry + at.warp * memory.width + at.tc * V, h);
-        if (count) {
-            if (marks && row0 % int(kCheckpointRows) == 0)
+        scan_warp<A, V, false, PACKED>(m, plan.log_lanes);
+        if (base != first || at.warp) {
+            if (warps > 1) take_over(link_before);
+            else __syncwarp();
+            const Pack<A, V> c = load_pack<A, V>(carry + at.warp * width);
 #pragma unroll
-                for (int v = 0; v < V; ++v) marks[int64_t(row0 / int(kCheckpointRows)) * dim + v] = h[v];
-            if (!events) {
-                X* to = out;
-                const int stored = out ? count : 0;
+            for (int v = 0; v < V; ++v) in[v] = c.v[v];
+        }
+        A h[V];
+        enter_rows<A, V, false>(m, plan.log_lanes, in, h, leaving);
+        if (warps > 1 && (at.warp + 1 < warps || base + span < rows)) give(link);
+        if (r.count) {
+            if (marks && row0 % int(kCheckpointRows) == 0) {
+                Pack<A, V> mark;
+#pragma unroll
+                for (int v = 0; v < V; ++v) mark.v[v] = h[v];
+                store_pack<A, V>(marks + int64_t(row0 / int(kCheckpointRows)) * dim, mark);
+            }
+            const int stored = out ? r.count : 0;
+            X* to = out;
+            if (!(PACKED && (r.e.starts | r.e.ends | r.e.dead))) {
                 if (stored == S) {
 #pragma unroll
                     for (int s = 0; s < S; ++s, to += dim) {
 #pragma unroll
-                        for (int v = 0; v < V; ++v) h[v] = fma_(a[s][v], h[v], u[s][v]);
+                        for (int v = 0; v < V; ++v) h[v] = fma_(r.a[s][v], h[v], r.u[s][v]);
                         store_pack<X, V>(to, narrow_pack<X, V>(h));
                     }
                 } else {
 #pragma unroll
                     for (int s = 0; s < S; ++s, to += dim) {
 #pragma unroll
-                        for (int v = 0; v < V; ++v) h[v] = fma_(a[s][v], h[v], u[s][v]);
+                        for (int v = 0; v < V; ++v) h[v] = fma_(r.a[s][v], h[v], r.u[s][v]);
                         if (s < stored) store_pack<X, V>(to, narrow_pack<X, V>(h));
                     }
                 }
             } else {
 #pragma unroll
-                for (int s = 0; s < S; ++s) {
+                for (int s = 0; s < S; ++s, to += dim) {
                     A y[V];
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
-                        h[v] = e.starts >> s & 1u ? u[s][v] : fma_(a[s][v], h[v], u[s][v]);
-                        y[v] = e.dead >> s & 1u ? A(0) : h[v];
+                        h[v] = r.e.starts >> s & 1u ? r.u[s][v] : fma_(r.a[s][v], h[v], r.u[s][v]);
+                        y[v] = r.e.dead >> s & 1u ? A(0) : h[v];
                     }
-                    if (out && s < count) store_pack<X, V>(out + s * dim, narrow_pack<X, V>(y));
-                    if (state && (e.ends >> s & 1u)) {
-                        A* to = state + sequence_of(walk, row0 + s) * dim;
+                    if (s < stored) store_pack<X, V>(to, narrow_pack<X, V>(y));
+                    if (state && (r.e.ends >> s & 1u)) {
+                        A* last = state + sequence_of(walk, row0 + s) * dim;
 #pragma unroll
-                        for (int v = 0; v < V; ++v) to[v] = h[v];
+                        for (int v = 0; v < V; ++v) last[v] = h[v];
                     }
                 }
             }
         }
         if (out) out += out_span;
     }
-    if (!PACKED && p.state && at.rank == 0)
-        for (int c = threadIdx.x; c < memory.width && at.first + c < p.dim; c += blockDim.x)
-            static_cast<A*>(p.state)[b * p.dim + at.first + c] = memory.run[c];
+    // what left the last warp's last part
+    if (!PACKED && state && live && at.segment + 1 == plan.segments && at.warp + 1 == warps && at.lane >= 32 - at.lanes)
+#pragma unroll
+        for (int v = 0; v < V; ++v) state[b * p.dim + v] = leaving[v];
 }
 
 // One iteration takes its rows backward and then, from a checkpoint, forward again (for h_{t-1}), both in
 // registers, so that x, the gates and the derivatives are read once and h, rounded or not, is not read at all.
+// Checkpoints are near enough for a warp to start from one, or from the warp before; the gradient goes round
+// the ring of warps, from the last to the first.
 // Shared gates: each thread sums its V channels, 1 << fold_log neighbouring lanes are folded by shuffles,
 // and `partial` takes one value per row and fold (dgate itself where a fold is a whole gate).
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED, bool COMPLEMENT>
 __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(const RecurrenceArgs p, const RecurrencePlan plan,
                                                                      Acc<X>* partial) {
     using A = Acc<X>;
-    constexpr int GV = SHARED ? 1 : V, kStages = Stages<X, G, V, GV, S, 2>::kCount;
+    constexpr int GV = SHARED ? 1 : V;
     extern __shared__ __align__(16) unsigned char smem[];
     const Place at(plan, p.dim, V);
     const uint64_t b = at.batch, c0 = at.c0;
     const bool live = at.live;
-    const int rows = int(p.rows);
+    const int stages = plan.stages, warps = plan.warps;
     const int64_t dim = int64_t(p.dim);
+    const int first = at.segment * plan.segment_rows, rows = min(int(p.rows), first + plan.segment_rows);
     const A* initial = p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr;
     const A* state_derivs = p.state_derivs ? static_cast<const A*>(p.state_derivs) + c0 : nullptr;
     A* dinitial = p.dinitial ? static_cast<A*>(p.dinitial) + c0 : nullptr;
-    const A* marks = static_cast<const A*>(p.marks) + b * ((p.rows + kCheckpointRows - 1) / kCheckpointRows) * p.dim + at.first;
 
     Prefetch<X, V, S> fx, fd;
     Prefetch<G, GV, S> fg;
     unsigned char* next = smem;
     fx.place(next, at.tc, plan.pairs);
-    next += kStages * fx.kStage;
+    next += stages * fx.kStage;
     fd.place(next, at.tc, plan.pairs);
-    next += kStages * fd.kStage;
+    next += stages * fd.kStage;
     fg.place(next, at.tc, plan.pairs);
-    next += kStages * fg.kStage;
-    ScanMemory<A> ahead, back;
-    ahead.place(next, at.lanes * V, plan.warps, 1);
-    next += ScanMemory<A>::bytes(ahead.width, plan.warps, 1);
-    back.place(next, ahead.width, plan.warps, at.cluster);
-    A* entering = reinterpret_cast<A*>(next + ScanMemory<A>::bytes(ahead.width, plan.warps, at.cluster));  // [stage][width]
-    for (int c = threadIdx.x; c < back.width; c += blockDim.x)
-        back.run[c] = !PACKED && p.state_derivs && at.first + c < p.dim ? static_cast<const A*>(p.state_derivs)[b * p.dim + at.first + c] : A(0);
-    const int block = plan.warps * at.parts * S, span = block * at.cluster;
-    int base = (rows - 1) / span * span, row0 = base + at.rank * block + at.part * S;
+    next += stages * fg.kStage;
+    const int width = at.lanes * V;
+    A* ahead = reinterpret_cast<A*>(next) + at.tc * V;  // [warp][width]: the state on its way into each warp
+    A* back = ahead + warps * width;                    // [warp][width]: the gradient
+    A* entering = back + (warps + at.warp) * width;     // [stage][warp][width]: checkpoints
+    next += sizeof(A) * width * warps * (2 + stages);
+
+    const int span = warps * at.parts * S;
+    int base = first + (rows - 1 - first) / span * span, row0 = base + at.part * S;
+    const int last_base = base;
     const X* x = static_cast<const X*>(p.x) + b * p.x_batch + (live ? c0 : 0);
     const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
     const X* derivs = static_cast<const X*>(p.derivs) + b * p.d_batch + (live ? c0 : 0);
@@ -678,22 +656,23 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
     const X* px = fx.start(x + int64_t(row0) * x_row, x_row);
     const G* pg = fg.start(gate + int64_t(row0) * gate_row, gate_row);
     const X* pd = fd.start(derivs + int64_t(row0) * d_row, d_row);
+    // warps whose first row is a checkpoint's start from it, the others from the warp before
+    const int warp_rows = at.parts * S;
+    const bool marked = at.warp * warp_rows % int(kCheckpointRows) == 0;
+    const bool passes = at.warp + 1 < warps && (at.warp + 1) * warp_rows % int(kCheckpointRows) != 0;
+    const A* marks = static_cast<const A*>(p.marks) + b * ((p.rows + kCheckpointRows - 1) / kCheckpointRows) * p.dim + c0;
     const int64_t out_span = span * dim;
-    X* dx = static_cast<X*>(p.dx) + (int64_t(b) * rows + row0) * dim + c0;
-    G* dgate = static_cast<G*>(p.dgate) + (SHARED ? 0 : (int64_t(b) * rows + row0) * dim + c0);
+    X* dx = static_cast<X*>(p.dx) + (int64_t(b * p.rows) + row0) * dim + c0;
+    G* dgate = static_cast<G*>(p.dgate) + (SHARED ? 0 : (int64_t(b * p.rows) + row0) * dim + c0);
     int coming = row0, coming_base = base;
     const auto fetch = [&](int stage) {
-        const int n = rows_left<S>(rows, coming, live);
+        const int n = coming_base >= first ? rows_left<S>(rows, coming, live) : 0;
         fx.issue(stage, x, px, x_row, n);
         fg.issue(stage, gate, pg, gate_row, n);
         fd.issue(stage, derivs, pd, d_row, n);
-        // the checkpoint that enters the CTA's rows: each column's thread copies its own
-        const int own = coming_base + at.rank * block;
-        const A* mark = marks + int64_t(own / int(kCheckpointRows)) * dim;
-        for (int c = threadIdx.x; c < ahead.width; c += blockDim.x) {
-            const bool on = own >= 0 && own < rows && at.first + c < p.dim;
-            copy_async<sizeof(A)>(entering + stage * ahead.width + c, on ? mark + c : static_cast<const A*>(p.marks), on);
-        }
+        const int own = coming_base + at.warp * warp_rows;  // the warp's first row
+        if (marked && live && at.lane < at.lanes && coming_base >= first && own < rows)
+            copy_async<sizeof(A) * V>(entering + stage * warps * width, marks + int64_t(own / int(kCheckpointRows)) * dim);
         commit_copies();
         px -= x_span;
         pg -= gate_span;
@@ -701,166 +680,258 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
         coming -= span;
         coming_base -= span;
     };
-    const auto hold = [&](int row) {
-        const int n = rows_left<S>(rows, row, live);
+    const auto hold = [&](int row, bool on) {
+        const int n = on ? rows_left<S>(rows, row, live) : 0;
         fx.hold(x + int64_t(row) * x_row, x_row, n);
         fg.hold(gate + int64_t(row) * gate_row, gate_row, n);
         fd.hold(derivs + int64_t(row) * d_row, d_row, n);
     };
-    for (int k = 0; k < kStages - 1; ++k) fetch(k);
-    hold(row0);
-    if (at.cluster > 1) cooperative_groups::this_cluster().sync();  // all of it runs before any writes to another
+    for (int k = 0; k < stages - 1; ++k) fetch(k);
+    hold(row0, true);
+    A w[V];  // the gradient that enters the warp's rows from behind
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        w[v] = !PACKED && state_derivs && live ? state_derivs[b * p.dim + v] : A(0);
+        if (at.warp + 1 == warps && live) w[v] = through_segments<A, true, PACKED>(plan, b, at.segment, p.dim, c0 + v, w[v]);
+    }
     SequenceWalk walk;
     if (PACKED) {
-        walk.open(p, reinterpret_cast<int*>(entering + kStages * ahead.width));
+        walk.open(p, reinterpret_cast<int*>(next));
         walk.seek(row0);
-        if (dinitial && live && at.rank == 0)
-            for (int j = at.part; j < walk.count; j += plan.warps * at.parts)
+        if (dinitial && live && at.segment == 0)
+            for (int j = at.part; j < walk.count; j += warps * at.parts)
                 if (offset_at(walk.offsets, walk.wide, j + 1) <= offset_at(walk.offsets, walk.wide, j))
                     for (int v = 0; v < V; ++v) dinitial[j * dim + v] = state_derivs ? state_derivs[j * dim + v] : A(0);
     }
-    int turn = 0, stage = 0;
-    for (; base >= 0; base -= span, row0 -= span, turn ^= 1, stage = stage + 1 == kStages ? 0 : stage + 1) {
-        const int count = rows_left<S>(rows, row0, live);
-        fetch(stage == 0 ? kStages - 1 : stage - 1);  // its slots were read in the last iteration, before a barrier
-        RowEvents e;
+    // hand-overs: 1 .. W of the gradient to the warp before (or from the first to the last), W + 1 .. of the state
+    const int link = 1 + at.warp, link_behind = at.warp + 1 == warps ? 1 : 2 + at.warp;
+    A* leaving = back + (at.warp ? at.warp - 1 : warps - 1) * width;
+    int stage = 0;
+    for (; base >= first; base -= span, row0 -= span, stage = stage + 1 == stages ? 0 : stage + 1) {
+        __syncwarp();
+        fetch(stage == 0 ? stages - 1 : stage - 1);  // its slots were read in the last iteration
+        Rows<A, V, S> r;  // u: derivatives, later their sums
+        r.count = rows_left<S>(rows, row0, live);
         if (PACKED) {
             walk.retreat(row0);
-            e = row_events<S>(walk, row0, rows);
+            r.e = row_events<S>(walk, row0, rows);
         }
-        A a[S][V], rest[S][V], x_[S][V], d[S][V];
-        await_copies<kStages - 1>();
-        factors<true, false>(p.form, fx, fg, stage, a, x_, rest);
+        A rest[S][V], x_[S][V];
+        await_copies(stages);
+        factors<true, false>(p.form, fx, fg, stage, r.a, x_, rest);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             const Pack<X, V> rd = fd.take(stage, s);
 #pragma unroll
-            for (int v = 0; v < V; ++v) d[s][v] = widen(rd.v[v]);
+            for (int v = 0; v < V; ++v) r.u[s][v] = widen(rd.v[v]);
         }
-        hold(row0 - span);
-        if (count < S || (PACKED && e.dead)) {
+        hold(row0 - span, base > first);
+        if (r.count < S || (PACKED && r.e.dead)) {
 #pragma unroll
             for (int s = 0; s < S; ++s)
-                if (s >= count || (e.dead >> s & 1u)) {
+                if (s >= r.count || (r.e.dead >> s & 1u)) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) { a[s][v] = A(1); rest[s][v] = x_[s][v] = d[s][v] = A(0); }
+                    for (int v = 0; v < V; ++v) rest[s][v] = x_[s][v] = A(0);
                 }
         }
-        const bool events = PACKED && e.starts | e.ends | e.dead;
-        // the gradient of a state joins the derivatives of the row that it was taken from
-        if (events && e.ends && state_derivs && live) {
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-                if (e.ends >> s & 1u) {
-                    const A* in = state_derivs + sequence_of(walk, row0 + s) * dim;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) d[s][v] += in[v];
-                }
-        }
-        Map<A, V> m, g;
-        m.clear();
-        g.clear();
+        settle_rows<true>(r, walk, row0, state_derivs, dim, live);
         const auto input = [&](int s, int v) { return COMPLEMENT ? rest[s][v] * x_[s][v] : x_[s][v]; };
-        if (!events) {
+        const auto first_state = [&](int s, A (&h)[V]) {
+            const A* from = initial && live ? initial + sequence_of(walk, row0 + s) * dim : nullptr;
 #pragma unroll
-            for (int s = 0; s < S; ++s)
+            for (int v = 0; v < V; ++v) h[v] = from ? from[v] : A(0);
+        };
+        Map<A, V> m, g;
+        g.clear();
+        append_rows<true, PACKED>(g, r);
+        m.clear();
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const int q = S - 1 - s;
-                    m.b[v] = s ? fma_(a[s][v], m.b[v], input(s, v)) : input(s, v);
-                    m.a[v] = s ? m.a[v] * a[s][v] : a[s][v];
-                    g.b[v] = a[q][v] * (s ? d[q][v] + g.b[v] : d[q][v]);
-                }
-        } else {
+        for (int s = 0; s < S; ++s) {
+            if (PACKED && (r.e.starts >> s & 1u)) first_state(s, m.b);
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-                if (e.starts >> s & 1u) {
-                    const A* in = initial && live ? initial + sequence_of(walk, row0 + s) * dim : nullptr;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) m.b[v] = in ? in[v] : A(0);
-                }
-                const int q = S - 1 - s;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    m.b[v] = fma_(a[s][v], m.b[v], input(s, v));
-                    m.a[v] *= a[s][v];
-                    g.b[v] = a[q][v] * (e.ends >> q & 1u ? d[q][v] : d[q][v] + g.b[v]);
-                }
-            }
-            m.drop = e.starts;
-            g.drop = e.ends;
+            for (int v = 0; v < V; ++v) m.b[v] = fma_(r.a[s][v], m.b[v], input(s, v));
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) g.a[v] = m.a[v];
+        for (int v = 0; v < V; ++v) m.a[v] = g.a[v];
+        m.drop = PACKED && r.e.starts;
         __syncwarp();
-        scan_warp<A, V, false, PACKED>(m, plan.log_lanes, ahead);
-        scan_warp<A, V, true, PACKED>(g, plan.log_lanes, back);
-        __syncthreads();
-        for (int c = threadIdx.x; c < ahead.width; c += blockDim.x) carry_through<A, false, PACKED>(ahead, plan.warps, c, entering[stage * ahead.width + c]);
-        if (at.cluster == 1) {
-            for (int c = threadIdx.x; c < back.width; c += blockDim.x)
-                back.run[c] = carry_through<A, true, PACKED>(back, plan.warps, c, back.run[c]);
-        } else {
-            carry_across<A, true, PACKED>(back, plan.warps, at.cluster, at.rank, turn);
+        scan_warp<A, V, false, PACKED>(m, plan.log_lanes);
+        scan_warp<A, V, true, PACKED>(g, plan.log_lanes);
+        // forward: the checkpoint, or what the warp before left
+        A in[V], h[V];
+        if (!marked) take_over(warps + at.warp);
+        {
+            const Pack<A, V> c = load_pack<A, V>(marked ? entering + stage * warps * width : ahead + at.warp * width);
+#pragma unroll
+            for (int v = 0; v < V; ++v) in[v] = c.v[v];
         }
-        __syncthreads();
-        A in[V], w[V];
-        enter_rows<A, V, false>(m, plan.log_lanes, ahead.carry + at.warp * ahead.width + at.tc * V, in);
-        enter_rows<A, V, true>(g, plan.log_lanes, back.carry + at.warp * back.width + at.tc * V, w);
-        // backward through the rows: d becomes g
+        enter_rows<A, V, false>(m, plan.log_lanes, in, h, ahead + (at.warp + 1 == warps ? 0 : at.warp + 1) * width);
+        if (passes) give(warps + 1 + at.warp);
+        // backward: the gradient
+        if (base != last_base || at.warp + 1 < warps) {
+            if (warps > 1) take_over(link_behind);
+            else __syncwarp();
+            const Pack<A, V> c = load_pack<A, V>(back + at.warp * width);
+#pragma unroll
+            for (int v = 0; v < V; ++v) w[v] = c.v[v];
+        }
+        A behind[V];
+        enter_rows<A, V, true>(g, plan.log_lanes, w, behind, leaving);
+        if (warps > 1 && (at.warp || base > first)) give(link);
+        // backward through the rows: the derivatives become g
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                if (!(PACKED && (e.ends >> s & 1u))) d[s][v] += w[v];
-                w[v] = a[s][v] * d[s][v];
+                if (!(PACKED && (r.e.ends >> s & 1u))) r.u[s][v] += behind[v];
+                behind[v] = r.a[s][v] * r.u[s][v];
             }
-            if (PACKED && dinitial && live && (e.starts >> s & 1u)) {
+            if (PACKED && dinitial && live && (r.e.starts >> s & 1u)) {
                 A* to = dinitial + sequence_of(walk, row0 + s) * dim;
 #pragma unroll
-                for (int v = 0; v < V; ++v) to[v] = w[v];
+                for (int v = 0; v < V; ++v) to[v] = behind[v];
             }
         }
-        // forward through them with h_{t-1} in `in`
+        // forward through them with h_{t-1} in `h`
         X* to_x = dx;
         G* to_gate = dgate;
         dx -= out_span;
         dgate -= SHARED ? 0 : out_span;
 #pragma unroll
         for (int s = 0; s < S; ++s, to_x += dim, to_gate += SHARED ? 0 : dim) {
-            if (PACKED && (e.starts >> s & 1u)) {
-                const A* from = initial && live ? initial + sequence_of(walk, row0 + s) * dim : nullptr;
-#pragma unroll
-                for (int v = 0; v < V; ++v) in[v] = from ? from[v] : A(0);
-            }
+            if (PACKED && (r.e.starts >> s & 1u)) first_state(s, h);
             A gx[V], gg[V], sum = A(0);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                gx[v] = COMPLEMENT ? rest[s][v] * d[s][v] : d[s][v];
-                gg[v] = d[s][v] * (COMPLEMENT ? in[v] - x_[s][v] : in[v]);
-                if (p.form != kGateValue) gg[v] *= a[s][v];
+                gx[v] = COMPLEMENT ? rest[s][v] * r.u[s][v] : r.u[s][v];
+                gg[v] = r.u[s][v] * (COMPLEMENT ? h[v] - x_[s][v] : h[v]);
+                if (p.form != kGateValue) gg[v] *= r.a[s][v];
                 if (p.form == kGateLogit) gg[v] *= rest[s][v];
-                if (PACKED && (e.dead >> s & 1u)) gx[v] = gg[v] = A(0);
+                if (PACKED && (r.e.dead >> s & 1u)) gx[v] = gg[v] = A(0);
                 sum += gg[v];
-                in[v] = fma_(a[s][v], in[v], input(s, v));
+                h[v] = fma_(r.a[s][v], h[v], input(s, v));
             }
-            if (s < count) store_pack<X, V>(to_x, narrow_pack<X, V>(gx));
+            if (s < r.count) store_pack<X, V>(to_x, narrow_pack<X, V>(gx));
             if (SHARED) {
-                sum = s < count ? sum : A(0);
+                sum = s < r.count ? sum : A(0);
                 for (int k = 1; k < 1 << plan.fold_log; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-                if (s < count && (at.tc & ((1 << plan.fold_log) - 1)) == 0) {
-                    const int64_t fold = int64_t(c0 / V) >> plan.fold_log, row = int64_t(b) * rows + row0 + s;
+                if (s < r.count && (at.tc & ((1 << plan.fold_log) - 1)) == 0) {
+                    const int64_t fold = int64_t(c0 / V) >> plan.fold_log, row = int64_t(b * p.rows) + row0 + s;
                     if (partial) partial[row * ((dim / V) >> plan.fold_log) + fold] = sum;
                     else to_gate[row * int64_t(p.gate_dim) + fold] = narrow<G>(sum);
                 }
-            } else if (s < count) {
+            } else if (s < r.count) {
                 if constexpr (std::is_same_v<Acc<G>, A>) store_pack<G, V>(to_gate, narrow_pack<G, V>(gg));
             }
         }
     }
-    if (!PACKED && p.dinitial && at.rank == 0)
-        for (int c = threadIdx.x; c < back.width && at.first + c < p.dim; c += blockDim.x)
-            static_cast<A*>(p.dinitial)[b * p.dim + at.first + c] = back.run[c];
+    // what left the first warp's first part
+    if (!PACKED && dinitial && live && at.segment == 0 && at.warp == 0 && at.lane < at.lanes)
+#pragma unroll
+        for (int v = 0; v < V; ++v) dinitial[b * p.dim + v] = leaving[v];
+}
+
+// Map of every segment of the rows: of the recurrence (x, initial states), or REVERSE of the gradient (derivatives in
+// the place of x, gradients of states).  Each thread takes a contiguous run of rows, S at a time, and
+// appends them to its map; parts and warps are composed once, at the end.
+template <typename X, typename G, int V, int S, bool SHARED, bool PACKED, bool REVERSE>
+__global__ void __launch_bounds__(kCtaThreads, 2) recurrence_maps_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
+    using A = Acc<X>;
+    constexpr int GV = SHARED ? 1 : V;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const Place at(plan, p.dim, V);
+    const uint64_t b = at.batch, c0 = at.c0;
+    const bool live = at.live;
+    const int stages = plan.stages, warps = plan.warps;
+    const int64_t dim = int64_t(p.dim);
+    const int run = plan.segment_rows / (warps * at.parts);  // rows of a thread
+    const int begin = at.segment * plan.segment_rows + at.part * run, end = min(int(p.rows), begin + run);
+    const A* joins = static_cast<const A*>(REVERSE ? p.state_derivs : p.initial);
+    if (joins) joins += c0;
+    const int64_t x_row = int64_t(REVERSE ? p.d_row : p.x_row), gate_row = int64_t(p.gate_row);
+    const X* x = static_cast<const X*>(REVERSE ? p.derivs : p.x) + b * (REVERSE ? p.d_batch : p.x_batch) + (live ? c0 : 0);
+    const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
+
+    Prefetch<X, V, S> fx;
+    Prefetch<G, GV, S> fg;
+    unsigned char* next = smem;
+    fx.place(next, at.tc, plan.pairs);
+    next += stages * fx.kStage;
+    fg.place(next, at.tc, plan.pairs);
+    next += stages * fg.kStage;
+    const int width = at.lanes * V;
+    A* maps = reinterpret_cast<A*>(next);  // [warp][A, B][width]
+    next += sizeof(A) * 2 * width * warps;
+    int* drops = reinterpret_cast<int*>(next);  // [warp]
+    next += sizeof(int) * warps;
+    SequenceWalk walk;
+    if (PACKED) {
+        walk.open(p, reinterpret_cast<int*>(next));
+        walk.seek(REVERSE ? begin + run : begin);
+    }
+    int coming = REVERSE ? begin + run - S : begin;
+    const auto fetch = [&](int stage) {
+        const int n = coming >= begin ? rows_left<S>(end, coming, live) : 0;
+        fx.issue(stage, x, fx.start(x + int64_t(coming) * x_row, x_row), x_row, n);
+        fg.issue(stage, gate, fg.start(gate + int64_t(coming) * gate_row, gate_row), gate_row, n);
+        commit_copies();
+        coming += REVERSE ? -S : S;
+    };
+    const auto hold = [&](int row) {
+        const int n = row >= begin ? rows_left<S>(end, row, live) : 0;
+        fx.hold(x + int64_t(row) * x_row, x_row, n);
+        fg.hold(gate + int64_t(row) * gate_row, gate_row, n);
+    };
+    hold(coming);
+    for (int k = 0; k < stages - 1; ++k) fetch(k);
+    Map<A, V> m;
+    m.clear();
+    int stage = 0;
+    for (int done = 0; done < run; done += S, stage = stage + 1 == stages ? 0 : stage + 1) {
+        const int row0 = REVERSE ? begin + run - S - done : begin + done;
+        __syncwarp();
+        fetch(stage == 0 ? stages - 1 : stage - 1);
+        Rows<A, V, S> r;
+        r.count = rows_left<S>(end, row0, live);
+        if (PACKED) {
+            if (REVERSE) walk.retreat(row0); else walk.advance(row0);
+            r.e = row_events<S>(walk, row0, end);
+        }
+        A unused[1][V];
+        await_copies(stages);
+        if (!REVERSE && p.complement) factors<false, true>(p.form, fx, fg, stage, r.a, r.u, unused);
+        else factors<false, false>(p.form, fx, fg, stage, r.a, r.u, unused);
+        hold(REVERSE ? row0 - S : row0 + S);
+        settle_rows<REVERSE>(r, walk, row0, joins, dim, live);
+        append_rows<REVERSE, PACKED>(m, r);
+    }
+    __syncwarp();
+    scan_warp<A, V, REVERSE, PACKED>(m, plan.log_lanes);
+    if (REVERSE ? at.lane < at.lanes : at.lane >= 32 - at.lanes) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            maps[2 * at.warp * width + at.tc * V + v] = m.a[v];
+            maps[(2 * at.warp + 1) * width + at.tc * V + v] = m.b[v];
+        }
+        if (at.tc == 0) drops[at.warp] = m.drop;
+    }
+    __syncthreads();
+    const uint64_t to = b * plan.segments + at.segment, strip = c0 - uint64_t(at.tc) * V;
+    for (int c = threadIdx.x; c < width && strip + c < p.dim; c += blockDim.x) {
+        A a = A(1), f = A(0);
+        int drop = 0;
+        for (int i = 0; i < warps; ++i) {
+            const int w = REVERSE ? warps - 1 - i : i;
+            const A wb = maps[(2 * w + 1) * width + c], wa = maps[2 * w * width + c];
+            f = drops[w] ? wb : fma_(wa, f, wb);
+            a *= wa;
+            drop |= drops[w];
+        }
+        A* map = static_cast<A*>(plan.maps) + 2 * to * p.dim + strip + c;
+        map[0] = a;
+        map[p.dim] = f;
+        if (c == 0 && strip == 0) plan.drops[to] = drop;
+    }
 }
 
 // dgate[row, h] = sum of the `count` partial sums of gate h, in their order.

@@ -21,8 +21,9 @@ inline size_t element_size(int type) { return type == kFloat64 ? 8 : type == kFl
 // States, checkpoints and their gradients: float64 for float64 inputs, else float32.
 inline size_t state_size(int type) { return type == kFloat64 ? 8 : 4; }
 
-// Rows between two checkpoints of a recurrence (the state entering rows 0, 64, 128, ..).
-constexpr uint64_t kCheckpointRows = 64;
+// Rows between two checkpoints of a recurrence (the state entering rows 0, 16, 32, ..): near enough for the
+// backward pass to start each warp's rows without waiting for the others', for 1/16 of a state's bytes a row.
+constexpr uint64_t kCheckpointRows = 16;
 
 // Rows are counted in 32 bits, with room for the blocks that an iteration looks ahead.
 constexpr uint64_t kMaxRows = 1ull << 30;

@@ -14,7 +14,7 @@ from .sequence_inputs import (batched_rows, call, check_like, check_state, conti
                               state_dtype, stream_of, zeros)
 
 GATE_FORMS = {"value": 0, "log": 1, "logit": 2}
-CHECKPOINT_ROWS = 64  # rows between two of the states kept for the backward pass
+CHECKPOINT_ROWS = 16  # rows between two of the states kept for the backward pass
 
 
 class _Recurrence:
@@ -113,7 +113,7 @@ def linear_recurrence(
         give wrong numbers.
     :param return_state: also return the state after the last row (``initial`` for an empty sequence),
         ready for ``linear_recurrence_step``.
-    :param return_checkpoints: also return the states before rows 0, 64, 128, .., which
+    :param return_checkpoints: also return the states before rows 0, 16, 32, .., which
         ``linear_recurrence_backprop`` would otherwise compute again.
     :return: ``h`` like ``x`` (contiguous), or a tuple ``(h, state, checkpoints)`` without the parts not
         asked for.

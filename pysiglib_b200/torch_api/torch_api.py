@@ -232,7 +232,7 @@ sig_coef.__doc__ = sig_coef_forward.__doc__
 
 
 class LinearRecurrence(torch.autograd.Function):
-    """Keeps x, the gates and one state of 64 for the backward pass, not h."""
+    """Keeps x, the gates and one state of 16 for the backward pass, not h."""
 
     @staticmethod
     def forward(ctx, x, gate, initial, gate_form, complement, offsets):

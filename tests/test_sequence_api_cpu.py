@@ -90,7 +90,7 @@ def test_recurrence_without_rows():
         x, g = np.zeros(shape, np.float32), np.zeros(gates, np.float32)
         start = np.arange(shape[0] * 6, dtype=np.float32).reshape(shape[0], 6)
         h, state, marks = psl.linear_recurrence(x, g, start, return_state=True, return_checkpoints=True)
-        assert h.shape == shape and marks.shape == (shape[0], -(-shape[1] // 64), 6)
+        assert h.shape == shape and marks.shape == (shape[0], -(-shape[1] // 16), 6)
         np.testing.assert_array_equal(state, start)
         dx, dg, ds = psl.linear_recurrence_backprop(x, x, g, start, state_derivs=start + 1, checkpoints=marks)
         assert dx.shape == shape and dg.shape == gates
