@@ -32,11 +32,15 @@ bool aligned_to(const RecurrenceArgs& p, size_t bytes) {
            (p.gate_dim != p.dim || fits(p.gate, element_size(p.gate_type), p.dim, p.gate_batch, p.gate_row));
 }
 
+#ifndef SIG_SEGW
+#define SIG_SEGW 8
+#endif
 // Up to 8 warps whose lanes lie side by side in the channels as far as 128 bytes of a row go (full lines), and
 // behind one another in the rows beyond that.  Two CTAs an SM are there at a time.  Where full lines make fewer
 // strips than there are SMs, half lines do if that is enough; else the rows are cut into segments.
 template <typename X>
 RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
+    constexpr uint64_t kResident = 16;  // warps an SM holds at 128 registers a thread
     const uint64_t per_row = (p.dim + V - 1) / V, sms = device_context(current_device()).sm_count;
     const int columns = log2_ceil(per_row), needed = log2_ceil((p.rows + S - 1) / S);
     RecurrencePlan plan{};
@@ -50,9 +54,13 @@ RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     if (ctas(plan.log_lanes) > 0x7fffffffull)
         throw std::invalid_argument("linear_recurrence: problem too large for one kernel launch");
     plan.strips = static_cast<unsigned>(((per_row - 1) >> plan.log_lanes) + 1);
-    const uint64_t span = uint64_t(plan.warps) * (32 >> plan.log_lanes) * S, blocks = (p.rows + span - 1) / span;
+    // shorter rings where there are many strips: all of them resident at a time, and fewer hand-overs
+    const uint64_t strips = ctas(plan.log_lanes), warp_rows = uint64_t(32 >> plan.log_lanes) * S;
+    while (plan.warps > 1 && strips * plan.warps > kResident * sms && plan.warps / 2 * warp_rows % kCheckpointRows == 0) plan.warps /= 2;
+    if (strips < sms) plan.warps = std::min(plan.warps, SIG_SEGW);
+    const uint64_t span = plan.warps * warp_rows, blocks = (p.rows + span - 1) / span;
     uint64_t segments = 1;
-    if (ctas(plan.log_lanes) < sms) segments = std::min(blocks, 2 * sms / ctas(plan.log_lanes));
+    if (strips < sms) segments = std::min(blocks, kResident * sms / (strips * plan.warps));
     const uint64_t length = (blocks + segments - 1) / segments;
     plan.segments = static_cast<int>((blocks + length - 1) / length);
     plan.segment_rows = static_cast<int>(length * span);
@@ -65,16 +73,19 @@ void check(const char* what) {
     if (err != cudaSuccess) throw CudaFailure(err, std::string(what) + ": " + cudaGetErrorString(err));
 }
 
-size_t offset_bytes(const RecurrenceArgs& p) {
-    return p.sequences && p.sequences < uint64_t(kLocalOffsets) ? (p.sequences + 1) * sizeof(int) : 0;
+// Shared memory behind the rings: the offsets of packed sequences and what composes the segments.
+template <typename A>
+size_t front_bytes(const RecurrenceArgs& p, const RecurrencePlan& plan, int width) {
+    const int values = std::max(32 * plan.warps, width);
+    return offset_room(p) + (plan.segments > 1 ? 2 * values * sizeof(A) + (values / width + 1) * sizeof(int) : 0);
 }
 
-// As many stages as two CTAs an SM have room for; returns the bytes of shared memory of a CTA.
-size_t shared_memory(RecurrencePlan& plan, size_t stage, size_t fixed) {
-    constexpr size_t kRoom = (228 * 1024 / 2) - 1024;
+// As many stages as the resident CTAs of an SM (16 warps) have room for; returns the bytes of shared memory of a CTA.
+size_t shared_memory(RecurrencePlan& plan, size_t stage_of_warp, size_t fixed) {
+    const size_t room = size_t(228) * 1024 / (16 / plan.warps) - 1024;
     plan.stages = 4;
-    while (plan.stages > 2 && fixed + plan.stages * stage > kRoom) --plan.stages;
-    return fixed + plan.stages * stage;
+    while (plan.stages > 2 && fixed + plan.stages * plan.warps * stage_of_warp > room) --plan.stages;
+    return fixed + plan.stages * plan.warps * stage_of_warp;
 }
 
 template <typename... Params, typename... Args>
@@ -93,9 +104,9 @@ size_t maps_bytes(const RecurrenceArgs& p, const RecurrencePlan& plan) {
 
 template <typename X, typename G, int V, bool SHARED, bool REVERSE>
 void reduce_segments(const RecurrenceArgs& p, RecurrencePlan plan, cudaStream_t stream) {
-    constexpr int S = V == 1 ? 8 : 4;  // divides the rows of a thread: a block's are a multiple of it
-    const size_t smem = shared_memory(plan, Prefetch<X, V, S>::kStage + Prefetch<G, SHARED ? 1 : V, S>::kStage,
-                                      plan.warps * (2 * sizeof(Acc<X>) * (V << plan.log_lanes) + sizeof(int)) + offset_bytes(p));
+        constexpr int S = V == 1 ? 8 : 4;  // divides the rows of a thread: a block's are a multiple of it
+    const size_t smem = shared_memory(plan, Prefetch<X, V, S, false>::kWarp + Prefetch<G, SHARED ? 1 : V, S, SHARED>::kWarp,
+                                      plan.warps * (2 * sizeof(Acc<X>) * (V << plan.log_lanes) + sizeof(int)) + 16 + offset_room(p));
     if (p.sequences) launch(recurrence_maps_kernel<X, G, V, S, SHARED, true, REVERSE>, p, plan, smem, stream);
     else launch(recurrence_maps_kernel<X, G, V, S, SHARED, false, REVERSE>, p, plan, smem, stream);
 }
@@ -115,8 +126,9 @@ void forward(const RecurrenceArgs& p, cudaStream_t stream) {
         place_maps<Acc<X>>(p, plan, maps.get());
         reduce_segments<X, G, V, SHARED, false>(p, plan, stream);
     }
-    const size_t smem = shared_memory(plan, Prefetch<X, V, S>::kStage + Prefetch<G, SHARED ? 1 : V, S>::kStage,
-                                      sizeof(Acc<X>) * (V << plan.log_lanes) * plan.warps + offset_bytes(p));
+    const int width = V << plan.log_lanes;
+    const size_t smem = shared_memory(plan, Prefetch<X, V, S, false>::kWarp + Prefetch<G, SHARED ? 1 : V, S, SHARED>::kWarp,
+                                      sizeof(Acc<X>) * width * plan.warps + front_bytes<Acc<X>>(p, plan, width));
     if (p.sequences) launch(recurrence_forward_kernel<X, G, V, S, SHARED, true>, p, plan, smem, stream);
     else launch(recurrence_forward_kernel<X, G, V, S, SHARED, false>, p, plan, smem, stream);
 }
@@ -139,9 +151,10 @@ void backward(const RecurrenceArgs& p, cudaStream_t stream) {
     const uint64_t n = p.batch * p.rows * p.gate_dim;
     Scratch scratch(per_gate > 1 ? checked_mul(n, per_gate * sizeof(Acc<X>), "linear_recurrence_backprop") : 0, stream);
     if (per_gate > 1) partial = scratch.as<Acc<X>>();
-    const size_t column = (V << plan.log_lanes) * sizeof(Acc<X>);
-    const size_t smem = shared_memory(plan, 2 * Prefetch<X, V, S>::kStage + Prefetch<G, SHARED ? 1 : V, S>::kStage + plan.warps * column,
-                                      2 * plan.warps * column + offset_bytes(p));
+    const int width = V << plan.log_lanes;
+    const size_t column = width * sizeof(Acc<X>);
+    const size_t smem = shared_memory(plan, 2 * Prefetch<X, V, S, false>::kWarp + Prefetch<G, SHARED ? 1 : V, S, SHARED>::kWarp + column,
+                                      2 * plan.warps * column + front_bytes<Acc<X>>(p, plan, width));
     if (p.complement) {
         if (p.sequences) launch(recurrence_backward_kernel<X, G, V, S, SHARED, true, true>, p, plan, smem, stream, partial);
         else launch(recurrence_backward_kernel<X, G, V, S, SHARED, false, true>, p, plan, smem, stream, partial);

@@ -58,6 +58,11 @@ __device__ __forceinline__ int offset_at(const void* offsets, bool wide, int i) 
 // Offsets of packed sequences that a CTA keeps in shared memory, where there are no more of them.
 constexpr int kLocalOffsets = 512;
 
+// Bytes of shared memory that they take.
+__host__ __device__ inline size_t offset_room(const RecurrenceArgs& p) {
+    return p.sequences && p.sequences < uint64_t(kLocalOffsets) ? (p.sequences + 4) / 4 * 16 : 0;
+}
+
 // Walks the packed sequences along the rows.  `seq` is the last sequence whose offset is at or before the row
 // (-1 before the first, `count` behind the last); it spans rows [begin, next).  Offsets are only compared
 // with rows, so values that are out of order or out of range take no access out of bounds.
@@ -165,7 +170,7 @@ __device__ __forceinline__ void gate_factors(A v, A& a, A& rest) {
 __device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_(double a, double b, double c) { return fma(a, b, c); }
 
-constexpr int kCtaThreads = 256;  // at most; also the stride of the prefetch slots
+constexpr int kCtaThreads = 256;  // at most
 
 // One copy of B bytes (4, 8 or 16) to shared memory, asynchronous; `on` false writes zeros.
 template <int B>
@@ -192,49 +197,54 @@ __device__ __forceinline__ void await_copies(int stages) {
 }
 
 // The coming iterations' S rows of V values of one array.  4 bytes and more go asynchronously to
-// slot [stage][row][thread] of shared memory; single 16-bit values, which that copy does not know, to
-// registers, one iteration ahead.  Rows from `count` on read as zero (as anything, where there are none).
+// slot [stage][warp][row][lane] of shared memory.  Single 16-bit values, which that copy does not know, and the
+// gates that channels share (REGISTERS), one for several lanes, go to registers, one iteration ahead.  Rows
+// from `count` on read as zero (as anything, where there are none).
 // Copies of less than 16 bytes pass through L1, whose free part bounds how many are in flight.  Where 8-byte
 // neighbours are aligned as a pair, the even thread therefore copies both of an even row and the odd thread
 // both of an odd row; a warp reads only what its own threads copied.
-template <typename T, int V, int S>
+template <typename T, int V, int S, bool REGISTERS>
 struct Prefetch {
     static constexpr int kBytes = sizeof(T) * V;
-    static constexpr bool kShared = kBytes >= 4, kPairs = V > 1 && kBytes == 8;
-    static constexpr size_t kStage = kShared ? size_t(kBytes) * S * kCtaThreads : 0;
+    static constexpr bool kShared = !REGISTERS && kBytes >= 4, kPairs = V > 1 && kBytes == 8;
+    static constexpr size_t kWarp = kShared ? size_t(kBytes) * S * 32 : 0;  // of a stage
     Pack<T, V> held[kShared ? 1 : S];
     Pack<T, V>* slot;
-    int odd;     // pairs: 1 for the thread that copies the odd rows
+    int per_stage;  // packs
+    int odd;        // pairs: 1 for the thread that copies the odd rows
     bool pairs;
 
-    __device__ __forceinline__ void place(unsigned char* at, int tc, bool in_pairs) {
-        slot = reinterpret_cast<Pack<T, V>*>(at) + threadIdx.x;
+    // takes `stages` stages of shared memory at `at` and returns its end
+    __device__ __forceinline__ unsigned char* place(unsigned char* at, int stages, int warps, int tc, bool in_pairs) {
+        slot = reinterpret_cast<Pack<T, V>*>(at) + (threadIdx.x >> 5) * S * 32 + (threadIdx.x & 31);
+        per_stage = warps * S * 32;
         pairs = kPairs && in_pairs;
         odd = pairs ? tc & 1 : 0;
+        return at + stages * warps * kWarp;
     }
     // where this thread's copies of the rows from `first` on start
     __device__ __forceinline__ const T* start(const T* first, int64_t stride) const { return odd ? first + stride - V : first; }
 
     __device__ __forceinline__ void issue(int stage, const T* base, const T* from, int64_t stride, int count) {
         if constexpr (kShared) {
-            Pack<T, V>* to = slot + stage * S * kCtaThreads;
+            Pack<T, V>* to = slot + stage * per_stage;
             if (kPairs && pairs) {
-                to += odd * (kCtaThreads - 1);
+                to += odd * 31;
                 const int left = count - odd;
                 stride *= 2;
                 if (count == S) {
 #pragma unroll
-                    for (int s = 0; s < S; s += 2, from += stride) copy_async<16>(to + s * kCtaThreads, from);
+                    for (int s = 0; s < S; s += 2, from += stride) copy_async<16>(to + s * 32, from);
                 } else if (count > 0) {
 #pragma unroll
-                    for (int s = 0; s < S; s += 2, from += stride) copy_async<16>(to + s * kCtaThreads, s < left ? from : base, s < left);
+                    for (int s = 0; s < S; s += 2, from += stride) copy_async<16>(to + s * 32, s < left ? from : base, s < left);
                 }
             } else if (count == S) {
 #pragma unroll
-                for (int s = 0; s < S; ++s, from += stride) copy_async<kBytes>(to + s * kCtaThreads, from);
+                for (int s = 0; s < S; ++s, from += stride) copy_async<kBytes>(to + s * 32, from);
             } else if (count > 0) {
 #pragma unroll
-                for (int s = 0; s < S; ++s, from += stride) copy_async<kBytes>(to + s * kCtaThreads, s < count ? from : base, s < count);
+                for (int s = 0; s < S; ++s, from += stride) copy_async<kBytes>(to + s * 32, s < count ? from : base, s < count);
             }
         }
     }
@@ -245,7 +255,7 @@ struct Prefetch {
         }
     }
     __device__ __forceinline__ Pack<T, V> take(int stage, int s) const {
-        if constexpr (kShared) return slot[(stage * S + s) * kCtaThreads];
+        if constexpr (kShared) return slot[stage * per_stage + s * 32];
         else return held[s];
     }
 };
@@ -319,24 +329,52 @@ __device__ __forceinline__ void take_over(int link) {
     asm volatile("bar.sync %0, 64;" ::"r"(link) : "memory");
 }
 
-// The state that enters a segment: `r`, which enters the first one in scan order, through the maps of those before
-// it.  A state of 0 meets no factor, so that a product of large gates that overflowed does no harm to it.
+// What enters the strip's columns of a segment: `first`, which enters the first segment in scan order (null: 0), through
+// the maps of the segments before this one.  All threads call it: groups of them compose runs of
+// segments, which then go one after another.  `memory`: [group][A, B][width] and [group] drops; the result is left
+// in its first `width` values.  A state of 0 meets no factor, so that a product of large gates that
+// overflowed does it no harm.
 template <typename A, bool REVERSE, bool PACKED>
-__device__ __forceinline__ A through_segments(const RecurrencePlan& plan, uint64_t batch, int segment, uint64_t dim, uint64_t c, A r) {
-    const int n = REVERSE ? plan.segments - 1 - segment : segment;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const uint64_t k = batch * plan.segments + (REVERSE ? plan.segments - 1 - i : i);
-        const A* map = static_cast<const A*>(plan.maps) + 2 * k * dim + c;
-        const A b = map[dim];
-        r = (PACKED && plan.drops[k]) || r == A(0) ? b : fma_(map[0], r, b);
+__device__ __forceinline__ void through_segments(const RecurrencePlan& plan, uint64_t batch, int segment, uint64_t dim, uint64_t strip,
+                                                 int width, const A* first, A* memory) {
+    const int groups = max(1, int(blockDim.x) / width), before = REVERSE ? plan.segments - 1 - segment : segment;
+    int* drops = reinterpret_cast<int*>(memory + 2 * groups * width);
+    const int run = (before + groups - 1) / groups;
+    for (int i = threadIdx.x; i < groups * width; i += blockDim.x) {
+        const int group = i / width, c = i - group * width;
+        A a = A(1), b = A(0);
+        int drop = 0;
+        if (strip + c < dim) {
+#pragma unroll 8
+            for (int k = group * run; k < min(before, (group + 1) * run); ++k) {
+                const uint64_t at = batch * plan.segments + (REVERSE ? plan.segments - 1 - k : k);
+                const A* map = static_cast<const A*>(plan.maps) + 2 * at * dim + strip + c;
+                const A ma = map[0], mb = map[dim];
+                const bool drops_here = PACKED && plan.drops[at];
+                b = drops_here || b == A(0) ? mb : fma_(ma, b, mb);
+                a *= ma;
+                drop |= drops_here;
+            }
+        }
+        memory[2 * group * width + c] = a;
+        memory[(2 * group + 1) * width + c] = b;
+        if (c == 0) drops[group] = drop;
     }
-    return r;
+    __syncthreads();
+    for (int c = threadIdx.x; c < width; c += blockDim.x) {
+        A r = first && strip + c < dim ? first[strip + c] : A(0);
+        for (int g = 0; g < groups; ++g) {
+            const A b = memory[(2 * g + 1) * width + c];
+            r = drops[g] || r == A(0) ? b : fma_(memory[2 * g * width + c], r, b);
+        }
+        memory[c] = r;  // this column's own
+    }
+    __syncthreads();
 }
 
 // a, x and, where REST, 1 - a of S rows from the prefetched inputs; without REST x is b already.
-template <int FORM, bool REST, bool COMPLEMENT, typename X, typename G, int V, int GV, int S, typename A>
-__device__ __forceinline__ void factors(const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, int stage, A (&a)[S][V],
+template <int FORM, bool REST, bool COMPLEMENT, typename X, typename G, int V, int GV, int S, bool R, typename A>
+__device__ __forceinline__ void factors(const Prefetch<X, V, S, false>& fx, const Prefetch<G, GV, S, R>& fg, int stage, A (&a)[S][V],
                                         A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
@@ -355,8 +393,8 @@ __device__ __forceinline__ void factors(const Prefetch<X, V, S>& fx, const Prefe
     }
 }
 
-template <bool REST, bool COMPLEMENT, typename X, typename G, int V, int GV, int S, typename A>
-__device__ __forceinline__ void factors(int form, const Prefetch<X, V, S>& fx, const Prefetch<G, GV, S>& fg, int stage, A (&a)[S][V],
+template <bool REST, bool COMPLEMENT, typename X, typename G, int V, int GV, int S, bool R, typename A>
+__device__ __forceinline__ void factors(int form, const Prefetch<X, V, S, false>& fx, const Prefetch<G, GV, S, R>& fg, int stage, A (&a)[S][V],
                                         A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
     if (form == kGateValue) factors<kGateValue, REST, COMPLEMENT>(fx, fg, stage, a, u, rest);
     else if (form == kGateLog) factors<kGateLog, REST, COMPLEMENT>(fx, fg, stage, a, u, rest);
@@ -472,13 +510,11 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
     A* marks = p.checkpoints
         ? static_cast<A*>(p.checkpoints) + b * ((p.rows + kCheckpointRows - 1) / kCheckpointRows) * p.dim + c0 : nullptr;
 
-    Prefetch<X, V, S> fx;
-    Prefetch<G, GV, S> fg;
+    Prefetch<X, V, S, false> fx;
+    Prefetch<G, GV, S, SHARED> fg;
     unsigned char* next = smem;
-    fx.place(next, at.tc, plan.pairs);
-    next += stages * fx.kStage;
-    fg.place(next, at.tc, plan.pairs);
-    next += stages * fg.kStage;
+    next = fx.place(next, stages, warps, at.tc, plan.pairs);
+    next = fg.place(next, stages, warps, at.tc, plan.pairs);
     const int width = at.lanes * V;
     A* carry = reinterpret_cast<A*>(next) + at.tc * V;  // [warp][width]: the state on its way into each warp
     next += sizeof(A) * width * warps;
@@ -511,9 +547,13 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
     hold(row0);
     A in[V];  // the state that enters the warp's rows
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        in[v] = !PACKED && initial && live ? initial[b * p.dim + v] : A(0);
-        if (at.warp == 0 && live) in[v] = through_segments<A, false, PACKED>(plan, b, at.segment, p.dim, c0 + v, in[v]);
+    for (int v = 0; v < V; ++v) in[v] = !PACKED && initial && live ? initial[b * p.dim + v] : A(0);
+    if (plan.segments > 1) {
+        A* fold = reinterpret_cast<A*>(next + offset_room(p));
+        through_segments<A, false, PACKED>(plan, b, at.segment, p.dim, c0 - uint64_t(at.tc) * V, width,
+                                           PACKED || !p.initial ? nullptr : static_cast<const A*>(p.initial) + b * p.dim, fold);
+#pragma unroll
+        for (int v = 0; v < V; ++v) in[v] = fold[at.tc * V + v];
     }
     SequenceWalk walk;
     if (PACKED) {
@@ -608,6 +648,27 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
         for (int v = 0; v < V; ++v) state[b * p.dim + v] = leaving[v];
 }
 
+// Sums S values each over 1 << log >= S neighbouring lanes.  Each of the first rounds halves the values a lane still
+// holds, so that S - 1 + log - log2 S exchanges do instead of S log.  Returns the value whose sum this lane's
+// sums[0] is, -1 where another lane has it too.
+template <typename A, int S>
+__device__ __forceinline__ int fold_rows(A (&sums)[S], int log, int tc) {
+    int row = 0;
+#pragma unroll
+    for (int half = S / 2, bit = 0; half >= 1; half /= 2, ++bit) {
+        const bool upper = tc >> bit & 1;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const A mine = upper ? sums[half + i] : sums[i], other = upper ? sums[i] : sums[half + i];
+            sums[i] = mine + __shfl_xor_sync(0xffffffffu, other, 1 << bit);
+        }
+        row += upper ? half : 0;
+    }
+    constexpr int kRounds = S == 8 ? 3 : S == 4 ? 2 : 1;
+    for (int k = kRounds; k < log; ++k) sums[0] += __shfl_xor_sync(0xffffffffu, sums[0], 1 << k);
+    return (tc & ((1 << log) - 1)) >> kRounds ? -1 : row;
+}
+
 // One iteration takes its rows backward and then, from a checkpoint, forward again (for h_{t-1}), both in
 // registers, so that x, the gates and the derivatives are read once and h, rounded or not, is not read at all.
 // Checkpoints are near enough for a warp to start from one, or from the warp before; the gradient goes round
@@ -630,15 +691,12 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
     const A* state_derivs = p.state_derivs ? static_cast<const A*>(p.state_derivs) + c0 : nullptr;
     A* dinitial = p.dinitial ? static_cast<A*>(p.dinitial) + c0 : nullptr;
 
-    Prefetch<X, V, S> fx, fd;
-    Prefetch<G, GV, S> fg;
+    Prefetch<X, V, S, false> fx, fd;
+    Prefetch<G, GV, S, SHARED> fg;
     unsigned char* next = smem;
-    fx.place(next, at.tc, plan.pairs);
-    next += stages * fx.kStage;
-    fd.place(next, at.tc, plan.pairs);
-    next += stages * fd.kStage;
-    fg.place(next, at.tc, plan.pairs);
-    next += stages * fg.kStage;
+    next = fx.place(next, stages, warps, at.tc, plan.pairs);
+    next = fd.place(next, stages, warps, at.tc, plan.pairs);
+    next = fg.place(next, stages, warps, at.tc, plan.pairs);
     const int width = at.lanes * V;
     A* ahead = reinterpret_cast<A*>(next) + at.tc * V;  // [warp][width]: the state on its way into each warp
     A* back = ahead + warps * width;                    // [warp][width]: the gradient
@@ -690,9 +748,13 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
     hold(row0, true);
     A w[V];  // the gradient that enters the warp's rows from behind
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        w[v] = !PACKED && state_derivs && live ? state_derivs[b * p.dim + v] : A(0);
-        if (at.warp + 1 == warps && live) w[v] = through_segments<A, true, PACKED>(plan, b, at.segment, p.dim, c0 + v, w[v]);
+    for (int v = 0; v < V; ++v) w[v] = !PACKED && state_derivs && live ? state_derivs[b * p.dim + v] : A(0);
+    if (plan.segments > 1) {
+        A* fold = reinterpret_cast<A*>(next + offset_room(p));
+        through_segments<A, true, PACKED>(plan, b, at.segment, p.dim, c0 - uint64_t(at.tc) * V, width,
+                                          PACKED || !p.state_derivs ? nullptr : static_cast<const A*>(p.state_derivs) + b * p.dim, fold);
+#pragma unroll
+        for (int v = 0; v < V; ++v) w[v] = fold[at.tc * V + v];
     }
     SequenceWalk walk;
     if (PACKED) {
@@ -793,6 +855,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
             }
         }
         // forward through them with h_{t-1} in `h`
+        A sums[SHARED ? S : 1];
         X* to_x = dx;
         G* to_gate = dgate;
         dx -= out_span;
@@ -812,16 +875,28 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
                 h[v] = fma_(r.a[s][v], h[v], input(s, v));
             }
             if (s < r.count) store_pack<X, V>(to_x, narrow_pack<X, V>(gx));
-            if (SHARED) {
-                sum = s < r.count ? sum : A(0);
-                for (int k = 1; k < 1 << plan.fold_log; k <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
-                if (s < r.count && (at.tc & ((1 << plan.fold_log) - 1)) == 0) {
-                    const int64_t fold = int64_t(c0 / V) >> plan.fold_log, row = int64_t(b * p.rows) + row0 + s;
-                    if (partial) partial[row * ((dim / V) >> plan.fold_log) + fold] = sum;
-                    else to_gate[row * int64_t(p.gate_dim) + fold] = narrow<G>(sum);
-                }
+            if constexpr (SHARED) {
+                sums[s] = sum;
             } else if (s < r.count) {
                 if constexpr (std::is_same_v<Acc<G>, A>) store_pack<G, V>(to_gate, narrow_pack<G, V>(gg));
+            }
+        }
+        if constexpr (SHARED) {
+            const int64_t fold = int64_t(c0 / V) >> plan.fold_log, folds = (dim / V) >> plan.fold_log;
+            const auto store = [&](int row, A sum) {
+                const int64_t place = (int64_t(b * p.rows) + row0 + row) * folds + fold;
+                if (partial) partial[place] = sum;
+                else dgate[place] = narrow<G>(sum);
+            };
+            if (1 << plan.fold_log >= S) {
+                const int row = fold_rows<A, S>(sums, plan.fold_log, at.tc);
+                if (row >= 0 && row < r.count) store(row, sums[0]);
+            } else {
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    for (int k = 1; k < 1 << plan.fold_log; k <<= 1) sums[s] += __shfl_xor_sync(0xffffffffu, sums[s], k);
+                    if (s < r.count && (at.tc & ((1 << plan.fold_log) - 1)) == 0) store(s, sums[s]);
+                }
             }
         }
     }
@@ -852,13 +927,11 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_maps_kernel(const R
     const X* x = static_cast<const X*>(REVERSE ? p.derivs : p.x) + b * (REVERSE ? p.d_batch : p.x_batch) + (live ? c0 : 0);
     const G* gate = static_cast<const G*>(p.gate) + b * p.gate_batch + (!live ? 0 : SHARED ? c0 / (p.dim / p.gate_dim) : c0);
 
-    Prefetch<X, V, S> fx;
-    Prefetch<G, GV, S> fg;
+    Prefetch<X, V, S, false> fx;
+    Prefetch<G, GV, S, SHARED> fg;
     unsigned char* next = smem;
-    fx.place(next, at.tc, plan.pairs);
-    next += stages * fx.kStage;
-    fg.place(next, at.tc, plan.pairs);
-    next += stages * fg.kStage;
+    next = fx.place(next, stages, warps, at.tc, plan.pairs);
+    next = fg.place(next, stages, warps, at.tc, plan.pairs);
     const int width = at.lanes * V;
     A* maps = reinterpret_cast<A*>(next);  // [warp][A, B][width]
     next += sizeof(A) * 2 * width * warps;
