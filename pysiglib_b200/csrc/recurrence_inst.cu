@@ -12,7 +12,7 @@ namespace {
 // widen to the same registers).
 template <typename X> constexpr int kWide = sizeof(X) == 8 ? 2 : 4;
 // Rows a thread holds: as many as leave the arrays of S * V values in registers and two CTAs an SM their stages.
-template <int V> constexpr int kBackwardRows = V == 1 ? 8 : 4;
+template <int V> constexpr int kBackwardRows = V > 1 ? 4 : 8;
 template <typename X, int V> constexpr int kForwardRows = V > 1 && sizeof(X) > 2 ? 4 : 8;
 
 int log2_ceil(uint64_t n) {
@@ -32,9 +32,6 @@ bool aligned_to(const RecurrenceArgs& p, size_t bytes) {
            (p.gate_dim != p.dim || fits(p.gate, element_size(p.gate_type), p.dim, p.gate_batch, p.gate_row));
 }
 
-#ifndef SIG_SEGW
-#define SIG_SEGW 8
-#endif
 // Up to 8 warps whose lanes lie side by side in the channels as far as 128 bytes of a row go (full lines), and
 // behind one another in the rows beyond that.  Two CTAs an SM are there at a time.  Where full lines make fewer
 // strips than there are SMs, half lines do if that is enough; else the rows are cut into segments.
@@ -47,6 +44,9 @@ RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     plan.log_lanes = std::min({columns, log2_ceil(128 / (V * sizeof(X))), 5});
     const auto ctas = [&](int log_lanes) { return p.batch * (((per_row - 1) >> log_lanes) + 1); };
     if (plan.log_lanes > 0 && ctas(plan.log_lanes) < sms && ctas(plan.log_lanes - 1) >= sms) --plan.log_lanes;
+    // as wide as leaves a strip for each SM and more, where that pads no more channels
+    while (plan.log_lanes < std::min(columns, 5) && 2 * ctas(plan.log_lanes + 1) >= 3 * sms && ctas(plan.log_lanes + 1) * 2 == ctas(plan.log_lanes))
+        ++plan.log_lanes;
     // short inputs: no more parts than there are rows for, the lanes go to the channels instead
     plan.log_lanes = std::max(plan.log_lanes, std::min(columns, 5 - std::min(needed, 5)));
     plan.warps = 1 << std::min(3, std::max(0, needed - (5 - plan.log_lanes)));
@@ -57,7 +57,6 @@ RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     // shorter rings where there are many strips: all of them resident at a time, and fewer hand-overs
     const uint64_t strips = ctas(plan.log_lanes), warp_rows = uint64_t(32 >> plan.log_lanes) * S;
     while (plan.warps > 1 && strips * plan.warps > kResident * sms && plan.warps / 2 * warp_rows % kCheckpointRows == 0) plan.warps /= 2;
-    if (strips < sms) plan.warps = std::min(plan.warps, SIG_SEGW);
     const uint64_t span = plan.warps * warp_rows, blocks = (p.rows + span - 1) / span;
     uint64_t segments = 1;
     if (strips < sms) segments = std::min(blocks, kResident * sms / (strips * plan.warps));

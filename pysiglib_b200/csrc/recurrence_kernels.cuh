@@ -131,7 +131,7 @@ __device__ __forceinline__ int64_t sequence_of(SequenceWalk walk, int row) {
     return walk.seq;
 }
 
-// a and 1 - a, neither by cancellation: exp and expm1 for logarithms; for logits, with e = e^-v kept finite,
+// a and 1 - a, neither by cancellation; for logits, with e = e^-v kept finite,
 // a = 1 / (1 + e) and 1 - a = e a.  The reciprocal is the hardware's (within 1 ulp).
 // FAST (gates of 16 bits): exponentials as 2^(v log2 e) in single precision, off by up to 2 + 1.2 |v| ulp.  A gate
 // of 8 or 11 bits leaves e^v uncertain by |v| 2^-9 or 2^-12 of itself, thousands of times more.
@@ -142,8 +142,25 @@ __device__ __forceinline__ float exponential(float v, bool fast) {
     return r;
 }
 __device__ __forceinline__ double exponential(double v, bool) { return exp(v); }
-__device__ __forceinline__ float minus_expm1(float v) { return -expm1f(v); }
-__device__ __forceinline__ double minus_expm1(double v) { return -expm1(v); }
+// a = e^v and 1 - a together: v = n ln 2 + f with |f| <= ln 2 / 2 (ln 2 in two parts), p = e^f - 1 by its Taylor
+// series (the first term left out, f^8 / 8!, is below 2^-25 of p), a = 2^n + 2^n p and 1 - a = (1 - 2^n) - 2^n p,
+// both halved on the way so that 2^n stays finite.  Below e^-87 a is 0.
+__device__ __forceinline__ void exponential_pair(float v, float& a, float& rest) {
+    float c;  // v within [-87, 89], NaN kept
+    asm("{\n .reg .f32 t;\n max.NaN.f32 t, %1, 0fC2AE0000;\n min.NaN.f32 %0, t, 0f42B20000;\n}" : "=f"(c) : "f"(v));
+    const float n = rintf(c * 1.4426950408889634f);
+    const float f = fmaf(n, 1.9046543e-9f, fmaf(n, -0.69314718246459961f, c));
+    float p = fmaf(f, 1.0f / 5040, 1.0f / 720);
+    p = fmaf(p, f, 1.0f / 120);
+    p = fmaf(p, f, 1.0f / 24);
+    p = fmaf(p, f, 1.0f / 6);
+    p = fmaf(p, f, 0.5f);
+    p = fmaf(p * f, f, f);
+    const float s = __int_as_float((__float2int_rn(n) + 126) << 23);  // 2^(n - 1), 0 for n = -126
+    a = 2.0f * fmaf(s, p, s);
+    rest = 2.0f * fmaf(-s, p, 0.5f - s);
+}
+__device__ __forceinline__ void exponential_pair(double v, double& a, double& rest) { a = exp(v); rest = -expm1(v); }
 __device__ __forceinline__ float below(float v) {  // at most 2^100, NaN kept
     float r;
     asm("min.NaN.f32 %0, %1, 0f71800000;" : "=f"(r) : "f"(v));
@@ -156,10 +173,14 @@ __device__ __forceinline__ float reciprocal(float v) {
     return r;
 }
 __device__ __forceinline__ double reciprocal(double v) { return 1.0 / v; }
-template <int FORM, bool FAST, typename A>
+// PAIR: 1 - a is wanted as well.
+template <int FORM, bool FAST, bool PAIR, typename A>
 __device__ __forceinline__ void gate_factors(A v, A& a, A& rest) {
     if (FORM == kGateValue) { a = v; rest = A(1) - v; }
-    else if (FORM == kGateLog) { a = exponential(v, FAST); rest = minus_expm1(v); }
+    else if (FORM == kGateLog) {
+        if (PAIR) exponential_pair(v, a, rest);
+        else a = exponential(v, FAST);
+    }
     else {
         const A e = below(exponential(-v, FAST));
         a = reciprocal(A(1) + e);
@@ -199,7 +220,7 @@ __device__ __forceinline__ void await_copies(int stages) {
 // The coming iterations' S rows of V values of one array.  4 bytes and more go asynchronously to
 // slot [stage][warp][row][lane] of shared memory.  Single 16-bit values, which that copy does not know, and the
 // gates that channels share (REGISTERS), one for several lanes, go to registers, one iteration ahead.  Rows
-// from `count` on read as zero (as anything, where there are none).
+// from `count` on read as zero.
 // Copies of less than 16 bytes pass through L1, whose free part bounds how many are in flight.  Where 8-byte
 // neighbours are aligned as a pair, the even thread therefore copies both of an even row and the odd thread
 // both of an odd row; a warp reads only what its own threads copied.
@@ -235,14 +256,14 @@ struct Prefetch {
                 if (count == S) {
 #pragma unroll
                     for (int s = 0; s < S; s += 2, from += stride) copy_async<16>(to + s * 32, from);
-                } else if (count > 0) {
+                } else {
 #pragma unroll
                     for (int s = 0; s < S; s += 2, from += stride) copy_async<16>(to + s * 32, s < left ? from : base, s < left);
                 }
             } else if (count == S) {
 #pragma unroll
                 for (int s = 0; s < S; ++s, from += stride) copy_async<kBytes>(to + s * 32, from);
-            } else if (count > 0) {
+            } else {
 #pragma unroll
                 for (int s = 0; s < S; ++s, from += stride) copy_async<kBytes>(to + s * 32, s < count ? from : base, s < count);
             }
@@ -372,33 +393,32 @@ __device__ __forceinline__ void through_segments(const RecurrencePlan& plan, uin
     __syncthreads();
 }
 
-// a, x and, where REST, 1 - a of S rows from the prefetched inputs; without REST x is b already.
-template <int FORM, bool REST, bool COMPLEMENT, typename X, typename G, int V, int GV, int S, bool R, typename A>
+// a and b of S rows from the prefetched inputs.
+template <int FORM, bool COMPLEMENT, typename X, typename G, int V, int GV, int S, bool R, typename A>
 __device__ __forceinline__ void factors(const Prefetch<X, V, S, false>& fx, const Prefetch<G, GV, S, R>& fg, int stage, A (&a)[S][V],
-                                        A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
+                                        A (&u)[S][V]) {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         const Pack<X, V> x = fx.take(stage, s);
         const Pack<G, GV> g = fg.take(stage, s);
         A ga[GV], gr[GV];
 #pragma unroll
-        for (int v = 0; v < GV; ++v) gate_factors<FORM, sizeof(G) == 2>(A(widen(g.v[v])), ga[v], gr[v]);
+        for (int v = 0; v < GV; ++v) gate_factors<FORM, sizeof(G) == 2, COMPLEMENT>(A(widen(g.v[v])), ga[v], gr[v]);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             a[s][v] = ga[v % GV];
             u[s][v] = widen(x.v[v]);
             if (COMPLEMENT) u[s][v] *= gr[v % GV];
-            if (REST) rest[s % (REST ? S : 1)][v] = gr[v % GV];
         }
     }
 }
 
-template <bool REST, bool COMPLEMENT, typename X, typename G, int V, int GV, int S, bool R, typename A>
+template <bool COMPLEMENT, typename X, typename G, int V, int GV, int S, bool R, typename A>
 __device__ __forceinline__ void factors(int form, const Prefetch<X, V, S, false>& fx, const Prefetch<G, GV, S, R>& fg, int stage, A (&a)[S][V],
-                                        A (&u)[S][V], A (&rest)[REST ? S : 1][V]) {
-    if (form == kGateValue) factors<kGateValue, REST, COMPLEMENT>(fx, fg, stage, a, u, rest);
-    else if (form == kGateLog) factors<kGateLog, REST, COMPLEMENT>(fx, fg, stage, a, u, rest);
-    else factors<kGateLogit, REST, COMPLEMENT>(fx, fg, stage, a, u, rest);
+                                        A (&u)[S][V]) {
+    if (form == kGateValue) factors<kGateValue, COMPLEMENT>(fx, fg, stage, a, u);
+    else if (form == kGateLog) factors<kGateLog, COMPLEMENT>(fx, fg, stage, a, u);
+    else factors<kGateLogit, COMPLEMENT>(fx, fg, stage, a, u);
 }
 
 // Where a thread stands: its strip, channels and segment of the rows.
@@ -576,10 +596,9 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
             walk.advance(row0);
             r.e = row_events<S>(walk, row0, rows);
         }
-        A unused[1][V];
         await_copies(stages);
-        if (p.complement) factors<false, true>(p.form, fx, fg, stage, r.a, r.u, unused);
-        else factors<false, false>(p.form, fx, fg, stage, r.a, r.u, unused);
+        if (p.complement) factors<true>(p.form, fx, fg, stage, r.a, r.u);
+        else factors<false>(p.form, fx, fg, stage, r.a, r.u);
         hold(row0 + span);
         settle_rows<false>(r, walk, row0, initial, dim, live);
         Map<A, V> m;
@@ -669,8 +688,100 @@ __device__ __forceinline__ int fold_rows(A (&sums)[S], int log, int tc) {
     return (tc & ((1 << log) - 1)) >> kRounds ? -1 : row;
 }
 
-// One iteration takes its rows backward and then, from a checkpoint, forward again (for h_{t-1}), both in
-// registers, so that x, the gates and the derivatives are read once and h, rounded or not, is not read at all.
+// What the backward pass takes twice from its slots, or keeps where they do not hold it: x and, for shared gates, 1 - a.
+template <typename A, int V, int GV, int S>
+struct Kept {
+    A x[V > 1 ? 1 : S][V], rest[GV > 1 ? 1 : S][GV];
+};
+
+// First walk of the backward pass through its rows, upward: a and the derivatives into `r`, the rows appended to the map
+// `m` of the state.  QUIET: all S rows are there and no sequence starts, ends or is missing in them.
+template <int FORM, bool COMPLEMENT, bool QUIET, typename X, typename G, int V, int GV, int S, bool R, typename A, typename Start>
+__device__ __forceinline__ void walk_up(const Prefetch<X, V, S, false>& fx, const Prefetch<X, V, S, false>& fd, const Prefetch<G, GV, S, R>& fg,
+                                        int stage, Rows<A, V, S>& r, Map<A, V>& m, Kept<A, V, GV, S>& kept, const Start& first_state) {
+    constexpr bool kPair = COMPLEMENT || (GV == 1 && FORM == kGateLogit);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const Pack<X, V> x = fx.take(stage, s), d = fd.take(stage, s);
+        const Pack<G, GV> g = fg.take(stage, s);
+        A ga[GV], gr[GV];
+#pragma unroll
+        for (int v = 0; v < GV; ++v) gate_factors<FORM, sizeof(G) == 2, kPair>(A(widen(g.v[v])), ga[v], gr[v]);
+        if (GV == 1 && kPair) kept.rest[GV > 1 ? 0 : s][0] = gr[0];
+        const bool gone = !QUIET && (s >= r.count || (r.e.dead >> s & 1u));
+        if (!QUIET && (r.e.starts >> s & 1u)) first_state(s, m.b);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const A in = widen(x.v[v]), b = COMPLEMENT ? gr[v % GV] * in : in;
+            if (V == 1) kept.x[V > 1 ? 0 : s][v] = in;
+            r.a[s][v] = gone ? A(1) : ga[v % GV];
+            r.u[s][v] = gone ? A(0) : A(widen(d.v[v]));
+            m.b[v] = fma_(r.a[s][v], m.b[v], gone ? A(0) : b);
+        }
+    }
+}
+
+template <bool COMPLEMENT, bool QUIET, typename X, typename G, int V, int GV, int S, bool R, typename A, typename Start>
+__device__ __forceinline__ void walk_up(int form, const Prefetch<X, V, S, false>& fx, const Prefetch<X, V, S, false>& fd,
+                                        const Prefetch<G, GV, S, R>& fg, int stage, Rows<A, V, S>& r, Map<A, V>& m, Kept<A, V, GV, S>& kept,
+                                        const Start& first_state) {
+    if (form == kGateValue) walk_up<kGateValue, COMPLEMENT, QUIET>(fx, fd, fg, stage, r, m, kept, first_state);
+    else if (form == kGateLog) walk_up<kGateLog, COMPLEMENT, QUIET>(fx, fd, fg, stage, r, m, kept, first_state);
+    else walk_up<kGateLogit, COMPLEMENT, QUIET>(fx, fd, fg, stage, r, m, kept, first_state);
+}
+
+// Last walk, upward again with h_{t-1} in `h` and the gradients g in r.u: dx and dgate of each row go to `store`.
+template <int FORM, bool COMPLEMENT, bool QUIET, typename X, typename G, int V, int GV, int S, bool R, typename A, typename Start, typename Store>
+__device__ __forceinline__ void walk_out(const Prefetch<X, V, S, false>& fx, const Prefetch<G, GV, S, R>& fg, int stage, const Rows<A, V, S>& r,
+                                         const Kept<A, V, GV, S>& kept, A (&h)[V], const Start& first_state, const Store& store) {
+    constexpr bool kPair = COMPLEMENT || FORM == kGateLogit;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        if (!QUIET && (r.e.starts >> s & 1u)) first_state(s, h);
+        A x[V], rest[GV], dx[V], dgate[V];
+        if (V > 1) {
+            const Pack<X, V> again = fx.take(stage, s);
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = widen(again.v[v]);
+        } else {
+            x[0] = kept.x[V > 1 ? 0 : s][0];
+        }
+        if (kPair && GV > 1) {
+            const Pack<G, GV> g = fg.take(stage, s);
+#pragma unroll
+            for (int v = 0; v < GV; ++v) {
+                A unused;
+                gate_factors<FORM, sizeof(G) == 2, true>(A(widen(g.v[v])), unused, rest[v]);
+            }
+        } else if (kPair) {
+            rest[0] = kept.rest[GV > 1 ? 0 : s][0];
+        }
+        const bool dead = !QUIET && (r.e.dead >> s & 1u);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const A g = r.u[s][v], a = r.a[s][v];
+            dx[v] = COMPLEMENT ? rest[v % GV] * g : g;
+            dgate[v] = g * (COMPLEMENT ? h[v] - x[v] : h[v]);
+            if (FORM != kGateValue) dgate[v] *= a;
+            if (FORM == kGateLogit) dgate[v] *= rest[v % GV];
+            if (dead) dx[v] = dgate[v] = A(0);
+            h[v] = fma_(a, h[v], COMPLEMENT ? rest[v % GV] * x[v] : x[v]);
+        }
+        store(s, dx, dgate);
+    }
+}
+
+template <bool COMPLEMENT, bool QUIET, typename X, typename G, int V, int GV, int S, bool R, typename A, typename Start, typename Store>
+__device__ __forceinline__ void walk_out(int form, const Prefetch<X, V, S, false>& fx, const Prefetch<G, GV, S, R>& fg, int stage,
+                                         const Rows<A, V, S>& r, const Kept<A, V, GV, S>& kept, A (&h)[V], const Start& first_state, const Store& store) {
+    if (form == kGateValue) walk_out<kGateValue, COMPLEMENT, QUIET>(fx, fg, stage, r, kept, h, first_state, store);
+    else if (form == kGateLog) walk_out<kGateLog, COMPLEMENT, QUIET>(fx, fg, stage, r, kept, h, first_state, store);
+    else walk_out<kGateLogit, COMPLEMENT, QUIET>(fx, fg, stage, r, kept, h, first_state, store);
+}
+
+// One iteration walks up its rows (factors and maps), down (gradients) and up again from a checkpoint (h_{t-1} and
+// the outputs), with a and the gradients in registers and x and the gates read again from shared memory, so that
+// x, the gates and the derivatives are read once and h, rounded or not, is not read at all.
 // Checkpoints are near enough for a warp to start from one, or from the warp before; the gradient goes round
 // the ring of warps, from the last to the first.
 // Shared gates: each thread sums its V channels, 1 << fold_log neighbouring lanes are folded by shuffles,
@@ -778,41 +889,22 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
             walk.retreat(row0);
             r.e = row_events<S>(walk, row0, rows);
         }
-        A rest[S][V], x_[S][V];
-        await_copies(stages);
-        factors<true, false>(p.form, fx, fg, stage, r.a, x_, rest);
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const Pack<X, V> rd = fd.take(stage, s);
-#pragma unroll
-            for (int v = 0; v < V; ++v) r.u[s][v] = widen(rd.v[v]);
-        }
-        hold(row0 - span, base > first);
-        if (r.count < S || (PACKED && r.e.dead)) {
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-                if (s >= r.count || (r.e.dead >> s & 1u)) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) rest[s][v] = x_[s][v] = A(0);
-                }
-        }
-        settle_rows<true>(r, walk, row0, state_derivs, dim, live);
-        const auto input = [&](int s, int v) { return COMPLEMENT ? rest[s][v] * x_[s][v] : x_[s][v]; };
         const auto first_state = [&](int s, A (&h)[V]) {
             const A* from = initial && live ? initial + sequence_of(walk, row0 + s) * dim : nullptr;
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = from ? from[v] : A(0);
         };
+        const bool quiet = r.count == S && !(PACKED && (r.e.starts | r.e.ends | r.e.dead));
         Map<A, V> m, g;
+        m.clear();
+        Kept<A, V, GV, S> kept;
+        await_copies(stages);
+        if (quiet) walk_up<COMPLEMENT, true>(p.form, fx, fd, fg, stage, r, m, kept, first_state);
+        else walk_up<COMPLEMENT, false>(p.form, fx, fd, fg, stage, r, m, kept, first_state);
+        hold(row0 - span, base > first);
+        if (PACKED && r.e.ends && state_derivs && live) settle_rows<true>(r, walk, row0, state_derivs, dim, live);
         g.clear();
         append_rows<true, PACKED>(g, r);
-        m.clear();
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            if (PACKED && (r.e.starts >> s & 1u)) first_state(s, m.b);
-#pragma unroll
-            for (int v = 0; v < V; ++v) m.b[v] = fma_(r.a[s][v], m.b[v], input(s, v));
-        }
 #pragma unroll
         for (int v = 0; v < V; ++v) m.a[v] = g.a[v];
         m.drop = PACKED && r.e.starts;
@@ -854,48 +946,42 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
                 for (int v = 0; v < V; ++v) to[v] = behind[v];
             }
         }
-        // forward through them with h_{t-1} in `h`
         A sums[SHARED ? S : 1];
         X* to_x = dx;
         G* to_gate = dgate;
         dx -= out_span;
         dgate -= SHARED ? 0 : out_span;
-#pragma unroll
-        for (int s = 0; s < S; ++s, to_x += dim, to_gate += SHARED ? 0 : dim) {
-            if (PACKED && (r.e.starts >> s & 1u)) first_state(s, h);
-            A gx[V], gg[V], sum = A(0);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                gx[v] = COMPLEMENT ? rest[s][v] * r.u[s][v] : r.u[s][v];
-                gg[v] = r.u[s][v] * (COMPLEMENT ? h[v] - x_[s][v] : h[v]);
-                if (p.form != kGateValue) gg[v] *= r.a[s][v];
-                if (p.form == kGateLogit) gg[v] *= rest[s][v];
-                if (PACKED && (r.e.dead >> s & 1u)) gx[v] = gg[v] = A(0);
-                sum += gg[v];
-                h[v] = fma_(r.a[s][v], h[v], input(s, v));
-            }
+        const auto store = [&](int s, const A (&gx)[V], const A (&gg)[V]) {
             if (s < r.count) store_pack<X, V>(to_x, narrow_pack<X, V>(gx));
+            to_x += dim;
             if constexpr (SHARED) {
+                A sum = gg[0];
+#pragma unroll
+                for (int v = 1; v < V; ++v) sum += gg[v];
                 sums[s] = sum;
-            } else if (s < r.count) {
-                if constexpr (std::is_same_v<Acc<G>, A>) store_pack<G, V>(to_gate, narrow_pack<G, V>(gg));
+            } else {
+                if constexpr (std::is_same_v<Acc<G>, A>)
+                    if (s < r.count) store_pack<G, V>(to_gate, narrow_pack<G, V>(gg));
+                to_gate += dim;
             }
-        }
+        };
+        if (quiet) walk_out<COMPLEMENT, true>(p.form, fx, fg, stage, r, kept, h, first_state, store);
+        else walk_out<COMPLEMENT, false>(p.form, fx, fg, stage, r, kept, h, first_state, store);
         if constexpr (SHARED) {
             const int64_t fold = int64_t(c0 / V) >> plan.fold_log, folds = (dim / V) >> plan.fold_log;
-            const auto store = [&](int row, A sum) {
+            const auto store_sum = [&](int row, A sum) {
                 const int64_t place = (int64_t(b * p.rows) + row0 + row) * folds + fold;
                 if (partial) partial[place] = sum;
                 else dgate[place] = narrow<G>(sum);
             };
             if (1 << plan.fold_log >= S) {
                 const int row = fold_rows<A, S>(sums, plan.fold_log, at.tc);
-                if (row >= 0 && row < r.count) store(row, sums[0]);
+                if (row >= 0 && row < r.count) store_sum(row, sums[0]);
             } else {
 #pragma unroll
                 for (int s = 0; s < S; ++s) {
                     for (int k = 1; k < 1 << plan.fold_log; k <<= 1) sums[s] += __shfl_xor_sync(0xffffffffu, sums[s], k);
-                    if (s < r.count && (at.tc & ((1 << plan.fold_log) - 1)) == 0) store(s, sums[s]);
+                    if (s < r.count && (at.tc & ((1 << plan.fold_log) - 1)) == 0) store_sum(s, sums[s]);
                 }
             }
         }
@@ -970,10 +1056,9 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_maps_kernel(const R
             if (REVERSE) walk.retreat(row0); else walk.advance(row0);
             r.e = row_events<S>(walk, row0, end);
         }
-        A unused[1][V];
         await_copies(stages);
-        if (!REVERSE && p.complement) factors<false, true>(p.form, fx, fg, stage, r.a, r.u, unused);
-        else factors<false, false>(p.form, fx, fg, stage, r.a, r.u, unused);
+        if (!REVERSE && p.complement) factors<true>(p.form, fx, fg, stage, r.a, r.u);
+        else factors<false>(p.form, fx, fg, stage, r.a, r.u);
         hold(REVERSE ? row0 - S : row0 + S);
         settle_rows<REVERSE>(r, walk, row0, joins, dim, live);
         append_rows<REVERSE, PACKED>(m, r);
@@ -1036,9 +1121,9 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(const RecurrenceAr
     for (int v = 0; v < V; ++v) {
         A a, rest, u = widen(x.v[v]);
         const A t = widen(g.v[SHARED ? 0 : v]);
-        if (p.form == kGateValue) gate_factors<kGateValue, sizeof(G) == 2>(t, a, rest);
-        else if (p.form == kGateLog) gate_factors<kGateLog, sizeof(G) == 2>(t, a, rest);
-        else gate_factors<kGateLogit, sizeof(G) == 2>(t, a, rest);
+        if (p.form == kGateValue) gate_factors<kGateValue, sizeof(G) == 2, true>(t, a, rest);
+        else if (p.form == kGateLog) gate_factors<kGateLog, sizeof(G) == 2, true>(t, a, rest);
+        else gate_factors<kGateLogit, sizeof(G) == 2, true>(t, a, rest);
         if (p.complement) u *= rest;
         h.v[v] = fma_(a, h.v[v], u);
         y.v[v] = narrow<X>(h.v[v]);
