@@ -258,7 +258,8 @@ uint64_t sigb200_noalloc_scratch_bytes(void);
 /* --- sequence operators ---------------------------------------------------------------
  * Element types: 0 float32, 1 float64, 2 bfloat16, 3 float16.  "State" arrays (initial, state,
  * checkpoints, state_derivs, dinitial) are float64 for float64 inputs, else float32, and contiguous.
- * Strides are in elements; channels are adjacent.  Device pointers run on the device that owns them, on
+ * Strides are in elements; channels are adjacent.  device: -1, or the ordinal of the device that the caller
+ * knows all pointers to be memory of, which saves looking them up.  Device pointers run on the device that owns them, on
  * `stream` (a cudaStream_t passed as void*), and return before completion unless synchronize != 0; host
  * pointers are staged (contiguous arrays only) and return when the result is there.  None of these
  * have a counterpart in the reference. */
@@ -279,7 +280,7 @@ int sigb200_linear_recurrence(int type, int gate_type, const void* x, const void
                               uint64_t length, uint64_t dimension, uint64_t gates, uint64_t sequences,
                               uint64_t x_batch_stride, uint64_t x_row_stride, uint64_t gate_batch_stride,
                               uint64_t gate_row_stride, int gate_form, bool complement, bool wide_offsets,
-                              void* stream, int synchronize);
+                              int device, void* stream, int synchronize);
 
 /* Backward of the recurrence: from the derivatives of out (derivs, like x) and of state (state_derivs,
  * optional) to dx (like out), dgate (batch, length, gates) and dinitial (optional).  checkpoints: those of
@@ -291,13 +292,13 @@ int sigb200_linear_recurrence_backprop(int type, int gate_type, const void* deri
                                        uint64_t sequences, uint64_t derivs_batch_stride, uint64_t derivs_row_stride,
                                        uint64_t x_batch_stride, uint64_t x_row_stride, uint64_t gate_batch_stride,
                                        uint64_t gate_row_stride, int gate_form, bool complement, bool wide_offsets,
-                                       void* stream, int synchronize);
+                                       int device, void* stream, int synchronize);
 
 /* One row for each of batch_size states: state (batch_size, dimension) becomes a state + b, out its
  * value in the type of x. */
 int sigb200_linear_recurrence_step(int type, int gate_type, const void* x, const void* gate, void* state, void* out,
                                    uint64_t batch_size, uint64_t dimension, uint64_t gates, uint64_t x_stride,
-                                   uint64_t gate_stride, int gate_form, bool complement, void* stream, int synchronize);
+                                   uint64_t gate_stride, int gate_form, bool complement, int device, void* stream, int synchronize);
 
 /* Rotary positions on x (outer, inner, length, dimension): the pair i < rotary_dimension / 2 of a row,
  * channels (i, i + rotary_dimension / 2) or, interleaved, (2i, 2i + 1), is turned by position *
@@ -309,7 +310,7 @@ int sigb200_rotary(int type, int position_type, const void* x, const double* fre
                    uint64_t rotary_dimension, uint64_t x_outer_stride, uint64_t x_inner_stride, uint64_t x_row_stride,
                    uint64_t out_outer_stride, uint64_t out_inner_stride, uint64_t out_row_stride,
                    uint64_t position_outer_stride, uint64_t position_inner_stride, uint64_t position_row_stride,
-                   bool interleaved, bool inverse, double scale, void* stream, int synchronize);
+                   bool interleaved, bool inverse, double scale, int device, void* stream, int synchronize);
 
 /* Number of coefficients of a signature, scalar term included; 0 on overflow.
  * Same contract as the CPU library's sig_length (siglib/cpsig/cp_utils.cpp:91-105). */

@@ -25,8 +25,9 @@ namespace {
 
 CallOptions sync_options() { return CallOptions{}; }
 
-CallOptions stream_options(void* stream, int synchronize, int* nonfinite) {
+CallOptions stream_options(void* stream, int synchronize, int* nonfinite, int known_device = -1) {
     CallOptions o;
+    o.known_device = known_device;
     o.stream = static_cast<cudaStream_t>(stream);
     o.synchronize = synchronize != 0;
     o.nonfinite = nonfinite;
@@ -329,13 +330,13 @@ SIG_API int sigb200_linear_recurrence(int type, int gate_type, const void* x, co
                                       uint64_t length, uint64_t dimension, uint64_t gates, uint64_t sequences,
                                       uint64_t x_batch_stride, uint64_t x_row_stride, uint64_t gate_batch_stride,
                                       uint64_t gate_row_stride, int gate_form, bool complement, bool wide_offsets,
-                                      void* stream, int synchronize) {
+                                      int device, void* stream, int synchronize) {
     RecurrenceArgs a{};
     a.type = type; a.gate_type = gate_type; a.batch = batch_size; a.rows = length; a.dim = dimension; a.gate_dim = gates;
     a.sequences = sequences; a.x = x; a.gate = gate; a.initial = initial; a.offsets = offsets; a.out = out; a.state = state;
     a.checkpoints = checkpoints; a.x_batch = x_batch_stride; a.x_row = x_row_stride; a.gate_batch = gate_batch_stride;
     a.gate_row = gate_row_stride; a.form = gate_form; a.complement = complement; a.wide_offsets = wide_offsets;
-    SIG_SAFE_CALL(recurrence_entry(a, stream_options(stream, synchronize, nullptr)));
+    SIG_SAFE_CALL(recurrence_entry(a, stream_options(stream, synchronize, nullptr, device)));
 }
 
 SIG_API int sigb200_linear_recurrence_backprop(int type, int gate_type, const void* derivs, const void* x, const void* gate,
@@ -346,7 +347,7 @@ SIG_API int sigb200_linear_recurrence_backprop(int type, int gate_type, const vo
                                                uint64_t derivs_row_stride, uint64_t x_batch_stride,
                                                uint64_t x_row_stride, uint64_t gate_batch_stride,
                                                uint64_t gate_row_stride, int gate_form, bool complement,
-                                               bool wide_offsets, void* stream, int synchronize) {
+                                               bool wide_offsets, int device, void* stream, int synchronize) {
     RecurrenceArgs a{};
     a.type = type; a.gate_type = gate_type; a.batch = batch_size; a.rows = length; a.dim = dimension; a.gate_dim = gates;
     a.sequences = sequences; a.derivs = derivs; a.x = x; a.gate = gate; a.initial = initial; a.offsets = offsets;
@@ -354,18 +355,17 @@ SIG_API int sigb200_linear_recurrence_backprop(int type, int gate_type, const vo
     a.d_batch = derivs_batch_stride; a.d_row = derivs_row_stride; a.x_batch = x_batch_stride; a.x_row = x_row_stride;
     a.gate_batch = gate_batch_stride; a.gate_row = gate_row_stride; a.form = gate_form; a.complement = complement;
     a.wide_offsets = wide_offsets;
-    SIG_SAFE_CALL(recurrence_backprop_entry(a, stream_options(stream, synchronize, nullptr)));
+    SIG_SAFE_CALL(recurrence_backprop_entry(a, stream_options(stream, synchronize, nullptr, device)));
 }
 
 SIG_API int sigb200_linear_recurrence_step(int type, int gate_type, const void* x, const void* gate, void* state, void* out,
                                            uint64_t batch_size, uint64_t dimension, uint64_t gates, uint64_t x_stride,
-                                           uint64_t gate_stride, int gate_form, bool complement, void* stream,
-                                           int synchronize) {
+                                           uint64_t gate_stride, int gate_form, bool complement, int device, void* stream, int synchronize) {
     RecurrenceArgs a{};
     a.type = type; a.gate_type = gate_type; a.batch = 1; a.rows = batch_size; a.dim = dimension; a.gate_dim = gates;
     a.x = x; a.gate = gate; a.state = state; a.out = out; a.x_row = x_stride; a.gate_row = gate_stride;
     a.form = gate_form; a.complement = complement;
-    SIG_SAFE_CALL(recurrence_step_entry(a, stream_options(stream, synchronize, nullptr)));
+    SIG_SAFE_CALL(recurrence_step_entry(a, stream_options(stream, synchronize, nullptr, device)));
 }
 
 SIG_API int sigb200_rotary(int type, int position_type, const void* x, const double* frequencies, const void* positions,
@@ -373,15 +373,14 @@ SIG_API int sigb200_rotary(int type, int position_type, const void* x, const dou
                            uint64_t rotary_dimension, uint64_t x_outer_stride, uint64_t x_inner_stride,
                            uint64_t x_row_stride, uint64_t out_outer_stride, uint64_t out_inner_stride,
                            uint64_t out_row_stride, uint64_t position_outer_stride, uint64_t position_inner_stride,
-                           uint64_t position_row_stride, bool interleaved, bool inverse, double scale, void* stream,
-                           int synchronize) {
+                           uint64_t position_row_stride, bool interleaved, bool inverse, double scale, int device, void* stream, int synchronize) {
     RotaryArgs a{};
     a.type = type; a.position_type = position_type; a.n0 = outer; a.n1 = inner; a.rows = length; a.dim = dimension;
     a.rotary_dim = rotary_dimension; a.x = x; a.frequencies = frequencies; a.positions = positions; a.out = out;
     a.x0 = x_outer_stride; a.x1 = x_inner_stride; a.x_row = x_row_stride; a.out0 = out_outer_stride;
     a.out1 = out_inner_stride; a.out_row = out_row_stride; a.p0 = position_outer_stride; a.p1 = position_inner_stride;
     a.p_row = position_row_stride; a.interleaved = interleaved; a.inverse = inverse; a.scale = scale;
-    SIG_SAFE_CALL(rotary_entry(a, stream_options(stream, synchronize, nullptr)));
+    SIG_SAFE_CALL(rotary_entry(a, stream_options(stream, synchronize, nullptr, device)));
 }
 
 SIG_API uint64_t sigb200_sig_length(uint64_t dimension, uint64_t degree) {

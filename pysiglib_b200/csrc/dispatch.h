@@ -12,6 +12,7 @@ namespace sigb200 {
 struct CallOptions {
     cudaStream_t stream = nullptr;  // stream for device-pointer calls (nullptr = legacy default stream)
     bool synchronize = true;        // wait for completion before returning (device-pointer calls)
+    int known_device = -1;          // device all pointers are known to be memory of (-1 = look them up)
     int device = -1;                // device used to stage host-pointer calls (-1 = current device)
     int* nonfinite = nullptr;       // host int: set to 1 if the forward output holds NaN / Inf
 };

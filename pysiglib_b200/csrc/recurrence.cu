@@ -80,8 +80,8 @@ void recurrence_entry(const RecurrenceArgs& args, const CallOptions& opt) {
     if (p.batch == 0 || p.rows == 0) return;
     const Sizes s = checked(p, who);
     if (!p.out) throw std::invalid_argument("linear_recurrence received a null pointer");
-    int device = -1;
-    if (all_on_device({p.x, p.gate, p.initial, p.offsets, p.out, p.state, p.checkpoints}, who, &device)) {
+    int device = opt.known_device;
+    if (device >= 0 || all_on_device({p.x, p.gate, p.initial, p.offsets, p.out, p.state, p.checkpoints}, who, &device)) {
         DeviceGuard guard(device);
         dispatch(RecurrencePass::forward, p, opt.stream);
         if (opt.synchronize) SIG_CUDA_CHECK(cudaStreamSynchronize(opt.stream));
@@ -107,8 +107,8 @@ void recurrence_backprop_entry(const RecurrenceArgs& args, const CallOptions& op
     if (p.batch == 0 || p.rows == 0) return;
     const Sizes s = checked(p, who);
     if (!p.derivs || !p.dx || !p.dgate) throw std::invalid_argument("linear_recurrence_backprop received a null pointer");
-    int device = -1;
-    if (all_on_device({p.derivs, p.x, p.gate, p.initial, p.offsets, p.state_derivs, p.marks, p.dx, p.dgate, p.dinitial}, who, &device)) {
+    int device = opt.known_device;
+    if (device >= 0 || all_on_device({p.derivs, p.x, p.gate, p.initial, p.offsets, p.state_derivs, p.marks, p.dx, p.dgate, p.dinitial}, who, &device)) {
         DeviceGuard guard(device);
         backward_on_device(p, s, opt.stream);
         if (opt.synchronize) SIG_CUDA_CHECK(cudaStreamSynchronize(opt.stream));
@@ -136,8 +136,8 @@ void recurrence_step_entry(const RecurrenceArgs& args, const CallOptions& opt) {
     if (p.rows == 0) return;
     const Sizes s = checked(p, who);
     if (!p.out || !p.state) throw std::invalid_argument("linear_recurrence_step received a null pointer");
-    int device = -1;
-    if (all_on_device({p.x, p.gate, p.out, p.state}, who, &device)) {
+    int device = opt.known_device;
+    if (device >= 0 || all_on_device({p.x, p.gate, p.out, p.state}, who, &device)) {
         DeviceGuard guard(device);
         dispatch(RecurrencePass::step, p, opt.stream);
         if (opt.synchronize) SIG_CUDA_CHECK(cudaStreamSynchronize(opt.stream));

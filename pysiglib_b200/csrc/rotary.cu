@@ -3,11 +3,13 @@
 // Mathematics.  (y_p, y_q) = scale * (x_p cos w - x_q sin w, x_p sin w + x_q cos w) with w = p_t f_i, for the
 // pairs (i, i + r/2) or (2i, 2i + 1) of the first r channels; the others are copied.  The adjoint is the
 // turn by -w.  Angles are formed in 64 bits as turns, p_t * (f_i / 2 pi) less the nearest integer, so that a
-// position of millions keeps all the bits that the sine needs; the sine and cosine of the remainder are
-// taken in the type of the arithmetic (32 bits, 64 for float64 rows) and each output is rounded once.
+// position of millions keeps all the bits that the sine needs.  The sine and cosine of the remainder are
+// taken in the type of the arithmetic (64 bits for float64 rows, else 32: the nearest quarter turn off, then
+// the Taylor series within an eighth of a turn) and each output is rounded once.
 //
-// Split.  One read and one write per value bound it, as long as the sines are shared: a thread takes V
-// pairs of one position and walks over the rows (heads, batch entries) that have that position.
+// Split.  One read and one write per value bound it, as long as the sines are shared: a thread takes V pairs of
+// one position and walks over the rows (heads, batch entries) that have that position, four in flight; where
+// every row has its own it takes four positions, loads them all, and turns one after the other.
 #include <algorithm>
 #include <type_traits>
 
@@ -19,92 +21,171 @@ namespace sigb200 {
 namespace {
 
 struct RotaryGrid {
-    uint64_t threads;                 // in all
-    uint32_t chunks, turned;          // chunks a row is cut into, the first `turned` of them hold pairs
-    uint64_t outer, outer1;           // rows that differ in position beside the row axis, and their inner axis
+    uint64_t threads, turning;        // in all; the first ones, which turn pairs
+    uint32_t turned, copied;          // chunks of a row that hold pairs, and that do not
+    uint64_t units;                   // row blocks, of one row where positions are shared, else of four
+    uint64_t outer1;                  // inner axis of the rows that differ in position beside the row axis
     uint64_t shared, shared1;         // rows that share a position, and their inner axis
     uint64_t per_thread, groups;      // shared rows of a thread, threads that share them out
-    uint64_t xo0, xo1, yo0, yo1, po0, po1, xs0, xs1, ys0, ys1;  // strides of those axes
+    int64_t xo0, xo1, yo0, yo1, po0, po1, xs0, xs1, ys0, ys1;  // strides of those axes
 };
 
-__device__ __forceinline__ void sine_cosine(double turns, float& s, float& c) { sincospif(2.0f * static_cast<float>(turns), &s, &c); }
-__device__ __forceinline__ void sine_cosine(double turns, double& s, double& c) { sincospi(2.0 * turns, &s, &c); }
+#ifndef ROT_WANT
+#define ROT_WANT 2048
+#endif
+#ifndef ROT_FLIGHT
+#define ROT_FLIGHT 4
+#endif
+constexpr int kInFlight = ROT_FLIGHT;
+
+// Sine and cosine of a number of turns.
+__device__ __forceinline__ void sine_cosine(double turns, float& s, float& c) {
+    constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+    const float t = static_cast<float>(turns - ((turns + kMagic) - kMagic));
+    const float quarter = rintf(4.0f * t);
+    const float u = fmaf(quarter, -0.25f, t) * 6.2831853071795865f, z = u * u;
+    float p = fmaf(z, 1.0f / 362880, -1.0f / 5040), q = fmaf(z, -1.0f / 3628800, 1.0f / 40320);
+    p = fmaf(p, z, 1.0f / 120);
+    q = fmaf(q, z, -1.0f / 720);
+    p = fmaf(p, z, -1.0f / 6);
+    q = fmaf(q, z, 1.0f / 24);
+    q = fmaf(q, z, -0.5f);
+    const float sine = fmaf(p * z, u, u), cosine = fmaf(q, z, 1.0f);
+    const int k = static_cast<int>(quarter);
+    const float a = k & 1 ? cosine : sine, b = k & 1 ? sine : cosine;
+    s = k & 2 ? -a : a;
+    c = (k + 1) & 2 ? -b : b;
+}
+__device__ __forceinline__ void sine_cosine(double turns, double& s, double& c) { sincospi(2.0 * (turns - rint(turns)), &s, &c); }
 
 template <typename P>
-__device__ __forceinline__ double position_at(const void* positions, uint64_t at, uint64_t row) {
+__device__ __forceinline__ double position_at(const void* positions, int64_t at, uint64_t row) {
     if constexpr (std::is_void_v<P>) return static_cast<double>(row);
     else return static_cast<double>(static_cast<const P*>(positions)[at]);
 }
 
-template <typename X, typename P, int V, bool INTERLEAVED>
+// The 2 V channels of V pairs, in the order they are loaded: V and V.
+template <typename X, int V>
+struct Pairs {
+    Pack<X, V> p, q;
+};
+
+template <typename X, int V, bool INTERLEAVED, typename A>
+__device__ __forceinline__ Pairs<X, V> turned(const Pairs<X, V>& x, const A (&s)[V], const A (&c)[V]) {
+    A yp[V], yq[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        // interleaved pairs lie side by side in the 2 V values of p and q together
+        const A a = widen(INTERLEAVED ? (2 * v < V ? x.p.v[(2 * v) % V] : x.q.v[(2 * v) % V]) : x.p.v[v]);
+        const A b = widen(INTERLEAVED ? (2 * v + 1 < V ? x.p.v[(2 * v + 1) % V] : x.q.v[(2 * v + 1) % V]) : x.q.v[v]);
+        const A ya = a * c[v] - b * s[v], yb = a * s[v] + b * c[v];
+        if (INTERLEAVED) {
+            (2 * v < V ? yp : yq)[(2 * v) % V] = ya;
+            (2 * v + 1 < V ? yp : yq)[(2 * v + 1) % V] = yb;
+        } else {
+            yp[v] = ya;
+            yq[v] = yb;
+        }
+    }
+    return {narrow_pack<X, V>(yp), narrow_pack<X, V>(yq)};
+}
+
+// SHARED: several rows have a thread's position.  Else each row has its own.
+template <typename X, typename P, int V, bool INTERLEAVED, bool SHARED>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs p, const RotaryGrid g) {
     using A = Acc<X>;
-    constexpr int U = 4;  // rows in flight
     uint64_t i = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= g.threads) return;
-    const uint32_t chunk = static_cast<uint32_t>(i % g.chunks);
-    i /= g.chunks;
-    const uint64_t row = i % p.rows;
-    i /= p.rows;
-    const uint64_t group = i % g.groups, outer = i / g.groups;
-    const uint64_t o0 = outer / g.outer1, o1 = outer % g.outer1;
-    const X* x = static_cast<const X*>(p.x) + o0 * g.xo0 + o1 * g.xo1 + row * p.x_row;
-    X* y = static_cast<X*>(p.out) + o0 * g.yo0 + o1 * g.yo1 + row * p.out_row;
-    const uint64_t first = group * g.per_thread, last = min(first + g.per_thread, g.shared);
-    uint64_t k0 = first / g.shared1, k1 = first % g.shared1;
+    const bool turning = i < g.turning;
+    if (!turning) i -= g.turning;
+    const uint32_t chunks = turning ? g.turned : g.copied;
+    const uint32_t chunk = static_cast<uint32_t>(i % chunks);
+    i /= chunks;
+    const uint64_t unit = i % g.units;
+    i /= g.units;
+    const uint64_t group = SHARED ? i % g.groups : 0, outer = SHARED ? i / g.groups : i;
+    const uint64_t o0 = outer / g.outer1, o1 = outer - o0 * g.outer1;
+    const uint64_t row = SHARED ? unit : unit * kInFlight;
+    const int64_t cp = turning ? (INTERLEAVED ? 2 * int64_t(chunk) * V : int64_t(chunk) * V) : int64_t(p.rotary_dim) + int64_t(chunk) * V;
+    const int64_t cq = INTERLEAVED ? V : int64_t(p.rotary_dim / 2);  // from cp on
+    const X* x = static_cast<const X*>(p.x) + int64_t(o0) * g.xo0 + int64_t(o1) * g.xo1 + int64_t(row) * int64_t(p.x_row) + cp;
+    X* y = static_cast<X*>(p.out) + int64_t(o0) * g.yo0 + int64_t(o1) * g.yo1 + int64_t(row) * int64_t(p.out_row) + cp;
 
-    if (chunk >= g.turned) {  // channels that are not turned
-        const uint64_t c = p.rotary_dim + uint64_t(chunk - g.turned) * V;
-        for (uint64_t k = first; k < last; ++k) {
-            store_pack<X, V>(y + k0 * g.ys0 + k1 * g.ys1 + c, load_pack<X, V>(x + k0 * g.xs0 + k1 * g.xs1 + c));
-            if (++k1 == g.shared1) { k1 = 0; ++k0; }
+    // the rows of this thread: `count` of them, `x_step` and `y_step` apart, with a jump after every `inner`
+    int64_t x_step = int64_t(p.x_row), y_step = int64_t(p.out_row), x_jump = 0, y_jump = 0;
+    uint64_t count = min(uint64_t(kInFlight), p.rows - row), inner = ~0ull, at = 0;
+    if (SHARED) {
+        const uint64_t first = group * g.per_thread, k0 = first / g.shared1;
+        count = min(g.per_thread, g.shared - first);
+        inner = g.shared1;
+        at = first - k0 * g.shared1;
+        x += int64_t(k0) * g.xs0 + int64_t(at) * g.xs1;
+        y += int64_t(k0) * g.ys0 + int64_t(at) * g.ys1;
+        x_step = g.xs1;
+        y_step = g.ys1;
+        x_jump = g.xs0 - int64_t(g.shared1) * g.xs1;
+        y_jump = g.ys0 - int64_t(g.shared1) * g.ys1;
+    }
+    uint64_t y_at = at;
+    const auto next_x = [&] {
+        x += x_step;
+        if (SHARED && ++at == inner) { at = 0; x += x_jump; }
+    };
+    const auto next_y = [&] {
+        y += y_step;
+        if (SHARED && ++y_at == inner) { y_at = 0; y += y_jump; }
+    };
+
+    if (!turning) {
+        for (uint64_t k = 0; k < count; k += kInFlight) {
+            Pack<X, V> r[kInFlight];
+#pragma unroll
+            for (int n = 0; n < kInFlight; ++n)
+                if (k + n < count) {
+                    r[n] = load_pack<X, V>(x);
+                    next_x();
+                }
+#pragma unroll
+            for (int n = 0; n < kInFlight; ++n)
+                if (k + n < count) {
+                    store_pack<X, V>(y, r[n]);
+                    next_y();
+                }
         }
         return;
     }
-    const uint64_t pair = uint64_t(chunk) * V;
-    const uint64_t cp = INTERLEAVED ? 2 * pair : pair, cq = INTERLEAVED ? 2 * pair + V : pair + p.rotary_dim / 2;
-    const double at = position_at<P>(p.positions, o0 * g.po0 + o1 * g.po1 + row * p.p_row, row);
     A s[V], c[V];
+    const double* frequencies = p.frequencies + uint64_t(chunk) * V;
+    const A scale = static_cast<A>(p.scale), signed_scale = static_cast<A>(p.inverse ? -p.scale : p.scale);
+    const auto turn_at = [&](double position) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const double turns = at * (p.frequencies[pair + v] * 0.15915494309189533577);
-        sine_cosine(turns - rint(turns), s[v], c[v]);
-        s[v] *= static_cast<A>(p.inverse ? -p.scale : p.scale);
-        c[v] *= static_cast<A>(p.scale);
-    }
-    for (uint64_t k = first; k < last; k += U) {
-        Pack<X, V> rp[U], rq[U];
-        uint64_t j0 = k0, j1 = k1;
+        for (int v = 0; v < V; ++v) {
+            sine_cosine(position * (frequencies[v] * 0.15915494309189533577), s[v], c[v]);
+            s[v] *= signed_scale;
+            c[v] *= scale;
+        }
+    };
+    const int64_t place = int64_t(o0) * g.po0 + int64_t(o1) * g.po1 + int64_t(row) * int64_t(p.p_row);
+    if (SHARED) turn_at(position_at<P>(p.positions, place, row));
+    for (uint64_t k = 0; k < count; k += kInFlight) {
+        Pairs<X, V> r[kInFlight];
+        double position[SHARED ? 1 : kInFlight];
 #pragma unroll
-        for (int n = 0; n < U; ++n)
-            if (k + n < last) {
-                const X* from = x + j0 * g.xs0 + j1 * g.xs1;
-                rp[n] = load_pack<X, V>(from + cp);
-                rq[n] = load_pack<X, V>(from + cq);
-                if (++j1 == g.shared1) { j1 = 0; ++j0; }
+        for (int n = 0; n < kInFlight; ++n)
+            if (k + n < count) {
+                r[n].p = load_pack<X, V>(x);
+                r[n].q = load_pack<X, V>(x + cq);
+                if (!SHARED) position[SHARED ? 0 : n] = position_at<P>(p.positions, place + n * int64_t(p.p_row), row + n);
+                next_x();
             }
 #pragma unroll
-        for (int n = 0; n < U; ++n)
-            if (k + n < last) {
-                Pack<X, V> up, uq;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    // interleaved pairs lie side by side in the 2 V values of rp and rq together
-                    const A a = widen(INTERLEAVED ? (2 * v < V ? rp[n].v[(2 * v) % V] : rq[n].v[(2 * v) % V]) : rp[n].v[v]);
-                    const A b = widen(INTERLEAVED ? (2 * v + 1 < V ? rp[n].v[(2 * v + 1) % V] : rq[n].v[(2 * v + 1) % V]) : rq[n].v[v]);
-                    const X ya = narrow<X>(a * c[v] - b * s[v]), yb = narrow<X>(a * s[v] + b * c[v]);
-                    if (INTERLEAVED) {
-                        (2 * v < V ? up : uq).v[(2 * v) % V] = ya;
-                        (2 * v + 1 < V ? up : uq).v[(2 * v + 1) % V] = yb;
-                    } else {
-                        up.v[v] = ya;
-                        uq.v[v] = yb;
-                    }
-                }
-                X* to = y + k0 * g.ys0 + k1 * g.ys1;
-                store_pack<X, V>(to + cp, up);
-                store_pack<X, V>(to + cq, uq);
-                if (++k1 == g.shared1) { k1 = 0; ++k0; }
+        for (int n = 0; n < kInFlight; ++n)
+            if (k + n < count) {
+                if (!SHARED) turn_at(position[SHARED ? 0 : n]);
+                const Pairs<X, V> t = turned<X, V, INTERLEAVED>(r[n], s, c);
+                store_pack<X, V>(y, t.p);
+                store_pack<X, V>(y + cq, t.q);
+                next_y();
             }
     }
 }
@@ -113,33 +194,43 @@ template <typename X, typename P, int V>
 void launch(const RotaryArgs& p, cudaStream_t stream) {
     RotaryGrid g{};
     g.turned = static_cast<uint32_t>(p.rotary_dim / 2 / V);
-    g.chunks = g.turned + static_cast<uint32_t>((p.dim - p.rotary_dim) / V);
+    g.copied = static_cast<uint32_t>((p.dim - p.rotary_dim) / V);
     // axes along which the positions do not change are walked by one thread
     const bool same0 = p.n0 == 1 || p.p0 == 0 || std::is_void_v<P>, same1 = p.n1 == 1 || p.p1 == 0 || std::is_void_v<P>;
-    g.outer = g.outer1 = g.shared = g.shared1 = 1;
+    uint64_t outer = 1;
+    g.outer1 = g.shared = g.shared1 = 1;
+    const auto x0 = int64_t(p.x0), x1 = int64_t(p.x1), y0 = int64_t(p.out0), y1 = int64_t(p.out1), p0 = int64_t(p.p0), p1 = int64_t(p.p1);
     if (same0 && same1) {
         g.shared = p.n0 * p.n1; g.shared1 = p.n1;
-        g.xs0 = p.x0; g.xs1 = p.x1; g.ys0 = p.out0; g.ys1 = p.out1;
+        g.xs0 = x0; g.xs1 = x1; g.ys0 = y0; g.ys1 = y1;
     } else if (same1) {
-        g.outer = p.n0; g.xo0 = p.x0; g.yo0 = p.out0; g.po0 = p.p0;
-        g.shared = g.shared1 = p.n1; g.xs1 = p.x1; g.ys1 = p.out1;
+        outer = p.n0; g.xo0 = x0; g.yo0 = y0; g.po0 = p0;
+        g.shared = g.shared1 = p.n1; g.xs1 = x1; g.ys1 = y1;
     } else if (same0) {
-        g.outer = p.n1; g.xo0 = p.x1; g.yo0 = p.out1; g.po0 = p.p1;
-        g.shared = g.shared1 = p.n0; g.xs1 = p.x0; g.ys1 = p.out0;
+        outer = p.n1; g.xo0 = x1; g.yo0 = y1; g.po0 = p1;
+        g.shared = g.shared1 = p.n0; g.xs1 = x0; g.ys1 = y0;
     } else {
-        g.outer = p.n0 * p.n1; g.outer1 = p.n1;
-        g.xo0 = p.x0; g.xo1 = p.x1; g.yo0 = p.out0; g.yo1 = p.out1; g.po0 = p.p0; g.po1 = p.p1;
+        outer = p.n0 * p.n1; g.outer1 = p.n1;
+        g.xo0 = x0; g.xo1 = x1; g.yo0 = y0; g.yo1 = y1; g.po0 = p0; g.po1 = p1;
     }
-    // enough threads for every SM twice over before one takes several of the rows that share a position
-    const uint64_t lines = g.chunks * p.rows * g.outer;
-    const uint64_t wanted = uint64_t(device_context(current_device()).sm_count) * 4096;
+    const bool shared = g.shared > 1;
+    g.units = shared ? p.rows : (p.rows + kInFlight - 1) / kInFlight;
+    // enough threads for every SM before one takes more of the rows that share a position
+    const uint64_t lines = uint64_t(g.turned + g.copied) * g.units * outer;
+    const uint64_t wanted = uint64_t(device_context(current_device()).sm_count) * ROT_WANT;
     g.groups = std::max<uint64_t>(1, std::min<uint64_t>(g.shared, (wanted + lines - 1) / lines));
     g.per_thread = (g.shared + g.groups - 1) / g.groups;
     g.groups = (g.shared + g.per_thread - 1) / g.per_thread;
+    g.turning = g.turned * g.units * outer * g.groups;
     g.threads = lines * g.groups;
     const unsigned grid = grid_1d(g.threads, 256);
-    if (p.interleaved) rotary_kernel<X, P, V, true><<<grid, 256, 0, stream>>>(p, g);
-    else rotary_kernel<X, P, V, false><<<grid, 256, 0, stream>>>(p, g);
+    if (p.interleaved) {
+        if (shared) rotary_kernel<X, P, V, true, true><<<grid, 256, 0, stream>>>(p, g);
+        else rotary_kernel<X, P, V, true, false><<<grid, 256, 0, stream>>>(p, g);
+    } else {
+        if (shared) rotary_kernel<X, P, V, false, true><<<grid, 256, 0, stream>>>(p, g);
+        else rotary_kernel<X, P, V, false, false><<<grid, 256, 0, stream>>>(p, g);
+    }
     check_launch("rotary kernel");
 }
 
@@ -197,8 +288,8 @@ void rotary_entry(const RotaryArgs& args, const CallOptions& opt) {
         throw std::invalid_argument("rotary received a null pointer");
     const void* positions = p.position_type == kPositionNone ? nullptr : p.positions;
     const void* frequencies = p.rotary_dim ? p.frequencies : nullptr;
-    int device = -1;
-    if (all_on_device({p.x, p.out, positions, frequencies}, who, &device)) {
+    int device = opt.known_device;
+    if (device >= 0 || all_on_device({p.x, p.out, positions, frequencies}, who, &device)) {
         DeviceGuard guard(device);
         run(p, opt.stream);
         if (opt.synchronize) SIG_CUDA_CHECK(cudaStreamSynchronize(opt.stream));

@@ -10,56 +10,68 @@ import numpy as np
 import torch
 
 from .param_checks import check_type
-from .sequence_inputs import (batched_rows, call, check_like, check_state, contiguous, element_type, empty, on_device, pointer,
-                              state_dtype, stream_of, zeros)
+from .sequence_inputs import (batched_rows, call, check_like, check_state, contiguous, element_type, empty, on_device,
+                              place_of, pointer, state_dtype)
 
 GATE_FORMS = {"value": 0, "log": 1, "logit": 2}
 CHECKPOINT_ROWS = 16  # rows between two of the states kept for the backward pass
+
+
+def _check_gate(x, gate, gate_form, complement):
+    """``(element type, gate type, gate form, gates)`` of inputs ``(..., dimension)`` and gates ``(..., G)``."""
+    code, gate_code = element_type(x, "x"), element_type(gate, "gate")
+    check_like(gate, "gate", x, "x")
+    if gate_code != code and not (gate_code == 0 and code >= 2):
+        raise TypeError("gate.dtype must be that of x, or float32 for 16-bit x; got %s for %s" % (gate.dtype, x.dtype))
+    form = GATE_FORMS.get(gate_form) if isinstance(gate_form, str) else None
+    if form is None:
+        check_type(gate_form, "gate_form", str)
+        raise ValueError("gate_form must be one of 'value', 'log' or 'logit', got %r" % gate_form)
+    if complement is not True and complement is not False:
+        check_type(complement, "complement", bool)
+    return code, gate_code, form
+
+
+def _check_gate_shape(shape, gate_shape):
+    dim, gates = shape[-1], gate_shape[-1] if len(gate_shape) else 0
+    if dim == 0:
+        raise ValueError("x has 0 channels (dimension). Its dimension must be at least 1.")
+    if gate_shape[:-1] != shape[:-1] or gates == 0 or dim % gates:
+        raise ValueError("gate must have shape %s + (G,) with G dividing %d, got %s" % (tuple(shape[:-1]), dim, tuple(gate_shape)))
+    return dim, gates
 
 
 class _Recurrence:
     """Checked and flattened arguments of one call."""
 
     def __init__(self, x, gate, initial, gate_form, complement, offsets):
-        self.type = element_type(x, "x")
-        self.gate_type = element_type(gate, "gate")
-        check_like(gate, "gate", x, "x")
-        if self.gate_type != self.type and not (self.gate_type == 0 and self.type >= 2):
-            raise TypeError("gate.dtype must be that of x, or float32 for 16-bit x; got %s for %s" % (gate.dtype, x.dtype))
-        check_type(gate_form, "gate_form", str)
-        if gate_form not in GATE_FORMS:
-            raise ValueError("gate_form must be one of 'value', 'log' or 'logit', got %r" % gate_form)
-        check_type(complement, "complement", bool)
-        self.form, self.complement = GATE_FORMS[gate_form], complement
-        shape = tuple(x.shape)
+        self.type, self.gate_type, self.form = _check_gate(x, gate, gate_form, complement)
+        self.complement = complement
+        shape = x.shape
         if len(shape) < 2:
             raise ValueError("x must have at least rank 2, got rank %d." % len(shape))
-        self.rows, self.dim = shape[-2:]
-        self.gates = gate.shape[-1] if len(gate.shape) else 0
-        if self.dim == 0:
-            raise ValueError("x has 0 channels (dimension). Its dimension must be at least 1.")
-        if tuple(gate.shape[:-1]) != shape[:-1] or self.gates == 0 or self.dim % self.gates:
-            raise ValueError("gate must have shape %s + (G,) with G dividing %d, got %s"
-                             % (shape[:-1], self.dim, tuple(gate.shape)))
-        self.shape, self.gate_shape = shape, tuple(gate.shape)
-        self.batch = prod(shape[:-2])
+        self.dim, self.gates = _check_gate_shape(shape, gate.shape)
+        self.rows, lead = shape[-2], shape[:-2]
+        self.batch = prod(lead)
         self.offsets, self.wide, self.sequences = None, False, 0
-        self.state_shape = (*shape[:-2], self.dim)
-        if offsets is not None:
+        if offsets is None:
+            self.state_shape = (*lead, self.dim)
+        else:
             self._set_offsets(offsets, x)
         self.initial = check_state(initial, "initial", self.state_shape, x)
         self.x, self.x_batch, self.x_row = batched_rows(x)
         self.gate, self.gate_batch, self.gate_row = batched_rows(gate)
-        self.marks_shape = (*shape[:-2], -(-self.rows // CHECKPOINT_ROWS), self.dim)
+        self.marks_shape = (*lead, -(-self.rows // CHECKPOINT_ROWS), self.dim)
         self.empty = self.batch == 0 or self.rows == 0
 
     def _set_offsets(self, offsets, x):
         check_type(offsets, "offsets", (np.ndarray, torch.Tensor))
-        if len(self.shape) != 2:
-            raise ValueError("packed sequences (offsets) need x of shape (rows, dimension), got %s" % (self.shape,))
+        if len(x.shape) != 2:
+            raise ValueError("packed sequences (offsets) need x of shape (rows, dimension), got %s" % (tuple(x.shape),))
         if len(offsets.shape) != 1 or offsets.shape[0] < 2:
             raise ValueError("offsets must be one row of at least 2 values, got shape %s" % (tuple(offsets.shape),))
-        if str(offsets.dtype).replace("torch.", "") not in ("int32", "int64"):
+        self.wide = offsets.dtype == (torch.int64 if isinstance(offsets, torch.Tensor) else np.int64)
+        if not self.wide and offsets.dtype != (torch.int32 if isinstance(offsets, torch.Tensor) else np.int32):
             raise TypeError("offsets.dtype must be int32 or int64, got %s instead" % offsets.dtype)
         if not on_device(offsets):
             values = np.asarray(offsets).astype(np.int64)
@@ -73,12 +85,11 @@ class _Recurrence:
         elif not isinstance(offsets, np.ndarray):
             check_like(offsets, "offsets", x, "x")
         self.offsets = contiguous(offsets)
-        self.wide = str(offsets.dtype).endswith("int64")
         self.sequences = offsets.shape[0] - 1
         self.state_shape = (self.sequences, self.dim)
 
     def tail(self, x):
-        return self.form, self.complement, self.wide, stream_of(x), 0
+        return self.form, self.complement, self.wide, *place_of(x), 0
 
 
 def linear_recurrence(
@@ -132,7 +143,7 @@ def linear_recurrence(
     check_type(return_state, "return_state", bool)
     check_type(return_checkpoints, "return_checkpoints", bool)
     r = _Recurrence(x, gate, initial, gate_form, complement, offsets)
-    h = empty(x, r.shape, x.dtype)
+    h = empty(x, x.shape, x.dtype)
     wide = state_dtype(x)
     state = empty(x, r.state_shape, wide) if return_state else None
     marks = empty(x, r.marks_shape, wide) if return_checkpoints else None
@@ -176,12 +187,12 @@ def linear_recurrence_backprop(
     check_like(derivs, "derivs", x, "x")
     if derivs.dtype != x.dtype:
         raise TypeError("derivs.dtype must be that of x, got %s for %s" % (derivs.dtype, x.dtype))
-    if tuple(derivs.shape) != r.shape:
-        raise ValueError("derivs must have the shape of x, %s, got %s" % (r.shape, tuple(derivs.shape)))
+    if derivs.shape != x.shape:
+        raise ValueError("derivs must have the shape of x, %s, got %s" % (tuple(x.shape), tuple(derivs.shape)))
     state_derivs = check_state(state_derivs, "state_derivs", r.state_shape, x)
     checkpoints = check_state(checkpoints, "checkpoints", r.marks_shape, x)
     d, d_batch, d_row = batched_rows(derivs)
-    dx, dgate = empty(x, r.shape, x.dtype), empty(x, r.gate_shape, gate.dtype)
+    dx, dgate = empty(x, x.shape, x.dtype), empty(gate, gate.shape, gate.dtype)
     dinitial = None if initial is None else empty(x, r.state_shape, state_dtype(x))
     if r.empty:
         if dinitial is not None:
@@ -211,28 +222,16 @@ def linear_recurrence_step(
 
     Stepping through a sequence gives what ``linear_recurrence`` gives for it, up to rounding.
     """
-    shape = tuple(getattr(x, "shape", ()))
-    code = element_type(x, "x")
-    gate_code = element_type(gate, "gate")
-    check_like(gate, "gate", x, "x")
+    code, gate_code, form = _check_gate(x, gate, gate_form, complement)
     check_like(state, "state", x, "x")
-    if gate_code != code and not (gate_code == 0 and code >= 2):
-        raise TypeError("gate.dtype must be that of x, or float32 for 16-bit x; got %s for %s" % (gate.dtype, x.dtype))
-    check_type(gate_form, "gate_form", str)
-    if gate_form not in GATE_FORMS:
-        raise ValueError("gate_form must be one of 'value', 'log' or 'logit', got %r" % gate_form)
-    check_type(complement, "complement", bool)
+    shape = x.shape
     if len(shape) < 1:
         raise ValueError("x must have at least rank 1, got rank 0.")
-    dim, gates = shape[-1], gate.shape[-1] if len(gate.shape) else 0
-    if dim == 0:
-        raise ValueError("x has 0 channels (dimension). Its dimension must be at least 1.")
-    if tuple(gate.shape[:-1]) != shape[:-1] or gates == 0 or dim % gates:
-        raise ValueError("gate must have shape %s + (G,) with G dividing %d, got %s" % (shape[:-1], dim, tuple(gate.shape)))
+    dim, gates = _check_gate_shape(shape, gate.shape)
     if state.dtype != state_dtype(x):
         raise TypeError("state.dtype must be %s for x of type %s, got %s instead" % (state_dtype(x), x.dtype, state.dtype))
-    if tuple(state.shape) != shape:
-        raise ValueError("state must have the shape of x, %s, got %s" % (shape, tuple(state.shape)))
+    if state.shape != shape:
+        raise ValueError("state must have the shape of x, %s, got %s" % (tuple(shape), tuple(state.shape)))
     if not (state.is_contiguous() if isinstance(state, torch.Tensor) else state.flags["C_CONTIGUOUS"] and state.flags["WRITEABLE"]):
         raise ValueError("state is overwritten: it must be contiguous and writeable")
     if isinstance(state, torch.Tensor) and state.requires_grad:
@@ -242,5 +241,5 @@ def linear_recurrence_step(
     batch = prod(shape[:-1])
     if batch:
         call("linear_recurrence_step", code, gate_code, pointer(x), pointer(gate), pointer(state), pointer(out), batch,
-             dim, gates, dim, gates, GATE_FORMS[gate_form], complement, stream_of(x), 0)
+             dim, gates, dim, gates, form, complement, *place_of(x), 0)
     return out

@@ -67,16 +67,16 @@ def _bind(lib):
     lib.sigb200_launch_count.restype = c_uint64
     u64 = c_uint64
     f = lib.sigb200_linear_recurrence
-    f.argtypes = (c_int, c_int) + (c_void_p,) * 7 + (u64,) * 9 + (c_int, c_bool, c_bool, c_void_p, c_int)
+    f.argtypes = (c_int, c_int) + (c_void_p,) * 7 + (u64,) * 9 + (c_int, c_bool, c_bool, c_int, c_void_p, c_int)
     f.restype = c_int
     f = lib.sigb200_linear_recurrence_backprop
-    f.argtypes = (c_int, c_int) + (c_void_p,) * 10 + (u64,) * 11 + (c_int, c_bool, c_bool, c_void_p, c_int)
+    f.argtypes = (c_int, c_int) + (c_void_p,) * 10 + (u64,) * 11 + (c_int, c_bool, c_bool, c_int, c_void_p, c_int)
     f.restype = c_int
     f = lib.sigb200_linear_recurrence_step
-    f.argtypes = (c_int, c_int) + (c_void_p,) * 4 + (u64,) * 5 + (c_int, c_bool, c_void_p, c_int)
+    f.argtypes = (c_int, c_int) + (c_void_p,) * 4 + (u64,) * 5 + (c_int, c_bool, c_int, c_void_p, c_int)
     f.restype = c_int
     f = lib.sigb200_rotary
-    f.argtypes = (c_int, c_int) + (c_void_p,) * 4 + (u64,) * 14 + (c_bool, c_bool, c_double, c_void_p, c_int)
+    f.argtypes = (c_int, c_int) + (c_void_p,) * 4 + (u64,) * 14 + (c_bool, c_bool, c_double, c_int, c_void_p, c_int)
     f.restype = c_int
     for suffix, real in (("f", c_float), ("d", c_double)):
         ptr = POINTER(real)

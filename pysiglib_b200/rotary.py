@@ -13,9 +13,10 @@ import numpy as np
 import torch
 
 from .param_checks import check_type
-from .sequence_inputs import call, check_like, contiguous, element_type, empty, on_device, pointer, stream_of
+from .sequence_inputs import call, check_like, contiguous, element_type, empty, on_device, place_of, pointer
 
-POSITION_TYPES = {"int32": 1, "int64": 2, "float32": 3, "float64": 4}
+POSITION_TYPES = {torch.int32: 1, torch.int64: 2, torch.float32: 3, torch.float64: 4, np.dtype(np.int32): 1,
+                  np.dtype(np.int64): 2, np.dtype(np.float32): 3, np.dtype(np.float64): 4}
 
 
 def rotary_frequencies(
@@ -66,52 +67,65 @@ def rotary_frequencies(
     return f
 
 
-def _common_axes(x, out, positions):
-    """``(n0, n1, x strides, out strides, position strides)`` with the lead axes of all three read as the same
-    two axes (outer, inner, then the row stride), or None."""
-    lead = x.dim() - 2
-    arrays = [x.stride(), out.stride(), (0,) * (lead + 1) if positions is None else positions.stride()]
+def _common_axes(shape, strides):
+    """``(n0, n1)`` and, for each array, its strides ``(outer, inner, row)``, with the lead axes of ``shape`` (lead
+    axes, rows, dimension) read as the same two axes of all arrays; None where that cannot be."""
+    lead = len(shape) - 2
+    if lead == 2:
+        return shape[0], shape[1], strides
+    if lead == 1:
+        return 1, shape[0], [(0, *s) for s in strides]
+    if lead == 0:
+        return 1, 1, [(0, 0, *s) for s in strides]
     merged = []
     for i in range(lead):
-        n = x.shape[i]
+        n = shape[i]
         if n == 1:
             continue
-        now = tuple(s[i] for s in arrays)
+        now = [s[i] for s in strides]
         if merged and all(outer == n * inner for outer, inner in zip(merged[-1][1], now)):
             merged[-1] = (merged[-1][0] * n, now)
         else:
             merged.append((n, now))
     if len(merged) > 2:
         return None
-    n1, inner = merged[-1] if merged else (1, (0, 0, 0))
-    n0, outer = merged[0] if len(merged) == 2 else (1, (0, 0, 0))
-    xs, ys, ps = ((o, i, s[lead]) for o, i, s in zip(outer, inner, arrays))
-    return n0, n1, xs, ys, ps
+    none = (1, [0] * len(strides))
+    n0, outer = merged[0] if len(merged) == 2 else none
+    n1, inner = merged[-1] if merged else none
+    return n0, n1, [(o, i, s[lead]) for o, i, s in zip(outer, inner, strides)]
+
+
+def _position_strides(positions, lead):
+    """Strides along the axes ``lead`` of an array that broadcasts to them."""
+    missing = len(lead) - positions.dim()
+    return (0,) * missing + tuple(0 if n == 1 else s for n, s in zip(positions.shape, positions.stride()))
 
 
 def _rotate(x, frequencies, positions, interleaved, scale, inverse, name):
     code = element_type(x, name)
     check_like(frequencies, "frequencies", x, name)
-    check_type(interleaved, "interleaved", bool)
+    if interleaved is not True and interleaved is not False:
+        check_type(interleaved, "interleaved", bool)
+    if inverse is not True and inverse is not False:
+        check_type(inverse, "inverse", bool)
     check_type(scale, "scale", float)
-    shape = tuple(x.shape)
+    shape = x.shape
     if len(shape) < 2:
         raise ValueError("%s must have at least rank 2, got rank %d." % (name, len(shape)))
-    if str(frequencies.dtype).replace("torch.", "") != "float64":
+    if POSITION_TYPES.get(frequencies.dtype) != 4:
         raise TypeError("frequencies.dtype must be float64, got %s instead" % frequencies.dtype)
     if len(frequencies.shape) != 1 or 2 * frequencies.shape[0] > shape[-1]:
         raise ValueError("frequencies must be one value for each of at most %d pairs of channels, got shape %s"
                          % (shape[-1] // 2, tuple(frequencies.shape)))
-    kind = 0
+    lead, kind = shape[:-1], 0
     if positions is not None:
         check_like(positions, "positions", x, name)
-        kind = POSITION_TYPES.get(str(positions.dtype).replace("torch.", ""))
+        kind = POSITION_TYPES.get(positions.dtype)
         if kind is None:
             raise TypeError("positions.dtype must be int32, int64, float32 or float64, got %s instead" % positions.dtype)
-        lead = shape[:-1]
-        tail = tuple(positions.shape)
-        if len(tail) < 1 or len(tail) > len(lead) or any(p not in (1, n) for p, n in zip(tail, lead[len(lead) - len(tail):])):
-            raise ValueError("positions must broadcast to %s, got %s" % (lead, tail))
+        tail = positions.shape
+        if len(tail) < 1 or len(tail) > len(lead) or any(p != 1 and p != n for p, n in zip(tail, lead[len(lead) - len(tail):])):
+            raise ValueError("positions must broadcast to %s, got %s" % (tuple(lead), tuple(tail)))
     frequencies = contiguous(frequencies)
     rows, dim = shape[-2:]
     if on_device(x):
@@ -119,29 +133,30 @@ def _rotate(x, frequencies, positions, interleaved, scale, inverse, name):
             x = x.contiguous()
         out = torch.empty_like(x)
         if out.stride(-1) != 1 and dim != 1:
-            out = torch.empty(shape, dtype=x.dtype, device=x.device)
-        if positions is not None:
-            positions = positions.expand(shape[:-1])
-        views = _common_axes(x, out, positions)
+            out = x.new_empty(shape)
+        p = (0,) * len(lead) if positions is None else _position_strides(positions, lead)
+        views = _common_axes(shape, [x.stride()[:-1], out.stride()[:-1], p])
         if views is None:  # lead axes that no two strides describe
             x = x.contiguous()
-            out = torch.empty(shape, dtype=x.dtype, device=x.device)
-            positions = positions.contiguous() if positions is not None else None
-            views = _common_axes(x, out, positions)
-        n0, n1, xs, ys, ps = views
+            out = x.new_empty(shape)
+            if positions is not None:
+                positions = positions.expand(lead).contiguous()
+                p = positions.stride()
+            views = _common_axes(shape, [x.stride()[:-1], out.stride()[:-1], p])
+        n0, n1, (xs, ys, ps) = views
     else:
         x = contiguous(x)
         out = empty(x, shape, x.dtype)
         if positions is not None:
-            positions = (positions.expand(shape[:-1]).contiguous() if isinstance(positions, torch.Tensor) else
-                         np.ascontiguousarray(np.broadcast_to(positions, shape[:-1])))
+            positions = (positions.expand(lead).contiguous() if isinstance(positions, torch.Tensor) else
+                         np.ascontiguousarray(np.broadcast_to(positions, lead)))
         n0, n1 = 1, prod(shape[:-2])
         xs = ys = (0, rows * dim, dim)
         ps = (0, rows, 1)
-    if prod(shape) == 0:
+    if 0 in shape:
         return out
     call("rotary", code, kind, pointer(x), pointer(frequencies), pointer(positions), pointer(out), n0, n1, rows, dim,
-         2 * frequencies.shape[0], *xs, *ys, *ps, interleaved, inverse, scale, stream_of(x), 0)
+         2 * frequencies.shape[0], *xs, *ys, *ps, interleaved, inverse, scale, *place_of(x), 0)
     return out
 
 
@@ -176,7 +191,6 @@ def rotary(
         f = torch.from_numpy(pysiglib_b200.rotary_frequencies(64)).cuda()
         q = pysiglib_b200.rotary(torch.randn(4, 8, 1000, 64, device="cuda"), f)
     """
-    check_type(inverse, "inverse", bool)
     return _rotate(x, frequencies, positions, interleaved, scale, inverse, "x")
 
 

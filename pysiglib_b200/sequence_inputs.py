@@ -13,16 +13,18 @@ from .param_checks import check_type
 TORCH_TYPES = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.float16: 3}
 NUMPY_TYPES = {np.dtype(np.float32): 0, np.dtype(np.float64): 1, np.dtype(np.float16): 3}
 
+# handle of a device's current stream, without building a torch.cuda.Stream around it
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
 
 def element_type(array, name):
     """Number of the element type in the C ABI."""
-    if isinstance(array, torch.Tensor):
-        code = TORCH_TYPES.get(array.dtype)
-    else:
-        check_type(array, name, (np.ndarray, torch.Tensor))
-        code = NUMPY_TYPES.get(array.dtype)
+    code = TORCH_TYPES.get(array.dtype) if isinstance(array, torch.Tensor) else None
     if code is None:
-        raise TypeError("%s.dtype must be float32, float64, float16 or bfloat16, got %s instead" % (name, array.dtype))
+        check_type(array, name, (np.ndarray, torch.Tensor))
+        code = NUMPY_TYPES.get(array.dtype) if isinstance(array, np.ndarray) else None
+        if code is None:
+            raise TypeError("%s.dtype must be float32, float64, float16 or bfloat16, got %s instead" % (name, array.dtype))
     return code
 
 
@@ -35,11 +37,13 @@ def state_dtype(array):
 
 def check_like(array, name, like, like_name):
     """Same kind and device as ``like``."""
+    if isinstance(array, torch.Tensor) and isinstance(like, torch.Tensor):
+        if array.device != like.device:
+            raise ValueError("%s and %s must be on the same device" % (name, like_name))
+        return
     check_type(array, name, (np.ndarray, torch.Tensor))
-    if isinstance(array, torch.Tensor) != isinstance(like, torch.Tensor):
+    if isinstance(array, torch.Tensor) or isinstance(like, torch.Tensor):
         raise ValueError("%s and %s must both be numpy arrays or both torch tensors" % (name, like_name))
-    if isinstance(array, torch.Tensor) and array.device != like.device:
-        raise ValueError("%s and %s must be on the same device" % (name, like_name))
 
 
 def check_state(array, name, shape, x):
@@ -49,7 +53,7 @@ def check_state(array, name, shape, x):
     check_like(array, name, x, "x")
     if array.dtype != state_dtype(x):
         raise TypeError("%s.dtype must be %s for x of type %s, got %s instead" % (name, state_dtype(x), x.dtype, array.dtype))
-    if tuple(array.shape) != tuple(shape):
+    if array.shape != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(array.shape)))
     return contiguous(array)
 
@@ -70,14 +74,10 @@ def pointer(array):
 
 def empty(like, shape, dtype):
     if isinstance(like, torch.Tensor):
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        if dtype is like.dtype and shape == like.shape and like.is_contiguous():
+            return torch.empty_like(like)
+        return like.new_empty(shape, dtype=dtype)
     return np.empty(shape, dtype=dtype)
-
-
-def zeros(like, shape, dtype):
-    if isinstance(like, torch.Tensor):
-        return torch.zeros(shape, dtype=dtype, device=like.device)
-    return np.zeros(shape, dtype=dtype)
 
 
 def batched_rows(array):
@@ -88,11 +88,12 @@ def batched_rows(array):
     if on_device(array):
         strides = array.stride()
         if strides[-1] == 1 or width == 1:
-            if array.dim() == 2:
+            rank = len(shape)
+            if rank == 2:
                 return array, 0, strides[0]
-            if array.dim() == 3:
+            if rank == 3:
                 return array, strides[0], strides[1]
-            axis = array.dim() - 3
+            axis = rank - 3
             while axis > 0 and (shape[axis - 1] == 1 or strides[axis - 1] == strides[axis] * shape[axis]):
                 axis -= 1
             if axis == 0:
@@ -101,8 +102,15 @@ def batched_rows(array):
     return array, rows * width, width
 
 
-def stream_of(array):
-    return torch.cuda.current_stream(array.device).cuda_stream if on_device(array) else None
+def place_of(array):
+    """``(device, stream)`` for a native call: a CUDA tensor's device, all of whose operands this package has
+    checked, and its current stream; (-1, None) where the library looks for itself."""
+    if not on_device(array):
+        return -1, None
+    device = array.get_device()
+    if _current_raw_stream is not None:
+        return device, _current_raw_stream(device)
+    return device, torch.cuda.current_stream(device).cuda_stream
 
 
 def call(name, *args):

@@ -159,7 +159,7 @@ def test_native_entry_points_refuse_without_a_gpu():
 
     def recurrence(type=0, gate_type=0, x=p, gate=p, offsets=None, out=p, batch=2, rows=4, dim=4, gates=4, sequences=0, form=0):
         return lib.sigb200_linear_recurrence(type, gate_type, x, gate, None, offsets, out, None, None, batch, rows, dim, gates,
-                                             sequences, rows * dim, dim, rows * gates, gates, form, False, True, None, 1)
+                                             sequences, rows * dim, dim, rows * gates, gates, form, False, True, -1, None, 1)
     for kw in ({"type": 4}, {"type": -1}, {"gate_type": 1}, {"type": 1, "gate_type": 0}, {"gates": 3}, {"gates": 0}, {"dim": 0},
                {"form": 3}, {"x": None}, {"gate": None}, {"out": None}, {"sequences": 1}, {"sequences": 1, "offsets": p}):
         assert recurrence(**kw) == 2, (kw, load_cusig.last_error_message())
@@ -170,7 +170,7 @@ def test_native_entry_points_refuse_without_a_gpu():
     def rotary(type=0, kind=0, x=p, f=p, positions=None, out=p, rows=4, dim=4, part=4):
         freq = ctypes.cast(f, ctypes.POINTER(ctypes.c_double)) if f else None
         return lib.sigb200_rotary(type, kind, x, f, positions, out, 1, 1, rows, dim, part, 0, 0, dim, 0, 0, dim, 0, 0, 1,
-                                  False, False, 1.0, None, 1)
+                                  False, False, 1.0, -1, None, 1)
     for kw in ({"type": 9}, {"kind": 5}, {"part": 3}, {"part": 6}, {"x": None}, {"f": None}, {"out": None}, {"kind": 2}):
         assert rotary(**kw) == 2, (kw, load_cusig.last_error_message())
     assert rotary(rows=0) == 0
