@@ -8,7 +8,7 @@
 // the Taylor series within an eighth of a turn) and each output is rounded once.
 //
 // Split.  One read and one write per value bound it, as long as the sines are shared: a thread takes V pairs of
-// one position and walks over the rows (heads, batch entries) that have that position, four in flight; where
+// one position and walks over the rows (heads, batch entries) that have that position; where
 // every row has its own it takes four positions, loads them all, and turns one after the other.
 #include <algorithm>
 #include <type_traits>
@@ -30,13 +30,7 @@ struct RotaryGrid {
     int64_t xo0, xo1, yo0, yo1, po0, po1, xs0, xs1, ys0, ys1;  // strides of those axes
 };
 
-#ifndef ROT_WANT
-#define ROT_WANT 2048
-#endif
-#ifndef ROT_FLIGHT
-#define ROT_FLIGHT 4
-#endif
-constexpr int kInFlight = ROT_FLIGHT;
+constexpr int kInFlight = 4;  // rows of an unshared position, or of a copy
 
 // Sine and cosine of a number of turns.
 __device__ __forceinline__ void sine_cosine(double turns, float& s, float& c) {
@@ -64,7 +58,9 @@ __device__ __forceinline__ double position_at(const void* positions, int64_t at,
     else return static_cast<double>(static_cast<const P*>(positions)[at]);
 }
 
-// The 2 V channels of V pairs, in the order they are loaded: V and V.
+// The 2 V channels of V pairs, in the order they are loaded: V and V.  Interleaved pairs lie side by side within each
+// of the two (a thread takes V / 2 pairs from either half of the channels, so that its neighbours' loads join
+// up); for V = 1 the two are the pair.
 template <typename X, int V>
 struct Pairs {
     Pack<X, V> p, q;
@@ -75,7 +71,6 @@ __device__ __forceinline__ Pairs<X, V> turned(const Pairs<X, V>& x, const A (&s)
     A yp[V], yq[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        // interleaved pairs lie side by side in the 2 V values of p and q together
         const A a = widen(INTERLEAVED ? (2 * v < V ? x.p.v[(2 * v) % V] : x.q.v[(2 * v) % V]) : x.p.v[v]);
         const A b = widen(INTERLEAVED ? (2 * v + 1 < V ? x.p.v[(2 * v + 1) % V] : x.q.v[(2 * v + 1) % V]) : x.q.v[v]);
         const A ya = a * c[v] - b * s[v], yb = a * s[v] + b * c[v];
@@ -92,7 +87,7 @@ __device__ __forceinline__ Pairs<X, V> turned(const Pairs<X, V>& x, const A (&s)
 
 // SHARED: several rows have a thread's position.  Else each row has its own.
 template <typename X, typename P, int V, bool INTERLEAVED, bool SHARED>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs p, const RotaryGrid g) {
+__global__ void __launch_bounds__(256, SHARED || sizeof(X) == 2 ? 2 : 3) rotary_kernel(const RotaryArgs p, const RotaryGrid g) {
     using A = Acc<X>;
     uint64_t i = uint64_t(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= g.threads) return;
@@ -106,8 +101,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs p, const R
     const uint64_t group = SHARED ? i % g.groups : 0, outer = SHARED ? i / g.groups : i;
     const uint64_t o0 = outer / g.outer1, o1 = outer - o0 * g.outer1;
     const uint64_t row = SHARED ? unit : unit * kInFlight;
-    const int64_t cp = turning ? (INTERLEAVED ? 2 * int64_t(chunk) * V : int64_t(chunk) * V) : int64_t(p.rotary_dim) + int64_t(chunk) * V;
-    const int64_t cq = INTERLEAVED ? V : int64_t(p.rotary_dim / 2);  // from cp on
+    const int64_t cp = turning ? (INTERLEAVED && V == 1 ? 2 * int64_t(chunk) : int64_t(chunk) * V) : int64_t(p.rotary_dim) + int64_t(chunk) * V;
+    const int64_t cq = INTERLEAVED && V == 1 ? 1 : int64_t(p.rotary_dim / 2);  // from cp on
     const X* x = static_cast<const X*>(p.x) + int64_t(o0) * g.xo0 + int64_t(o1) * g.xo1 + int64_t(row) * int64_t(p.x_row) + cp;
     X* y = static_cast<X*>(p.out) + int64_t(o0) * g.yo0 + int64_t(o1) * g.yo1 + int64_t(row) * int64_t(p.out_row) + cp;
 
@@ -137,55 +132,93 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs p, const R
     };
 
     if (!turning) {
-        for (uint64_t k = 0; k < count; k += kInFlight) {
-            Pack<X, V> r[kInFlight];
+        Pack<X, V> r[kInFlight], ahead[kInFlight];
+        const auto read = [&](Pack<X, V> (&to)[kInFlight], uint64_t k) {
 #pragma unroll
             for (int n = 0; n < kInFlight; ++n)
                 if (k + n < count) {
-                    r[n] = load_pack<X, V>(x);
+                    to[n] = load_pack<X, V>(x);
                     next_x();
                 }
+        };
+        read(r, 0);
+        for (uint64_t k = 0; k < count; k += kInFlight) {
+            read(ahead, k + kInFlight);
 #pragma unroll
             for (int n = 0; n < kInFlight; ++n)
                 if (k + n < count) {
                     store_pack<X, V>(y, r[n]);
                     next_y();
+                    r[n] = ahead[n];
                 }
         }
         return;
     }
     A s[V], c[V];
-    const double* frequencies = p.frequencies + uint64_t(chunk) * V;
+    double per_turn[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const uint64_t pair = !INTERLEAVED || V == 1 ? uint64_t(chunk) * V + v : (v < V / 2 ? cp : cp + cq - V) / 2 + v;
+        per_turn[v] = p.frequencies[pair] * 0.15915494309189533577;
+    }
     const A scale = static_cast<A>(p.scale), signed_scale = static_cast<A>(p.inverse ? -p.scale : p.scale);
     const auto turn_at = [&](double position) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            sine_cosine(position * (frequencies[v] * 0.15915494309189533577), s[v], c[v]);
+            sine_cosine(position * per_turn[v], s[v], c[v]);
             s[v] *= signed_scale;
             c[v] *= scale;
         }
     };
     const int64_t place = int64_t(o0) * g.po0 + int64_t(o1) * g.po1 + int64_t(row) * int64_t(p.p_row);
-    if (SHARED) turn_at(position_at<P>(p.positions, place, row));
-    for (uint64_t k = 0; k < count; k += kInFlight) {
+    const auto load = [&] {
+        Pairs<X, V> r;
+        r.p = load_pack<X, V>(x);
+        r.q = load_pack<X, V>(x + cq);
+        next_x();
+        return r;
+    };
+    const auto store = [&](const Pairs<X, V>& r) {
+        const Pairs<X, V> t = turned<X, V, INTERLEAVED>(r, s, c);
+        store_pack<X, V>(y, t.p);
+        store_pack<X, V>(y + cq, t.q);
+        next_y();
+    };
+    if constexpr (SHARED) {
+        // two rows in flight while two are turned
+        Pairs<X, V> r[2], ahead[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+            if (uint64_t(n) < count) r[n] = load();
+        turn_at(position_at<P>(p.positions, place, row));
+        uint64_t k = 0;
+        for (; k + 4 <= count; k += 2) {
+            ahead[0] = load();
+            ahead[1] = load();
+            store(r[0]);
+            store(r[1]);
+            r[0] = ahead[0];
+            r[1] = ahead[1];
+        }
+        if (k + 3 == count) ahead[0] = load();
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+            if (k + n < count) store(r[n]);
+        if (k + 3 == count) store(ahead[0]);
+    } else {
         Pairs<X, V> r[kInFlight];
-        double position[SHARED ? 1 : kInFlight];
+        double position[kInFlight];
 #pragma unroll
         for (int n = 0; n < kInFlight; ++n)
-            if (k + n < count) {
-                r[n].p = load_pack<X, V>(x);
-                r[n].q = load_pack<X, V>(x + cq);
-                if (!SHARED) position[SHARED ? 0 : n] = position_at<P>(p.positions, place + n * int64_t(p.p_row), row + n);
-                next_x();
+            if (uint64_t(n) < count) {
+                r[n] = load();
+                position[n] = position_at<P>(p.positions, place + n * int64_t(p.p_row), row + n);
             }
 #pragma unroll
         for (int n = 0; n < kInFlight; ++n)
-            if (k + n < count) {
-                if (!SHARED) turn_at(position[SHARED ? 0 : n]);
-                const Pairs<X, V> t = turned<X, V, INTERLEAVED>(r[n], s, c);
-                store_pack<X, V>(y, t.p);
-                store_pack<X, V>(y + cq, t.q);
-                next_y();
+            if (uint64_t(n) < count) {
+                turn_at(position[n]);
+                store(r[n]);
             }
     }
 }
@@ -217,7 +250,7 @@ void launch(const RotaryArgs& p, cudaStream_t stream) {
     g.units = shared ? p.rows : (p.rows + kInFlight - 1) / kInFlight;
     // enough threads for every SM before one takes more of the rows that share a position
     const uint64_t lines = uint64_t(g.turned + g.copied) * g.units * outer;
-    const uint64_t wanted = uint64_t(device_context(current_device()).sm_count) * ROT_WANT;
+    const uint64_t wanted = uint64_t(device_context(current_device()).sm_count) * 1024;
     g.groups = std::max<uint64_t>(1, std::min<uint64_t>(g.shared, (wanted + lines - 1) / lines));
     g.per_thread = (g.shared + g.groups - 1) / g.groups;
     g.groups = (g.shared + g.per_thread - 1) / g.per_thread;
