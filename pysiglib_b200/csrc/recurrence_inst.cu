@@ -1,6 +1,7 @@
 // Launchers of the recurrence kernels for one pair of element types (SIG_RECURRENCE_PART picks it; one
 // object each, so that the pairs compile side by side).
 #include <algorithm>
+#include <atomic>
 
 #include "recurrence.h"
 #include "recurrence_kernels.cuh"
@@ -14,6 +15,8 @@ template <typename X> constexpr int kWide = sizeof(X) == 8 ? 2 : 4;
 // Rows a thread holds: as many as leave the arrays of S * V values in registers and two CTAs an SM their stages.
 template <int V> constexpr int kBackwardRows = V > 1 ? 4 : 8;
 template <typename X, int V> constexpr int kForwardRows = V > 1 && sizeof(X) > 2 ? 4 : 8;
+
+constexpr int kMostShared = 227 * 1024;  // of a CTA
 
 int log2_ceil(uint64_t n) {
     int k = 0;
@@ -87,11 +90,19 @@ size_t shared_memory(RecurrencePlan& plan, size_t stage_of_warp, size_t fixed) {
     return fixed + plan.stages * plan.warps * stage_of_warp;
 }
 
-template <typename... Params, typename... Args>
-void launch(void (*kernel)(Params...), const RecurrenceArgs& p, const RecurrencePlan& plan, size_t smem, cudaStream_t stream, Args... args) {
-    if (smem > 48 * 1024) SIG_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+// The kernels' limit of shared memory is raised once on each device.
+template <auto Kernel, typename... Args>
+void launch(const RecurrenceArgs& p, const RecurrencePlan& plan, size_t smem, cudaStream_t stream, Args... args) {
+    static std::atomic<uint64_t> raised{0};
+    if (smem > 48 * 1024) {
+        const uint64_t bit = 1ull << (current_device() & 63);
+        if (!(raised.load(std::memory_order_acquire) & bit)) {
+            SIG_CUDA_CHECK(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared));
+            if (current_device() < 64) raised.fetch_or(bit, std::memory_order_release);
+        }
+    }
     const unsigned grid = static_cast<unsigned>(p.batch) * plan.strips * unsigned(plan.segments);
-    kernel<<<grid, 32 * plan.warps, smem, stream>>>(p, plan, args...);
+    Kernel<<<grid, 32 * plan.warps, smem, stream>>>(p, plan, args...);
     check("linear recurrence kernel");
 }
 
@@ -106,8 +117,8 @@ void reduce_segments(const RecurrenceArgs& p, RecurrencePlan plan, cudaStream_t 
         constexpr int S = V == 1 ? 8 : 4;  // divides the rows of a thread: a block's are a multiple of it
     const size_t smem = shared_memory(plan, Prefetch<X, V, S, false>::kWarp + Prefetch<G, SHARED ? 1 : V, S, SHARED>::kWarp,
                                       plan.warps * (2 * sizeof(Acc<X>) * (V << plan.log_lanes) + sizeof(int)) + 16 + offset_room(p));
-    if (p.sequences) launch(recurrence_maps_kernel<X, G, V, S, SHARED, true, REVERSE>, p, plan, smem, stream);
-    else launch(recurrence_maps_kernel<X, G, V, S, SHARED, false, REVERSE>, p, plan, smem, stream);
+    if (p.sequences) launch<recurrence_maps_kernel<X, G, V, S, SHARED, true, REVERSE>>(p, plan, smem, stream);
+    else launch<recurrence_maps_kernel<X, G, V, S, SHARED, false, REVERSE>>(p, plan, smem, stream);
 }
 
 template <typename A>
@@ -128,8 +139,8 @@ void forward(const RecurrenceArgs& p, cudaStream_t stream) {
     const int width = V << plan.log_lanes;
     const size_t smem = shared_memory(plan, Prefetch<X, V, S, false>::kWarp + Prefetch<G, SHARED ? 1 : V, S, SHARED>::kWarp,
                                       sizeof(Acc<X>) * width * plan.warps + front_bytes<Acc<X>>(p, plan, width));
-    if (p.sequences) launch(recurrence_forward_kernel<X, G, V, S, SHARED, true>, p, plan, smem, stream);
-    else launch(recurrence_forward_kernel<X, G, V, S, SHARED, false>, p, plan, smem, stream);
+    if (p.sequences) launch<recurrence_forward_kernel<X, G, V, S, SHARED, true>>(p, plan, smem, stream);
+    else launch<recurrence_forward_kernel<X, G, V, S, SHARED, false>>(p, plan, smem, stream);
 }
 
 template <typename X, typename G, int V, bool SHARED>
@@ -155,11 +166,11 @@ void backward(const RecurrenceArgs& p, cudaStream_t stream) {
     const size_t smem = shared_memory(plan, 2 * Prefetch<X, V, S, false>::kWarp + Prefetch<G, SHARED ? 1 : V, S, SHARED>::kWarp + column,
                                       2 * plan.warps * column + front_bytes<Acc<X>>(p, plan, width));
     if (p.complement) {
-        if (p.sequences) launch(recurrence_backward_kernel<X, G, V, S, SHARED, true, true>, p, plan, smem, stream, partial);
-        else launch(recurrence_backward_kernel<X, G, V, S, SHARED, false, true>, p, plan, smem, stream, partial);
+        if (p.sequences) launch<recurrence_backward_kernel<X, G, V, S, SHARED, true, true>>(p, plan, smem, stream, partial);
+        else launch<recurrence_backward_kernel<X, G, V, S, SHARED, false, true>>(p, plan, smem, stream, partial);
     } else {
-        if (p.sequences) launch(recurrence_backward_kernel<X, G, V, S, SHARED, true, false>, p, plan, smem, stream, partial);
-        else launch(recurrence_backward_kernel<X, G, V, S, SHARED, false, false>, p, plan, smem, stream, partial);
+        if (p.sequences) launch<recurrence_backward_kernel<X, G, V, S, SHARED, true, false>>(p, plan, smem, stream, partial);
+        else launch<recurrence_backward_kernel<X, G, V, S, SHARED, false, false>>(p, plan, smem, stream, partial);
     }
     if (partial) {
         if (n / 256 >= 0x7fffffffull) throw std::invalid_argument("linear_recurrence_backprop: problem too large for one kernel launch");

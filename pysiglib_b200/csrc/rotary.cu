@@ -2,9 +2,9 @@
 //
 // Mathematics.  (y_p, y_q) = scale * (x_p cos w - x_q sin w, x_p sin w + x_q cos w) with w = p_t f_i, for the
 // pairs (i, i + r/2) or (2i, 2i + 1) of the first r channels; the others are copied.  The adjoint is the
-// turn by -w.  Angles are formed in 64 bits as turns, p_t * (f_i / 2 pi) less the nearest integer, so that a
+// turn by -w.  Angles are formed in 64 bits, as turns p_t * (f_i / 2 pi) less the nearest integer, so that a
 // position of millions keeps all the bits that the sine needs.  The sine and cosine of the remainder are
-// taken in the type of the arithmetic (64 bits for float64 rows, else 32: the nearest quarter turn off, then
+// taken in the type of the arithmetic (64 bits for float64 rows, of radians; else 32: the nearest quarter turn off, then
 // the Taylor series within an eighth of a turn) and each output is rounded once.
 //
 // Split.  One read and one write per value bound it, as long as the sines are shared: a thread takes V pairs of
@@ -50,7 +50,11 @@ __device__ __forceinline__ void sine_cosine(double turns, float& s, float& c) {
     s = k & 2 ? -a : a;
     c = (k + 1) & 2 ? -b : b;
 }
-__device__ __forceinline__ void sine_cosine(double turns, double& s, double& c) { sincospi(2.0 * (turns - rint(turns)), &s, &c); }
+// In 64 bits of an angle: less the nearest number of whole turns, 2 pi in two parts.
+__device__ __forceinline__ void sine_cosine(double angle, double& s, double& c) {
+    const double n = rint(angle * 0.15915494309189533577);
+    sincos(fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586232, angle)), &s, &c);
+}
 
 template <typename P>
 __device__ __forceinline__ double position_at(const void* positions, int64_t at, uint64_t row) {
@@ -155,17 +159,17 @@ __global__ void __launch_bounds__(256, SHARED || sizeof(X) == 2 ? 2 : 3) rotary_
         return;
     }
     A s[V], c[V];
-    double per_turn[V];
+    double rate[V];  // turns (float64: radians) for each unit of position
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const uint64_t pair = !INTERLEAVED || V == 1 ? uint64_t(chunk) * V + v : (v < V / 2 ? cp : cp + cq - V) / 2 + v;
-        per_turn[v] = p.frequencies[pair] * 0.15915494309189533577;
+        rate[v] = p.frequencies[pair] * (std::is_same_v<A, double> ? 1.0 : 0.15915494309189533577);
     }
     const A scale = static_cast<A>(p.scale), signed_scale = static_cast<A>(p.inverse ? -p.scale : p.scale);
     const auto turn_at = [&](double position) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            sine_cosine(position * per_turn[v], s[v], c[v]);
+            sine_cosine(position * rate[v], s[v], c[v]);
             s[v] *= signed_scale;
             c[v] *= scale;
         }
