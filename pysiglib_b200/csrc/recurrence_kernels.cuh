@@ -135,13 +135,8 @@ __device__ __forceinline__ int64_t sequence_of(SequenceWalk walk, int row) {
 // a = 1 / (1 + e) and 1 - a = e a.  The reciprocal is the hardware's (within 1 ulp).
 // FAST (gates of 16 bits): exponentials as 2^(v log2 e) in single precision, off by up to 2 + 1.2 |v| ulp.  A gate
 // of 8 or 11 bits leaves e^v uncertain by |v| 2^-9 or 2^-12 of itself, thousands of times more.
-__device__ __forceinline__ float exponential(float v, bool fast) {
-    if (!fast) return expf(v);
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.4426950408889634f));
-    return r;
-}
-__device__ __forceinline__ double exponential(double v, bool) { return exp(v); }
+__device__ __forceinline__ float exponential(float v) { return expf(v); }
+__device__ __forceinline__ double exponential(double v) { return exp(v); }
 // a = e^v and 1 - a together: v = n ln 2 + f with |f| <= ln 2 / 2 (ln 2 in two parts), p = e^f - 1 by its Taylor
 // series (the first term left out, f^8 / 8!, is below 2^-25 of p), a = 2^n + 2^n p and 1 - a = (1 - 2^n) - 2^n p,
 // both halved on the way so that 2^n stays finite.  Below e^-87 a is 0.
@@ -173,23 +168,118 @@ __device__ __forceinline__ float reciprocal(float v) {
     return r;
 }
 __device__ __forceinline__ double reciprocal(double v) { return 1.0 / v; }
-// PAIR: 1 - a is wanted as well.
-template <int FORM, bool FAST, bool PAIR, typename A>
-__device__ __forceinline__ void gate_factors(A v, A& a, A& rest) {
-    if (FORM == kGateValue) { a = v; rest = A(1) - v; }
-    else if (FORM == kGateLog) {
-        if (PAIR) exponential_pair(v, a, rest);
-        else a = exponential(v, FAST);
-    }
-    else {
-        const A e = below(exponential(-v, FAST));
-        a = reciprocal(A(1) + e);
-        rest = e * a;
-    }
-}
-
 __device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_(double a, double b, double c) { return fma(a, b, c); }
+
+// r = a b + c, a b, a + b and a - b on V values: two at a time where they are float32, which halves the issue slots
+// (what bounds these kernels for 16-bit inputs).
+template <typename A, int V> constexpr bool kTwo = std::is_same_v<A, float> && V % 2 == 0;
+template <typename A, int V>
+__device__ __forceinline__ void v_fma(A (&r)[V], const A (&a)[V], const A (&b)[V], const A (&c)[V]) {
+    if constexpr (kTwo<A, V>) {
+#pragma unroll
+        for (int v = 0; v < V; v += 2) {
+            const float2 t = __ffma2_rn(make_float2(a[v], a[v + 1]), make_float2(b[v], b[v + 1]), make_float2(c[v], c[v + 1]));
+            r[v] = t.x;
+            r[v + 1] = t.y;
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = fma_(a[v], b[v], c[v]);
+    }
+}
+template <typename A, int V>
+__device__ __forceinline__ void v_mul(A (&r)[V], const A (&a)[V], const A (&b)[V]) {
+    if constexpr (kTwo<A, V>) {
+#pragma unroll
+        for (int v = 0; v < V; v += 2) {
+            const float2 t = __fmul2_rn(make_float2(a[v], a[v + 1]), make_float2(b[v], b[v + 1]));
+            r[v] = t.x;
+            r[v + 1] = t.y;
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = a[v] * b[v];
+    }
+}
+template <typename A, int V>
+__device__ __forceinline__ void v_add(A (&r)[V], const A (&a)[V], const A (&b)[V]) {
+    if constexpr (kTwo<A, V>) {
+#pragma unroll
+        for (int v = 0; v < V; v += 2) {
+            const float2 t = __fadd2_rn(make_float2(a[v], a[v + 1]), make_float2(b[v], b[v + 1]));
+            r[v] = t.x;
+            r[v + 1] = t.y;
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = a[v] + b[v];
+    }
+}
+template <typename A, int V>
+__device__ __forceinline__ void v_sub(A (&r)[V], const A (&a)[V], const A (&b)[V]) {
+    if constexpr (kTwo<A, V>) {
+#pragma unroll
+        for (int v = 0; v < V; v += 2) {  // -1 b + a is exact up to its one rounding
+            const float2 t = __ffma2_rn(make_float2(b[v], b[v + 1]), make_float2(-1.0f, -1.0f), make_float2(a[v], a[v + 1]));
+            r[v] = t.x;
+            r[v + 1] = t.y;
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = a[v] - b[v];
+    }
+}
+template <typename A, int V>
+__device__ __forceinline__ void v_fill(A (&r)[V], A value) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) r[v] = value;
+}
+
+// a, and where PAIR 1 - a, of V gate values.
+template <int FORM, bool FAST, bool PAIR, typename A, int V>
+__device__ __forceinline__ void gate_factors(const A (&g)[V], A (&a)[V], A (&rest)[V]) {
+    if constexpr (FORM == kGateValue) {
+        A one[V];
+        v_fill(one, A(1));
+#pragma unroll
+        for (int v = 0; v < V; ++v) a[v] = g[v];
+        if (PAIR) v_sub(rest, one, g);
+    } else if constexpr (FORM == kGateLog && PAIR) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) exponential_pair(g[v], a[v], rest[v]);
+    } else if constexpr (std::is_same_v<A, float> && FAST) {
+        A t[V], unit[V];
+        v_fill(t, FORM == kGateLogit ? -1.4426950408889634f : 1.4426950408889634f);
+        v_mul(t, t, g);
+#pragma unroll
+        for (int v = 0; v < V; ++v) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t[v]) : "f"(t[v]));
+        if constexpr (FORM == kGateLog) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) a[v] = t[v];
+        } else {
+            if (PAIR) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) t[v] = below(t[v]);
+            }
+            v_fill(unit, 1.0f);
+            v_add(unit, unit, t);
+#pragma unroll
+            for (int v = 0; v < V; ++v) a[v] = reciprocal(unit[v]);
+            if (PAIR) v_mul(rest, t, a);
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if constexpr (FORM == kGateLog) a[v] = exponential(g[v]);
+            else {
+                const A e = PAIR ? below(exponential(-g[v])) : exponential(-g[v]);
+                a[v] = reciprocal(A(1) + e);
+                rest[v] = e * a[v];
+            }
+        }
+    }
+}
 
 constexpr int kCtaThreads = 256;  // at most
 
@@ -310,15 +400,17 @@ __device__ __forceinline__ void scan_warp(Map<A, V>& m, int log_lanes) {
     for (int k = 1; k < parts; k <<= 1) {
         const bool earlier_drop = PACKED && from(int(m.drop), k << log_lanes);
         const bool take = part >= k && !(PACKED && m.drop);
+        A ea[V], eb[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const A ea = from(m.a[v], k << log_lanes), eb = from(m.b[v], k << log_lanes);
-            if (take) {
-                m.b[v] = fma_(m.a[v], eb, m.b[v]);
-                m.a[v] *= ea;
-            }
+            ea[v] = from(m.a[v], k << log_lanes);
+            eb[v] = from(m.b[v], k << log_lanes);
         }
-        if (take) m.drop = earlier_drop;
+        if (take) {
+            v_fma(m.b, m.a, eb, m.b);
+            v_mul(m.a, m.a, ea);
+            m.drop = earlier_drop;
+        }
     }
 }
 
@@ -328,8 +420,11 @@ template <typename A, int V, bool REVERSE>
 __device__ __forceinline__ void enter_rows(const Map<A, V>& m, int log_lanes, const A (&in)[V], A (&h)[V], A* leaving) {
     const int lane = threadIdx.x & 31, lanes = 1 << log_lanes;
     Pack<A, V> behind;
+    v_fma(behind.v, m.a, in, m.b);
+    if (m.drop) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) behind.v[v] = m.drop ? m.b[v] : fma_(m.a[v], in[v], m.b[v]);
+        for (int v = 0; v < V; ++v) behind.v[v] = m.b[v];
+    }
     if (REVERSE ? lane < lanes : lane >= 32 - lanes) store_pack<A, V>(leaving, behind);
     const bool first = REVERSE ? lane >= 32 - lanes : lane < lanes;
 #pragma unroll
@@ -401,15 +496,17 @@ __device__ __forceinline__ void factors(const Prefetch<X, V, S, false>& fx, cons
     for (int s = 0; s < S; ++s) {
         const Pack<X, V> x = fx.take(stage, s);
         const Pack<G, GV> g = fg.take(stage, s);
-        A ga[GV], gr[GV];
+        A wide[GV], ga[GV], gr[GV], rest[V];
 #pragma unroll
-        for (int v = 0; v < GV; ++v) gate_factors<FORM, sizeof(G) == 2, COMPLEMENT>(A(widen(g.v[v])), ga[v], gr[v]);
+        for (int v = 0; v < GV; ++v) wide[v] = widen(g.v[v]);
+        gate_factors<FORM, sizeof(G) == 2, COMPLEMENT>(wide, ga, gr);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             a[s][v] = ga[v % GV];
+            rest[v] = gr[v % GV];
             u[s][v] = widen(x.v[v]);
-            if (COMPLEMENT) u[s][v] *= gr[v % GV];
         }
+        if (COMPLEMENT) v_mul(u[s], u[s], rest);
     }
 }
 
@@ -504,12 +601,13 @@ __device__ __forceinline__ void append_rows(Map<A, V>& m, const Rows<A, V, S>& r
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             const int s = REVERSE ? S - 1 - i : i;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                if (REVERSE) m.b[v] = r.a[s][v] * (r.u[s][v] + m.b[v]);
-                else m.b[v] = fma_(r.a[s][v], m.b[v], r.u[s][v]);
-                m.a[v] *= r.a[s][v];
+            if (REVERSE) {
+                v_add(m.b, r.u[s], m.b);
+                v_mul(m.b, r.a[s], m.b);
+            } else {
+                v_fma(m.b, r.a[s], m.b, r.u[s]);
             }
+            v_mul(m.a, m.a, r.a[s]);
         }
     }
 }
@@ -629,15 +727,13 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
                 if (stored == S) {
 #pragma unroll
                     for (int s = 0; s < S; ++s, to += dim) {
-#pragma unroll
-                        for (int v = 0; v < V; ++v) h[v] = fma_(r.a[s][v], h[v], r.u[s][v]);
+                        v_fma(h, r.a[s], h, r.u[s]);
                         store_pack<X, V>(to, narrow_pack<X, V>(h));
                     }
                 } else {
 #pragma unroll
                     for (int s = 0; s < S; ++s, to += dim) {
-#pragma unroll
-                        for (int v = 0; v < V; ++v) h[v] = fma_(r.a[s][v], h[v], r.u[s][v]);
+                        v_fma(h, r.a[s], h, r.u[s]);
                         if (s < stored) store_pack<X, V>(to, narrow_pack<X, V>(h));
                     }
                 }
@@ -704,20 +800,24 @@ __device__ __forceinline__ void walk_up(const Prefetch<X, V, S, false>& fx, cons
     for (int s = 0; s < S; ++s) {
         const Pack<X, V> x = fx.take(stage, s), d = fd.take(stage, s);
         const Pack<G, GV> g = fg.take(stage, s);
-        A ga[GV], gr[GV];
+        A wide[GV], ga[GV], gr[GV], rest[V], b[V];
 #pragma unroll
-        for (int v = 0; v < GV; ++v) gate_factors<FORM, sizeof(G) == 2, kPair>(A(widen(g.v[v])), ga[v], gr[v]);
+        for (int v = 0; v < GV; ++v) wide[v] = widen(g.v[v]);
+        gate_factors<FORM, sizeof(G) == 2, kPair>(wide, ga, gr);
         if (GV == 1 && kPair) kept.rest[GV > 1 ? 0 : s][0] = gr[0];
         const bool gone = !QUIET && (s >= r.count || (r.e.dead >> s & 1u));
         if (!QUIET && (r.e.starts >> s & 1u)) first_state(s, m.b);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const A in = widen(x.v[v]), b = COMPLEMENT ? gr[v % GV] * in : in;
-            if (V == 1) kept.x[V > 1 ? 0 : s][v] = in;
+            b[v] = widen(x.v[v]);
+            rest[v] = gr[v % GV];
+            if (V == 1) kept.x[V > 1 ? 0 : s][v] = b[v];
             r.a[s][v] = gone ? A(1) : ga[v % GV];
             r.u[s][v] = gone ? A(0) : A(widen(d.v[v]));
-            m.b[v] = fma_(r.a[s][v], m.b[v], gone ? A(0) : b);
         }
+        if (COMPLEMENT) v_mul(b, b, rest);
+        if (gone) v_fill(b, A(0));
+        v_fma(m.b, r.a[s], m.b, b);
     }
 }
 
@@ -738,7 +838,7 @@ __device__ __forceinline__ void walk_out(const Prefetch<X, V, S, false>& fx, con
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         if (!QUIET && (r.e.starts >> s & 1u)) first_state(s, h);
-        A x[V], rest[GV], dx[V], dgate[V];
+        A x[V], rest[V], dx[V], dgate[V];
         if (V > 1) {
             const Pack<X, V> again = fx.take(stage, s);
 #pragma unroll
@@ -746,28 +846,34 @@ __device__ __forceinline__ void walk_out(const Prefetch<X, V, S, false>& fx, con
         } else {
             x[0] = kept.x[V > 1 ? 0 : s][0];
         }
-        if (kPair && GV > 1) {
+        if constexpr (kPair && GV > 1) {
             const Pack<G, GV> g = fg.take(stage, s);
+            A wide[GV], unused[GV];
 #pragma unroll
-            for (int v = 0; v < GV; ++v) {
-                A unused;
-                gate_factors<FORM, sizeof(G) == 2, true>(A(widen(g.v[v])), unused, rest[v]);
-            }
+            for (int v = 0; v < GV; ++v) wide[v] = widen(g.v[v]);
+            gate_factors<FORM, sizeof(G) == 2, true>(wide, unused, rest);
         } else if (kPair) {
-            rest[0] = kept.rest[GV > 1 ? 0 : s][0];
+            v_fill(rest, kept.rest[GV > 1 ? 0 : s][0]);
         }
         const bool dead = !QUIET && (r.e.dead >> s & 1u);
+        if (COMPLEMENT) {
+            v_mul(dx, rest, r.u[s]);
+            v_sub(dgate, h, x);
+            v_mul(dgate, dgate, r.u[s]);
+            v_mul(x, x, rest);
+        } else {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const A g = r.u[s][v], a = r.a[s][v];
-            dx[v] = COMPLEMENT ? rest[v % GV] * g : g;
-            dgate[v] = g * (COMPLEMENT ? h[v] - x[v] : h[v]);
-            if (FORM != kGateValue) dgate[v] *= a;
-            if (FORM == kGateLogit) dgate[v] *= rest[v % GV];
-            if (dead) dx[v] = dgate[v] = A(0);
-            h[v] = fma_(a, h[v], COMPLEMENT ? rest[v % GV] * x[v] : x[v]);
+            for (int v = 0; v < V; ++v) dx[v] = r.u[s][v];
+            v_mul(dgate, h, r.u[s]);
         }
-        store(s, dx, dgate);
+        if (FORM != kGateValue) v_mul(dgate, dgate, r.a[s]);
+        if (FORM == kGateLogit) v_mul(dgate, dgate, rest);
+        if (dead) {
+            v_fill(dx, A(0));
+            v_fill(dgate, A(0));
+        }
+        v_fma(h, r.a[s], h, x);
+        store(std::bool_constant<QUIET>{}, s, dx, dgate);
     }
 }
 
@@ -935,11 +1041,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
         // backward through the rows: the derivatives become g
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                if (!(PACKED && (r.e.ends >> s & 1u))) r.u[s][v] += behind[v];
-                behind[v] = r.a[s][v] * r.u[s][v];
-            }
+            if (!(PACKED && (r.e.ends >> s & 1u))) v_add(r.u[s], r.u[s], behind);
+            v_mul(behind, r.a[s], r.u[s]);
             if (PACKED && dinitial && live && (r.e.starts >> s & 1u)) {
                 A* to = dinitial + sequence_of(walk, row0 + s) * dim;
 #pragma unroll
@@ -951,8 +1054,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
         G* to_gate = dgate;
         dx -= out_span;
         dgate -= SHARED ? 0 : out_span;
-        const auto store = [&](int s, const A (&gx)[V], const A (&gg)[V]) {
-            if (s < r.count) store_pack<X, V>(to_x, narrow_pack<X, V>(gx));
+        const auto store = [&](auto all, int s, const A (&gx)[V], const A (&gg)[V]) {
+            if (all || s < r.count) store_pack<X, V>(to_x, narrow_pack<X, V>(gx));
             to_x += dim;
             if constexpr (SHARED) {
                 A sum = gg[0];
@@ -961,7 +1064,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
                 sums[s] = sum;
             } else {
                 if constexpr (std::is_same_v<Acc<G>, A>)
-                    if (s < r.count) store_pack<G, V>(to_gate, narrow_pack<G, V>(gg));
+                    if (all || s < r.count) store_pack<G, V>(to_gate, narrow_pack<G, V>(gg));
                 to_gate += dim;
             }
         };
@@ -1117,15 +1220,18 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(const RecurrenceAr
     A* at = static_cast<A*>(p.state) + row * p.dim + c0;
     Pack<A, V> h = load_pack<A, V>(at);
     Pack<X, V> y;
+    constexpr int GV = SHARED ? 1 : V;
+    A wide[GV], a[GV], rest[GV];
+#pragma unroll
+    for (int v = 0; v < GV; ++v) wide[v] = widen(g.v[v]);
+    if (p.form == kGateValue) gate_factors<kGateValue, sizeof(G) == 2, true>(wide, a, rest);
+    else if (p.form == kGateLog) gate_factors<kGateLog, sizeof(G) == 2, true>(wide, a, rest);
+    else gate_factors<kGateLogit, sizeof(G) == 2, true>(wide, a, rest);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        A a, rest, u = widen(x.v[v]);
-        const A t = widen(g.v[SHARED ? 0 : v]);
-        if (p.form == kGateValue) gate_factors<kGateValue, sizeof(G) == 2, true>(t, a, rest);
-        else if (p.form == kGateLog) gate_factors<kGateLog, sizeof(G) == 2, true>(t, a, rest);
-        else gate_factors<kGateLogit, sizeof(G) == 2, true>(t, a, rest);
-        if (p.complement) u *= rest;
-        h.v[v] = fma_(a, h.v[v], u);
+        A u = widen(x.v[v]);
+        if (p.complement) u *= rest[v % GV];
+        h.v[v] = fma_(a[v % GV], h.v[v], u);
         y.v[v] = narrow<X>(h.v[v]);
     }
     store_pack<A, V>(at, h);
