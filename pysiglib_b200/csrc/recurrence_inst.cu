@@ -13,7 +13,7 @@ namespace {
 // widen to the same registers).
 template <typename X> constexpr int kWide = sizeof(X) == 8 ? 2 : 4;
 // Rows a thread holds: as many as leave the arrays of S * V values in registers and two CTAs an SM their stages.
-template <int V> constexpr int kBackwardRows = V > 1 ? 4 : 8;
+template <typename X, int V> constexpr int kBackwardRows = V > 1 && sizeof(X) > 2 ? 4 : 8;
 template <typename X, int V> constexpr int kForwardRows = V > 1 && sizeof(X) > 2 ? 4 : 8;
 
 constexpr int kMostShared = 227 * 1024;  // of a CTA
@@ -145,7 +145,7 @@ void forward(const RecurrenceArgs& p, cudaStream_t stream) {
 
 template <typename X, typename G, int V, bool SHARED>
 void backward(const RecurrenceArgs& p, cudaStream_t stream) {
-    constexpr int S = kBackwardRows<V>;
+    constexpr int S = kBackwardRows<X, V>;
     RecurrencePlan plan = make_plan<X>(p, V, S);
     Scratch maps(maps_bytes<Acc<X>>(p, plan), stream);
     if (plan.segments > 1) {

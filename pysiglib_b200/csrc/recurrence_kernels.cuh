@@ -415,9 +415,9 @@ __device__ __forceinline__ void scan_warp(Map<A, V>& m, int log_lanes) {
 }
 
 // The state that enters this thread's rows, from `in`, which enters its warp's, and the maps of scan_warp; lanes of the
-// part that comes last leave what leaves the warp at `leaving`.
-template <typename A, int V, bool REVERSE>
-__device__ __forceinline__ void enter_rows(const Map<A, V>& m, int log_lanes, const A (&in)[V], A (&h)[V], A* leaving) {
+// part that comes last put what leaves the warp at `leaving`, before `pass_on`.
+template <typename A, int V, bool REVERSE, typename PassOn>
+__device__ __forceinline__ void enter_rows(const Map<A, V>& m, int log_lanes, const A (&in)[V], A (&h)[V], A* leaving, const PassOn& pass_on) {
     const int lane = threadIdx.x & 31, lanes = 1 << log_lanes;
     Pack<A, V> behind;
     v_fma(behind.v, m.a, in, m.b);
@@ -426,6 +426,7 @@ __device__ __forceinline__ void enter_rows(const Map<A, V>& m, int log_lanes, co
         for (int v = 0; v < V; ++v) behind.v[v] = m.b[v];
     }
     if (REVERSE ? lane < lanes : lane >= 32 - lanes) store_pack<A, V>(leaving, behind);
+    pass_on();  // the next warp waits for it
     const bool first = REVERSE ? lane >= 32 - lanes : lane < lanes;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -712,8 +713,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
             for (int v = 0; v < V; ++v) in[v] = c.v[v];
         }
         A h[V];
-        enter_rows<A, V, false>(m, plan.log_lanes, in, h, leaving);
-        if (warps > 1 && (at.warp + 1 < warps || base + span < rows)) give(link);
+        enter_rows<A, V, false>(m, plan.log_lanes, in, h, leaving,
+                                [&] { if (warps > 1 && (at.warp + 1 < warps || base + span < rows)) give(link); });
         if (r.count) {
             if (marks && row0 % int(kCheckpointRows) == 0) {
                 Pack<A, V> mark;
@@ -1025,8 +1026,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
 #pragma unroll
             for (int v = 0; v < V; ++v) in[v] = c.v[v];
         }
-        enter_rows<A, V, false>(m, plan.log_lanes, in, h, ahead + (at.warp + 1 == warps ? 0 : at.warp + 1) * width);
-        if (passes) give(warps + 1 + at.warp);
+        enter_rows<A, V, false>(m, plan.log_lanes, in, h, ahead + (at.warp + 1 == warps ? 0 : at.warp + 1) * width,
+                                [&] { if (passes) give(warps + 1 + at.warp); });
         // backward: the gradient
         if (base != last_base || at.warp + 1 < warps) {
             if (warps > 1) take_over(link_behind);
@@ -1036,8 +1037,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
             for (int v = 0; v < V; ++v) w[v] = c.v[v];
         }
         A behind[V];
-        enter_rows<A, V, true>(g, plan.log_lanes, w, behind, leaving);
-        if (warps > 1 && (at.warp || base > first)) give(link);
+        enter_rows<A, V, true>(g, plan.log_lanes, w, behind, leaving, [&] { if (warps > 1 && (at.warp || base > first)) give(link); });
         // backward through the rows: the derivatives become g
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {
