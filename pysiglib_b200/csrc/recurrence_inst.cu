@@ -47,8 +47,9 @@ RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     plan.log_lanes = std::min({columns, log2_ceil(128 / (V * sizeof(X))), 5});
     const auto ctas = [&](int log_lanes) { return p.batch * (((per_row - 1) >> log_lanes) + 1); };
     if (plan.log_lanes > 0 && ctas(plan.log_lanes) < sms && ctas(plan.log_lanes - 1) >= sms) --plan.log_lanes;
-    // as wide as leaves a strip for each SM and more, where that pads no more channels
-    while (plan.log_lanes < std::min(columns, 5) && 2 * ctas(plan.log_lanes + 1) >= 3 * sms && ctas(plan.log_lanes + 1) * 2 == ctas(plan.log_lanes))
+    // two lines wide where that pads no more channels and leaves strips for one and a half rounds of the SMs:
+    // half the parts to compose (bf16 64x500x768 36 against 40 us, float32 40x600x512 30 against 35 us)
+    if (plan.log_lanes < std::min(columns, 5) && 2 * ctas(plan.log_lanes + 1) >= 3 * sms && ctas(plan.log_lanes + 1) * 2 == ctas(plan.log_lanes))
         ++plan.log_lanes;
     // short inputs: no more parts than there are rows for, the lanes go to the channels instead
     plan.log_lanes = std::max(plan.log_lanes, std::min(columns, 5 - std::min(needed, 5)));
@@ -57,9 +58,12 @@ RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     if (ctas(plan.log_lanes) > 0x7fffffffull)
         throw std::invalid_argument("linear_recurrence: problem too large for one kernel launch");
     plan.strips = static_cast<unsigned>(((per_row - 1) >> plan.log_lanes) + 1);
-    // shorter rings where there are many strips: all of them resident at a time, and fewer hand-overs
-    const uint64_t strips = ctas(plan.log_lanes), warp_rows = uint64_t(32 >> plan.log_lanes) * S;
-    while (plan.warps > 1 && strips * plan.warps > kResident * sms && plan.warps / 2 * warp_rows % kCheckpointRows == 0) plan.warps /= 2;
+    const uint64_t strips = ctas(plan.log_lanes), warp_rows = uint64_t(32 >> plan.log_lanes) * S, round = 2 * sms;
+    // rings of four warps where CTAs of eight would leave most of a second round empty, or where all CTAs of four
+    // just fit one (float32 64x512x272, 576 strips: 24.6 against 26.7 us; at 512 strips eight take 289, four 334 us)
+    if (plan.warps == 8 && ((strips > round && 2 * strips <= 3 * round) || (20 * strips > 38 * round && strips <= 2 * round)) &&
+        4 * warp_rows % kCheckpointRows == 0)
+        plan.warps = 4;
     const uint64_t span = plan.warps * warp_rows, blocks = (p.rows + span - 1) / span;
     uint64_t segments = 1;
     if (strips < sms) segments = std::min(blocks, kResident * sms / (strips * plan.warps));
