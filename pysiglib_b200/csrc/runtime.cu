@@ -142,11 +142,24 @@ Scratch::~Scratch() {
     if (ptr_) (void)cudaFreeAsync(ptr_, stream_);
 }
 
+namespace {
+
+// The calls that set a device up touch no stream being captured: the first call of a process may be a
+// captured one.
+struct SetUpDuringCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    SetUpDuringCapture() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~SetUpDuringCapture() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+}  // namespace
+
 DeviceContext& device_context(int device) {
     std::lock_guard<std::mutex> lock(g_contexts_mu);
     auto it = g_contexts.find(device);
     if (it != g_contexts.end()) return *it->second;
     DeviceGuard guard(device);
+    SetUpDuringCapture relaxed;
     auto ctx = std::make_unique<DeviceContext>();
     ctx->device = device;
     SIG_CUDA_CHECK(cudaStreamCreateWithFlags(&ctx->copy_in, cudaStreamNonBlocking));

@@ -302,3 +302,121 @@ def test_host_arrays(dtype):
     one = so.recurrence(x[:5, None], gate[:5, None], start, "logit", True)
     so.check(torch.from_numpy(out), (one["h"][0][:, 0], one["h"][1][:, 0]), "step")
     so.check(torch.from_numpy(s), one["state"], "state")
+
+
+@pytest.mark.parametrize("dtype,gate_dtype", TYPES)
+@pytest.mark.parametrize("rows,dim,gates,sequences", [(5000, 64, 64, 0), (3001, 33, 33, 0), (4100, 128, 2, 9), (2500, 20, 20, 40)])
+def test_rows_cut_into_segments(dtype, gate_dtype, rows, dim, gates, sequences):
+    """One batch entry, few channels: the rows are shared out over the SMs and joined."""
+    form = "log" if sequences else "logit"
+    run_and_check(make(rows + dim, 1, rows, dim, gates, dtype, gate_dtype, form, True, sequences), form, dim == 64, rows % 2 == 0)
+
+
+@pytest.mark.parametrize("batch,rows,dim,dtype", [(80, 150, 128, F32), (64, 70, 1024, BF16), (700, 40, 64, F16), (3, 40, 8200, F32),
+                                                  (2500, 9, 16, F64), (130, 33, 130, BF16)])
+def test_many_strips(batch, rows, dim, dtype):
+    run_and_check(make(batch, batch, rows, dim, dim, dtype, dtype, "logit", True), "logit", False)
+
+
+@pytest.mark.parametrize("dim", [4, 12, 20, 36])
+@pytest.mark.parametrize("dtype,gate_dtype", [(BF16, BF16), (F16, F32)])
+def test_sixteen_bit_rows_aligned_to_eight_bytes(dim, dtype, gate_dtype):
+    run_and_check(make(dim, 2, 100, dim, dim, dtype, gate_dtype, "logit", True), "logit", True)
+    g = torch.Generator().manual_seed(dim)
+    wide = torch.randn(2, 90, 64, generator=g).to(dtype)
+    view = lambda t: t[..., 4:4 + dim]  # dense rows of 128 bytes that start 8 bytes in
+    gate = torch.randn(2, 90, dim, generator=g).to(gate_dtype)
+    expect = so.recurrence(view(wide).contiguous(), gate, None, "logit", False, None, view(wide).contiguous())
+    W = wide.cuda()
+    dx, dgate, _ = psl.linear_recurrence_backprop(view(W), view(W), gate.cuda(), gate_form="logit")
+    so.check(psl.linear_recurrence(view(W), gate.cuda(), gate_form="logit"), expect["h"], "h")
+    so.check(dx, expect["dx"], "dx")
+    so.check(dgate, expect["dgate"], "dgate")
+
+
+def test_a_captured_training_step():
+    """Warmed up on a side stream, as torch asks for: a graph that was made eagerly on the default stream and still
+    lives would tie the leaves to that stream, for any torch operation."""
+    x, gate, start, derivs, tail, _ = make(50, 2, 300, 32, 4, F32, F32, "logit", True)
+    expect = so.recurrence(x, gate, start, "logit", True, None, derivs, tail)
+    X, G, S = (cuda(t).requires_grad_() for t in (x, gate, start))
+    D, T = cuda(derivs), cuda(tail)
+
+    def step():
+        h, state = torch_api.linear_recurrence(X, G, S, gate_form="logit", complement=True, return_state=True)
+        return torch.autograd.grad((h, state), (X, G, S), (D, T))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = step()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for name, got in zip(("dx", "dgate", "dinitial"), grads):
+        so.check(got, expect[name], name)
+
+
+def test_calls_from_two_threads():
+    import threading
+    sets = [make(60 + k, 1, 2000, 64, 2, BF16, F32, "log", True, 7) for k in range(2)]
+    expects = [so.recurrence(*s[:3], "log", False, s[5], s[3]) for s in sets]
+    failures = []
+
+    def work(k):
+        try:
+            x, gate, start, derivs, _, offsets = (cuda(t) for t in sets[k])
+            stream = torch.cuda.Stream()
+            stream.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    h = psl.linear_recurrence(x, gate, start, gate_form="log", offsets=offsets)
+                    grads = psl.linear_recurrence_backprop(derivs, x, gate, start, gate_form="log", offsets=offsets)
+            stream.synchronize()
+            for name, got in zip(("h", "dx", "dgate", "dinitial"), (h, *grads)):
+                so.check(got, expects[k][name], name)
+        except BaseException as e:  # noqa: BLE001
+            failures.append(e)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failures, failures
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    code = ("import torch, pysiglib_b200 as psl\n"
+            "x = torch.randn(2, 300, 48, device='cuda'); g = torch.randn(2, 300, 1, device='cuda')\n"
+            "graph = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(graph):\n"
+            "    h = psl.linear_recurrence(x, g, gate_form='logit')\n"
+            "    d = psl.linear_recurrence_backprop(x, x, g, gate_form='logit')[1]\n"
+            "graph.replay(); torch.cuda.synchronize()\n"
+            "assert torch.equal(h, psl.linear_recurrence(x, g, gate_form='logit'))\n"
+            "assert torch.equal(d, psl.linear_recurrence_backprop(x, x, g, gate_form='logit')[1])\n")
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_offsets_that_are_out_of_order_stay_in_bounds():
+    """Device offsets are trusted; wrong ones give wrong numbers for their own sequences and nothing else: memory around
+    the arrays stays as it was."""
+    rows, dim = 200, 16
+    whole = torch.full((3 * rows, dim), 7.0, device="cuda")
+    x = whole[rows:2 * rows]
+    gate = torch.full((rows, dim), 0.5, device="cuda")
+    for bad in ([0, 150, 50, 200], [-5, 10, 300], [90, 80, 70, 60], [2 ** 40, -2 ** 40, 5], [200, 200, 200]):
+        offsets = torch.tensor(bad, device="cuda")
+        start = torch.zeros(len(bad) - 1, dim, device="cuda")
+        psl.linear_recurrence(x, gate, start, offsets=offsets, return_state=True)
+        psl.linear_recurrence_backprop(x, x, gate, start, offsets=offsets)
+    torch.cuda.synchronize()
+    assert (whole == 7.0).all()
+    expect = so.recurrence(x.cpu()[None], gate.cpu()[None], None, "value", False)["h"]
+    so.check(psl.linear_recurrence(x, gate), tuple(t[0] for t in expect), "h")
