@@ -10,8 +10,8 @@ import numpy as np
 import torch
 
 from .param_checks import check_type
-from .sequence_inputs import (batched_rows, call, check_like, check_state, contiguous, element_type, empty, on_device,
-                              place_of, pointer, state_dtype)
+from .sequence_inputs import (TORCH_TYPES, batched_rows, call, check_like, check_state, contiguous, element_type, empty,
+                              on_device, place_of, pointer, raw_stream, state_dtype)
 
 GATE_FORMS = {"value": 0, "log": 1, "logit": 2}
 CHECKPOINT_ROWS = 16  # rows between two of the states kept for the backward pass
@@ -19,8 +19,13 @@ CHECKPOINT_ROWS = 16  # rows between two of the states kept for the backward pas
 
 def _check_gate(x, gate, gate_form, complement):
     """``(element type, gate type, gate form, gates)`` of inputs ``(..., dimension)`` and gates ``(..., G)``."""
-    code, gate_code = element_type(x, "x"), element_type(gate, "gate")
-    check_like(gate, "gate", x, "x")
+    if isinstance(x, torch.Tensor) and isinstance(gate, torch.Tensor) and x.device == gate.device:
+        code, gate_code = TORCH_TYPES.get(x.dtype), TORCH_TYPES.get(gate.dtype)
+    else:
+        code = gate_code = None
+    if code is None or gate_code is None:
+        code, gate_code = element_type(x, "x"), element_type(gate, "gate")
+        check_like(gate, "gate", x, "x")
     if gate_code != code and not (gate_code == 0 and code >= 2):
         raise TypeError("gate.dtype must be that of x, or float32 for 16-bit x; got %s for %s" % (gate.dtype, x.dtype))
     form = GATE_FORMS.get(gate_form) if isinstance(gate_form, str) else None
@@ -223,19 +228,29 @@ def linear_recurrence_step(
     Stepping through a sequence gives what ``linear_recurrence`` gives for it, up to rounding.
     """
     code, gate_code, form = _check_gate(x, gate, gate_form, complement)
-    check_like(state, "state", x, "x")
+    if not isinstance(state, torch.Tensor) or state.device != getattr(x, "device", None):
+        check_like(state, "state", x, "x")
     shape = x.shape
     if len(shape) < 1:
         raise ValueError("x must have at least rank 1, got rank 0.")
     dim, gates = _check_gate_shape(shape, gate.shape)
+    torch_state = isinstance(state, torch.Tensor)
     if state.dtype != state_dtype(x):
         raise TypeError("state.dtype must be %s for x of type %s, got %s instead" % (state_dtype(x), x.dtype, state.dtype))
     if state.shape != shape:
         raise ValueError("state must have the shape of x, %s, got %s" % (tuple(shape), tuple(state.shape)))
-    if not (state.is_contiguous() if isinstance(state, torch.Tensor) else state.flags["C_CONTIGUOUS"] and state.flags["WRITEABLE"]):
+    if not (state.is_contiguous() if torch_state else state.flags["C_CONTIGUOUS"] and state.flags["WRITEABLE"]):
         raise ValueError("state is overwritten: it must be contiguous and writeable")
-    if isinstance(state, torch.Tensor) and state.requires_grad:
+    if torch_state and state.requires_grad:
         raise ValueError("state is overwritten: it cannot require a gradient (use linear_recurrence to differentiate)")
+    if torch_state and state.is_cuda:
+        x, gate = x.contiguous(), gate.contiguous()
+        out = torch.empty_like(x)
+        if out.numel():
+            device = x.get_device()
+            call("linear_recurrence_step", code, gate_code, x.data_ptr(), gate.data_ptr(), state.data_ptr(), out.data_ptr(),
+                 out.numel() // dim, dim, gates, dim, gates, form, complement, device, raw_stream(device), 0)
+        return out
     x, gate = contiguous(x), contiguous(gate)
     out = empty(x, shape, x.dtype)
     batch = prod(shape[:-1])

@@ -13,7 +13,7 @@ import numpy as np
 import torch
 
 from .param_checks import check_type
-from .sequence_inputs import call, check_like, contiguous, element_type, empty, on_device, place_of, pointer
+from .sequence_inputs import TORCH_TYPES, call, check_like, contiguous, element_type, empty, pointer, raw_stream
 
 POSITION_TYPES = {torch.int32: 1, torch.int64: 2, torch.float32: 3, torch.float64: 4, np.dtype(np.int32): 1,
                   np.dtype(np.int64): 2, np.dtype(np.float32): 3, np.dtype(np.float64): 4}
@@ -97,18 +97,25 @@ def _common_axes(shape, strides):
 
 def _position_strides(positions, lead):
     """Strides along the axes ``lead`` of an array that broadcasts to them."""
-    missing = len(lead) - positions.dim()
-    return (0,) * missing + tuple(0 if n == 1 else s for n, s in zip(positions.shape, positions.stride()))
+    strides = positions.stride()
+    if positions.shape == lead:
+        return strides
+    return (0,) * (len(lead) - len(strides)) + tuple([0 if n == 1 else s for n, s in zip(positions.shape, strides)])
 
 
 def _rotate(x, frequencies, positions, interleaved, scale, inverse, name):
-    code = element_type(x, name)
-    check_like(frequencies, "frequencies", x, name)
+    on_device = isinstance(x, torch.Tensor) and x.is_cuda
+    code = TORCH_TYPES.get(x.dtype) if on_device else None
+    if code is None:
+        code = element_type(x, name)
+    if not (on_device and isinstance(frequencies, torch.Tensor) and frequencies.device == x.device):
+        check_like(frequencies, "frequencies", x, name)
     if interleaved is not True and interleaved is not False:
         check_type(interleaved, "interleaved", bool)
     if inverse is not True and inverse is not False:
         check_type(inverse, "inverse", bool)
-    check_type(scale, "scale", float)
+    if not isinstance(scale, float):
+        check_type(scale, "scale", float)
     shape = x.shape
     if len(shape) < 2:
         raise ValueError("%s must have at least rank 2, got rank %d." % (name, len(shape)))
@@ -119,16 +126,18 @@ def _rotate(x, frequencies, positions, interleaved, scale, inverse, name):
                          % (shape[-1] // 2, tuple(frequencies.shape)))
     lead, kind = shape[:-1], 0
     if positions is not None:
-        check_like(positions, "positions", x, name)
+        if not (on_device and isinstance(positions, torch.Tensor) and positions.device == x.device):
+            check_like(positions, "positions", x, name)
         kind = POSITION_TYPES.get(positions.dtype)
         if kind is None:
             raise TypeError("positions.dtype must be int32, int64, float32 or float64, got %s instead" % positions.dtype)
         tail = positions.shape
-        if len(tail) < 1 or len(tail) > len(lead) or any(p != 1 and p != n for p, n in zip(tail, lead[len(lead) - len(tail):])):
+        if tail != lead and (len(tail) < 1 or len(tail) > len(lead) or
+                             any(p != 1 and p != n for p, n in zip(tail, lead[len(lead) - len(tail):]))):
             raise ValueError("positions must broadcast to %s, got %s" % (tuple(lead), tuple(tail)))
     frequencies = contiguous(frequencies)
-    rows, dim = shape[-2:]
-    if on_device(x):
+    rows, dim = shape[-2], shape[-1]
+    if on_device:
         if x.stride(-1) != 1 and dim != 1:
             x = x.contiguous()
         out = torch.empty_like(x)
@@ -143,20 +152,22 @@ def _rotate(x, frequencies, positions, interleaved, scale, inverse, name):
                 positions = positions.expand(lead).contiguous()
                 p = positions.stride()
             views = _common_axes(shape, [x.stride()[:-1], out.stride()[:-1], p])
-        n0, n1, (xs, ys, ps) = views
-    else:
-        x = contiguous(x)
-        out = empty(x, shape, x.dtype)
-        if positions is not None:
-            positions = (positions.expand(lead).contiguous() if isinstance(positions, torch.Tensor) else
-                         np.ascontiguousarray(np.broadcast_to(positions, lead)))
-        n0, n1 = 1, prod(shape[:-2])
-        xs = ys = (0, rows * dim, dim)
-        ps = (0, rows, 1)
-    if 0 in shape:
+        n0, n1, ((x0, x1, x_row), (y0, y1, y_row), (p0, p1, p_row)) = views
+        if out.numel():
+            device = x.get_device()
+            call("rotary", code, kind, x.data_ptr(), frequencies.data_ptr(), positions.data_ptr() if kind else None, out.data_ptr(),
+                 n0, n1, rows, dim, 2 * frequencies.shape[0], x0, x1, x_row, y0, y1, y_row, p0, p1, p_row, interleaved, inverse, scale,
+                 device, raw_stream(device), 0)
         return out
-    call("rotary", code, kind, pointer(x), pointer(frequencies), pointer(positions), pointer(out), n0, n1, rows, dim,
-         2 * frequencies.shape[0], *xs, *ys, *ps, interleaved, inverse, scale, *place_of(x), 0)
+    x = contiguous(x)
+    out = empty(x, shape, x.dtype)
+    if positions is not None:
+        positions = (positions.expand(lead).contiguous() if isinstance(positions, torch.Tensor) else
+                     np.ascontiguousarray(np.broadcast_to(positions, lead)))
+    if 0 not in shape:
+        call("rotary", code, kind, pointer(x), pointer(frequencies), pointer(positions), pointer(out), 1, prod(shape[:-2]), rows,
+             dim, 2 * frequencies.shape[0], 0, rows * dim, dim, 0, rows * dim, dim, 0, rows, 1, interleaved, inverse, scale, -1,
+             None, 0)
     return out
 
 

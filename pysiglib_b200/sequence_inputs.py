@@ -14,7 +14,8 @@ TORCH_TYPES = {torch.float32: 0, torch.float64: 1, torch.bfloat16: 2, torch.floa
 NUMPY_TYPES = {np.dtype(np.float32): 0, np.dtype(np.float64): 1, np.dtype(np.float16): 3}
 
 # handle of a device's current stream, without building a torch.cuda.Stream around it
-_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def element_type(array, name):
@@ -84,11 +85,10 @@ def batched_rows(array):
     """``(array, batch stride, row stride)`` of (..., L, C) with the batch axes read as one: in place where
     the strides allow it, else a contiguous copy."""
     shape = array.shape
-    width, rows = shape[-1], shape[-2]
-    if on_device(array):
+    rank, width, rows = len(shape), shape[-1], shape[-2]
+    if isinstance(array, torch.Tensor) and array.is_cuda:
         strides = array.stride()
         if strides[-1] == 1 or width == 1:
-            rank = len(shape)
             if rank == 2:
                 return array, 0, strides[0]
             if rank == 3:
@@ -108,13 +108,22 @@ def place_of(array):
     if not on_device(array):
         return -1, None
     device = array.get_device()
-    if _current_raw_stream is not None:
-        return device, _current_raw_stream(device)
-    return device, torch.cuda.current_stream(device).cuda_stream
+    return device, raw_stream(device)
+
+
+_natives = {}
+
+
+def native(name):
+    """The native function sigb200_<name>, looked up once."""
+    f = _natives.get(name)
+    if f is None:
+        f = _natives[name] = getattr(load_cusig.library(), "sigb200_" + name)
+    return f
 
 
 def call(name, *args):
     """One native call; raises what the package's other operators raise."""
-    code = getattr(load_cusig.library(), "sigb200_" + name)(*args)
+    code = native(name)(*args)
     if code:
         raise Exception("Error in pysiglib.%s: %s" % (name, err_msg(code)))
