@@ -624,10 +624,9 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
     const int stages = plan.stages, warps = plan.warps;
     const int64_t dim = int64_t(p.dim);
     const int first = at.segment * plan.segment_rows, rows = min(int(p.rows), first + plan.segment_rows);
-    const A* initial = p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr;
-    A* state = p.state ? static_cast<A*>(p.state) + c0 : nullptr;
-    A* marks = p.checkpoints
-        ? static_cast<A*>(p.checkpoints) + b * ((p.rows + kCheckpointRows - 1) / kCheckpointRows) * p.dim + c0 : nullptr;
+    // made where they are needed, rather than held in registers all along
+    const auto initial = [&] { return p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr; };
+    const auto state = [&] { return static_cast<A*>(p.state) + c0; };
 
     Prefetch<X, V, S, false> fx;
     Prefetch<G, GV, S, SHARED> fg;
@@ -650,8 +649,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
     int coming = row0;  // the row that the next copies are for
     const auto fetch = [&](int stage) {
         const int n = rows_left<S>(rows, coming, live);
-        fx.issue(stage, x, px, x_row, n);
-        fg.issue(stage, gate, pg, gate_row, n);
+        fx.issue(stage, static_cast<const X*>(p.x), px, x_row, n);
+        fg.issue(stage, static_cast<const G*>(p.gate), pg, gate_row, n);
         commit_copies();
         px += x_span;
         pg += gate_span;
@@ -666,7 +665,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
     hold(row0);
     A in[V];  // the state that enters the warp's rows
 #pragma unroll
-    for (int v = 0; v < V; ++v) in[v] = !PACKED && initial && live ? initial[b * p.dim + v] : A(0);
+    for (int v = 0; v < V; ++v) in[v] = !PACKED && p.initial && live ? initial()[b * p.dim + v] : A(0);
     if (plan.segments > 1) {
         A* fold = reinterpret_cast<A*>(next + offset_room(p));
         through_segments<A, false, PACKED>(plan, b, at.segment, p.dim, c0 - uint64_t(at.tc) * V, width,
@@ -678,10 +677,10 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
     if (PACKED) {
         walk.open(p, reinterpret_cast<int*>(next));
         walk.seek(row0);
-        if (state && live && at.segment == 0)  // sequences without rows hand their initial state on
+        if (p.state && live && at.segment == 0)  // sequences without rows hand their initial state on
             for (int j = at.part; j < walk.count; j += warps * at.parts)
                 if (offset_at(walk.offsets, walk.wide, j + 1) <= offset_at(walk.offsets, walk.wide, j))
-                    for (int v = 0; v < V; ++v) state[j * dim + v] = initial ? initial[j * dim + v] : A(0);
+                    for (int v = 0; v < V; ++v) state()[j * dim + v] = p.initial ? initial()[j * dim + v] : A(0);
     }
     const int link = 1 + at.warp, link_before = at.warp ? at.warp : warps;
     A* leaving = carry + (at.warp + 1 == warps ? 0 : at.warp + 1) * width;
@@ -699,7 +698,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
         if (p.complement) factors<true>(p.form, fx, fg, stage, r.a, r.u);
         else factors<false>(p.form, fx, fg, stage, r.a, r.u);
         hold(row0 + span);
-        settle_rows<false>(r, walk, row0, initial, dim, live);
+        settle_rows<false>(r, walk, row0, initial(), dim, live);
         Map<A, V> m;
         m.clear();
         append_rows<false, PACKED>(m, r);
@@ -716,11 +715,12 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
         enter_rows<A, V, false>(m, plan.log_lanes, in, h, leaving,
                                 [&] { if (warps > 1 && (at.warp + 1 < warps || base + span < rows)) give(link); });
         if (r.count) {
-            if (marks && row0 % int(kCheckpointRows) == 0) {
+            if (p.checkpoints && row0 % int(kCheckpointRows) == 0) {
                 Pack<A, V> mark;
 #pragma unroll
                 for (int v = 0; v < V; ++v) mark.v[v] = h[v];
-                store_pack<A, V>(marks + int64_t(row0 / int(kCheckpointRows)) * dim, mark);
+                const int64_t n = b * ((p.rows + kCheckpointRows - 1) / kCheckpointRows) + row0 / int(kCheckpointRows);
+                store_pack<A, V>(static_cast<A*>(p.checkpoints) + n * dim + c0, mark);
             }
             const int stored = out ? r.count : 0;
             X* to = out;
@@ -748,8 +748,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
                         y[v] = r.e.dead >> s & 1u ? A(0) : h[v];
                     }
                     if (s < stored) store_pack<X, V>(to, narrow_pack<X, V>(y));
-                    if (state && (r.e.ends >> s & 1u)) {
-                        A* last = state + sequence_of(walk, row0 + s) * dim;
+                    if (p.state && (r.e.ends >> s & 1u)) {
+                        A* last = state() + sequence_of(walk, row0 + s) * dim;
 #pragma unroll
                         for (int v = 0; v < V; ++v) last[v] = h[v];
                     }
@@ -759,9 +759,9 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
         if (out) out += out_span;
     }
     // what left the last warp's last part
-    if (!PACKED && state && live && at.segment + 1 == plan.segments && at.warp + 1 == warps && at.lane >= 32 - at.lanes)
+    if (!PACKED && p.state && live && at.segment + 1 == plan.segments && at.warp + 1 == warps && at.lane >= 32 - at.lanes)
 #pragma unroll
-        for (int v = 0; v < V; ++v) state[b * p.dim + v] = leaving[v];
+        for (int v = 0; v < V; ++v) state()[b * p.dim + v] = leaving[v];
 }
 
 // Sums S values each over 1 << log >= S neighbouring lanes.  Each of the first rounds halves the values a lane still
@@ -905,9 +905,10 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
     const int stages = plan.stages, warps = plan.warps;
     const int64_t dim = int64_t(p.dim);
     const int first = at.segment * plan.segment_rows, rows = min(int(p.rows), first + plan.segment_rows);
-    const A* initial = p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr;
-    const A* state_derivs = p.state_derivs ? static_cast<const A*>(p.state_derivs) + c0 : nullptr;
-    A* dinitial = p.dinitial ? static_cast<A*>(p.dinitial) + c0 : nullptr;
+    // made where they are needed, rather than held in registers all along
+    const auto initial = [&] { return p.initial ? static_cast<const A*>(p.initial) + c0 : nullptr; };
+    const auto state_derivs = [&] { return p.state_derivs ? static_cast<const A*>(p.state_derivs) + c0 : nullptr; };
+    const auto dinitial = [&] { return static_cast<A*>(p.dinitial) + c0; };
 
     Prefetch<X, V, S, false> fx, fd;
     Prefetch<G, GV, S, SHARED> fg;
@@ -943,9 +944,9 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
     int coming = row0, coming_base = base;
     const auto fetch = [&](int stage) {
         const int n = coming_base >= first ? rows_left<S>(rows, coming, live) : 0;
-        fx.issue(stage, x, px, x_row, n);
-        fg.issue(stage, gate, pg, gate_row, n);
-        fd.issue(stage, derivs, pd, d_row, n);
+        fx.issue(stage, static_cast<const X*>(p.x), px, x_row, n);
+        fg.issue(stage, static_cast<const G*>(p.gate), pg, gate_row, n);
+        fd.issue(stage, static_cast<const X*>(p.derivs), pd, d_row, n);
         const int own = coming_base + at.warp * warp_rows;  // the warp's first row
         if (marked && live && at.lane < at.lanes && coming_base >= first && own < rows)
             copy_async<sizeof(A) * V>(entering + stage * warps * width, marks + int64_t(own / int(kCheckpointRows)) * dim);
@@ -966,7 +967,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
     hold(row0, true);
     A w[V];  // the gradient that enters the warp's rows from behind
 #pragma unroll
-    for (int v = 0; v < V; ++v) w[v] = !PACKED && state_derivs && live ? state_derivs[b * p.dim + v] : A(0);
+    for (int v = 0; v < V; ++v) w[v] = !PACKED && p.state_derivs && live ? state_derivs()[b * p.dim + v] : A(0);
     if (plan.segments > 1) {
         A* fold = reinterpret_cast<A*>(next + offset_room(p));
         through_segments<A, true, PACKED>(plan, b, at.segment, p.dim, c0 - uint64_t(at.tc) * V, width,
@@ -978,10 +979,10 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
     if (PACKED) {
         walk.open(p, reinterpret_cast<int*>(next));
         walk.seek(row0);
-        if (dinitial && live && at.segment == 0)
+        if (p.dinitial && live && at.segment == 0)
             for (int j = at.part; j < walk.count; j += warps * at.parts)
                 if (offset_at(walk.offsets, walk.wide, j + 1) <= offset_at(walk.offsets, walk.wide, j))
-                    for (int v = 0; v < V; ++v) dinitial[j * dim + v] = state_derivs ? state_derivs[j * dim + v] : A(0);
+                    for (int v = 0; v < V; ++v) dinitial()[j * dim + v] = p.state_derivs ? state_derivs()[j * dim + v] : A(0);
     }
     // hand-overs: 1 .. W of the gradient to the warp before (or from the first to the last), W + 1 .. of the state
     const int link = 1 + at.warp, link_behind = at.warp + 1 == warps ? 1 : 2 + at.warp;
@@ -997,7 +998,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
             r.e = row_events<S>(walk, row0, rows);
         }
         const auto first_state = [&](int s, A (&h)[V]) {
-            const A* from = initial && live ? initial + sequence_of(walk, row0 + s) * dim : nullptr;
+            const A* from = p.initial && live ? initial() + sequence_of(walk, row0 + s) * dim : nullptr;
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = from ? from[v] : A(0);
         };
@@ -1009,7 +1010,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
         if (quiet) walk_up<COMPLEMENT, true>(p.form, fx, fd, fg, stage, r, m, kept, first_state);
         else walk_up<COMPLEMENT, false>(p.form, fx, fd, fg, stage, r, m, kept, first_state);
         hold(row0 - span, base > first);
-        if (PACKED && r.e.ends && state_derivs && live) settle_rows<true>(r, walk, row0, state_derivs, dim, live);
+        if (PACKED && r.e.ends && p.state_derivs && live) settle_rows<true>(r, walk, row0, state_derivs(), dim, live);
         g.clear();
         append_rows<true, PACKED>(g, r);
 #pragma unroll
@@ -1043,8 +1044,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
         for (int s = S - 1; s >= 0; --s) {
             if (!(PACKED && (r.e.ends >> s & 1u))) v_add(r.u[s], r.u[s], behind);
             v_mul(behind, r.a[s], r.u[s]);
-            if (PACKED && dinitial && live && (r.e.starts >> s & 1u)) {
-                A* to = dinitial + sequence_of(walk, row0 + s) * dim;
+            if (PACKED && p.dinitial && live && (r.e.starts >> s & 1u)) {
+                A* to = dinitial() + sequence_of(walk, row0 + s) * dim;
 #pragma unroll
                 for (int v = 0; v < V; ++v) to[v] = behind[v];
             }
@@ -1090,9 +1091,9 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
         }
     }
     // what left the first warp's first part
-    if (!PACKED && dinitial && live && at.segment == 0 && at.warp == 0 && at.lane < at.lanes)
+    if (!PACKED && p.dinitial && live && at.segment == 0 && at.warp == 0 && at.lane < at.lanes)
 #pragma unroll
-        for (int v = 0; v < V; ++v) dinitial[b * p.dim + v] = leaving[v];
+        for (int v = 0; v < V; ++v) dinitial()[b * p.dim + v] = leaving[v];
 }
 
 // Map of every segment of the rows: of the recurrence (x, initial states), or REVERSE of the gradient (derivatives in
