@@ -36,8 +36,9 @@ bool aligned_to(const RecurrenceArgs& p, size_t bytes) {
 }
 
 // Up to 8 warps whose lanes lie side by side in the channels as far as 128 bytes of a row go (full lines), and
-// behind one another in the rows beyond that.  Two CTAs an SM are there at a time.  Where full lines make fewer
-// strips than there are SMs, half lines do if that is enough; else the rows are cut into segments.
+// behind one another in the rows beyond that; an SM holds two such CTAs.  Where full lines make fewer strips
+// than there are SMs, half lines do if that is enough; else the rows are cut into segments, as many as fill the
+// SMs (float32 1x65536x192, forward: 50 segments 52 us; 8 CTAs of a cluster to each strip took 71 us, one CTA 246 us).
 template <typename X>
 RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     constexpr uint64_t kResident = 16;  // warps an SM holds at 128 registers a thread
@@ -118,7 +119,7 @@ size_t maps_bytes(const RecurrenceArgs& p, const RecurrencePlan& plan) {
 
 template <typename X, typename G, int V, bool SHARED, bool REVERSE>
 void reduce_segments(const RecurrenceArgs& p, RecurrencePlan plan, cudaStream_t stream) {
-        constexpr int S = V == 1 ? 8 : 4;  // divides the rows of a thread: a block's are a multiple of it
+    constexpr int S = V == 1 ? 8 : 4;  // divides the rows of a thread: a block's are a multiple of it
     const size_t smem = shared_memory(plan, Prefetch<X, V, S, false>::kWarp + Prefetch<G, SHARED ? 1 : V, S, SHARED>::kWarp,
                                       plan.warps * (2 * sizeof(Acc<X>) * (V << plan.log_lanes) + sizeof(int)) + 16 + offset_room(p));
     if (p.sequences) launch<recurrence_maps_kernel<X, G, V, S, SHARED, true, REVERSE>>(p, plan, smem, stream);

@@ -131,10 +131,6 @@ __device__ __forceinline__ int64_t sequence_of(SequenceWalk walk, int row) {
     return walk.seq;
 }
 
-// a and 1 - a, neither by cancellation; for logits, with e = e^-v kept finite,
-// a = 1 / (1 + e) and 1 - a = e a.  The reciprocal is the hardware's (within 1 ulp).
-// FAST (gates of 16 bits): exponentials as 2^(v log2 e) in single precision, off by up to 2 + 1.2 |v| ulp.  A gate
-// of 8 or 11 bits leaves e^v uncertain by |v| 2^-9 or 2^-12 of itself, thousands of times more.
 __device__ __forceinline__ float exponential(float v) { return expf(v); }
 __device__ __forceinline__ double exponential(double v) { return exp(v); }
 // a = e^v and 1 - a together: v = n ln 2 + f with |f| <= ln 2 / 2 (ln 2 in two parts), p = e^f - 1 by its Taylor
@@ -236,7 +232,10 @@ __device__ __forceinline__ void v_fill(A (&r)[V], A value) {
     for (int v = 0; v < V; ++v) r[v] = value;
 }
 
-// a, and where PAIR 1 - a, of V gate values.
+// a, and where PAIR 1 - a, of V gate values, neither by cancellation; for logits, with e = e^-v kept finite,
+// a = 1 / (1 + e) and 1 - a = e a.  The reciprocal is the hardware's (within 1 ulp).
+// FAST (gates of 16 bits): exponentials as 2^(v log2 e) in single precision, off by up to 2 + 1.2 |v| ulp.  A gate
+// of 8 or 11 bits leaves e^v uncertain by |v| 2^-9 or 2^-12 of itself, thousands of times more.
 template <int FORM, bool FAST, bool PAIR, typename A, int V>
 __device__ __forceinline__ void gate_factors(const A (&g)[V], A (&a)[V], A (&rest)[V]) {
     if constexpr (FORM == kGateValue) {
@@ -381,10 +380,6 @@ struct Map {
 #pragma unroll
         for (int v = 0; v < V; ++v) { a[v] = A(1); b[v] = A(0); }
         drop = false;
-    }
-    __device__ __forceinline__ void apply(A (&h)[V]) const {
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = drop ? b[v] : fma_(a[v], h[v], b[v]);
     }
 };
 
