@@ -119,7 +119,10 @@ size_t maps_bytes(const RecurrenceArgs& p, const RecurrencePlan& plan) {
 
 template <typename X, typename G, int V, bool SHARED, bool REVERSE>
 void reduce_segments(const RecurrenceArgs& p, RecurrencePlan plan, cudaStream_t stream) {
-    constexpr int S = V == 1 ? 8 : 4;  // divides the rows of a thread: a block's are a multiple of it
+#ifndef MAPS_16
+#define MAPS_16 8
+#endif
+    constexpr int S = V == 1 ? 8 : sizeof(X) == 2 ? MAPS_16 : 4;
     const size_t smem = shared_memory(plan, Prefetch<X, V, S, false>::kWarp + Prefetch<G, SHARED ? 1 : V, S, SHARED>::kWarp,
                                       plan.warps * (2 * sizeof(Acc<X>) * (V << plan.log_lanes) + sizeof(int)) + 16 + offset_room(p));
     if (p.sequences) launch<recurrence_maps_kernel<X, G, V, S, SHARED, true, REVERSE>>(p, plan, smem, stream);

@@ -1104,8 +1104,6 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_maps_kernel(const R
     const bool live = at.live;
     const int stages = plan.stages, warps = plan.warps;
     const int64_t dim = int64_t(p.dim);
-    const int run = plan.segment_rows / (warps * at.parts);  // rows of a thread
-    const int begin = at.segment * plan.segment_rows + at.part * run, end = min(int(p.rows), begin + run);
     const A* joins = static_cast<const A*>(REVERSE ? p.state_derivs : p.initial);
     if (joins) joins += c0;
     const int64_t x_row = int64_t(REVERSE ? p.d_row : p.x_row), gate_row = int64_t(p.gate_row);
@@ -1122,11 +1120,19 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_maps_kernel(const R
     next += sizeof(A) * 2 * width * warps;
     int* drops = reinterpret_cast<int*>(next);  // [warp]
     next += sizeof(int) * warps;
+    int first = at.segment * plan.segment_rows, rows = min(int(p.rows), first + plan.segment_rows);
     SequenceWalk walk;
-    if (PACKED) {
+    if (PACKED) {  // nothing leaves the segment from before its last sequence (from behind its first)
         walk.open(p, reinterpret_cast<int*>(next));
-        walk.seek(REVERSE ? begin + run : begin);
+        walk.seek(REVERSE ? first : rows - 1);
+        if (walk.inside()) {
+            if (REVERSE) rows = min(rows, walk.next);
+            else first = max(first, walk.begin);
+        }
     }
+    const int round = warps * at.parts * S, run = (rows - first + round - 1) / round * S;  // rows of a thread
+    const int begin = first + at.part * run, end = min(rows, begin + run);
+    if (PACKED) walk.seek(REVERSE ? begin + run : begin);
     int coming = REVERSE ? begin + run - S : begin;
     const auto fetch = [&](int stage) {
         const int n = coming >= begin ? rows_left<S>(end, coming, live) : 0;
