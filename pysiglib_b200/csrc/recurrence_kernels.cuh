@@ -1035,14 +1035,22 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
         A behind[V];
         enter_rows<A, V, true>(g, plan.log_lanes, w, behind, leaving, [&] { if (warps > 1 && (at.warp || base > first)) give(link); });
         // backward through the rows: the derivatives become g
+        if (PACKED && !quiet) {
 #pragma unroll
-        for (int s = S - 1; s >= 0; --s) {
-            if (!(PACKED && (r.e.ends >> s & 1u))) v_add(r.u[s], r.u[s], behind);
-            v_mul(behind, r.a[s], r.u[s]);
-            if (PACKED && p.dinitial && live && (r.e.starts >> s & 1u)) {
-                A* to = dinitial() + sequence_of(walk, row0 + s) * dim;
+            for (int s = S - 1; s >= 0; --s) {
+                if (!(r.e.ends >> s & 1u)) v_add(r.u[s], r.u[s], behind);
+                v_mul(behind, r.a[s], r.u[s]);
+                if (p.dinitial && live && (r.e.starts >> s & 1u)) {
+                    A* to = dinitial() + sequence_of(walk, row0 + s) * dim;
 #pragma unroll
-                for (int v = 0; v < V; ++v) to[v] = behind[v];
+                    for (int v = 0; v < V; ++v) to[v] = behind[v];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int s = S - 1; s >= 0; --s) {
+                v_add(r.u[s], r.u[s], behind);
+                v_mul(behind, r.a[s], r.u[s]);
             }
         }
         A sums[SHARED ? S : 1];
