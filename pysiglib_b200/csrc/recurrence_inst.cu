@@ -106,9 +106,19 @@ void launch(const RecurrenceArgs& p, const RecurrencePlan& plan, size_t smem, cu
             if (current_device() < 64) raised.fetch_or(bit, std::memory_order_release);
         }
     }
-    const unsigned grid = static_cast<unsigned>(p.batch) * plan.strips * unsigned(plan.segments);
-    Kernel<<<grid, 32 * plan.warps, smem, stream>>>(p, plan, args...);
-    check("linear recurrence kernel");
+    cudaLaunchAttribute overlap{};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(p.batch) * plan.strips * unsigned(plan.segments));
+    config.blockDim = dim3(32 * plan.warps);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    config.attrs = &overlap;
+    config.numAttrs = plan.follows ? 1 : 0;
+    count_launch();
+    const cudaError_t err = cudaLaunchKernelEx(&config, Kernel, p, plan, args...);
+    if (err != cudaSuccess) throw CudaFailure(err, std::string("linear recurrence kernel: ") + cudaGetErrorString(err));
 }
 
 // Scratch for the segments' maps and, behind them, their drops.
@@ -119,10 +129,7 @@ size_t maps_bytes(const RecurrenceArgs& p, const RecurrencePlan& plan) {
 
 template <typename X, typename G, int V, bool SHARED, bool REVERSE>
 void reduce_segments(const RecurrenceArgs& p, RecurrencePlan plan, cudaStream_t stream) {
-#ifndef MAPS_16
-#define MAPS_16 8
-#endif
-    constexpr int S = V == 1 ? 8 : sizeof(X) == 2 ? MAPS_16 : 4;
+    constexpr int S = V == 1 || sizeof(X) == 2 ? 8 : 4;  // float32 as in the main kernels; 4 for 16 bits: packed 16000x1536 56 -> 62 us
     const size_t smem = shared_memory(plan, Prefetch<X, V, S, false>::kWarp + Prefetch<G, SHARED ? 1 : V, S, SHARED>::kWarp,
                                       plan.warps * (2 * sizeof(Acc<X>) * (V << plan.log_lanes) + sizeof(int)) + 16 + offset_room(p));
     if (p.sequences) launch<recurrence_maps_kernel<X, G, V, S, SHARED, true, REVERSE>>(p, plan, smem, stream);
@@ -143,6 +150,7 @@ void forward(const RecurrenceArgs& p, cudaStream_t stream) {
     if (plan.segments > 1) {
         place_maps<Acc<X>>(p, plan, maps.get());
         reduce_segments<X, G, V, SHARED, false>(p, plan, stream);
+        plan.follows = true;
     }
     const int width = V << plan.log_lanes;
     const size_t smem = shared_memory(plan, Prefetch<X, V, S, false>::kWarp + Prefetch<G, SHARED ? 1 : V, S, SHARED>::kWarp,
@@ -159,6 +167,7 @@ void backward(const RecurrenceArgs& p, cudaStream_t stream) {
     if (plan.segments > 1) {
         place_maps<Acc<X>>(p, plan, maps.get());
         reduce_segments<X, G, V, SHARED, true>(p, plan, stream);
+        plan.follows = true;
     }
     Acc<X>* partial = nullptr;
     uint64_t per_gate = 0;

@@ -44,6 +44,7 @@ struct RecurrencePlan {
     int fold_log;      // backward, shared gates: lanes folded into one partial sum, log2
     void* maps;        // [batch][segment][A, B][dim] of the segments, and
     int* drops;        // [batch][segment]
+    bool follows;      // the launch right behind the one of those maps: it may begin before they are there
 };
 
 namespace {
@@ -662,6 +663,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
 #pragma unroll
     for (int v = 0; v < V; ++v) in[v] = !PACKED && p.initial && live ? initial()[b * p.dim + v] : A(0);
     if (plan.segments > 1) {
+        cudaGridDependencySynchronize();  // the maps; what is above runs beside the kernel that makes them
         A* fold = reinterpret_cast<A*>(next + offset_room(p));
         through_segments<A, false, PACKED>(plan, b, at.segment, p.dim, c0 - uint64_t(at.tc) * V, width,
                                            PACKED || !p.initial ? nullptr : static_cast<const A*>(p.initial) + b * p.dim, fold);
@@ -964,6 +966,7 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
 #pragma unroll
     for (int v = 0; v < V; ++v) w[v] = !PACKED && p.state_derivs && live ? state_derivs()[b * p.dim + v] : A(0);
     if (plan.segments > 1) {
+        cudaGridDependencySynchronize();  // the maps; what is above runs beside the kernel that makes them
         A* fold = reinterpret_cast<A*>(next + offset_room(p));
         through_segments<A, true, PACKED>(plan, b, at.segment, p.dim, c0 - uint64_t(at.tc) * V, width,
                                           PACKED || !p.state_derivs ? nullptr : static_cast<const A*>(p.state_derivs) + b * p.dim, fold);
@@ -1106,6 +1109,7 @@ template <typename X, typename G, int V, int S, bool SHARED, bool PACKED, bool R
 __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_maps_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
     using A = Acc<X>;
     constexpr int GV = SHARED ? 1 : V;
+    cudaTriggerProgrammaticLaunchCompletion();  // the main kernel's CTAs may come as these leave
     extern __shared__ __align__(16) unsigned char smem[];
     const Place at(plan, p.dim, V);
     const uint64_t b = at.batch, c0 = at.c0;
