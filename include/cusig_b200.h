@@ -270,7 +270,8 @@ uint64_t sigb200_noalloc_scratch_bytes(void);
  * gate (batch, length, gates) then serves dimension / gates neighbouring channels each.  gate_type is
  * `type`, or 0 for 16-bit types.  Written: out (batch, length, dimension), contiguous; state (batch,
  * dimension), the last h, optional; checkpoints (batch, ceil(length / 16), dimension), the states that
- * enter rows 0, 16, .., optional, for the backward pass.  length and sequences are below 2^30.
+ * enter rows 0, 16, .., optional, for the backward pass.  length and sequences are below 2^30.  A batch or
+ * a length of 0 writes nothing.
  * sequences > 0: packed sequences, batch 1; sequence i holds rows offsets[i] to offsets[i + 1] - 1
  * (sequences + 1 non-decreasing values within 0 .. length; int64 with wide_offsets, else int32), initial
  * and state are (sequences, dimension); rows of no sequence come out as 0.  Offsets in device

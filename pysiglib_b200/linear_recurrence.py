@@ -250,6 +250,7 @@ def linear_recurrence_step(
             device = x.get_device()
             call("linear_recurrence_step", code, gate_code, x.data_ptr(), gate.data_ptr(), state.data_ptr(), out.data_ptr(),
                  out.numel() // dim, dim, gates, dim, gates, form, complement, device, raw_stream(device), 0)
+            torch.autograd.graph.increment_version(state)  # a graph that has kept it must not go on with it
         return out
     x, gate = contiguous(x), contiguous(gate)
     out = empty(x, shape, x.dtype)
@@ -257,4 +258,6 @@ def linear_recurrence_step(
     if batch:
         call("linear_recurrence_step", code, gate_code, pointer(x), pointer(gate), pointer(state), pointer(out), batch,
              dim, gates, dim, gates, form, complement, *place_of(x), 0)
+        if torch_state:
+            torch.autograd.graph.increment_version(state)
     return out

@@ -268,7 +268,7 @@ def linear_recurrence(x, gate, initial=None, *, gate_form: str = "value", comple
                                          return_state=return_state, return_checkpoints=return_checkpoints)
     check_type(return_state, "return_state", bool)
     if isinstance(offsets, np.ndarray):
-        offsets = torch.from_numpy(offsets)
+        offsets = torch.from_numpy(offsets.copy())  # kept for the backward pass
     h, state = LinearRecurrence.apply(x, gate, initial, gate_form, complement, offsets)
     return (h, state) if return_state else h
 

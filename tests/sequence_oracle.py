@@ -2,8 +2,8 @@
 correct implementation can add up to.
 
 Unit roundoff of the arithmetic: u = eps / 2 of the state type.  One row of the recurrence costs at most ROUNDINGS
-of them relative to |a| |h| + |b|: the gate factor (exp and a quotient of CUDA's library within 4 units, expm1
-within 2, their product with x 1), the product of a run's factors 1 and the multiply-add 1.  Errors already
+of them relative to |a| |h| + |b|: the gate factor (an exponential and a quotient, by CUDA's library or a Taylor series,
+within 4 units, 1 - a within 2, its product with x 1), the product of a run's factors 1 and the multiply-add 1.  Errors already
 made are handed on through |a|.  For gates of 16 bits e^v is taken by CUDA's __expf, whose documented error is
 2 + floor(1.173 |v|) ulp (2 units each) where exp's is within the 4 units above: 2.4 |v| units more.  The
 bounds below are that recursion, written out."""

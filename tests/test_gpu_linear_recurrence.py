@@ -420,3 +420,33 @@ def test_offsets_that_are_out_of_order_stay_in_bounds():
     assert (whole == 7.0).all()
     expect = so.recurrence(x.cpu()[None], gate.cpu()[None], None, "value", False)["h"]
     so.check(psl.linear_recurrence(x, gate), tuple(t[0] for t in expect), "h")
+
+
+def test_what_a_graph_has_kept_is_not_overwritten_unseen():
+    x, gate, start, derivs, _, _ = make(60, 1, 40, 8, 8, F32, F32, "logit", True)
+    X = cuda(x[0]).requires_grad_()
+    G, S = cuda(gate[0])[None], cuda(start)
+    h = torch_api.linear_recurrence(X[None], G, S, gate_form="logit")
+    psl.linear_recurrence_step(X[:1].detach(), G[0, :1], S, gate_form="logit")
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+    # offsets on the host are the caller's again after the call
+    offsets = np.array([0, 15, 40])
+    h = torch_api.linear_recurrence(X, G[0], gate_form="logit", offsets=offsets)
+    offsets[1] = 3
+    (got,) = torch.autograd.grad(h, X, cuda(derivs[0]))
+    expect = psl.linear_recurrence_backprop(cuda(derivs[0]), X.detach(), G[0], gate_form="logit", offsets=np.array([0, 15, 40]))[0]
+    assert torch.equal(got, expect)
+
+
+@pytest.mark.parametrize("lengths", [(900, 3, 0, 0, 1100, 997), (1, 2998, 1), (0, 3000, 0), (7,) * 400, (100, 2000)])
+def test_segments_of_packed_rows_that_begin_and_end_in_sequences(lengths):
+    """Sequence bounds before, in, at and behind the cuts between segments; rows before the first and behind the last."""
+    rows = 3000
+    x, gate, _, derivs, _, _ = make(61, 1, rows, 24, 24, F32, F32, "log", False)
+    x, gate, derivs = x[0], gate[0], derivs[0]
+    bounds = np.cumsum([0, *lengths])
+    bounds = bounds + min(5, rows - bounds[-1])
+    rng = np.random.default_rng(62)
+    start, tail = (torch.from_numpy(rng.standard_normal((len(lengths), 24)).astype(np.float32)) for _ in range(2))
+    run_and_check((x, gate, start, derivs, tail, torch.from_numpy(bounds)), "log", True)
