@@ -38,7 +38,7 @@ bool aligned_to(const RecurrenceArgs& p, size_t bytes) {
 // Up to 8 warps whose lanes lie side by side in the channels as far as 128 bytes of a row go (full lines), and
 // behind one another in the rows beyond that; an SM holds two such CTAs.  Where full lines make fewer strips
 // than there are SMs, half lines do if that is enough; else the rows are cut into segments, as many as fill the
-// SMs (float32 1x65536x192, forward: 50 segments 52 us; 8 CTAs of a cluster to each strip took 71 us, one CTA 246 us).
+// SMs (float32 1x65536x192, forward: 47 segments 48 us; 8 CTAs of a cluster to each strip took 71 us, one CTA 246 us).
 template <typename X>
 RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     constexpr uint64_t kResident = 16;  // warps an SM holds at 128 registers a thread

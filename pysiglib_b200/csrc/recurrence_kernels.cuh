@@ -609,6 +609,10 @@ __device__ __forceinline__ void append_rows(Map<A, V>& m, const Rows<A, V, S>& r
     }
 }
 
+// Measured (B200, event times; the bytes alone would take what stands behind the bar): bfloat16 8x4096x2048 76 us | 61,
+// 8x8192x4096 277 | 245, float32 64x512x272 23 | 16: about 21 instructions a value at 59 % of the issue slots.  In
+// segments, with the kernel of their maps: float32 1x65536x192 48 us | 23, bfloat16 16000x1536 in 23 sequences
+// 52 | 15; there 16 warps an SM, all that 128 registers a thread admit, wait for one another.
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED>
 __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
     using A = Acc<X>;
@@ -890,6 +894,8 @@ __device__ __forceinline__ void walk_out(int form, const Prefetch<X, V, S, false
 // the ring of warps, from the last to the first.
 // Shared gates: each thread sums its V channels, 1 << fold_log neighbouring lanes are folded by shuffles,
 // and `partial` takes one value per row and fold (dgate itself where a fold is a whole gate).
+// Measured (as above): bfloat16 8x4096x2048 151 us | 102, float32 64x512x272 38 | 27: about 42 instructions a value
+// at 55 % of the issue slots; in segments float32 1x65536x192 64 us | 38, bfloat16 16000x1536 89 | 23.
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED, bool COMPLEMENT>
 __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(const RecurrenceArgs p, const RecurrencePlan plan,
                                                                      Acc<X>* partial) {
@@ -1105,6 +1111,9 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
 // Map of every segment of the rows: of the recurrence (x, initial states), or REVERSE of the gradient (derivatives in
 // the place of x, gradients of states).  Each thread takes a contiguous run of rows, S at a time, and
 // appends them to its map; parts and warps are composed once, at the end.
+// Of packed sequences only the last (REVERSE: the first) one in a segment decides what leaves it: the rows before
+// (behind) it are not read.  Measured: float32 1x65536x192, 101 MB in 21 us, 62 % of the HBM's rate; bfloat16
+// 16000x1536 in 23 sequences 17 us instead of 24.
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED, bool REVERSE>
 __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_maps_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
     using A = Acc<X>;
@@ -1221,6 +1230,7 @@ __global__ void fold_partials_kernel(const A* __restrict__ partial, G* __restric
 
 // One row for each state: state = a state + b, out = the new state rounded.  Two reads, one read and write
 // of the state and one write; a grid over all values, since nothing is shared between them.
+// A launch is what it costs: float32 16x512 takes 6 us between two events, as an empty kernel would.
 template <typename X, typename G, int V, bool SHARED>
 __global__ void __launch_bounds__(256) recurrence_step_kernel(const RecurrenceArgs p) {
     using A = Acc<X>;
