@@ -1230,7 +1230,7 @@ __global__ void fold_partials_kernel(const A* __restrict__ partial, G* __restric
 
 // One row for each state: state = a state + b, out = the new state rounded.  Two reads, one read and write
 // of the state and one write; a grid over all values, since nothing is shared between them.
-// A launch is what it costs: float32 16x512 takes 6 us between two events, as an empty kernel would.
+// The launch is most of it: float32 16x512 takes 6 us between two events, its 164 KB would take 0.03 us.
 template <typename X, typename G, int V, bool SHARED>
 __global__ void __launch_bounds__(256) recurrence_step_kernel(const RecurrenceArgs p) {
     using A = Acc<X>;
