@@ -12,8 +12,10 @@ namespace {
 // Channels a thread holds: 16 bytes of float32 or float64, 8 of the 16-bit types (whose gates and states
 // widen to the same registers).
 template <typename X> constexpr int kWide = sizeof(X) == 8 ? 2 : 4;
-// Rows a thread holds: as many as leave the arrays of S * V values in registers and two CTAs an SM their stages.
-template <typename X, int V> constexpr int kBackwardRows = V > 1 && sizeof(X) > 2 ? 4 : 8;
+// Rows a thread holds: as many as leave the arrays of S * V values in registers and two CTAs an SM their stages
+// (float16 with float32 gates, packed 8000x1536 backward: 4 rows 74 us, 8 rows 107 us).
+template <typename X, typename G, int V, bool SHARED>
+constexpr int kBackwardRows = V > 1 && (sizeof(X) > 2 || (!SHARED && sizeof(G) > 2)) ? 4 : 8;
 template <typename X, int V> constexpr int kForwardRows = V > 1 && sizeof(X) > 2 ? 4 : 8;
 
 constexpr int kMostShared = 227 * 1024;  // of a CTA
@@ -38,7 +40,7 @@ bool aligned_to(const RecurrenceArgs& p, size_t bytes) {
 // Up to 8 warps whose lanes lie side by side in the channels as far as 128 bytes of a row go (full lines), and
 // behind one another in the rows beyond that; an SM holds two such CTAs.  Where full lines make fewer strips
 // than there are SMs, half lines do if that is enough; else the rows are cut into segments, as many as fill the
-// SMs (float32 1x65536x192, forward: 47 segments 48 us; 8 CTAs of a cluster to each strip took 71 us, one CTA 246 us).
+// SMs (float32 1x65536x192, forward: 94 segments 46 us; 8 CTAs of a cluster to each strip took 71 us, one CTA 246 us).
 template <typename X>
 RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     constexpr uint64_t kResident = 16;  // warps an SM holds at 128 registers a thread
@@ -51,6 +53,10 @@ RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     // two lines wide where that pads no more channels and leaves strips for one and a half rounds of the SMs:
     // half the parts to compose (bf16 64x500x768 36 against 40 us, float32 40x600x512 30 against 35 us)
     if (plan.log_lanes < std::min(columns, 5) && 2 * ctas(plan.log_lanes + 1) >= 3 * sms && ctas(plan.log_lanes + 1) * 2 == ctas(plan.log_lanes))
+        ++plan.log_lanes;
+    // and where there will be segments: the rows make up for the strips (float32 1x65536x192 training 108 against
+    // 112 us, bfloat16 16000x1536 packed 132 against 140 us)
+    else if (plan.log_lanes < std::min(columns, 5) && ctas(plan.log_lanes) < sms && ctas(plan.log_lanes + 1) * 2 == ctas(plan.log_lanes))
         ++plan.log_lanes;
     // short inputs: no more parts than there are rows for, the lanes go to the channels instead
     plan.log_lanes = std::max(plan.log_lanes, std::min(columns, 5 - std::min(needed, 5)));
@@ -82,9 +88,9 @@ void check(const char* what) {
 
 // Shared memory behind the rings: the offsets of packed sequences and what composes the segments.
 template <typename A>
-size_t front_bytes(const RecurrenceArgs& p, const RecurrencePlan& plan, int width) {
+size_t front_bytes(const RecurrenceArgs& p, const RecurrencePlan& plan, int width, bool in_ring = false) {
     const int values = std::max(32 * plan.warps, width);
-    return offset_room(p) + (plan.segments > 1 ? 2 * values * sizeof(A) + (values / width + 1) * sizeof(int) : 0);
+    return offset_room(p) + (plan.segments > 1 && !in_ring ? 2 * values * sizeof(A) + (values / width + 1) * sizeof(int) : 0);
 }
 
 // As many stages as the resident CTAs of an SM (16 warps) have room for; returns the bytes of shared memory of a CTA.
@@ -161,7 +167,7 @@ void forward(const RecurrenceArgs& p, cudaStream_t stream) {
 
 template <typename X, typename G, int V, bool SHARED>
 void backward(const RecurrenceArgs& p, cudaStream_t stream) {
-    constexpr int S = kBackwardRows<X, V>;
+    constexpr int S = kBackwardRows<X, G, V, SHARED>;
     RecurrencePlan plan = make_plan<X>(p, V, S);
     Scratch maps(maps_bytes<Acc<X>>(p, plan), stream);
     if (plan.segments > 1) {
@@ -181,7 +187,7 @@ void backward(const RecurrenceArgs& p, cudaStream_t stream) {
     const int width = V << plan.log_lanes;
     const size_t column = width * sizeof(Acc<X>);
     const size_t smem = shared_memory(plan, 2 * Prefetch<X, V, S, false>::kWarp + Prefetch<G, SHARED ? 1 : V, S, SHARED>::kWarp + column,
-                                      2 * plan.warps * column + front_bytes<Acc<X>>(p, plan, width));
+                                      2 * plan.warps * column + front_bytes<Acc<X>>(p, plan, width, fold_in_ring(width)));
     if (p.complement) {
         if (p.sequences) launch<recurrence_backward_kernel<X, G, V, S, SHARED, true, true>>(p, plan, smem, stream, partial);
         else launch<recurrence_backward_kernel<X, G, V, S, SHARED, false, true>>(p, plan, smem, stream, partial);

@@ -56,8 +56,9 @@ __device__ __forceinline__ int offset_at(const void* offsets, bool wide, int i) 
     return wide ? saturated(static_cast<const long long*>(offsets)[i]) : static_cast<const int*>(offsets)[i];
 }
 
-// Offsets of packed sequences that a CTA keeps in shared memory, where there are no more of them.
-constexpr int kLocalOffsets = 512;
+// Offsets of packed sequences that a CTA keeps in shared memory, where there are no more of them: what is left
+// beside the backward pass's stages of 16-bit inputs with two CTAs an SM.
+constexpr int kLocalOffsets = 240;
 
 // Bytes of shared memory that they take.
 __host__ __device__ inline size_t offset_room(const RecurrenceArgs& p) {
@@ -441,6 +442,10 @@ __device__ __forceinline__ void take_over(int link) {
     __syncwarp();
     asm volatile("bar.sync %0, 64;" ::"r"(link) : "memory");
 }
+
+// Backward: whether the memory of through_segments is that of the rings (2 W rows of `width`), which are not yet in
+// use: a strip of 64 channels and more leaves it room there.
+__host__ __device__ constexpr bool fold_in_ring(int width) { return width >= 64; }
 
 // What enters the strip's columns of a segment: `first`, which enters the first segment in scan order (null: 0), through
 // the maps of the segments before this one.  All threads call it: groups of them compose runs of
@@ -973,11 +978,12 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
     for (int v = 0; v < V; ++v) w[v] = !PACKED && p.state_derivs && live ? state_derivs()[b * p.dim + v] : A(0);
     if (plan.segments > 1) {
         cudaGridDependencySynchronize();  // the maps; what is above runs beside the kernel that makes them
-        A* fold = reinterpret_cast<A*>(next + offset_room(p));
+        A* fold = fold_in_ring(width) ? ahead - at.tc * V : reinterpret_cast<A*>(next + offset_room(p));
         through_segments<A, true, PACKED>(plan, b, at.segment, p.dim, c0 - uint64_t(at.tc) * V, width,
                                           PACKED || !p.state_derivs ? nullptr : static_cast<const A*>(p.state_derivs) + b * p.dim, fold);
 #pragma unroll
         for (int v = 0; v < V; ++v) w[v] = fold[at.tc * V + v];
+        if (fold_in_ring(width)) __syncthreads();
     }
     SequenceWalk walk;
     if (PACKED) {
