@@ -616,8 +616,8 @@ __device__ __forceinline__ void append_rows(Map<A, V>& m, const Rows<A, V, S>& r
 
 // Measured (B200, event times; the bytes alone would take what stands behind the bar): bfloat16 8x4096x2048 76 us | 61,
 // 8x8192x4096 277 | 245, float32 64x512x272 23 | 16: about 21 instructions a value at 59 % of the issue slots.  In
-// segments, with the kernel of their maps: float32 1x65536x192 48 us | 23, bfloat16 16000x1536 in 23 sequences
-// 52 | 15; there 16 warps an SM, all that 128 registers a thread admit, wait for one another.
+// segments, with the kernel of their maps: float32 1x65536x192 46 us | 23, bfloat16 16000x1536 in 23 sequences
+// 50 | 15; there 16 warps an SM, all that 128 registers a thread admit, wait for one another.
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED>
 __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
     using A = Acc<X>;
@@ -900,7 +900,7 @@ __device__ __forceinline__ void walk_out(int form, const Prefetch<X, V, S, false
 // Shared gates: each thread sums its V channels, 1 << fold_log neighbouring lanes are folded by shuffles,
 // and `partial` takes one value per row and fold (dgate itself where a fold is a whole gate).
 // Measured (as above): bfloat16 8x4096x2048 151 us | 102, float32 64x512x272 38 | 27: about 42 instructions a value
-// at 55 % of the issue slots; in segments float32 1x65536x192 64 us | 38, bfloat16 16000x1536 89 | 23.
+// at 55 % of the issue slots; in segments float32 1x65536x192 62 us | 38, bfloat16 16000x1536 83 | 23.
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED, bool COMPLEMENT>
 __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(const RecurrenceArgs p, const RecurrencePlan plan,
                                                                      Acc<X>* partial) {
