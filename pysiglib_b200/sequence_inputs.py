@@ -93,11 +93,10 @@ def batched_rows(array):
                 return array, 0, strides[0]
             if rank == 3:
                 return array, strides[0], strides[1]
-            axis = rank - 3
-            while axis > 0 and (shape[axis - 1] == 1 or strides[axis - 1] == strides[axis] * shape[axis]):
-                axis -= 1
-            if axis == 0:
-                return array, strides[-3], strides[-2]
+            # axes of one entry take no part: their strides lead nowhere
+            batch = [(n, s) for n, s in zip(shape[:-2], strides) if n != 1]
+            if all(outer[1] == inner[0] * inner[1] for outer, inner in zip(batch, batch[1:])):
+                return array, batch[-1][1] if batch else 0, strides[-2]
     array = contiguous(array)
     return array, rows * width, width
 

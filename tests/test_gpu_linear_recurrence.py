@@ -450,3 +450,20 @@ def test_segments_of_packed_rows_that_begin_and_end_in_sequences(lengths):
     rng = np.random.default_rng(62)
     start, tail = (torch.from_numpy(rng.standard_normal((len(lengths), 24)).astype(np.float32)) for _ in range(2))
     run_and_check((x, gate, start, derivs, tail, torch.from_numpy(bounds)), "log", True)
+
+
+@pytest.mark.parametrize("view", [lambda t: t[:, None, :3], lambda t: t[:, None, :1], lambda t: t[None, :, 1:4, None],
+                                  lambda t: t[1:2, None, :1].expand(3, 7, 1, -1, -1), lambda t: t[:, None].transpose(0, 2)])
+def test_views_with_axes_of_one_entry(view):
+    """Three and more batch axes, some of one entry, as x, gate and derivatives."""
+    g = torch.Generator().manual_seed(70)
+    bases = [torch.randn(4, 5, 40, 12, generator=g) for _ in range(3)]
+    X, G, D = (view(t.cuda()) for t in bases)
+    batch = X.shape[:-2].numel()
+    flat = [view(t).reshape(batch, 40, 12) for t in bases]
+    expect = so.recurrence(flat[0], flat[1], None, "logit", True, None, flat[2])
+    h, marks = psl.linear_recurrence(X, G, gate_form="logit", complement=True, return_checkpoints=True)
+    dx, dgate, _ = psl.linear_recurrence_backprop(D, X, G, gate_form="logit", complement=True, checkpoints=marks)
+    for name, got in (("h", h), ("dx", dx), ("dgate", dgate)):
+        assert got.shape == X.shape
+        so.check(got.reshape(batch, 40, 12), expect[name], name)
