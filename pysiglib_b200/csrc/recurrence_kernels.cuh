@@ -337,6 +337,8 @@ struct Prefetch {
     // where this thread's copies of the rows from `first` on start
     __device__ __forceinline__ const T* start(const T* first, int64_t stride) const { return odd ? first + stride - V : first; }
 
+    // `base`: the array's start, the source of the copies that bring zeros.  They too have to be aligned to their
+    // size, which a thread's own channels need not be where pairs are copied.
     __device__ __forceinline__ void issue(int stage, const T* base, const T* from, int64_t stride, int count) {
         if constexpr (kShared) {
             Pack<T, V>* to = slot + stage * per_stage;
@@ -1163,8 +1165,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_maps_kernel(const R
     int coming = REVERSE ? begin + run - S : begin;
     const auto fetch = [&](int stage) {
         const int n = coming >= begin ? rows_left<S>(end, coming, live) : 0;
-        fx.issue(stage, x, fx.start(x + int64_t(coming) * x_row, x_row), x_row, n);
-        fg.issue(stage, gate, fg.start(gate + int64_t(coming) * gate_row, gate_row), gate_row, n);
+        fx.issue(stage, static_cast<const X*>(REVERSE ? p.derivs : p.x), fx.start(x + int64_t(coming) * x_row, x_row), x_row, n);
+        fg.issue(stage, static_cast<const G*>(p.gate), fg.start(gate + int64_t(coming) * gate_row, gate_row), gate_row, n);
         commit_copies();
         coming += REVERSE ? -S : S;
     };
