@@ -154,12 +154,6 @@ __device__ __forceinline__ void exponential_pair(float v, float& a, float& rest)
     rest = 2.0f * fmaf(-s, p, 0.5f - s);
 }
 __device__ __forceinline__ void exponential_pair(double v, double& a, double& rest) { a = exp(v); rest = -expm1(v); }
-__device__ __forceinline__ float below(float v) {  // at most 2^100, NaN kept
-    float r;
-    asm("min.NaN.f32 %0, %1, 0f71800000;" : "=f"(r) : "f"(v));
-    return r;
-}
-__device__ __forceinline__ double below(double v) { return v > 0x1p1000 ? 0x1p1000 : v; }
 __device__ __forceinline__ float reciprocal(float v) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -234,8 +228,13 @@ __device__ __forceinline__ void v_fill(A (&r)[V], A value) {
     for (int v = 0; v < V; ++v) r[v] = value;
 }
 
-// a, and where PAIR 1 - a, of V gate values, neither by cancellation; for logits, with e = e^-v kept finite,
-// a = 1 / (1 + e) and 1 - a = e a.  The reciprocal is the hardware's (within 1 ulp).
+// 1 - a for a = 1 / (1 + e): e a, and 1 from 2^60 on, where it is 1 to the last bit long before a becomes 0 and e a
+// meaningless (a gate of -infinity closes exactly).  NaN is kept.
+template <typename A>
+__device__ __forceinline__ A complement_of(A e, A a) { return e >= A(0x1p60) ? A(1) : e * a; }
+
+// a, and where PAIR 1 - a, of V gate values, neither by cancellation; for logits, with e = e^-v, a = 1 / (1 + e) and
+// 1 - a = e a.  The reciprocal is the hardware's (within 1 ulp).
 // FAST (gates of 16 bits): exponentials as 2^(v log2 e) in single precision, off by up to 2 + 1.2 |v| ulp.  A gate
 // of 8 or 11 bits leaves e^v uncertain by |v| 2^-9 or 2^-12 of itself, thousands of times more.
 template <int FORM, bool FAST, bool PAIR, typename A, int V>
@@ -259,24 +258,23 @@ __device__ __forceinline__ void gate_factors(const A (&g)[V], A (&a)[V], A (&res
 #pragma unroll
             for (int v = 0; v < V; ++v) a[v] = t[v];
         } else {
-            if (PAIR) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) t[v] = below(t[v]);
-            }
             v_fill(unit, 1.0f);
             v_add(unit, unit, t);
 #pragma unroll
             for (int v = 0; v < V; ++v) a[v] = reciprocal(unit[v]);
-            if (PAIR) v_mul(rest, t, a);
+            if (PAIR) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) rest[v] = complement_of(t[v], a[v]);
+            }
         }
     } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             if constexpr (FORM == kGateLog) a[v] = exponential(g[v]);
             else {
-                const A e = PAIR ? below(exponential(-g[v])) : exponential(-g[v]);
+                const A e = exponential(-g[v]);
                 a[v] = reciprocal(A(1) + e);
-                rest[v] = e * a[v];
+                rest[v] = complement_of(e, a[v]);
             }
         }
     }

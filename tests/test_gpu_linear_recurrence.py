@@ -467,3 +467,30 @@ def test_views_with_axes_of_one_entry(view):
     for name, got in (("h", h), ("dx", dx), ("dgate", dgate)):
         assert got.shape == X.shape
         so.check(got.reshape(batch, 40, 12), expect[name], name)
+
+
+@pytest.mark.parametrize("dtype,gate_dtype", TYPES)
+def test_gates_far_below_zero(dtype, gate_dtype):
+    """Logits whose gate is tiny or 0: a state as large as its type lets through what the gate says and no more, with
+    `complement` and in the gradients too.  Smallest gate: 2^-100 of float32's range, 2^-1000 of float64's."""
+    far = {F32: [-60.0, -66.0, -75.0, -80.0], F64: [-60.0, -600.0, -695.0, -700.0]}[so.state_type(dtype)] + [-float("inf")]
+    dim = len(far) * 4
+    gate = torch.tensor(far, dtype=F64).repeat_interleave(4).to(gate_dtype).expand(2, 3, dim).contiguous()
+    x = torch.zeros(2, 3, dim, dtype=dtype)
+    big = 1e30 if so.state_type(dtype) is F32 else 1e300
+    start = torch.full((2, dim), big, dtype=so.state_type(dtype))
+    closed = torch.isinf(gate[0, 0])
+    for complement in (False, True):
+        # -inf is exact below; the oracle's bound for 16-bit gates grows with the finite ones alone
+        bound = so.recurrence(x[..., ~closed], gate[..., ~closed], start[:, ~closed], "logit", complement, None,
+                              torch.ones_like(x[..., ~closed]))
+        X, G, S = cuda(x), cuda(gate), cuda(start)
+        h, state = psl.linear_recurrence(X, G, S, gate_form="logit", complement=complement, return_state=True)
+        dx, dgate, dinitial = psl.linear_recurrence_backprop(torch.ones_like(X), X, G, S, gate_form="logit", complement=complement)
+        for name, got in (("h", h), ("state", state), ("dx", dx), ("dgate", dgate), ("dinitial", dinitial)):
+            so.check(got[..., ~closed], bound[name], name)
+            assert (got[..., closed].cpu() == (1.0 if name == "dx" else 0.0)).all(), name
+        step_state = S.clone()
+        psl.linear_recurrence_step(X[:, 0], G[:, 0], step_state, gate_form="logit", complement=complement)
+        so.check(step_state[:, ~closed], so.recurrence(x[:, :1, ~closed], gate[:, :1, ~closed], start[:, ~closed], "logit", complement)["state"], "step")
+        assert (step_state[:, closed] == 0).all()
