@@ -558,7 +558,7 @@ struct Rows {
 };
 
 // Rows that are not there, or in no sequence, become the identity; the initial state of a sequence that starts here
-// joins b, and its first row is then b alone (in the backward direction: the gradient of a state joins
+// (0 without one, which a gate that is not finite does not leave 0) joins b, and its first row is then b alone (in the backward direction: the gradient of a state joins
 // the derivatives of the row it was taken from).
 template <bool REVERSE, typename A, int V, int S>
 __device__ __forceinline__ void settle_rows(Rows<A, V, S>& r, const SequenceWalk& walk, int row0, const A* joins, int64_t dim, bool live) {
@@ -571,13 +571,13 @@ __device__ __forceinline__ void settle_rows(Rows<A, V, S>& r, const SequenceWalk
             }
     }
     const unsigned at = REVERSE ? r.e.ends : r.e.starts;
-    if (at && joins && live) {
+    if (at && (joins || !REVERSE) && live) {
 #pragma unroll
         for (int s = 0; s < S; ++s)
             if (at >> s & 1u) {
-                const A* in = joins + sequence_of(walk, row0 + s) * dim;
+                const A* in = joins ? joins + sequence_of(walk, row0 + s) * dim : nullptr;
 #pragma unroll
-                for (int v = 0; v < V; ++v) r.u[s][v] = REVERSE ? r.u[s][v] + in[v] : fma_(r.a[s][v], in[v], r.u[s][v]);
+                for (int v = 0; v < V; ++v) r.u[s][v] = REVERSE ? r.u[s][v] + in[v] : fma_(r.a[s][v], in ? in[v] : A(0), r.u[s][v]);
             }
     }
 }

@@ -494,3 +494,16 @@ def test_gates_far_below_zero(dtype, gate_dtype):
         psl.linear_recurrence_step(X[:, 0], G[:, 0], step_state, gate_form="logit", complement=complement)
         so.check(step_state[:, ~closed], so.recurrence(x[:, :1, ~closed], gate[:, :1, ~closed], start[:, ~closed], "logit", complement)["state"], "step")
         assert (step_state[:, closed] == 0).all()
+
+
+@pytest.mark.parametrize("rows", [40, 3000])
+def test_a_first_gate_that_is_not_finite(rows):
+    """a_0 times an absent state is a_0 times 0, NaN here, in a packed sequence as in a dense one; the next is clean."""
+    x, gate, _, derivs, _, _ = make(71, 1, rows, 8, 8, F32, F32, "value", False)
+    gate[0, 0, 0], gate[0, 0, 1] = float("nan"), float("inf")
+    X, G, cut = cuda(x[0]), cuda(gate[0]), rows - 10
+    dense, packed = psl.linear_recurrence(X, G), psl.linear_recurrence(X, G, offsets=torch.tensor([0, cut, rows]))
+    assert torch.isnan(dense[:, :2]).all() and torch.isnan(packed[:cut, :2]).all()
+    expect = so.recurrence(x[0], gate[0].clamp(-1, 1).nan_to_num(0.0), None, "value", False, torch.tensor([0, cut, rows]))["h"]
+    so.check(packed[:, 2:], tuple(t[:, 2:] for t in expect), "h")
+    so.check(packed[cut:], tuple(t[cut:] for t in expect), "h")
