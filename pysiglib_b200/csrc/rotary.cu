@@ -2,10 +2,10 @@
 //
 // Mathematics.  (y_p, y_q) = scale * (x_p cos w - x_q sin w, x_p sin w + x_q cos w) with w = p_t f_i, for the
 // pairs (i, i + r/2) or (2i, 2i + 1) of the first r channels; the others are copied.  The adjoint is the
-// turn by -w.  Angles are formed in 64 bits, as turns p_t * (f_i / 2 pi) less the nearest integer, so that a
+// turn by -w.  Angles are formed in 64 bits, as quarter turns p_t * (f_i 2 / pi) less the nearest integer, so that a
 // position of millions keeps all the bits that the sine needs.  The sine and cosine of the remainder are
-// taken in the type of the arithmetic (64 bits for float64 rows, of radians; else 32: the nearest quarter turn off, then
-// the Taylor series within an eighth of a turn) and each output is rounded once.
+// taken in the type of the arithmetic (64 bits for float64 rows, of radians; else 32: the Taylor series within an
+// eighth of a turn) and each output is rounded once.
 //
 // Split.  One read and one write per value bound it, as long as the sines are shared: a thread takes V pairs of
 // one position and walks over the rows (heads, batch entries) that have that position; where
@@ -35,20 +35,26 @@ struct RotaryGrid {
 
 constexpr int kInFlight = 4;  // rows of an unshared position, or of a copy
 
-// Sine and cosine of a number of turns.
-__device__ __forceinline__ void sine_cosine(double turns, float& s, float& c) {
-    constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
-    const float t = static_cast<float>(turns - ((turns + kMagic) - kMagic));
-    const float quarter = rintf(4.0f * t);
-    const float u = fmaf(quarter, -0.25f, t) * 6.2831853071795865f, z = u * u;
-    float p = fmaf(z, 1.0f / 362880, -1.0f / 5040), q = fmaf(z, -1.0f / 3628800, 1.0f / 40320);
-    p = fmaf(p, z, 1.0f / 120);
-    q = fmaf(q, z, -1.0f / 720);
-    p = fmaf(p, z, -1.0f / 6);
-    q = fmaf(q, z, 1.0f / 24);
-    q = fmaf(q, z, -0.5f);
-    const float sine = fmaf(p * z, u, u), cosine = fmaf(q, z, 1.0f);
-    const int k = static_cast<int>(quarter);
+// Sine and cosine of a number of quarter turns.  The nearest integer comes off in 64 bits; what is left, t of at most a
+// half, is rounded to 32 bits once, and the series in t have the powers of pi / 2 in their coefficients (the first
+// one in two parts).  Where 64 bits hold no fraction of a turn any more, t is 0.
+__device__ __forceinline__ void sine_cosine(double quarters, float& s, float& c) {
+    constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer, its last bits
+    constexpr double h = 1.57079632679489661923, h2 = h * h, h4 = h2 * h2, h8 = h4 * h4;
+    constexpr float kHigh = float(h), kLow = float(h - kHigh);
+    const double whole = quarters + kMagic;
+    float t = static_cast<float>(quarters - (whole - kMagic));
+    if (fabsf(t) > 0.5f) t = 0.0f;
+    const float z = t * t;
+    float p = fmaf(z, float(h8 * h / 362880), float(-h4 * h2 * h / 5040)), q = fmaf(z, float(-h8 * h2 / 3628800), float(h8 / 40320));
+    p = fmaf(p, z, float(h4 * h / 120));
+    q = fmaf(q, z, float(-h4 * h2 / 720));
+    p = fmaf(p, z, float(-h2 * h / 6));
+    q = fmaf(q, z, float(h4 / 24));
+    p = fmaf(p, z, kLow);
+    q = fmaf(q, z, float(-h2 / 2));
+    const float sine = fmaf(t, kHigh, t * p), cosine = fmaf(q, z, 1.0f);
+    const int k = __double2loint(whole);
     const float a = k & 1 ? cosine : sine, b = k & 1 ? sine : cosine;
     s = k & 2 ? -a : a;
     c = (k + 1) & 2 ? -b : b;
@@ -162,11 +168,11 @@ __global__ void __launch_bounds__(256, SHARED || sizeof(X) == 2 ? 2 : 3) rotary_
         return;
     }
     A s[V], c[V];
-    double rate[V];  // turns (float64: radians) for each unit of position
+    double rate[V];  // quarter turns (float64: radians) for each unit of position
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const uint64_t pair = !INTERLEAVED || V == 1 ? uint64_t(chunk) * V + v : (v < V / 2 ? cp : cp + cq - V) / 2 + v;
-        rate[v] = p.frequencies[pair] * (std::is_same_v<A, double> ? 1.0 : 0.15915494309189533577);
+        rate[v] = p.frequencies[pair] * (std::is_same_v<A, double> ? 1.0 : 0.63661977236758134308);
     }
     const A scale = static_cast<A>(p.scale), signed_scale = static_cast<A>(p.inverse ? -p.scale : p.scale);
     const auto turn_at = [&](double position) {

@@ -207,3 +207,35 @@ def test_a_float32_chain_in_training():
     for leaf in (x, gate, start):
         assert leaf.grad is not None and torch.isfinite(leaf.grad).all() and float(leaf.grad.abs().max()) > 0
     assert float(state[1].abs().max()) == 0
+
+
+def near_quarter_turns(odd):
+    """Angles (the frequency is 1) 1e-4 to 1e-2 from odd or even quarter turns, whose cosine or sine is that small."""
+    rng = np.random.default_rng(17)
+    k = 2.0 * rng.integers(-1000, 1000, 4000) + odd
+    return k * (np.pi / 2) + rng.choice([-1.0, 1.0], 4000) * 10.0 ** rng.uniform(-4, -2, 4000)
+
+
+@pytest.mark.parametrize("odd", [0, 1])
+def test_small_sines_and_cosines_keep_their_digits(odd):
+    """float32 rows: what is left of the angle is rounded once, relative to itself (1 unit of 2^-24), its sine is
+    within 2 units more (the series' product, a tenth of a unit, its sum, one, and its rest); the angle itself is
+    within 4 units of 2^-53."""
+    angle = near_quarter_turns(odd)
+    x = torch.zeros(4000, 2)
+    x[:, 0] = 1.0
+    for interleaved in (False, True):
+        y = psl.rotary(x.cuda(), torch.ones(1, dtype=F64).cuda(), torch.from_numpy(angle).cuda(), interleaved=interleaved).cpu().double().numpy()
+        exact = (np.cos if odd else np.sin)(angle.astype(np.longdouble)).astype(np.float64)
+        off = np.abs(y[:, 0 if odd else 1] - exact) - (4 * 2.0 ** -24 * np.abs(exact) + 4 * 2.0 ** -53 * np.abs(angle))
+        assert off.max() <= 0, off.max()
+
+
+@pytest.mark.parametrize("dtype", [F32, F64])
+def test_turns_past_counting_keep_the_length(dtype):
+    """Angles so large that 64 bits hold no fraction of a turn any more are some angle all the same."""
+    angle = torch.tensor([2.0 ** 49 + 0.25, 2.0 ** 51 + 1, 2.0 ** 53 + 2, 1e17, 1e30, -1e40, 1e200, 1e300], dtype=F64)
+    x = torch.zeros(8, 2, dtype=dtype)
+    x[:, 0] = 1.0
+    y = psl.rotary(x.cuda(), torch.ones(1, dtype=F64).cuda(), angle.cuda()).cpu().double()
+    assert float((y.square().sum(1) - 1).abs().max()) < 16 * so.unit(dtype)  # twice 4 units each for sine and cosine
