@@ -59,10 +59,18 @@ __device__ __forceinline__ void sine_cosine(double quarters, float& s, float& c)
     s = k & 2 ? -a : a;
     c = (k + 1) & 2 ? -b : b;
 }
-// In 64 bits of an angle: less the nearest number of whole turns, 2 pi in two parts.
+// In 64 bits of an angle: less the nearest number of whole turns, 2 pi in two parts.  What the remainder r loses when
+// it is rounded is the angle's error; kept as `low`, it turns sine and cosine by its first-order term.
 __device__ __forceinline__ void sine_cosine(double angle, double& s, double& c) {
+    constexpr double kHigh = 6.283185307179586232, kLow = 2.4492935982947064e-16;
     const double n = rint(angle * 0.15915494309189533577);
-    sincos(fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586232, angle)), &s, &c);
+    const double product = __dmul_rn(n, kHigh), rest = __dsub_rn(angle, product);  // rest is exact
+    const double off = fma(n, kLow, fma(n, kHigh, -product)), r = __dsub_rn(rest, off);
+    const double low = fabs(r) < 4.0 ? __dsub_rn(__dsub_rn(rest, r), off) : 0.0;  // past 2^53 turns any angle will do
+    double sine, cosine;
+    sincos(r, &sine, &cosine);
+    s = fma(cosine, low, sine);
+    c = fma(-sine, low, cosine);
 }
 
 template <typename P>

@@ -239,3 +239,17 @@ def test_turns_past_counting_keep_the_length(dtype):
     x[:, 0] = 1.0
     y = psl.rotary(x.cuda(), torch.ones(1, dtype=F64).cuda(), angle.cuda()).cpu().double()
     assert float((y.square().sum(1) - 1).abs().max()) < 16 * so.unit(dtype)  # twice 4 units each for sine and cosine
+
+
+@pytest.mark.parametrize("odd", [0, 1])
+def test_small_sines_and_cosines_keep_their_digits_in_float64(odd):
+    """CUDA's sincos is within 2 ulp (4 units), the remainder's low part adds one rounding."""
+    if np.finfo(np.longdouble).nmant < 63:
+        pytest.skip("needs an oracle of more than 64 bits")
+    angle = near_quarter_turns(odd)
+    x = torch.zeros(4000, 2, dtype=F64)
+    x[:, 0] = 1.0
+    y = psl.rotary(x.cuda(), torch.ones(1, dtype=F64).cuda(), torch.from_numpy(angle).cuda()).cpu().numpy()
+    exact = (np.cos if odd else np.sin)(angle.astype(np.longdouble))
+    off = np.abs(y[:, 0 if odd else 1].astype(np.longdouble) - exact) - 6 * 2.0 ** -53 * np.abs(exact)
+    assert off.max() <= 0, off.max()
