@@ -51,12 +51,18 @@ RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
     const auto ctas = [&](int log_lanes) { return p.batch * (((per_row - 1) >> log_lanes) + 1); };
     if (plan.log_lanes > 0 && ctas(plan.log_lanes) < sms && ctas(plan.log_lanes - 1) >= sms) --plan.log_lanes;
     // two lines wide where that pads no more channels and leaves strips for one and a half rounds of the SMs:
-    // half the parts to compose (bf16 64x500x768 36 against 40 us, float32 40x600x512 30 against 35 us)
+    // half the parts to compose (training, two lines against one: float32 48x400x320 40 against 48 us, 100x300x256 47
+    // against 57, 20x800x1024 97 against 105, 40x600x512 76 against 78, 64x2000x512 365 against 356; bfloat16 64x500x768
+    // 89 against 92, 16x2000x2048 203 against 202, 12x3000x2304 245 against 246)
     if (plan.log_lanes < std::min(columns, 5) && 2 * ctas(plan.log_lanes + 1) >= 3 * sms && ctas(plan.log_lanes + 1) * 2 == ctas(plan.log_lanes))
         ++plan.log_lanes;
-    // and where there will be segments: the rows make up for the strips (float32 1x65536x192 training 108 against
-    // 112 us, bfloat16 16000x1536 packed 132 against 140 us)
-    else if (plan.log_lanes < std::min(columns, 5) && ctas(plan.log_lanes) < sms && ctas(plan.log_lanes + 1) * 2 == ctas(plan.log_lanes))
+    // and where there will be segments: the rows make up for the strips, as long as a thread of a CTA composes no more
+    // than 32 of the segments' maps (through_segments), which are twice as many then.  Training, two lines wide against
+    // one: 25 maps float32 1x65536x192 108 against 111 us, 1x90000x192 146 against 149; 30 bfloat16 5x30000x128 89
+    // against 94; 25 1x50000x768 166 against 174; 12 16000x1536 packed 132 against 140; 37 float32 1x50000x128 66
+    // against 64; 49 bfloat16 3x30000x128 73 against 71; 148 1x30000x128 49 against 41
+    else if (plan.log_lanes < std::min(columns, 5) && ctas(plan.log_lanes) < sms && ctas(plan.log_lanes + 1) * 2 == ctas(plan.log_lanes) &&
+             kResident * sms * (V << (plan.log_lanes + 1)) <= 32 * 8 * kCtaThreads * ctas(plan.log_lanes + 1))
         ++plan.log_lanes;
     // short inputs: no more parts than there are rows for, the lanes go to the channels instead
     plan.log_lanes = std::max(plan.log_lanes, std::min(columns, 5 - std::min(needed, 5)));
@@ -66,10 +72,14 @@ RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
         throw std::invalid_argument("linear_recurrence: problem too large for one kernel launch");
     plan.strips = static_cast<unsigned>(((per_row - 1) >> plan.log_lanes) + 1);
     const uint64_t strips = ctas(plan.log_lanes), warp_rows = uint64_t(32 >> plan.log_lanes) * S, round = 2 * sms;
-    // rings of four warps where CTAs of eight would leave most of a second round empty, or where all CTAs of four
-    // just fit one (float32 64x512x272, 576 strips: 24.6 against 26.7 us; at 512 strips eight take 289, four 334 us)
-    if (plan.warps == 8 && ((strips > round && 2 * strips <= 3 * round) || (20 * strips > 38 * round && strips <= 2 * round)) &&
-        4 * warp_rows % kCheckpointRows == 0)
+    // Rings of four warps, twice as many on an SM, where CTAs of eight would leave most of a second round empty or have
+    // few iterations, whose start and end then count: three at most, or four where all CTAs of four warps fit one
+    // round.  Four against eight warps, forward and backward, in float32, float64 and bfloat16 of three widths: 330
+    // strips of 140 to 1200 rows 0.81 to 1.02 of the time, mostly 0.9; 480 to 2000 strips of 140 rows 0.69 to 0.86, of
+    // 257 rows 0.78 to 0.97; 480 and 560 strips of 400 rows 0.82 to 0.95, of 512 rows 0.89 to 1.04, of 640 rows 0.93 to
+    // 1.12; 640 to 2000 strips of 400 rows 0.83 to 1.07, of 512 rows 0.92 to 1.20.
+    const uint64_t iterations = (p.rows + 8 * warp_rows - 1) / (8 * warp_rows);
+    if (plan.warps == 8 && strips > round && (2 * strips <= 3 * round || iterations <= (strips <= 2 * round ? 4 : 3)) && 4 * warp_rows % kCheckpointRows == 0)
         plan.warps = 4;
     const uint64_t span = plan.warps * warp_rows, blocks = (p.rows + span - 1) / span;
     uint64_t segments = 1;

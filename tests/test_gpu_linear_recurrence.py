@@ -507,3 +507,11 @@ def test_a_first_gate_that_is_not_finite(rows):
     expect = so.recurrence(x[0], gate[0].clamp(-1, 1).nan_to_num(0.0), None, "value", False, torch.tensor([0, cut, rows]))["h"]
     so.check(packed[:, 2:], tuple(t[:, 2:] for t in expect), "h")
     so.check(packed[cut:], tuple(t[cut:] for t in expect), "h")
+
+
+@pytest.mark.parametrize("batch,rows,dim,gates,dtype,gate_dtype", [
+    (310, 140, 32, 32, F32, F32), (420, 30, 32, 1, F32, F32), (200, 384, 48, 48, F32, F32), (310, 385, 32, 32, F32, F32),
+    (600, 100, 16, 16, F64, F64), (600, 160, 7, 7, F32, F32), (310, 96, 64, 64, BF16, F32), (150, 130, 192, 3, BF16, BF16)])
+def test_short_rows_of_many_strips(batch, rows, dim, gates, dtype, gate_dtype):
+    """More strips than fit the GPU at once, of few iterations and of one more."""
+    run_and_check(make(batch + rows, batch, rows, dim, gates, dtype, gate_dtype, "logit", True), "logit", rows % 2 == 0)
