@@ -66,6 +66,7 @@ RecurrencePlan make_plan(const RecurrenceArgs& p, int V, int S) {
         ++plan.log_lanes;
     // short inputs: no more parts than there are rows for, the lanes go to the channels instead
     plan.log_lanes = std::max(plan.log_lanes, std::min(columns, 5 - std::min(needed, 5)));
+    // fewer than eight warps hold all rows in one iteration
     plan.warps = 1 << std::min(3, std::max(0, needed - (5 - plan.log_lanes)));
     plan.pairs = plan.log_lanes > 0 && aligned_to(p, 16);
     if (ctas(plan.log_lanes) > 0x7fffffffull)

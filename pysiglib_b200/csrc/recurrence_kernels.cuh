@@ -710,16 +710,15 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(cons
         append_rows<false, PACKED>(m, r);
         __syncwarp();
         scan_warp<A, V, false, PACKED>(m, plan.log_lanes);
-        if (base != first || at.warp) {
-            if (warps > 1) take_over(link_before);
-            else __syncwarp();
+        if (base != first || at.warp) {  // one warp alone has one iteration (make_plan)
+            take_over(link_before);
             const Pack<A, V> c = load_pack<A, V>(carry + at.warp * width);
 #pragma unroll
             for (int v = 0; v < V; ++v) in[v] = c.v[v];
         }
         A h[V];
         enter_rows<A, V, false>(m, plan.log_lanes, in, h, leaving,
-                                [&] { if (warps > 1 && (at.warp + 1 < warps || base + span < rows)) give(link); });
+                                [&] { if (at.warp + 1 < warps || base + span < rows) give(link); });
         if (r.count) {
             if (p.checkpoints && row0 % int(kCheckpointRows) == 0) {
                 Pack<A, V> mark;
@@ -1041,14 +1040,13 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
                                 [&] { if (passes) give(warps + 1 + at.warp); });
         // backward: the gradient
         if (base != last_base || at.warp + 1 < warps) {
-            if (warps > 1) take_over(link_behind);
-            else __syncwarp();
+            take_over(link_behind);
             const Pack<A, V> c = load_pack<A, V>(back + at.warp * width);
 #pragma unroll
             for (int v = 0; v < V; ++v) w[v] = c.v[v];
         }
         A behind[V];
-        enter_rows<A, V, true>(g, plan.log_lanes, w, behind, leaving, [&] { if (warps > 1 && (at.warp || base > first)) give(link); });
+        enter_rows<A, V, true>(g, plan.log_lanes, w, behind, leaving, [&] { if (at.warp || base > first) give(link); });
         // backward through the rows: the derivatives become g
         if (PACKED && !quiet) {
 #pragma unroll
