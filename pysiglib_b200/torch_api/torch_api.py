@@ -232,15 +232,18 @@ sig_coef.__doc__ = sig_coef_forward.__doc__
 
 
 class LinearRecurrence(torch.autograd.Function):
-    """Keeps x, the gates and one state of 16 for the backward pass, not h."""
+    """Keeps x, the gates and one state of 16 for the backward pass (`keep`), not h."""
 
     @staticmethod
-    def forward(ctx, x, gate, initial, gate_form, complement, offsets):
-        h, state, marks = linear_recurrence_forward(x, gate, initial, gate_form=gate_form, complement=complement,
-                                                    offsets=offsets, return_state=True, return_checkpoints=True)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, gate, initial, offsets, marks)
-        ctx.args = (gate_form, complement)
+    def forward(ctx, x, gate, initial, gate_form, complement, offsets, return_state=True, keep=True):
+        out = linear_recurrence_forward(x, gate, initial, gate_form=gate_form, complement=complement, offsets=offsets,
+                                        return_state=return_state, return_checkpoints=keep)
+        h, *rest = out if return_state or keep else (out,)
+        state = rest.pop(0) if return_state else None
+        if keep:
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(x, gate, initial, offsets, *rest)
+            ctx.args = (gate_form, complement)
         return h, state
 
     @staticmethod
@@ -250,26 +253,26 @@ class LinearRecurrence(torch.autograd.Function):
         gate_form, complement = ctx.args
         if grad_h is None:
             if grad_state is None:
-                return (None,) * 6
+                return (None,) * 8
             grad_h = torch.zeros_like(x)
         dx, dgate, dinitial = linear_recurrence_backprop(grad_h, x, gate, initial, gate_form=gate_form,
                                                          complement=complement, offsets=offsets,
                                                          state_derivs=grad_state, checkpoints=marks)
-        return dx, dgate, dinitial, None, None, None
+        return dx, dgate, dinitial, None, None, None, None, None
 
 
 def linear_recurrence(x, gate, initial=None, *, gate_form: str = "value", complement: bool = False, offsets=None,
                       return_state: bool = False, return_checkpoints: bool = False):
+    keep = torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, gate, initial))
     if not isinstance(x, torch.Tensor) or return_checkpoints:
-        if isinstance(x, torch.Tensor) and torch.is_grad_enabled() and any(
-                isinstance(t, torch.Tensor) and t.requires_grad for t in (x, gate, initial)):
+        if isinstance(x, torch.Tensor) and keep:
             raise ValueError("checkpoints are kept by the autograd graph: return_checkpoints needs inputs without gradients")
         return linear_recurrence_forward(x, gate, initial, gate_form=gate_form, complement=complement, offsets=offsets,
                                          return_state=return_state, return_checkpoints=return_checkpoints)
     check_type(return_state, "return_state", bool)
-    if isinstance(offsets, np.ndarray):
+    if isinstance(offsets, np.ndarray) and keep:
         offsets = torch.from_numpy(offsets.copy())  # kept for the backward pass
-    h, state = LinearRecurrence.apply(x, gate, initial, gate_form, complement, offsets)
+    h, state = LinearRecurrence.apply(x, gate, initial, gate_form, complement, offsets, return_state, keep)
     return (h, state) if return_state else h
 
 

@@ -198,3 +198,25 @@ def test_the_oracle_is_the_definition(form):
     got = so.recurrence(x.detach(), gate.detach(), start.detach(), form, True, offsets, d, tail)
     for name, want in zip(("h", "state", "dx", "dgate", "dinitial"), (h, state, *grads)):
         torch.testing.assert_close(got[name][0], want.detach(), rtol=1e-12, atol=1e-12)
+
+
+def test_autograd_asks_for_what_somebody_reads(monkeypatch):
+    """Checkpoints only where a gradient may be asked for, the state there or where the caller wants it."""
+    import sys
+    module = sys.modules[torch_api.linear_recurrence.__module__]
+    asked = []
+
+    def forward(x, gate, initial=None, *, return_state, return_checkpoints, **how):
+        asked.append((return_state, return_checkpoints))
+        parts = [x * 1.0] + [x[:, -1] * 1.0] * return_state + [x[:, :1] * 1.0] * return_checkpoints
+        return tuple(parts) if len(parts) > 1 else parts[0]
+    monkeypatch.setattr(module, "linear_recurrence_forward", forward)
+    x, gate, leaf = torch.zeros(2, 5, 6), torch.zeros(2, 5, 6), torch.zeros(2, 5, 6, requires_grad=True)
+    for return_state in (False, True):
+        for args, keep in (((x, gate), False), ((leaf, gate), True), ((x, leaf), True), ((x, gate, leaf[:, 0]), True)):
+            for grad_mode in (True, False):
+                with torch.set_grad_enabled(grad_mode):
+                    out = torch_api.linear_recurrence(*args, return_state=return_state)
+                assert asked.pop() == (return_state, keep and grad_mode)
+                h = out[0] if return_state else out
+                assert h.requires_grad == (keep and grad_mode) and (not return_state or out[1].shape == (2, 6))
