@@ -222,8 +222,11 @@ def linear_recurrence_step(
 
     :param x: the new rows, ``(..., dimension)``.
     :param gate: their gates, ``(..., G)`` as in ``linear_recurrence``.
-    :param state: ``(..., dimension)``, contiguous, float64 for float64 ``x``, else float32.  Overwritten.
+    :param state: ``(..., dimension)``, contiguous, float64 for float64 ``x``, else float32.  Overwritten; shares
+        no memory with ``x`` and ``gate``.
     :return: the new state in the type of ``x``.
+
+    No gradient passes through a step: with gradients enabled, inputs that require one are refused.
 
     Stepping through a sequence gives what ``linear_recurrence`` gives for it, up to rounding.
     """
@@ -243,6 +246,9 @@ def linear_recurrence_step(
         raise ValueError("state is overwritten: it must be contiguous and writeable")
     if torch_state and state.requires_grad:
         raise ValueError("state is overwritten: it cannot require a gradient (use linear_recurrence to differentiate)")
+    if torch_state and (x.requires_grad or gate.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("a step has no gradient: detach x and gate, step under torch.no_grad(), or differentiate "
+                         "torch_api.linear_recurrence")
     if torch_state and state.is_cuda:
         x, gate = x.contiguous(), gate.contiguous()
         out = torch.empty_like(x)

@@ -220,3 +220,13 @@ def test_autograd_asks_for_what_somebody_reads(monkeypatch):
                 assert asked.pop() == (return_state, keep and grad_mode)
                 h = out[0] if return_state else out
                 assert h.requires_grad == (keep and grad_mode) and (not return_state or out[1].shape == (2, 6))
+
+
+def test_a_step_does_not_drop_a_gradient_unseen():
+    x, gate, state = torch.zeros(0, 6), torch.zeros(0, 3), torch.zeros(0, 6)
+    for args in ((x.clone().requires_grad_(), gate), (x, gate.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="a step has no gradient"):
+            psl.linear_recurrence_step(*args, state)
+        with torch.no_grad():
+            assert psl.linear_recurrence_step(*args, state).shape == (0, 6)
+        assert psl.linear_recurrence_step(*(t.detach() for t in args), state).shape == (0, 6)
