@@ -515,3 +515,34 @@ def test_a_first_gate_that_is_not_finite(rows):
 def test_short_rows_of_many_strips(batch, rows, dim, gates, dtype, gate_dtype):
     """More strips than fit the GPU at once, of few iterations and of one more."""
     run_and_check(make(batch + rows, batch, rows, dim, gates, dtype, gate_dtype, "logit", True), "logit", rows % 2 == 0)
+
+
+@pytest.mark.parametrize("rows", [200, 3000])  # in one piece and in segments
+@pytest.mark.parametrize("dim", [16, 7])
+@pytest.mark.parametrize("bad", ["swapped", "outside", "falling", "far", "at the end"])
+def test_offsets_that_are_out_of_order_write_nothing_outside(rows, dim, bad):
+    """Every output lies between guards, which a row before it or behind it would change."""
+    from pysiglib_b200.sequence_inputs import native
+    offsets = {"swapped": [0, rows - 50, 50, rows], "outside": [-5, 10, rows + 100], "falling": [rows - 110, 80, 70, 60],
+               "far": [2 ** 40, -2 ** 40, 5], "at the end": [rows, rows, rows]}[bad]
+    count, guard, kept = len(offsets) - 1, 64 * dim, []
+
+    def guarded(*shape):
+        n = int(np.prod(shape))
+        kept.append(torch.full((n + 2 * guard,), 7.0, device="cuda"))
+        return kept[-1][guard:guard + n].view(shape)
+    offsets = torch.tensor(offsets, device="cuda")
+    g = torch.Generator().manual_seed(80)
+    x, gate, derivs = (torch.rand(rows, dim, generator=g).cuda() for _ in range(3))
+    start, tail = (torch.rand(count, dim, generator=g).cuda() for _ in range(2))
+    out, state, marks = guarded(rows, dim), guarded(count, dim), guarded(-(-rows // 16), dim)
+    dx, dgate, dinitial = guarded(rows, dim), guarded(rows, dim), guarded(count, dim)
+    stream, p = torch.cuda.current_stream().cuda_stream, lambda t: t.data_ptr()
+    assert native("linear_recurrence")(0, 0, p(x), p(gate), p(start), p(offsets), p(out), p(state), p(marks), 1, rows, dim, dim, count,
+                                       0, dim, 0, dim, 0, False, True, -1, stream, 1) == 0
+    assert native("linear_recurrence_backprop")(0, 0, p(derivs), p(x), p(gate), p(start), p(offsets), p(tail), p(marks), p(dx), p(dgate),
+                                                p(dinitial), 1, rows, dim, dim, count, 0, dim, 0, dim, 0, dim, 0, False, True, -1,
+                                                stream, 1) == 0
+    for whole in kept:
+        assert (whole[:guard] == 7.0).all() and (whole[-guard:] == 7.0).all()
+    assert (out != 7.0).all() and (dx != 7.0).all() and (dgate != 7.0).all()  # rows are written whatever the offsets say
