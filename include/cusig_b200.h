@@ -261,8 +261,8 @@ uint64_t sigb200_noalloc_scratch_bytes(void);
  * Strides are in elements; channels are adjacent.  device: -1, or the ordinal of the device that the caller
  * knows all pointers to be memory of, which saves looking them up.  Device pointers run on the device that owns them, on
  * `stream` (a cudaStream_t passed as void*), and return before completion unless synchronize != 0; host
- * pointers are staged (contiguous arrays only) and return when the result is there.  None of these
- * have a counterpart in the reference. */
+ * pointers are staged (contiguous arrays only) and return when the result is there.  Outputs overlap neither
+ * inputs nor one another.  None of these have a counterpart in the reference. */
 
 /* Gated linear recurrence along the rows of x (batch, length, dimension):
  *   h_t = a_t h_{t-1} + b_t,   b_t = complement ? (1 - a_t) x_t : x_t,   h_{-1} = initial (or 0),

@@ -558,8 +558,8 @@ struct Rows {
 };
 
 // Rows that are not there, or in no sequence, become the identity; the initial state of a sequence that starts here
-// (0 without one, which a gate that is not finite does not leave 0) joins b, and its first row is then b alone (in the backward direction: the gradient of a state joins
-// the derivatives of the row it was taken from).
+// (0 without one, which a gate that is not finite does not leave 0) joins b, and its first row is then b alone (in
+// the backward direction: the gradient of a state joins the derivatives of the row it was taken from).
 template <bool REVERSE, typename A, int V, int S>
 __device__ __forceinline__ void settle_rows(Rows<A, V, S>& r, const SequenceWalk& walk, int row0, const A* joins, int64_t dim, bool live) {
     if (r.count < S || r.e.dead) {
@@ -614,10 +614,11 @@ __device__ __forceinline__ void append_rows(Map<A, V>& m, const Rows<A, V, S>& r
     }
 }
 
-// Measured (B200, event times; the bytes alone would take what stands behind the bar): bfloat16 8x4096x2048 76 us | 61,
-// 8x8192x4096 277 | 245, float32 64x512x272 23 | 16: about 21 instructions a value at 59 % of the issue slots.  In
-// segments, with the kernel of their maps: float32 1x65536x192 46 us | 23, bfloat16 16000x1536 in 23 sequences
-// 50 | 15; there 16 warps an SM, all that 128 registers a thread admit, wait for one another.
+// Measured (B200, eight launches between two events; the bytes alone would take what stands behind the bar): bfloat16
+// 8x4096x2048 81 us | 61, 8x8192x4096 268 to 287 | 245 (the power cap moves the clock), float32 64x512x272 21 | 16: about
+// 23 instructions a value at 61 % of the issue slots, 13.5 of the 16 warps an SM that 128 registers a thread admit.
+// In segments, with the kernel of their maps: float32 1x65536x192 45 us | 23, bfloat16 16000x1536 in 23 sequences
+// 48 | 15; there the warps wait for one another.
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED>
 __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_forward_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
     using A = Acc<X>;
@@ -898,8 +899,9 @@ __device__ __forceinline__ void walk_out(int form, const Prefetch<X, V, S, false
 // the ring of warps, from the last to the first.
 // Shared gates: each thread sums its V channels, 1 << fold_log neighbouring lanes are folded by shuffles,
 // and `partial` takes one value per row and fold (dgate itself where a fold is a whole gate).
-// Measured (as above): bfloat16 8x4096x2048 151 us | 102, float32 64x512x272 38 | 27: about 42 instructions a value
-// at 55 % of the issue slots; in segments float32 1x65536x192 62 us | 38, bfloat16 16000x1536 83 | 23.
+// Measured (as above): bfloat16 8x4096x2048 153 us | 102, float32 64x512x272 38 | 27: about 45 instructions a value
+// at 60 % of the issue slots, 256 CTAs for 296 places; in segments float32 1x65536x192 62 us | 38, bfloat16 16000x1536
+// 79 | 23.
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED, bool COMPLEMENT>
 __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(const RecurrenceArgs p, const RecurrencePlan plan,
                                                                      Acc<X>* partial) {
@@ -1116,8 +1118,8 @@ __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_backward_kernel(con
 // the place of x, gradients of states).  Each thread takes a contiguous run of rows, S at a time, and
 // appends them to its map; parts and warps are composed once, at the end.
 // Of packed sequences only the last (REVERSE: the first) one in a segment decides what leaves it: the rows before
-// (behind) it are not read.  Measured: float32 1x65536x192, 101 MB in 21 us, 62 % of the HBM's rate; bfloat16
-// 16000x1536 in 23 sequences 17 us instead of 24.
+// (behind) it are not read.  Measured: float32 1x65536x192, 101 MB in 21 us, 60 % of the HBM's rate; bfloat16
+// 16000x1536 in 23 sequences 17 to 19 us instead of 24.
 template <typename X, typename G, int V, int S, bool SHARED, bool PACKED, bool REVERSE>
 __global__ void __launch_bounds__(kCtaThreads, 2) recurrence_maps_kernel(const RecurrenceArgs p, const RecurrencePlan plan) {
     using A = Acc<X>;
@@ -1234,7 +1236,8 @@ __global__ void fold_partials_kernel(const A* __restrict__ partial, G* __restric
 
 // One row for each state: state = a state + b, out = the new state rounded.  Two reads, one read and write
 // of the state and one write; a grid over all values, since nothing is shared between them.
-// The launch is most of it: float32 16x512 takes 6 us between two events, its 164 KB would take 0.03 us.
+// The launch is most of it: bfloat16 16x512 with float32 gates takes 3.2 us, one launch behind the other, its 131 KB
+// would take 0.02 us.
 template <typename X, typename G, int V, bool SHARED>
 __global__ void __launch_bounds__(256) recurrence_step_kernel(const RecurrenceArgs p) {
     using A = Acc<X>;

@@ -10,7 +10,7 @@
 // Split.  One read and one write per value bound it, as long as the sines are shared: a thread takes V pairs of
 // one position and walks over the rows (heads, batch entries) that have that position; where
 // every row has its own it takes four positions, loads them all, and turns one after the other.
-// Measured (B200, kernel alone; the copy alone would take what stands behind the bar): bfloat16 2x32768x16x128 195 us | 164,
+// Measured (B200, eight launches between two events; the copy alone would take what stands behind the bar): bfloat16 2x32768x16x128 193 us | 164,
 // 4x2048x32x128 33 | 20; float32 64x1023x272 with a time stamp a row 56 | 43.  What is left is the sines where they
 // are not shared and the loads' latency at the start and the end of short threads.
 #include <algorithm>
@@ -306,7 +306,7 @@ bool fits(const RotaryArgs& p, uint64_t V, size_t size) {
     return reinterpret_cast<uintptr_t>(p.x) % (V * size) == 0 && reinterpret_cast<uintptr_t>(p.out) % (V * size) == 0;
 }
 
-// 16 bytes a load where all is aligned to it; else two values where that fits (bfloat16 8x4096x8x132, 68 turned: 47
+// 16 bytes a load where all is aligned to it; else two values where that fits (bfloat16 8x4096x8x132, 68 turned: 44
 // against 70 us one by one), else one.
 template <typename X>
 void launch_type(const RotaryArgs& p, cudaStream_t stream) {
