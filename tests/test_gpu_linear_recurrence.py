@@ -546,3 +546,57 @@ def test_offsets_that_are_out_of_order_write_nothing_outside(rows, dim, bad):
     for whole in kept:
         assert (whole[:guard] == 7.0).all() and (whole[-guard:] == 7.0).all()
     assert (out != 7.0).all() and (dx != 7.0).all() and (dgate != 7.0).all()  # rows are written whatever the offsets say
+
+
+def test_a_captured_step_goes_on_with_its_state():
+    """Serving: one captured step, replayed for each new row, in inference mode as outside it."""
+    x, gate, start, *_ = make(90, 5, 12, 24, 3, BF16, F32, "log", True)
+    expect = so.recurrence(x, gate, start, "log", True)
+    for mode in (torch.inference_mode, torch.no_grad):
+        with mode():
+            X, G, S = cuda(x), cuda(gate), cuda(start)
+            row, row_gate = X[:, 0].clone(), G[:, 0].clone()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = psl.linear_recurrence_step(row, row_gate, S, gate_form="log", complement=True)
+            for t in range(12):
+                row.copy_(X[:, t])
+                row_gate.copy_(G[:, t])
+                graph.replay()
+                so.check(out, (expect["h"][0][:, t], expect["h"][1][:, t]), "row %d" % t)
+            so.check(S, expect["state"], "state")
+
+
+def test_recomputed_and_graphed_layers():
+    """The layer under torch's activation checkpointing and as a graphed callable gives the gradients it gives alone."""
+    from torch.utils.checkpoint import checkpoint
+    x, gate, start, derivs, tail, _ = make(91, 3, 200, 40, 8, F32, F32, "logit", True)
+
+    class Layer(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.bias = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+
+        def forward(self, x, gate):
+            return torch_api.linear_recurrence(x, gate + self.bias, gate_form="logit", complement=True)
+
+    expect = so.recurrence(x, gate, None, "logit", True, None, derivs)
+    layer, X, G = Layer(), cuda(x).requires_grad_(), cuda(gate).requires_grad_()
+
+    def grads(f):
+        h = f(X, G)
+        so.check(h, expect["h"], "h")
+        return torch.autograd.grad(h, (X, G, layer.bias), cuda(derivs))
+    # the graphed one first: no eager graph of the same leaves lives beside its capture
+    sample = tuple(torch.randn_like(t).requires_grad_() for t in (X, G))
+    graphed = torch.cuda.make_graphed_callables(layer, sample)
+    for _ in range(2):
+        for name, got in zip(("dx", "dgate"), grads(graphed)):
+            so.check(got, expect[name], name)
+    plain = Layer()
+    for f in (plain, lambda x, g: checkpoint(plain, x, g, use_reentrant=False)):
+        h = f(X, G)
+        dx, dgate, dbias = torch.autograd.grad(h, (X, G, plain.bias), cuda(derivs))
+        so.check(dx, expect["dx"], "dx")
+        so.check(dgate, expect["dgate"], "dgate")
+        assert torch.equal(dbias, dgate.sum((0, 1)))
