@@ -571,14 +571,21 @@ __device__ __forceinline__ void settle_rows(Rows<A, V, S>& r, const SequenceWalk
             }
     }
     const unsigned at = REVERSE ? r.e.ends : r.e.starts;
-    if (at && (joins || !REVERSE) && live) {
+    if (at && live) {
+        if (joins) {
 #pragma unroll
-        for (int s = 0; s < S; ++s)
-            if (at >> s & 1u) {
-                const A* in = joins ? joins + sequence_of(walk, row0 + s) * dim : nullptr;
+            for (int s = 0; s < S; ++s)
+                if (at >> s & 1u) {
+                    const A* in = joins + sequence_of(walk, row0 + s) * dim;
 #pragma unroll
-                for (int v = 0; v < V; ++v) r.u[s][v] = REVERSE ? r.u[s][v] + in[v] : fma_(r.a[s][v], in ? in[v] : A(0), r.u[s][v]);
-            }
+                    for (int v = 0; v < V; ++v) r.u[s][v] = REVERSE ? r.u[s][v] + in[v] : fma_(r.a[s][v], in[v], r.u[s][v]);
+                }
+        } else if (!REVERSE) {
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int v = 0; v < V; ++v) r.u[s][v] = at >> s & 1u ? fma_(r.a[s][v], A(0), r.u[s][v]) : r.u[s][v];
+        }
     }
 }
 
