@@ -4,8 +4,8 @@
 // pairs (i, i + r/2) or (2i, 2i + 1) of the first r channels; the others are copied.  The adjoint is the
 // turn by -w.  Angles are formed in 64 bits, as quarter turns p_t * (f_i 2 / pi) less the nearest integer, so that a
 // position of millions keeps all the bits that the sine needs.  The sine and cosine of the remainder are
-// taken in the type of the arithmetic (64 bits for float64 rows, of radians; else 32: the Taylor series within an
-// eighth of a turn) and each output is rounded once.
+// taken in the type of the arithmetic (64 bits for float64 rows, of radians; else 32) by their Taylor series within an
+// eighth of a turn, and each output is rounded once.
 //
 // Split.  One read and one write per value bound it, as long as the sines are shared: a thread takes V pairs of
 // one position and walks over the rows (heads, batch entries) that have that position; where
@@ -59,18 +59,37 @@ __device__ __forceinline__ void sine_cosine(double quarters, float& s, float& c)
     s = k & 2 ? -a : a;
     c = (k + 1) & 2 ? -b : b;
 }
-// In 64 bits of an angle: less the nearest number of whole turns, 2 pi in two parts.  What the remainder r loses when
-// it is rounded is the angle's error; kept as `low`, it turns sine and cosine by its first-order term.
+// In 64 bits of an angle: less the nearest number of quarter turns, pi / 2 in two parts, then the Taylor series (the
+// terms left out are below 2^-60 of what they belong to).  What the remainder t loses when it is rounded is the angle's
+// error; kept as `low`, it turns sine and cosine by its first-order term.  Where an angle's neighbours are more than a
+// turn away, t is 0.
 __device__ __forceinline__ void sine_cosine(double angle, double& s, double& c) {
-    constexpr double kHigh = 6.283185307179586232, kLow = 2.4492935982947064e-16;
-    const double n = rint(angle * 0.15915494309189533577);
+    constexpr double kMagic = 6755399441055744.0, kHigh = 1.57079632679489661923, kLow = 6.123233995736766e-17;
+    const double whole = fma(angle, 0.63661977236758134308, kMagic), n = whole - kMagic;
     const double product = __dmul_rn(n, kHigh), rest = __dsub_rn(angle, product);  // rest is exact
-    const double off = fma(n, kLow, fma(n, kHigh, -product)), r = __dsub_rn(rest, off);
-    const double low = fabs(r) < 4.0 ? __dsub_rn(__dsub_rn(rest, r), off) : 0.0;  // past 2^53 turns any angle will do
-    double sine, cosine;
-    sincos(r, &sine, &cosine);
-    s = fma(cosine, low, sine);
-    c = fma(-sine, low, cosine);
+    const double off = fma(n, kLow, fma(n, kHigh, -product));
+    double t = __dsub_rn(rest, off), low = __dsub_rn(__dsub_rn(rest, t), off);
+    if (fabs(t) > 1.0) t = low = 0.0;
+    const double z = t * t;
+    double p = fma(z, 1.0 / 355687428096000, -1.0 / 1307674368000), q = fma(z, 1.0 / 20922789888000, -1.0 / 87178291200);
+    p = fma(p, z, 1.0 / 6227020800);
+    q = fma(q, z, 1.0 / 479001600);
+    p = fma(p, z, -1.0 / 39916800);
+    q = fma(q, z, -1.0 / 3628800);
+    p = fma(p, z, 1.0 / 362880);
+    q = fma(q, z, 1.0 / 40320);
+    p = fma(p, z, -1.0 / 5040);
+    q = fma(q, z, -1.0 / 720);
+    p = fma(p, z, 1.0 / 120);
+    q = fma(q, z, 1.0 / 24);
+    p = fma(p, z, -1.0 / 6);
+    q = fma(q, z, -0.5);
+    const double first = fma(p * z, t, t), second = fma(q, z, 1.0);
+    const double sine = fma(second, low, first), cosine = fma(-first, low, second);
+    const int k = __double2loint(whole);
+    const double a = k & 1 ? cosine : sine, b = k & 1 ? sine : cosine;
+    s = k & 2 ? -a : a;
+    c = (k + 1) & 2 ? -b : b;
 }
 
 template <typename P>

@@ -243,7 +243,7 @@ def test_turns_past_counting_keep_the_length(dtype):
 
 @pytest.mark.parametrize("odd", [0, 1])
 def test_small_sines_and_cosines_keep_their_digits_in_float64(odd):
-    """CUDA's sincos is within 2 ulp (4 units), the remainder's low part adds one rounding."""
+    """The series are within 2 units of 2^-53 each, the remainder within one, its low part adds one rounding."""
     if np.finfo(np.longdouble).nmant < 63:
         pytest.skip("needs an oracle of more than 64 bits")
     angle = near_quarter_turns(odd)
