@@ -125,8 +125,8 @@ def linear_recurrence(
     :param offsets: packed sequences: ``x`` is ``(rows, dimension)`` and sequence ``i`` holds the rows
         ``offsets[i]`` to ``offsets[i + 1] - 1`` (int32 or int64, ``n + 1`` values that do not decrease).
         Sequences may be empty; rows of no sequence come out as 0.  ``initial`` and the state are
-        ``(n, dimension)``.  Values on the host are checked, those on the device are trusted: wrong ones
-        give wrong numbers.
+        ``(n, dimension)``.  Values on the host are checked and copied to the device, which waits for the
+        copy and cannot be captured; those on the device are trusted: wrong ones give wrong numbers.
     :param return_state: also return the state after the last row (``initial`` for an empty sequence),
         ready for ``linear_recurrence_step``.
     :param return_checkpoints: also return the states before rows 0, 16, 32, .., which
